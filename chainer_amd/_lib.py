@@ -199,6 +199,14 @@ SIGNATURES = {
     'hipcx_lstm_step': (_INT, [_A, _A, _A, _A, _A, _A, _A, _A, _V]),
     'hipcx_softmax_cross_entropy_workspace_size': (_SZ, [_A]),
     'hipcx_softmax_cross_entropy': (_INT, [_A, _A, _A, _V, _SZ, _V]),
+    'hipcx_dropout': (_INT, [_A, ctypes.c_double, _A, ctypes.c_int64, _A, _A, _V]),
+    'hipcx_causal_conv': (_INT, [_A] * 5 + [_INT] + [_A] * 2 + [_V]),
+    'hipcx_causal_conv_grad_workspace_size': (_SZ, [_A, _A]),
+    'hipcx_causal_conv_grad': (_INT, [_A] * 5 + [_INT] + [_A] * 6 + [_V, _SZ, _V]),
+    'hipcx_selective_scan_workspace_size': (_SZ, [_A, _A]),
+    'hipcx_selective_scan': (_INT, [_A] * 8 + [_INT] + [_A] * 4 + [_V, _SZ, _V]),
+    'hipcx_selective_scan_grad_workspace_size': (_SZ, [_A, _A, _A]),
+    'hipcx_selective_scan_grad': (_INT, [_A] * 8 + [_INT] + [_A] * 13 + [_V, _SZ, _V]),
     'hipcx_profile_start': (_INT, []),
     'hipcx_profile_stop': (_INT, [_I64P, ctypes.POINTER(ctypes.c_double), ctypes.POINTER(ctypes.c_double),
                                   ctypes.POINTER(ctypes.c_double)]),

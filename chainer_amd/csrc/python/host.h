@@ -187,7 +187,7 @@ inline void Call(F&& f) {
 void Parse(const char* fn, PyObject* const* args, Py_ssize_t nargs, PyObject* kwnames, PyObject* const* names, int n_names, int n_required,
            PyObject** out);
 struct Names {  // interned argument names
-    static constexpr int kMax = 12;
+    static constexpr int kMax = 16;
     PyObject* v[kMax];
     int n = 0;
     Names(std::initializer_list<const char*> names) {
@@ -202,5 +202,10 @@ struct Names {  // interned argument names
 inline bool Given(PyObject* x) { return x != nullptr && x != Py_None; }
 
 extern PyMethodDef kRoutines[];  // routines.cc
+HOST_FN(Dropout);                // sequence.cc
+HOST_FN(CausalConv);
+HOST_FN(CausalConvGrad);
+HOST_FN(SelectiveScan);
+HOST_FN(SelectiveScanGrad);
 
 }  // namespace host

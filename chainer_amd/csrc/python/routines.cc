@@ -1402,6 +1402,11 @@ PyMethodDef kRoutines[] = {
         ROUTINE("lstm_step_direct", LstmStep, nullptr),
         ROUTINE("rnn_forward", RnnForward, nullptr),
         ROUTINE("rnn_backward", RnnBackward, nullptr),
+        ROUTINE("dropout", Dropout, nullptr),
+        ROUTINE("causal_conv", CausalConv, nullptr),
+        ROUTINE("causal_conv_grad", CausalConvGrad, nullptr),
+        ROUTINE("selective_scan", SelectiveScan, nullptr),
+        ROUTINE("selective_scan_grad", SelectiveScanGrad, nullptr),
         {nullptr, nullptr, 0, nullptr}};
 
 }  // namespace host

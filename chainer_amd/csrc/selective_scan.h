@@ -1,0 +1,138 @@
+// What the selective scan and its gradients share.
+//   h[t][n] = exp(dt[t] a[n]) h[t-1][n] + dt[t] u[t] b[t][n],  y[t] = (sum over n of c[t][n] h[t][n] + d u[t]) silu(z[t])
+// for every sequence and channel; dt = delta + bias, or softplus of it.  b and c belong to a group of channels.
+#pragma once
+
+#include "sequence.h"
+
+namespace hipcx {
+
+// Rows of b or c, [batch, time, group, state]; strides in elements.
+struct ScanShared {
+    void* data;
+    int64_t batch, row, group;
+};
+
+struct ScanArgs {
+    SequenceRows u, delta, z, y;
+    ScanShared b, c;
+    const float *a, *d, *bias;  // [channels][states], [channels] or null
+    const float* state;         // [batch][channels][states] or null
+    float* new_state;
+    SequenceLengths lengths;
+    int64_t batch, length;
+    int channels, states, group_channels;
+    int group_blocks, blocks;   // workgroups along the channels of a group, of all groups
+    int chunks, chunk_rows;     // of the time axis; whole tiles of rows
+    float* ends;                // [batch][chunks][channels][states]: the state that the sequence starts from, then what each chunk but the last adds
+    float* steps;               // [batch][chunks - 1][channels]: dt summed over the chunk
+    int softplus;
+};
+
+// Four lanes (a quad) belong to a channel: each keeps a quarter of its states, and they take the rows' other work in turns.  A wave has 16 channels.
+constexpr int kScanChannels = 64;  // to a workgroup of four waves
+constexpr int kScanTile = 16;      // rows whose b and c are in LDS
+
+template <int S>
+__device__ __forceinline__ float OfQuadLane(float v) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), S * 0x55, 0xf, 0xf, true));
+}
+__device__ __forceinline__ float QuadSwap1(float v) { return __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), 0xB1, 0xf, 0xf, true)); }
+__device__ __forceinline__ float QuadSwap2(float v) { return __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), 0x4E, 0xf, 0xf, true)); }
+
+// Lane q of a quad gets the sum of v[q] over the quad.
+__device__ __forceinline__ float QuadTransposedSum(const float (&v)[4], int q) {
+    const bool odd = (q & 1) != 0, high = (q & 2) != 0;
+    const float r0 = (odd ? v[1] : v[0]) + QuadSwap1(odd ? v[0] : v[1]);
+    const float r1 = (odd ? v[3] : v[2]) + QuadSwap1(odd ? v[2] : v[3]);
+    return (high ? r1 : r0) + QuadSwap2(high ? r0 : r1);
+}
+
+// log(1 + exp(x)) = max(x, 0) + log(1 + e), e = exp(-|x|); the logarithm as 2 artanh(s), s = e / (2 + e) <= 1/3, by seven terms of its series (the eighth is 1.4e-8 of
+// the sum): a step of 1e-3 keeps its 24 bits, which it loses in 1 + e.
+__device__ __forceinline__ float SoftplusOf(float x) {
+    const float e = __builtin_amdgcn_exp2f(-kLog2E * __builtin_fabsf(x));
+    const float s = e * __builtin_amdgcn_rcpf(2.f + e), q = s * s;
+    float r = 1.f / 13;
+    r = __builtin_fmaf(r, q, 1.f / 11);
+    r = __builtin_fmaf(r, q, 1.f / 9);
+    r = __builtin_fmaf(r, q, 1.f / 7);
+    r = __builtin_fmaf(r, q, 1.f / 5);
+    r = __builtin_fmaf(r, q, 1.f / 3);
+    return __builtin_fmaxf(x, 0.f) + 2.f * __builtin_fmaf(s * q, r, s);
+}
+
+// States n0 .. n0 + NPL - 1 of `all`, which the padding follows; one access where they are all there.
+template <int NPL>
+struct __attribute__((packed, aligned(4))) LaneStates {
+    float v[NPL];
+};
+template <int NPL>
+__device__ __forceinline__ void LoadStates(const float* p, int n0, int all, float (&v)[NPL]) {
+    if (n0 + NPL <= all) {
+        const LaneStates<NPL> s = *reinterpret_cast<const LaneStates<NPL>*>(p + n0);
+#pragma unroll
+        for (int i = 0; i < NPL; ++i) v[i] = s.v[i];
+    } else {
+#pragma unroll
+        for (int i = 0; i < NPL; ++i) v[i] = n0 + i < all ? p[n0 + i] : 0.f;
+    }
+}
+template <int NPL>
+__device__ __forceinline__ void StoreStates(float* p, int n0, int all, const float (&v)[NPL]) {
+    if (n0 + NPL <= all) {
+        LaneStates<NPL> s;
+#pragma unroll
+        for (int i = 0; i < NPL; ++i) s.v[i] = v[i];
+        *reinterpret_cast<LaneStates<NPL>*>(p + n0) = s;
+    } else {
+#pragma unroll
+        for (int i = 0; i < NPL; ++i) {
+            if (n0 + i < all) p[n0 + i] = v[i];
+        }
+    }
+}
+
+// Where a thread stands: its sequence, chunk, channel and lane of the quad.
+struct ScanPlace {
+    int64_t b;
+    int chunk, group, channel, q;
+    bool inside;  // else it repeats the group's last channel and stores nothing
+    __device__ __forceinline__ ScanPlace(const ScanArgs& p, unsigned block, int chunks) {
+        const unsigned line = block / static_cast<unsigned>(p.blocks), of_channels = block % static_cast<unsigned>(p.blocks);
+        chunk = static_cast<int>(line % static_cast<unsigned>(chunks));
+        b = line / static_cast<unsigned>(chunks);
+        group = static_cast<int>(of_channels) / p.group_blocks;
+        const int within = (static_cast<int>(of_channels) - group * p.group_blocks) * kScanChannels + (static_cast<int>(threadIdx.x) >> 2);
+        inside = within < p.group_channels;
+        channel = group * p.group_channels + (inside ? within : p.group_channels - 1);
+        q = static_cast<int>(threadIdx.x) & 3;
+    }
+};
+
+template <typename T>
+__device__ __forceinline__ float ScanRead(const SequenceRows& r, int64_t b, int64_t row, int channel) {
+    return static_cast<float>(static_cast<const T*>(r.data)[b * r.batch + row * r.row + channel]);
+}
+
+// The NPL of a call: a lane's share of the states, rounded up to a power of two.
+template <typename F>
+void VisitScan(int dtype, int states, F&& f) {
+    const auto visit = [&](auto tag) {
+        const int share = (states + 3) / 4;
+        if (share <= 1) f(tag, std::integral_constant<int, 1>{});
+        else if (share <= 2) f(tag, std::integral_constant<int, 2>{});
+        else if (share <= 4) f(tag, std::integral_constant<int, 4>{});
+        else if (share <= 8) f(tag, std::integral_constant<int, 8>{});
+        else f(tag, std::integral_constant<int, 16>{});
+    };
+    if (dtype == HIPCX_FLOAT16) visit(Tag<half_t>{});
+    else visit(Tag<float>{});
+}
+
+// Checks the inputs that the scan and its gradients share and describes them, except for the cut along time.
+ScanArgs DescribeScan(const std::string& what, const hipcx_array* u, const hipcx_array* delta, const hipcx_array* a, const hipcx_array* b, const hipcx_array* c,
+                      const hipcx_array* d, const hipcx_array* z, const hipcx_array* delta_bias, int delta_softplus, const hipcx_array* state,
+                      const hipcx_array* lengths);
+
+}  // namespace hipcx

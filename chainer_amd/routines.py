@@ -7,6 +7,7 @@ LogSoftmax, the Lstm cell, softmax cross entropy) runs as one kernel where its a
 except by the opt-in ``conv_bn_act``.
 """
 import builtins as _py
+import collections
 import ctypes
 
 import numpy
@@ -1756,6 +1757,48 @@ def n_step_birnn(n_layers, hx, ws, bs, xs, activation='tanh', kernel=False):
         (hy, _), ys, _ = rnn(n_layers, hx, None, ws, bs, xs, True, 'rnn', activation)
         return hy, ys
     return _n_step_rnn_impl(_rnn_impl, n_layers, hx, None, ws, bs, xs, True, activation)
+
+
+# ---------------------------------------------------------------------------------------------
+# layers of a recurrent block that the reference has no kernels for: the causal convolution, the selective scan, dropout
+# ---------------------------------------------------------------------------------------------
+def dropout(x, ratio, key, site=0, residual=None):
+    """Dropout (chainer/functions/noise/dropout.py): ``x`` scaled by 1 / (1 - ratio) where it is kept, else 0, plus ``residual``, in one kernel.  The mask is
+    drawn from a counter-based generator (Philox4x32-10) and never stored: the gradient is ``dropout`` of the gradient with the same ratio, ``key`` and ``site`` (a
+    residual's gradient is the gradient itself).  ``key``: an int64 array of a seed and a step, one for all layers of a network; a captured graph draws another mask
+    once the step has been changed.  ``site``: the layer's number.  The mask depends on the element's position in C order alone, not on the dtype; the ratio is
+    rounded to a multiple of 2^-16, below 1, and the scale is that of the rounded one."""
+    return _host.dropout(x, ratio, key, site, residual)
+
+
+def causal_conv(x, w, b=None, state=None, lengths=None, activation=None, out_state=None):
+    """A convolution of every channel along time that sees the past alone: y[:, t] = b + sum over k of w[:, k] * rows[:, t + k], ``rows`` being the taps - 1 rows of
+    ``state`` (zeros) with ``x`` behind them; ``activation``: None or 'silu'.  x [batch, time, channels], w [channels, taps] with up to 8 taps, b [channels], state
+    [batch, taps - 1, channels]; float16 or float32.  ``lengths``: the rows of each sequence of a padded batch.  Returns (y, new state); the next token or
+    piece of the sequence is a call with that state.  ``out_state``: where to put it, the state itself for one."""
+    return _host.causal_conv(x, w, b, state, lengths, activation, out_state)
+
+
+def causal_conv_grad(x, w, b, gy, state=None, lengths=None, activation=None, gnew_state=None):
+    """The gradients (gx, gw, gb, gstate) of ``causal_conv`` from those of its results; None for a ``b`` or ``state`` that is not given."""
+    return _host.causal_conv_grad(x, w, b, gy, state, lengths, activation, gnew_state)
+
+
+def selective_scan(u, delta, a, b, c, d=None, z=None, delta_bias=None, delta_softplus=False, state=None, lengths=None, out_state=None):
+    """A recurrent layer whose states decay by what the input says: with dt = delta + delta_bias, or softplus of it, h[t] = exp(dt[t] * a) * h[t - 1] + dt[t] * u[t] *
+    b[t] and y[t] = (sum(c[t] * h[t]) + d * u[t]) * z[t] * sigmoid(z[t]) for every channel and its states.  u, delta, z [batch, time, channels], b and c [batch, time,
+    states] or [batch, time, groups, states]: float16 or float32; a [channels, states], d, delta_bias [channels], state [batch, channels, states]: float32; up to 64
+    states.  ``lengths``: the rows of each sequence of a padded batch.  Returns (y, new state); the next token or piece of the sequence is a call with that state.
+    ``out_state``: where to put it, the state itself for one."""
+    return _host.selective_scan(u, delta, a, b, c, d, z, delta_bias, delta_softplus, state, lengths, out_state)
+
+
+SelectiveScanGradients = collections.namedtuple('SelectiveScanGradients', ['u', 'delta', 'a', 'b', 'c', 'd', 'z', 'delta_bias', 'state'])
+
+
+def selective_scan_grad(u, delta, a, b, c, gy, d=None, z=None, delta_bias=None, delta_softplus=False, state=None, lengths=None, gnew_state=None):
+    """The gradients of ``selective_scan`` from those of its results, by name; None for what is not given.  The states are computed again."""
+    return SelectiveScanGradients(*_host.selective_scan_grad(u, delta, a, b, c, gy, d, z, delta_bias, delta_softplus, state, lengths, gnew_state))
 
 
 def softmax_cross_entropy(x, t):

@@ -437,6 +437,55 @@ size_t hipcx_softmax_cross_entropy_workspace_size(const hipcx_array* x);
 int hipcx_softmax_cross_entropy(const hipcx_array* x, const hipcx_array* t, const hipcx_array* out, void* workspace, size_t workspace_bytes,
                                 void* stream);
 
+/* ---- layers of a recurrent block: additions to the reference, whose links are LSTM, GRU and RNN (chainer/links/rnn) ----
+ * Arrays are [batch, time, ...] and may be parts of wider ones: the last axis is dense, the others have any strides.  `lengths` (int32 or int64 [batch], or
+ * NULL): the rows that each sequence of a padded batch has, taken as 0 or as all rows where they lie outside; later rows are not looked at and give zeros, and the
+ * new state is the one behind the sequence's last row (the given one, of a sequence without rows).  A state that is NULL is zeros.  new_state may be state. */
+enum hipcx_activation { HIPCX_ACTIVATION_NONE = 0, HIPCX_ACTIVATION_SILU = 1 };
+
+/* hipcx_dropout: Dropout (chainer/functions/noise/dropout.py, y = x * mask / (1 - ratio)) whose mask is drawn from the counter-based generator
+ *   Philox4x32-10 and not stored.  Element i (in C order) takes the 16 bits at 16 * (i % 8) of the generator's output for counter {i / 8, site, low and high half of
+ *   key[1]} and key {low and high half of key[0]}, and is kept where they are at least t = min(65535, floor(65536 ratio + 1/2)): out = x * 65536 / (65536 - t) +
+ *   residual, rounded once; elsewhere out = residual, whatever x is.  Floating point, C-contiguous arrays of up to 2^35 elements; residual may be NULL.  `key`:
+ *   int64 [2] in device memory, a seed and a step, so that a captured graph draws another mask after the step has been changed; `site`: the layer, in [0, 2^32).
+ *   The gradient is the same call on the gradient.  out may be x or residual. */
+int hipcx_dropout(const hipcx_array* x, double ratio, const hipcx_array* key, int64_t site, const hipcx_array* residual, const hipcx_array* out,
+                  void* stream);
+
+/* hipcx_causal_conv: s[t] = b + sum over k of w[:, k] in[t + k], y = s or s / (1 + exp(-s)), where `in` is the taps - 1 rows of `state` with x behind them;
+ *   new_state: the taps - 1 rows of `in` that end with the sequence's last.  x and y [batch, time, channels], w [channels, taps] with 1 to 8 taps, b [channels] or
+ *   NULL, state and new_state [batch, taps - 1, channels], of one dtype, float16 or float32, summed in float32.
+ * hipcx_causal_conv_grad: from gy and gnew_state (or NULL, zeros) the gradients of x, w, b and state; gb and gstate may be NULL.  Sums over rows run in float32 in
+ *   an order that depends on the sizes alone. */
+int hipcx_causal_conv(const hipcx_array* x, const hipcx_array* w, const hipcx_array* b, const hipcx_array* state, const hipcx_array* lengths, int activation,
+                      const hipcx_array* y, const hipcx_array* new_state, void* stream);
+size_t hipcx_causal_conv_grad_workspace_size(const hipcx_array* x, const hipcx_array* w);
+int hipcx_causal_conv_grad(const hipcx_array* x, const hipcx_array* w, const hipcx_array* b, const hipcx_array* state, const hipcx_array* lengths,
+                           int activation, const hipcx_array* gy, const hipcx_array* gnew_state, const hipcx_array* gx, const hipcx_array* gw,
+                           const hipcx_array* gb, const hipcx_array* gstate, void* workspace, size_t workspace_bytes, void* stream);
+
+/* hipcx_selective_scan: for every sequence, channel and state n
+ *     h[t][n] = exp(dt[t] a[n]) h[t-1][n] + dt[t] u[t] b[t][n],   y[t] = (sum over n of c[t][n] h[t][n] + d u[t]) z[t] / (1 + exp(-z[t]))
+ *   with dt = delta + delta_bias, or log(1 + exp(delta + delta_bias)) with delta_softplus; h[-1] is `state`, new_state the last h; d and delta_bias (zeros) and z (no gate)
+ *   may be NULL.  u, delta, z, y [batch, time, channels]; b, c [batch, time, states] or [batch, time, groups, states], a group for channels / groups neighbours:
+ *   float16 or float32.  a [channels, states], d, delta_bias [channels], state, new_state [batch, channels, states]: float32, C-contiguous.  1 to 64 states, of
+ *   float32.
+ * hipcx_selective_scan_grad: the gradients of all that was given, from gy and gnew_state (or NULL, zeros); gz goes with z, gd, gdelta_bias and gstate may be NULL.
+ *   ga, gb, gc, gd, gdelta_bias, gnew_state and gstate are C-contiguous.  The states are computed again; sums run in float32 in an order that depends on the sizes
+ *   alone. */
+size_t hipcx_selective_scan_workspace_size(const hipcx_array* u, const hipcx_array* a);
+int hipcx_selective_scan(const hipcx_array* u, const hipcx_array* delta, const hipcx_array* a, const hipcx_array* b, const hipcx_array* c,
+                         const hipcx_array* d, const hipcx_array* z, const hipcx_array* delta_bias, int delta_softplus, const hipcx_array* state,
+                         const hipcx_array* lengths, const hipcx_array* y, const hipcx_array* new_state, void* workspace, size_t workspace_bytes,
+                         void* stream);
+size_t hipcx_selective_scan_grad_workspace_size(const hipcx_array* u, const hipcx_array* a, const hipcx_array* b);
+int hipcx_selective_scan_grad(const hipcx_array* u, const hipcx_array* delta, const hipcx_array* a, const hipcx_array* b, const hipcx_array* c,
+                              const hipcx_array* d, const hipcx_array* z, const hipcx_array* delta_bias, int delta_softplus, const hipcx_array* state,
+                              const hipcx_array* lengths, const hipcx_array* gy, const hipcx_array* gnew_state, const hipcx_array* gu,
+                              const hipcx_array* gdelta, const hipcx_array* ga, const hipcx_array* gb, const hipcx_array* gc, const hipcx_array* gd,
+                              const hipcx_array* gz, const hipcx_array* gdelta_bias, const hipcx_array* gstate, void* workspace, size_t workspace_bytes,
+                              void* stream);
+
 /* Measurement aid (no counterpart in the reference): between start and stop every implicit-GEMM launch made by
  * hipcx_dot / hipcx_conv from the calling process is bracketed by a pair of HIP events on its stream.  stop waits for them
  * and returns the number of launches, the sum of their durations, and their algorithmic flops (2 per multiply-add) and
