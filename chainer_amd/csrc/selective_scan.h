@@ -24,7 +24,7 @@ struct ScanArgs {
     int channels, states, group_channels;
     int group_blocks, blocks;   // workgroups along the channels of a group, of all groups
     int chunks, chunk_rows;     // of the time axis; whole tiles of rows
-    float* ends;                // [batch][chunks][channels][states]: the state that the sequence starts from, then what each chunk but the last adds
+    float* ends;                // [batch][chunks][channels][states]: the state that the sequence starts from, then where each chunk but the last ends that starts from zeros
     float* steps;               // [batch][chunks - 1][channels]: dt summed over the chunk
     int softplus;
 };
@@ -110,10 +110,94 @@ struct ScanPlace {
     }
 };
 
-template <typename T>
-__device__ __forceinline__ float ScanRead(const SequenceRows& r, int64_t b, int64_t row, int channel) {
-    return static_cast<float>(static_cast<const T*>(r.data)[b * r.batch + row * r.row + channel]);
-}
+// A tile's rows of a channel, which a quad's lanes take in turns: the tile starts at an address that is the same for the whole workgroup, and a lane's place in it is a
+// number of 32 bits, so that a load costs one more vector instruction at most.  `held`: what Fetch() has asked for.
+template <typename T, int ROWS>
+struct TileRows {
+    static constexpr int kGroups = ROWS / 4;
+    char* base;
+    int group;  // bytes to the next four rows
+    unsigned offset;
+    T held[kGroups];
+    __device__ __forceinline__ TileRows(const SequenceRows& r, const ScanPlace& at, int64_t t) {
+        const int64_t row = r.row * static_cast<int64_t>(sizeof(T)), low = row < 0 ? (ROWS - 1) * row : 0;
+        base = static_cast<char*>(r.data) + at.b * r.batch * static_cast<int64_t>(sizeof(T)) + t * row + low;
+        group = static_cast<int>(4 * row);
+        offset = static_cast<unsigned>(at.q * row - low + at.channel * static_cast<int64_t>(sizeof(T)));
+        asm("" : "+v"(offset));  // (the compiler would put 64-bit addresses together)
+#pragma unroll
+        for (int g = 0; g < kGroups; ++g) held[g] = static_cast<T>(0);
+    }
+    __device__ __forceinline__ T& operator[](int g) const { return *reinterpret_cast<T*>(base + (offset + static_cast<unsigned>(g * group))); }
+    // A lane's rows of the tile, all of them or those before `rows`.
+    template <bool WHOLE>
+    __device__ __forceinline__ void Fetch(int q, int rows) {
+#pragma unroll
+        for (int g = 0; g < kGroups; ++g) {
+            T v = static_cast<T>(0);
+            if (WHOLE || 4 * g + q < rows) v = (*this)[g];
+            held[g] = v;
+        }
+    }
+    __device__ __forceinline__ float Held(int g) const { return static_cast<float>(held[g]); }
+    __device__ __forceinline__ void Move(int tiles) {
+        base += static_cast<int64_t>(tiles) * kGroups * group;
+        asm("" : "+v"(offset));  // else a register for each group's offset is kept from tile to tile
+    }
+};
+constexpr int64_t kMaxScanRow = int64_t{1} << 26;  // elements from one row to the next: a tile and the channels fit those 32 bits
+
+// A tile of b, or of b and c, on its way to LDS: workgroups of 256 threads take an element each, or a few.
+template <typename T, int NPL, int ROWS, int PARTS>
+struct TileShared {
+    static constexpr int kNP = 4 * NPL, kEach = (ROWS * kNP + 255) / 256;
+    const T* from[PARTS][kEach];
+    int64_t step[PARTS];
+    bool is_state[kEach];
+    T held[PARTS][kEach];
+    __device__ __forceinline__ TileShared(const ScanArgs& p, const ScanPlace& at, int64_t t) {
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) {
+            const int e = i * 256 + static_cast<int>(threadIdx.x), r = e / kNP, n = e % kNP;
+            is_state[i] = r < ROWS && n < p.states;
+#pragma unroll
+            for (int k = 0; k < PARTS; ++k) {
+                const ScanShared& s = k == 0 ? p.b : p.c;
+                from[k][i] = static_cast<const T*>(s.data) + at.b * s.batch + at.group * s.group + (t + r) * s.row + n;
+                step[k] = ROWS * s.row;
+                held[k][i] = static_cast<T>(0);
+            }
+        }
+    }
+    template <bool WHOLE>
+    __device__ __forceinline__ void Fetch(int rows) {
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) {
+            const bool counts = is_state[i] && (WHOLE || (i * 256 + static_cast<int>(threadIdx.x)) / kNP < rows);
+#pragma unroll
+            for (int k = 0; k < PARTS; ++k) {
+                T v = static_cast<T>(0);
+                if (counts) v = *from[k][i];
+                held[k][i] = v;
+            }
+        }
+    }
+    __device__ __forceinline__ void Move(int tiles) {
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) {
+#pragma unroll
+            for (int k = 0; k < PARTS; ++k) from[k][i] += tiles * step[k];
+        }
+    }
+    template <int K>
+    __device__ __forceinline__ void Stage(float (&to)[ROWS][kNP]) const {
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) {
+            const int e = i * 256 + static_cast<int>(threadIdx.x);
+            if (e < ROWS * kNP) to[e / kNP][e % kNP] = static_cast<float>(held[K][i]);
+        }
+    }
+};
 
 // The NPL of a call: a lane's share of the states, rounded up to a power of two.
 template <typename F>
@@ -129,6 +213,9 @@ void VisitScan(int dtype, int states, F&& f) {
     if (dtype == HIPCX_FLOAT16) visit(Tag<half_t>{});
     else visit(Tag<float>{});
 }
+
+// Cuts the time axis into chunks of `least` tiles or more, for `each` workgroups to a compute unit, where sequences and channels alone do not give it `enough`.
+void CutScan(ScanArgs* p, int enough, int each, int least);
 
 // Checks the inputs that the scan and its gradients share and describes them, except for the cut along time.
 ScanArgs DescribeScan(const std::string& what, const hipcx_array* u, const hipcx_array* delta, const hipcx_array* a, const hipcx_array* b, const hipcx_array* c,

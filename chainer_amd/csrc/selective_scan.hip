@@ -4,13 +4,15 @@
 namespace hipcx {
 namespace {
 
-// A workgroup's part of the sequence: 64 channels, a chunk of rows.  Rows go by in tiles of 16, whose b and c lie in LDS; a lane reads u, delta and z of every fourth row
+// A workgroup's part of the sequence: 64 channels, a chunk of rows.  Chunks that come after others need the state there, and a state goes through a chunk linearly:
+// h -> exp(a * sum of dt) h + what the chunk makes of zeros.  So ENDS runs the chunks but the last from zeros, without outputs, and the second launch runs all of them
+// from the states that it puts together on the way.  Rows go by in tiles of 16, whose b and c lie in LDS; a lane reads u, delta and z of every fourth row
 // of its channel, prepares dt, dt u and the gate once, and hands them to the quad's other lanes.
-template <typename T, int NPL>
+template <typename T, int NPL, bool ENDS>
 __global__ __launch_bounds__(256) void SelectiveScanKernel(ScanArgs p) {
-    constexpr int NP = 4 * NPL, kEach = (kScanTile * NP + 255) / 256;
-    __shared__ float bs[2][kScanTile][NP], cs[2][kScanTile][NP];
-    const ScanPlace at(p, blockIdx.x, p.chunks);
+    constexpr int NP = 4 * NPL;
+    __shared__ float bs[2][kScanTile][NP], cs[ENDS ? 1 : 2][ENDS ? 1 : kScanTile][NP];
+    const ScanPlace at(p, blockIdx.x, ENDS ? p.chunks - 1 : p.chunks);
     const int64_t len = LengthOf(p.lengths, at.b, p.length);
     const int64_t t0 = static_cast<int64_t>(at.chunk) * p.chunk_rows, end = std::min(t0 + p.chunk_rows, p.length), last = std::min(end, len);
     const int n0 = at.q * NPL;
@@ -18,52 +20,42 @@ __global__ __launch_bounds__(256) void SelectiveScanKernel(ScanArgs p) {
     LoadStates<NPL>(p.a + static_cast<int64_t>(at.channel) * p.states, n0, p.states, a);
 #pragma unroll
     for (int i = 0; i < NPL; ++i) a[i] *= kLog2E, h[i] = 0.f;
-    const int64_t of_state = (at.b * p.channels + at.channel) * p.states;
-    if (p.state != nullptr) LoadStates<NPL>(p.state + of_state, n0, p.states, h);
+    const int64_t of_state = (at.b * p.channels + at.channel) * p.states, per_chunk = static_cast<int64_t>(p.channels) * p.states;
+    float* const ends = p.ends + (at.b * p.chunks * p.channels + at.channel) * p.states;
+    const float* const steps = p.steps + at.b * (p.chunks - 1) * p.channels + at.channel;
+    if (ENDS || p.chunks == 1) {
+        if (p.state != nullptr) LoadStates<NPL>(p.state + of_state, n0, p.states, h);
+        if (ENDS) {  // the other launch writes new_state, which may be state, and so does not read it
+            if (at.chunk == 0 && at.inside) StoreStates<NPL>(ends, n0, p.states, h);
+#pragma unroll
+            for (int i = 0; i < NPL; ++i) h[i] = 0.f;
+        }
+    } else {
+        LoadStates<NPL>(ends, n0, p.states, h);
+        for (int j = 0; j < at.chunk; ++j) {
+            float end[NPL];
+            LoadStates<NPL>(ends + (j + 1) * per_chunk, n0, p.states, end);
+            const float dt = steps[static_cast<int64_t>(j) * p.channels];
+#pragma unroll
+            for (int i = 0; i < NPL; ++i) h[i] = __builtin_fmaf(__builtin_amdgcn_exp2f(dt * a[i]), h[i], end[i]);
+        }
+    }
+    float all_steps = 0.f;
     const float bias = p.bias != nullptr ? p.bias[at.channel] : 0.f, d = p.d != nullptr ? p.d[at.channel] : 0.f;
-    const T* const b = static_cast<const T*>(p.b.data) + at.b * p.b.batch + at.group * p.b.group;
-    const T* const c = static_cast<const T*>(p.c.data) + at.b * p.c.batch + at.group * p.c.group;
-
-    float ub[4], db[4], zb[4], bb[kEach], cb[kEach];  // of the next tile
-    const auto fetch = [&](int64_t t) {
-#pragma unroll
-        for (int g = 0; g < 4; ++g) {
-            const int64_t row = t + 4 * g + at.q;
-            ub[g] = db[g] = zb[g] = 0.f;
-            if (row < last) {
-                ub[g] = ScanRead<T>(p.u, at.b, row, at.channel);
-                db[g] = ScanRead<T>(p.delta, at.b, row, at.channel);
-                if (p.z.data != nullptr) zb[g] = ScanRead<T>(p.z, at.b, row, at.channel);
-            }
-        }
-#pragma unroll
-        for (int i = 0; i < kEach; ++i) {
-            const int e = i * 256 + static_cast<int>(threadIdx.x), r = e / NP, n = e % NP;
-            bb[i] = cb[i] = 0.f;
-            if (r < kScanTile && n < p.states && t + r < last) {
-                bb[i] = static_cast<float>(b[(t + r) * p.b.row + n]);
-                cb[i] = static_cast<float>(c[(t + r) * p.c.row + n]);
-            }
-        }
+    TileRows<T, kScanTile> us(p.u, at, t0), ds(p.delta, at, t0), zs(p.z, at, t0), ys(p.y, at, t0);
+    TileShared<T, NPL, kScanTile, ENDS ? 1 : 2> shared(p, at, t0);
+    const bool gated = !ENDS && p.z.data != nullptr;
+    const auto fetch = [&](int rows, auto whole) __attribute__((always_inline)) {
+        constexpr bool kWhole = decltype(whole)::value;
+        us.template Fetch<kWhole>(at.q, rows);
+        ds.template Fetch<kWhole>(at.q, rows);
+        if (gated) zs.template Fetch<kWhole>(at.q, rows);
+        shared.template Fetch<kWhole>(rows);
+        us.Move(1), ds.Move(1), zs.Move(1), shared.Move(1);
     };
-    fetch(t0);
-    int buffer = 0;
-    for (int64_t t = t0; t < last; t += kScanTile, buffer ^= 1) {
-#pragma unroll
-        for (int i = 0; i < kEach; ++i) {
-            const int e = i * 256 + static_cast<int>(threadIdx.x);
-            if (e < kScanTile * NP) bs[buffer][e / NP][e % NP] = bb[i], cs[buffer][e / NP][e % NP] = cb[i];
-        }
-        __syncthreads();
-        float u[4], dt[4], z[4];
-#pragma unroll
-        for (int g = 0; g < 4; ++g) {
-            const bool counts = t + 4 * g + at.q < last;
-            u[g] = ub[g], z[g] = zb[g];
-            const float raw = db[g] + bias;
-            dt[g] = counts ? (p.softplus != 0 ? SoftplusOf(raw) : raw) : 0.f;
-        }
-        fetch(t + kScanTile);
+    // `rows` of the tile at t, all 16 of them or fewer
+    const auto run = [&](int64_t t, int buffer, const float (&u)[4], const float (&z)[4], const float (&dt)[4], auto whole) __attribute__((always_inline)) {
+        constexpr bool kWhole = decltype(whole)::value;
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
             const float x = dt[g] * u[g];
@@ -76,7 +68,7 @@ __global__ __launch_bounds__(256) void SelectiveScanKernel(ScanArgs p) {
                 for (int i = 0; i < NPL; ++i) {
                     const float e = __builtin_amdgcn_exp2f(dts * a[i]);
                     h[i] = __builtin_fmaf(xs, bs[buffer][4 * g + S][n0 + i], e * h[i]);
-                    sum = __builtin_fmaf(cs[buffer][4 * g + S][n0 + i], h[i], sum);
+                    if constexpr (!ENDS) sum = __builtin_fmaf(cs[buffer][4 * g + S][n0 + i], h[i], sum);
                 }
                 sums[S] = sum;
             };
@@ -84,16 +76,119 @@ __global__ __launch_bounds__(256) void SelectiveScanKernel(ScanArgs p) {
             step(std::integral_constant<int, 1>{});
             step(std::integral_constant<int, 2>{});
             step(std::integral_constant<int, 3>{});
-            float y = __builtin_fmaf(d, u[g], QuadTransposedSum(sums, at.q));
-            if (p.z.data != nullptr) y *= z[g] * LogisticOf(z[g]);
-            const int64_t row = t + 4 * g + at.q;
-            if (at.inside && row < last) static_cast<T*>(p.y.data)[at.b * p.y.batch + row * p.y.row + at.channel] = static_cast<T>(y);
+            if constexpr (!ENDS) {
+                float y = __builtin_fmaf(d, u[g], QuadTransposedSum(sums, at.q));
+                if (gated) y *= z[g] * LogisticOf(z[g]);
+                if (at.inside && (kWhole || t + 4 * g + at.q < last)) ys[g] = static_cast<T>(y);
+            }
         }
+    };
+    const auto fetch_tile = [&](int64_t t) {
+        if (t + kScanTile <= last) fetch(kScanTile, std::true_type{});
+        else if (t < last) fetch(static_cast<int>(last - t), std::false_type{});
+    };
+    fetch_tile(t0);
+    int buffer = 0;
+    for (int64_t t = t0; t < last; t += kScanTile, buffer ^= 1) {
+        shared.template Stage<0>(bs[buffer]);
+        if constexpr (!ENDS) shared.template Stage<1>(cs[buffer]);
+        __syncthreads();
+        float u[4], dt[4], z[4];
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            u[g] = us.Held(g), z[g] = zs.Held(g);
+            const float raw = ds.Held(g) + bias;
+            dt[g] = p.softplus != 0 ? SoftplusOf(raw) : raw;
+        }
+        fetch_tile(t + kScanTile);
+        if (t + kScanTile <= last) {
+            run(t, buffer, u, z, dt, std::true_type{});
+        } else {
+#pragma unroll
+            for (int g = 0; g < 4; ++g) dt[g] = t + 4 * g + at.q < last ? dt[g] : 0.f;
+            run(t, buffer, u, z, dt, std::false_type{});
+        }
+        ys.Move(1);
+        if constexpr (ENDS) all_steps += (dt[0] + dt[1]) + (dt[2] + dt[3]);
     }
     if (!at.inside) return;
+    if constexpr (ENDS) {
+        StoreStates<NPL>(ends + (at.chunk + 1) * per_chunk, n0, p.states, h);
+        all_steps += QuadSwap1(all_steps);
+        all_steps += QuadSwap2(all_steps);
+        if (at.q == 0) p.steps[(at.b * (p.chunks - 1) + at.chunk) * p.channels + at.channel] = all_steps;
+        return;
+    }
     for (int64_t row = std::max(t0, len) + at.q; row < end; row += 4) static_cast<T*>(p.y.data)[at.b * p.y.batch + row * p.y.row + at.channel] = static_cast<T>(0);
     if (at.chunk == p.chunks - 1) StoreStates<NPL>(p.new_state + of_state, n0, p.states, h);
 }
+
+// One row of each sequence: what a token costs is its states, read and written once.  Four threads to a channel, each with a quarter of the states.
+template <typename T, int NPL>
+__global__ __launch_bounds__(256) void ScanTokenKernel(ScanArgs p, int64_t first) {
+    const int64_t index = first + static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x, line = index >> 2;
+    if (line >= p.batch * p.channels) return;  // whole quads
+    const int64_t b = line / p.channels;
+    const int channel = static_cast<int>(line % p.channels), group = channel / p.group_channels, n0 = (static_cast<int>(threadIdx.x) & 3) * NPL;
+    float h[NPL] = {}, a[NPL], bs[NPL], cs[NPL];
+    if (p.state != nullptr) LoadStates<NPL>(p.state + line * p.states, n0, p.states, h);
+    T* const y = static_cast<T*>(p.y.data) + b * p.y.batch + channel;
+    const bool counts = LengthOf(p.lengths, b, 1) != 0;
+    if (counts) {
+        LoadStates<NPL>(p.a + static_cast<int64_t>(channel) * p.states, n0, p.states, a);
+        const T* const from_b = static_cast<const T*>(p.b.data) + b * p.b.batch + group * p.b.group;
+        const T* const from_c = static_cast<const T*>(p.c.data) + b * p.c.batch + group * p.c.group;
+#pragma unroll
+        for (int i = 0; i < NPL; ++i) {
+            const bool is = n0 + i < p.states;
+            bs[i] = is ? static_cast<float>(from_b[n0 + i]) : 0.f, cs[i] = is ? static_cast<float>(from_c[n0 + i]) : 0.f;
+        }
+        const float u = static_cast<float>(static_cast<const T*>(p.u.data)[b * p.u.batch + channel]);
+        const float raw = static_cast<float>(static_cast<const T*>(p.delta.data)[b * p.delta.batch + channel]) + (p.bias != nullptr ? p.bias[channel] : 0.f);
+        const float dt = p.softplus != 0 ? SoftplusOf(raw) : raw, x = dt * u;
+        float sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < NPL; ++i) {
+            h[i] = __builtin_fmaf(x, bs[i], __builtin_amdgcn_exp2f(dt * (a[i] * kLog2E)) * h[i]);
+            sum = __builtin_fmaf(cs[i], h[i], sum);
+        }
+        sum += QuadSwap1(sum);
+        sum += QuadSwap2(sum);
+        if (n0 == 0) {
+            float out = __builtin_fmaf(p.d != nullptr ? p.d[channel] : 0.f, u, sum);
+            if (p.z.data != nullptr) {
+                const float z = static_cast<float>(static_cast<const T*>(p.z.data)[b * p.z.batch + channel]);
+                out *= z * LogisticOf(z);
+            }
+            *y = static_cast<T>(out);
+        }
+    } else if (n0 == 0) {
+        *y = static_cast<T>(0);
+    }
+    StoreStates<NPL>(p.new_state + line * p.states, n0, p.states, h);
+}
+
+}  // namespace
+
+void CutScan(ScanArgs* p, int enough, int each, int least) {
+    const int64_t tiles = DivUp(p->length, kScanTile), lines = p->batch * DivUp(p->channels, kScanChannels);
+    int64_t chunks = 1;
+    if (lines > 0 && lines < int64_t{NumCUs()} * enough) chunks = std::max<int64_t>(1, std::min<int64_t>(int64_t{NumCUs()} * each / lines, tiles / least));
+    const int64_t to_chunk = std::max<int64_t>(1, (tiles + chunks - 1) / chunks);
+    p->chunk_rows = static_cast<int>(to_chunk) * kScanTile;
+    p->chunks = static_cast<int>(std::max<int64_t>(1, (tiles + to_chunk - 1) / to_chunk));
+}
+
+namespace {
+
+struct ScanWorkspace {
+    int64_t ends, steps;  // floats
+    explicit ScanWorkspace(const ScanArgs& p) : ends(0), steps(0) {
+        if (p.chunks == 1) return;
+        ends = p.batch * p.chunks * p.channels * p.states, steps = p.batch * (p.chunks - 1) * p.channels;
+    }
+    size_t Bytes() const { return static_cast<size_t>(ends + steps) * sizeof(float); }
+};
 
 }  // namespace
 
@@ -126,6 +221,9 @@ ScanArgs DescribeScan(const std::string& what, const hipcx_array* u, const hipcx
     RequireShape(state, {batch, channels, states}, HIPCX_FLOAT32, what + ": state");
     for (const hipcx_array* s : {a, d, delta_bias, state}) RequireDense(s, what + ": a, d, delta_bias and state");
     ScanArgs p{};
+    for (const hipcx_array* s : {u, delta, z, b, c}) {
+        HIPCX_REQUIRE(s == nullptr || std::abs(s->strides[1]) < kMaxScanRow * ItemSize(s->dtype), HIPCX_NOT_IMPLEMENTED_ERROR, what + ": rows 2^26 elements apart or more");
+    }
     p.u = RowsOf(u, "u"), p.delta = RowsOf(delta, "delta"), p.z = RowsOf(z, "z");
     const auto shared = [&](const hipcx_array* s, const char* name) {
         const SequenceRows r = RowsOf(s, name);
@@ -149,8 +247,11 @@ using namespace hipcx;
 extern "C" {
 
 size_t hipcx_selective_scan_workspace_size(const hipcx_array* u, const hipcx_array* a) {
-    (void)u, (void)a;
-    return 0;
+    if (u == nullptr || a == nullptr || u->ndim != 3 || a->ndim != 2 || u->shape[0] < 0 || u->shape[1] < 0 || u->shape[2] < 0) return 0;
+    ScanArgs p{};
+    p.batch = u->shape[0], p.length = u->shape[1], p.channels = static_cast<int>(u->shape[2]), p.states = static_cast<int>(a->shape[1]);
+    CutScan(&p, 4, 8, 2);
+    return ScanWorkspace(p).Bytes();
 }
 
 int hipcx_selective_scan(const hipcx_array* u, const hipcx_array* delta, const hipcx_array* a, const hipcx_array* b, const hipcx_array* c, const hipcx_array* d,
@@ -163,16 +264,30 @@ int hipcx_selective_scan(const hipcx_array* u, const hipcx_array* delta, const h
         RequireShape(y, {p.batch, p.length, p.channels}, u->dtype, what + ": y");
         RequireShape(new_state, {p.batch, p.channels, p.states}, HIPCX_FLOAT32, what + ": new_state");
         RequireDense(new_state, what + ": new_state");
+        HIPCX_REQUIRE(std::abs(y->strides[1]) < kMaxScanRow * ItemSize(y->dtype), HIPCX_NOT_IMPLEMENTED_ERROR, what + ": rows 2^26 elements apart or more");
         p.y = RowsOf(y, "y"), p.new_state = static_cast<float*>(new_state->data);
         if (p.batch == 0 || p.channels == 0) return;
-        const size_t need = hipcx_selective_scan_workspace_size(u, a);
-        HIPCX_REQUIRE(workspace_bytes >= need && (need == 0 || workspace != nullptr), HIPCX_CHAINERX_ERROR, what + ": the workspace is too small");
-        p.chunks = 1, p.chunk_rows = static_cast<int>(DivUp(p.length, kScanTile)) * kScanTile;
+        CutScan(&p, 4, 8, 2);
+        const ScanWorkspace w(p);
+        HIPCX_REQUIRE(workspace_bytes >= w.Bytes() && (w.Bytes() == 0 || workspace != nullptr), HIPCX_CHAINERX_ERROR, what + ": the workspace is too small");
+        p.ends = static_cast<float*>(workspace), p.steps = p.ends + w.ends;
         const int64_t blocks = p.batch * p.chunks * p.blocks;
-        HIPCX_REQUIRE(blocks <= kBlocksPerLaunch, HIPCX_NOT_IMPLEMENTED_ERROR, what + ": too many elements");
+        HIPCX_REQUIRE(p.length == 1 || blocks <= kBlocksPerLaunch, HIPCX_NOT_IMPLEMENTED_ERROR, what + ": too many elements");
         VisitScan(u->dtype, p.states, [&](auto tag, auto share) {
             using T = typename decltype(tag)::type;
-            hipLaunchKernelGGL((SelectiveScanKernel<T, decltype(share)::value>), dim3(static_cast<unsigned>(blocks)), dim3(256), 0, AsStream(stream), p);
+            constexpr int NPL = decltype(share)::value;
+            if (p.length == 1) {
+                ForLaunches(p.batch * p.channels * 4, [&](dim3 grid, int64_t first) {
+                    hipLaunchKernelGGL((ScanTokenKernel<T, NPL>), grid, dim3(256), 0, AsStream(stream), p, first);
+                    CheckLaunch("selective_scan");
+                });
+                return;
+            }
+            if (p.chunks > 1) {
+                hipLaunchKernelGGL((SelectiveScanKernel<T, NPL, true>), dim3(static_cast<unsigned>(blocks - p.batch * p.blocks)), dim3(256), 0, AsStream(stream), p);
+                CheckLaunch("selective_scan");
+            }
+            hipLaunchKernelGGL((SelectiveScanKernel<T, NPL, false>), dim3(static_cast<unsigned>(blocks)), dim3(256), 0, AsStream(stream), p);
             CheckLaunch("selective_scan");
         });
     });

@@ -11,15 +11,17 @@ struct ScanGradArgs {
     SequenceRows gy, gu, gdelta, gz;
     const float* gnew;  // gradient of the new state, or null
     float* gstate;      // or null
-    float* states;      // [batch][tiles][channels][states]: where each tile starts
+    float* states;      // [batch][tiles][channels][states]: where each tile starts, of a chunk that starts from zeros
+    float* passed;      // [batch][tiles][channels]: dt summed over the chunk's rows before the tile
     float* shared_parts;   // [batch][length][blocks][2][states]: gb and gc by workgroups along the channels
     float* channel_parts;  // [batch * chunks][channels][states + 2]: ga, gd, gbias
+    float* starts;         // [batch][chunks][channels][states]: what a chunk's outputs give the state before it (of s.ends: where a chunk ends that starts from zeros)
     int tiles;             // of a sequence
 };
 
 // Rows whose states a lane keeps in registers on the way back: 64 states.
 template <int NPL>
-constexpr int kGradTile = NPL <= 4 ? 16 : 64 / NPL;
+constexpr int kGradTile = NPL <= 2 ? 16 : NPL == 4 ? 8 : 4;
 
 __device__ __forceinline__ float AddRowRotations(float v) {  // over the four quads of 16 lanes
     v += __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), 0x128, 0xf, 0xf, true));
@@ -49,48 +51,90 @@ __device__ __forceinline__ void SumOverChannels(const float (&v)[4 * NPL], float
     }
 }
 
-// The states that each tile starts from: the forward recurrence, without its outputs.
-template <typename T, int NPL>
-__global__ __launch_bounds__(256) void ScanStatesKernel(ScanGradArgs pg) {
+// dt, and dt u, of the rows that a lane has fetched; zeros behind the sequence's end.
+template <typename T, int ROWS>
+__device__ __forceinline__ void ScanSteps(const ScanArgs& p, const TileRows<T, ROWS>& us, const TileRows<T, ROWS>& ds, int q, int rows, float bias, float (&dt)[ROWS / 4],
+                                          float (&x)[ROWS / 4]) {
+#pragma unroll
+    for (int g = 0; g < ROWS / 4; ++g) {
+        const float raw = ds.Held(g) + bias;
+        dt[g] = 4 * g + q < rows ? (p.softplus != 0 ? SoftplusOf(raw) : raw) : 0.f;
+        x[g] = dt[g] * us.Held(g);
+    }
+}
+
+// Chunks by themselves, from zeros: the states that their tiles start from, where they end, and what a chunk's outputs give the state before it -- the sum over its rows
+// of g0 c times the decay since the chunk began, which runs forwards too.  CHUNKS: there is more than one, else the last two are not needed.
+template <typename T, int NPL, bool CHUNKS>
+__global__ __launch_bounds__(256) void ScanGradStatesKernel(ScanGradArgs pg) {
     const ScanArgs& p = pg.s;
-    constexpr int NP = 4 * NPL, kEach = (kScanTile * NP + 255) / 256, kTile = kGradTile<NPL>;
-    __shared__ float bs[2][kScanTile][NP];
-    const ScanPlace at(p, blockIdx.x, 1);
+    constexpr int NP = 4 * NPL, kTile = kGradTile<NPL>;
+    __shared__ float bs[2][kScanTile][NP], cs[CHUNKS ? 2 : 1][CHUNKS ? kScanTile : 1][NP];
+    const ScanPlace at(p, blockIdx.x, p.chunks);
     const int64_t len = LengthOf(p.lengths, at.b, p.length);
+    const int64_t t0 = static_cast<int64_t>(at.chunk) * p.chunk_rows, last = std::min(std::min(t0 + p.chunk_rows, p.length), len);
     const int n0 = at.q * NPL;
-    float a[NPL], h[NPL];
+    const int64_t per_tile = static_cast<int64_t>(p.channels) * p.states;
+    float a[NPL], h[NPL], start[NPL], decay[NPL];
     LoadStates<NPL>(p.a + static_cast<int64_t>(at.channel) * p.states, n0, p.states, a);
 #pragma unroll
-    for (int i = 0; i < NPL; ++i) a[i] *= kLog2E, h[i] = 0.f;
-    if (p.state != nullptr) LoadStates<NPL>(p.state + (at.b * p.channels + at.channel) * p.states, n0, p.states, h);
+    for (int i = 0; i < NPL; ++i) a[i] *= kLog2E, h[i] = start[i] = 0.f, decay[i] = 1.f;
     const float bias = p.bias != nullptr ? p.bias[at.channel] : 0.f;
-    const T* const b = static_cast<const T*>(p.b.data) + at.b * p.b.batch + at.group * p.b.group;
+    const bool gated = CHUNKS && p.z.data != nullptr;
+    float* const states = pg.states + (at.b * pg.tiles * p.channels + at.channel) * p.states;
+    float* const passed = pg.passed + at.b * pg.tiles * p.channels + at.channel;
+    TileRows<T, kScanTile> us(p.u, at, t0), ds(p.delta, at, t0), zs(p.z, at, t0), gs(pg.gy, at, t0);
+    TileShared<T, NPL, kScanTile, CHUNKS ? 2 : 1> shared(p, at, t0);
+    const auto fetch_rows = [&](int rows, auto whole) __attribute__((always_inline)) {
+        constexpr bool kWhole = decltype(whole)::value;
+        us.template Fetch<kWhole>(at.q, rows);
+        ds.template Fetch<kWhole>(at.q, rows);
+        if constexpr (CHUNKS) gs.template Fetch<kWhole>(at.q, rows);
+        if (gated) zs.template Fetch<kWhole>(at.q, rows);
+        shared.template Fetch<kWhole>(rows);
+        us.Move(1), ds.Move(1), zs.Move(1), gs.Move(1), shared.Move(1);
+    };
+    const auto fetch = [&](int64_t t) {
+        if (t + kScanTile <= last) fetch_rows(kScanTile, std::true_type{});
+        else if (t < last) fetch_rows(static_cast<int>(last - t), std::false_type{});
+    };
+    fetch(t0);
+    float all_steps = 0.f;
     int buffer = 0;
-    for (int64_t t = 0; t < len; t += kScanTile, buffer ^= 1) {
-#pragma unroll
-        for (int i = 0; i < kEach; ++i) {
-            const int e = i * 256 + static_cast<int>(threadIdx.x), r = e / NP, n = e % NP;
-            if (e < kScanTile * NP) bs[buffer][r][n] = n < p.states && t + r < len ? static_cast<float>(b[(t + r) * p.b.row + n]) : 0.f;
-        }
+    for (int64_t t = t0; t < last; t += kScanTile, buffer ^= 1) {
+        shared.template Stage<0>(bs[buffer]);
+        if constexpr (CHUNKS) shared.template Stage<1>(cs[buffer]);
         __syncthreads();
+        float dt[4], x[4], g0[4];
+        ScanSteps(p, us, ds, at.q, static_cast<int>(std::min<int64_t>(last - t, kScanTile)), bias, dt, x);
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
-            const int64_t row = t + 4 * g + at.q;
-            float dt = 0.f, x = 0.f;
-            if (row < len) {
-                const float raw = ScanRead<T>(p.delta, at.b, row, at.channel) + bias;
-                dt = p.softplus != 0 ? SoftplusOf(raw) : raw;
-                x = dt * ScanRead<T>(p.u, at.b, row, at.channel);
-            }
-            if (4 * g % kTile == 0 && t + 4 * g < len && at.inside) {
-                float* const to = pg.states + ((at.b * pg.tiles + (t + 4 * g) / kTile) * p.channels + at.channel) * p.states;
-                StoreStates<NPL>(to, n0, p.states, h);
-            }
-            const auto step = [&](auto lane) {
-                constexpr int S = decltype(lane)::value;
-                const float dts = OfQuadLane<S>(dt), xs = OfQuadLane<S>(x);
+            g0[g] = CHUNKS ? gs.Held(g) : 0.f;
+            if (gated) g0[g] *= zs.Held(g) * LogisticOf(zs.Held(g));
+        }
+        fetch(t + kScanTile);
 #pragma unroll
-                for (int i = 0; i < NPL; ++i) h[i] = __builtin_fmaf(xs, bs[buffer][4 * g + S][n0 + i], __builtin_amdgcn_exp2f(dts * a[i]) * h[i]);
+        for (int g = 0; g < 4; ++g) {
+            if (4 * g % kTile == 0 && t + 4 * g < last && at.inside) {
+                const int64_t tile = (t + 4 * g) / kTile;
+                StoreStates<NPL>(states + tile * per_tile, n0, p.states, h);
+                if (at.q == 0) passed[tile * p.channels] = all_steps;
+            }
+            float four = dt[g] + QuadSwap1(dt[g]);
+            four += QuadSwap2(four);
+            all_steps += four;
+            const auto step = [&](auto lane) __attribute__((always_inline)) {
+                constexpr int S = decltype(lane)::value;
+                const float dts = OfQuadLane<S>(dt[g]), xs = OfQuadLane<S>(x[g]), gys = OfQuadLane<S>(g0[g]);
+#pragma unroll
+                for (int i = 0; i < NPL; ++i) {
+                    const float e = __builtin_amdgcn_exp2f(dts * a[i]);
+                    h[i] = __builtin_fmaf(xs, bs[buffer][4 * g + S][n0 + i], e * h[i]);
+                    if constexpr (CHUNKS) {
+                        decay[i] *= e;
+                        start[i] = __builtin_fmaf(gys * cs[buffer][4 * g + S][n0 + i], decay[i], start[i]);
+                    }
+                }
             };
             step(std::integral_constant<int, 0>{});
             step(std::integral_constant<int, 1>{});
@@ -98,62 +142,99 @@ __global__ __launch_bounds__(256) void ScanStatesKernel(ScanGradArgs pg) {
             step(std::integral_constant<int, 3>{});
         }
     }
+    if (!CHUNKS || !at.inside) return;
+    const int64_t line = (at.b * p.chunks + at.chunk) * p.channels + at.channel;
+    StoreStates<NPL>(p.ends + line * p.states, n0, p.states, h);
+    StoreStates<NPL>(pg.starts + line * p.states, n0, p.states, start);
+    if (at.q == 0) p.steps[line] = all_steps;
 }
 
+// A chunk from its last tile to its first: the tile's states again, in registers, from those that it starts from, and the gradients.
 template <typename T, int NPL>
-__global__ __launch_bounds__(256) void SelectiveScanGradKernel(ScanGradArgs pg) {
+__global__ __launch_bounds__(256, 2) void SelectiveScanGradKernel(ScanGradArgs pg) {
     const ScanArgs& p = pg.s;
     constexpr int NP = 4 * NPL, kTile = kGradTile<NPL>, kGroups = kTile / 4;
-    __shared__ float bs[kTile][NP], cs[kTile][NP], sums[4][kTile][2][NP];
-    const ScanPlace at(p, blockIdx.x, 1);
+    __shared__ float bs[2][kTile][NP], cs[2][kTile][NP], sums[2][4][kTile][2][NP];
+    const ScanPlace at(p, blockIdx.x, p.chunks);
     const int64_t len = LengthOf(p.lengths, at.b, p.length);
+    const int64_t t0 = static_cast<int64_t>(at.chunk) * p.chunk_rows, end = std::min(t0 + p.chunk_rows, p.length), last = std::min(end, len);
     const int n0 = at.q * NPL, lane = static_cast<int>(threadIdx.x) & 63, wave = static_cast<int>(threadIdx.x) >> 6;
-    const int64_t of_state = (at.b * p.channels + at.channel) * p.states;
-    float a[NPL], q[NPL], ga[NPL];
+    const int64_t of_state = (at.b * p.channels + at.channel) * p.states, per_chunk = static_cast<int64_t>(p.channels) * p.states;
+    float a[NPL], q[NPL], ga[NPL], first[NPL];  // first: the state that the chunk starts from
     LoadStates<NPL>(p.a + static_cast<int64_t>(at.channel) * p.states, n0, p.states, a);
 #pragma unroll
-    for (int i = 0; i < NPL; ++i) a[i] *= kLog2E, q[i] = ga[i] = 0.f;
-    if (pg.gnew != nullptr && at.inside) LoadStates<NPL>(pg.gnew + of_state, n0, p.states, q);
+    for (int i = 0; i < NPL; ++i) a[i] *= kLog2E, q[i] = ga[i] = first[i] = 0.f;
     const float bias = p.bias != nullptr ? p.bias[at.channel] : 0.f, d = p.d != nullptr ? p.d[at.channel] : 0.f;
-    const T* const b = static_cast<const T*>(p.b.data) + at.b * p.b.batch + at.group * p.b.group;
-    const T* const c = static_cast<const T*>(p.c.data) + at.b * p.c.batch + at.group * p.c.group;
+    const int64_t first_line = at.b * p.chunks * p.channels + at.channel;  // of the first chunk
+    if (at.inside) {  // a lane that stands for no channel keeps zeros: it adds nothing to the sums over channels
+        if (p.state != nullptr) LoadStates<NPL>(p.state + of_state, n0, p.states, first);
+        for (int j = 0; j < at.chunk; ++j) {
+            float from[NPL];
+            LoadStates<NPL>(p.ends + first_line * p.states + j * per_chunk, n0, p.states, from);
+            const float dt = p.steps[first_line + static_cast<int64_t>(j) * p.channels];
+#pragma unroll
+            for (int i = 0; i < NPL; ++i) first[i] = __builtin_fmaf(__builtin_amdgcn_exp2f(dt * a[i]), first[i], from[i]);
+        }
+        if (pg.gnew != nullptr) LoadStates<NPL>(pg.gnew + of_state, n0, p.states, q);
+        for (int j = p.chunks - 1; j > at.chunk; --j) {
+            float from[NPL];
+            LoadStates<NPL>(pg.starts + first_line * p.states + j * per_chunk, n0, p.states, from);
+            const float dt = p.steps[first_line + static_cast<int64_t>(j) * p.channels];
+#pragma unroll
+            for (int i = 0; i < NPL; ++i) q[i] = __builtin_fmaf(__builtin_amdgcn_exp2f(dt * a[i]), q[i], from[i]);
+        }
+    }
+    const float* const states = pg.states + (at.b * pg.tiles * p.channels + at.channel) * p.states;
+    const float* const passed = pg.passed + at.b * pg.tiles * p.channels + at.channel;
     const unsigned of_channels = blockIdx.x % static_cast<unsigned>(p.blocks);
     float gd = 0.f, gbias = 0.f;
-    for (int64_t tile = (len + kTile - 1) / kTile - 1; tile >= 0; --tile) {
-        const int64_t t = tile * kTile;
-        for (int e = threadIdx.x; e < kTile * NP; e += 256) {
-            const int r = e / NP, n = e % NP;
-            const bool is = n < p.states && t + r < len;
-            bs[r][n] = is ? static_cast<float>(b[(t + r) * p.b.row + n]) : 0.f;
-            cs[r][n] = is ? static_cast<float>(c[(t + r) * p.c.row + n]) : 0.f;
+    const bool gated = p.z.data != nullptr;
+    const int64_t tiles = last > t0 ? (last - t0 + kTile - 1) / kTile : 0, top = t0 + (tiles - 1) * kTile;
+    TileRows<T, kTile> us(p.u, at, top), ds(p.delta, at, top), zs(p.z, at, top), gys(pg.gy, at, top), gus(pg.gu, at, top), gds(pg.gdelta, at, top), gzs(pg.gz, at, top);
+    TileShared<T, NPL, kTile, 2> shared(p, at, top);
+    float next[NPL] = {}, next_passed = 0.f;  // where the fetched tile starts
+    const auto fetch_rows = [&](int rows, auto whole) __attribute__((always_inline)) {
+        constexpr bool kWhole = decltype(whole)::value;
+        us.template Fetch<kWhole>(at.q, rows);
+        ds.template Fetch<kWhole>(at.q, rows);
+        gys.template Fetch<kWhole>(at.q, rows);
+        if (gated) zs.template Fetch<kWhole>(at.q, rows);
+    };
+    const auto fetch = [&](int64_t t) __attribute__((always_inline)) {
+        if (at.inside) {
+            if (t + kTile <= last) fetch_rows(kTile, std::true_type{});
+            else fetch_rows(static_cast<int>(last - t), std::false_type{});
+            LoadStates<NPL>(states + t / kTile * per_chunk, n0, p.states, next);
+            next_passed = passed[t / kTile * p.channels];
         }
+        shared.template Fetch<false>(static_cast<int>(std::min<int64_t>(last - t, kTile)));
+        us.Move(-1), ds.Move(-1), zs.Move(-1), gys.Move(-1), shared.Move(-1);
+    };
+    int buffer = 0;
+    if (tiles > 0) {
+        fetch(top);
+        shared.template Stage<0>(bs[0]);
+        shared.template Stage<1>(cs[0]);
+        __syncthreads();
+    }
+    for (int64_t t = top; t >= t0; t -= kTile, buffer ^= 1) {
+        const int rows = static_cast<int>(std::min<int64_t>(last - t, kTile)), own_rows = at.inside ? rows : 0;
         float u[kGroups], dt[kGroups], x[kGroups], g0[kGroups], gy[kGroups], slope[kGroups], z[kGroups];
-#pragma unroll
-        for (int g = 0; g < kGroups; ++g) {
-            const int64_t row = t + 4 * g + at.q;
-            u[g] = dt[g] = x[g] = g0[g] = gy[g] = z[g] = 0.f, slope[g] = 1.f;
-            if (row < len && at.inside) {  // a lane that stands for no channel keeps zeros: it adds nothing to the sums over channels
-                const float raw = ScanRead<T>(p.delta, at.b, row, at.channel) + bias;
-                u[g] = ScanRead<T>(p.u, at.b, row, at.channel);
-                dt[g] = p.softplus != 0 ? SoftplusOf(raw) : raw;
-                if (p.softplus != 0) slope[g] = LogisticOf(raw);
-                x[g] = dt[g] * u[g];
-                g0[g] = gy[g] = ScanRead<T>(pg.gy, at.b, row, at.channel);
-                if (p.z.data != nullptr) {
-                    z[g] = ScanRead<T>(p.z, at.b, row, at.channel);
-                    g0[g] *= z[g] * LogisticOf(z[g]);
-                }
-            }
-        }
+        ScanSteps(p, us, ds, at.q, own_rows, bias, dt, x);
         float h[kTile + 1][NPL], e[kTile][NPL];
 #pragma unroll
-        for (int i = 0; i < NPL; ++i) h[0][i] = 0.f;
-        if (at.inside) LoadStates<NPL>(pg.states + ((at.b * pg.tiles + tile) * p.channels + at.channel) * p.states, n0, p.states, h[0]);
-        __syncthreads();
+        for (int g = 0; g < kGroups; ++g) {
+            u[g] = us.Held(g), g0[g] = gy[g] = gys.Held(g), z[g] = zs.Held(g);
+            slope[g] = p.softplus != 0 ? LogisticOf(ds.Held(g) + bias) : 1.f;
+            if (gated) g0[g] *= z[g] * LogisticOf(z[g]);
+        }
+#pragma unroll
+        for (int i = 0; i < NPL; ++i) h[0][i] = __builtin_fmaf(__builtin_amdgcn_exp2f(next_passed * a[i]), first[i], next[i]);
+        if (t > t0) fetch(t - kTile);
 #pragma unroll
         for (int g = 0; g < kGroups; ++g) {
             float y[4];
-            const auto step = [&](auto which) {
+            const auto step = [&](auto which) __attribute__((always_inline)) {
                 constexpr int S = decltype(which)::value;
                 const int r = 4 * g + S;
                 const float dts = OfQuadLane<S>(dt[g]), xs = OfQuadLane<S>(x[g]);
@@ -161,36 +242,33 @@ __global__ __launch_bounds__(256) void SelectiveScanGradKernel(ScanGradArgs pg) 
 #pragma unroll
                 for (int i = 0; i < NPL; ++i) {
                     e[r][i] = __builtin_amdgcn_exp2f(dts * a[i]);
-                    h[r + 1][i] = __builtin_fmaf(xs, bs[r][n0 + i], e[r][i] * h[r][i]);
-                    y[S] = __builtin_fmaf(cs[r][n0 + i], h[r + 1][i], y[S]);
+                    h[r + 1][i] = __builtin_fmaf(xs, bs[buffer][r][n0 + i], e[r][i] * h[r][i]);
+                    y[S] = __builtin_fmaf(cs[buffer][r][n0 + i], h[r + 1][i], y[S]);
                 }
             };
             step(std::integral_constant<int, 0>{});
             step(std::integral_constant<int, 1>{});
             step(std::integral_constant<int, 2>{});
             step(std::integral_constant<int, 3>{});
-            if (p.z.data != nullptr) {
+            if (gated) {
                 const float y0 = __builtin_fmaf(d, u[g], QuadTransposedSum(y, at.q)), l = LogisticOf(z[g]);
-                const int64_t row = t + 4 * g + at.q;
-                if (at.inside && row < len) {
-                    static_cast<T*>(pg.gz.data)[at.b * pg.gz.batch + row * pg.gz.row + at.channel] = static_cast<T>(gy[g] * y0 * l * __builtin_fmaf(z[g], 1.f - l, 1.f));
-                }
+                if (4 * g + at.q < own_rows) gzs[g] = static_cast<T>(gy[g] * y0 * l * __builtin_fmaf(z[g], 1.f - l, 1.f));
             }
         }
 #pragma unroll
         for (int g = kGroups - 1; g >= 0; --g) {
             float qb[4], xa[4], of_b[4 * NPL], of_c[4 * NPL];
-            const auto step = [&](auto which) {
+            const auto step = [&](auto which) __attribute__((always_inline)) {
                 constexpr int S = decltype(which)::value;
                 const int r = 4 * g + S;
                 const float dts = OfQuadLane<S>(dt[g]), xs = OfQuadLane<S>(x[g]), gs = OfQuadLane<S>(g0[g]);
                 qb[S] = xa[S] = 0.f;
 #pragma unroll
                 for (int i = 0; i < NPL; ++i) {
-                    q[i] = __builtin_fmaf(gs, cs[r][n0 + i], q[i]);
+                    q[i] = __builtin_fmaf(gs, cs[buffer][r][n0 + i], q[i]);
                     of_c[S * NPL + i] = gs * h[r + 1][i];
                     of_b[S * NPL + i] = q[i] * xs;
-                    qb[S] = __builtin_fmaf(q[i], bs[r][n0 + i], qb[S]);
+                    qb[S] = __builtin_fmaf(q[i], bs[buffer][r][n0 + i], qb[S]);
                     q[i] *= e[r][i];
                     const float xi = q[i] * h[r][i];
                     ga[i] = __builtin_fmaf(dts, xi, ga[i]);
@@ -203,28 +281,30 @@ __global__ __launch_bounds__(256) void SelectiveScanGradKernel(ScanGradArgs pg) 
             step(std::integral_constant<int, 0>{});
             const float qb_sum = QuadTransposedSum(qb, at.q), xa_sum = QuadTransposedSum(xa, at.q) * (1.f / kLog2E);
             const float gdelta = __builtin_fmaf(u[g], qb_sum, xa_sum) * slope[g];
-            const int64_t row = t + 4 * g + at.q;
-            if (row < len) {
+            if (4 * g + at.q < own_rows) {
                 gbias += gdelta;
                 gd = __builtin_fmaf(g0[g], u[g], gd);
-                if (at.inside) {
-                    static_cast<T*>(pg.gu.data)[at.b * pg.gu.batch + row * pg.gu.row + at.channel] = static_cast<T>(__builtin_fmaf(d, g0[g], dt[g] * qb_sum));
-                    static_cast<T*>(pg.gdelta.data)[at.b * pg.gdelta.batch + row * pg.gdelta.row + at.channel] = static_cast<T>(gdelta);
-                }
+                gus[g] = static_cast<T>(__builtin_fmaf(d, g0[g], dt[g] * qb_sum));
+                gds[g] = static_cast<T>(gdelta);
             }
             float sum_b[NPL], sum_c[NPL];
             SumOverChannels<NPL>(of_b, sum_b);
             SumOverChannels<NPL>(of_c, sum_c);
             if (((lane >> 2) & 3) == 0) {
 #pragma unroll
-                for (int i = 0; i < NPL; ++i) sums[wave][4 * g + (lane >> 4)][0][n0 + i] = sum_b[i], sums[wave][4 * g + (lane >> 4)][1][n0 + i] = sum_c[i];
+                for (int i = 0; i < NPL; ++i) sums[buffer][wave][4 * g + (lane >> 4)][0][n0 + i] = sum_b[i], sums[buffer][wave][4 * g + (lane >> 4)][1][n0 + i] = sum_c[i];
             }
         }
-        __syncthreads();
+        gus.Move(-1), gds.Move(-1), gzs.Move(-1);
+        if (t > t0) {
+            shared.template Stage<0>(bs[buffer ^ 1]);
+            shared.template Stage<1>(cs[buffer ^ 1]);
+        }
+        __syncthreads();  // of the other buffers, what was read before the last one of these
         for (int i = threadIdx.x; i < kTile * 2 * NP; i += 256) {
             const int r = i / (2 * NP), of = i / NP % 2, n = i % NP;
-            if (n < p.states && t + r < len) {
-                const float s = (sums[0][r][of][n] + sums[1][r][of][n]) + (sums[2][r][of][n] + sums[3][r][of][n]);
+            if (n < p.states && r < rows) {
+                const float s = (sums[buffer][0][r][of][n] + sums[buffer][1][r][of][n]) + (sums[buffer][2][r][of][n] + sums[buffer][3][r][of][n]);
                 pg.shared_parts[(((at.b * p.length + t + r) * p.blocks + of_channels) * 2 + of) * p.states + n] = s;
             }
         }
@@ -232,13 +312,13 @@ __global__ __launch_bounds__(256) void SelectiveScanGradKernel(ScanGradArgs pg) 
     gd += QuadSwap1(gd), gbias += QuadSwap1(gbias);
     gd += QuadSwap2(gd), gbias += QuadSwap2(gbias);
     if (!at.inside) return;
-    for (int64_t row = len + at.q; row < p.length; row += 4) {
+    for (int64_t row = std::max(t0, len) + at.q; row < end; row += 4) {
         for (const SequenceRows* r : {&pg.gu, &pg.gdelta, &pg.gz}) {
             if (r->data != nullptr) static_cast<T*>(r->data)[at.b * r->batch + row * r->row + at.channel] = static_cast<T>(0);
         }
     }
-    if (pg.gstate != nullptr) StoreStates<NPL>(pg.gstate + of_state, n0, p.states, q);
-    float* const parts = pg.channel_parts + (at.b * p.channels + at.channel) * (p.states + 2);
+    if (pg.gstate != nullptr && at.chunk == 0) StoreStates<NPL>(pg.gstate + of_state, n0, p.states, q);
+    float* const parts = pg.channel_parts + (first_line + static_cast<int64_t>(at.chunk) * p.channels) * (p.states + 2);
     StoreStates<NPL>(parts, n0, p.states, ga);
     if (at.q == 0) parts[p.states] = gd, parts[p.states + 1] = gbias;
 }
@@ -280,15 +360,19 @@ __global__ __launch_bounds__(256) void ScanChannelSumKernel(const float* parts, 
     else if (n > states && gbias != nullptr) gbias[channel] = all;
 }
 
-int GradTileOf(int states) { return states <= 16 ? 16 : states <= 32 ? 8 : 4; }
+int GradTileOf(int states) { return states <= 8 ? 16 : states <= 16 ? 8 : 4; }
 
 struct GradWorkspace {
-    int64_t states, shared, channels;  // floats
-    GradWorkspace(const ScanArgs& p)
-        : states(p.batch * ((p.length + GradTileOf(p.states) - 1) / GradTileOf(p.states)) * p.channels * p.states),
-          shared(p.batch * p.length * p.blocks * 2 * p.states), channels(p.batch * p.channels * (p.states + 2)) {}
-    size_t Bytes() const { return static_cast<size_t>(states + shared + channels) * sizeof(float); }
+    int64_t states, passed, shared, channels, ends, steps;  // floats
+    explicit GradWorkspace(const ScanArgs& p)
+        : states(p.batch * ((p.length + GradTileOf(p.states) - 1) / GradTileOf(p.states)) * p.channels * p.states), passed(states / p.states), shared(p.batch * p.length * p.blocks * 2 * p.states),
+          channels(p.batch * p.chunks * p.channels * (p.states + 2)), ends(0), steps(0) {
+        if (p.chunks > 1) ends = p.batch * p.chunks * p.channels * p.states, steps = p.batch * p.chunks * p.channels;
+    }
+    size_t Bytes() const { return static_cast<size_t>(states + passed + shared + channels + 2 * ends + steps) * sizeof(float); }
 };
+
+void CutScanGrad(ScanArgs* p) { CutScan(p, 2, 4, 2); }
 
 }  // namespace
 }  // namespace hipcx
@@ -304,6 +388,7 @@ size_t hipcx_selective_scan_grad_workspace_size(const hipcx_array* u, const hipc
     if (groups < 1 || u->shape[0] <= 0 || u->shape[2] <= 0 || u->shape[2] % groups != 0) return 0;
     p.batch = u->shape[0], p.length = u->shape[1], p.channels = static_cast<int>(u->shape[2]), p.states = static_cast<int>(a->shape[1]);
     p.blocks = static_cast<int>(groups) * DivUp(u->shape[2] / groups, kScanChannels);
+    CutScanGrad(&p);
     return GradWorkspace(p).Bytes();
 }
 
@@ -328,21 +413,27 @@ int hipcx_selective_scan_grad(const hipcx_array* u, const hipcx_array* delta, co
         for (const hipcx_array* x : {gd, gdelta_bias}) RequireShape(x, {s.channels}, HIPCX_FLOAT32, what + ": gd and gdelta_bias");
         for (const hipcx_array* x : {gnew_state, gstate}) RequireShape(x, {s.batch, s.channels, s.states}, HIPCX_FLOAT32, what + ": gnew_state and gstate");
         for (const hipcx_array* x : {ga, gb, gc, gd, gdelta_bias, gnew_state, gstate}) RequireDense(x, what + ": ga, gb, gc, gd, gdelta_bias, gnew_state and gstate");
+        for (const hipcx_array* x : {gy, gu, gdelta, gz}) {
+            HIPCX_REQUIRE(x == nullptr || std::abs(x->strides[1]) < kMaxScanRow * ItemSize(x->dtype), HIPCX_NOT_IMPLEMENTED_ERROR, what + ": rows 2^26 elements apart or more");
+        }
         p.gy = RowsOf(gy, "gy"), p.gu = RowsOf(gu, "gu"), p.gdelta = RowsOf(gdelta, "gdelta"), p.gz = RowsOf(gz, "gz");
         const auto floats = [](const hipcx_array* x) { return x != nullptr ? static_cast<float*>(x->data) : nullptr; };
         p.gnew = floats(gnew_state), p.gstate = floats(gstate);
+        CutScanGrad(&p.s);
         const GradWorkspace w(s);
         const size_t need = w.Bytes();
         HIPCX_REQUIRE(workspace_bytes >= need && (need == 0 || workspace != nullptr), HIPCX_CHAINERX_ERROR, what + ": the workspace is too small");
-        p.states = static_cast<float*>(workspace), p.shared_parts = p.states + w.states, p.channel_parts = p.shared_parts + w.shared;
+        p.states = static_cast<float*>(workspace), p.passed = p.states + w.states, p.shared_parts = p.passed + w.passed, p.channel_parts = p.shared_parts + w.shared;
+        p.s.ends = p.channel_parts + w.channels, p.starts = p.s.ends + w.ends, p.s.steps = p.starts + w.ends;
         p.tiles = DivUp(s.length, GradTileOf(s.states));
-        const int64_t blocks = s.batch * s.blocks;
+        const int64_t blocks = s.batch * s.chunks * s.blocks;
         HIPCX_REQUIRE(blocks <= kBlocksPerLaunch, HIPCX_NOT_IMPLEMENTED_ERROR, what + ": too many elements");
         VisitScan(u->dtype, s.states, [&](auto tag, auto share) {
             using T = typename decltype(tag)::type;
             constexpr int NPL = decltype(share)::value;
             if (blocks != 0) {
-                hipLaunchKernelGGL((ScanStatesKernel<T, NPL>), dim3(static_cast<unsigned>(blocks)), dim3(256), 0, AsStream(stream), p);
+                if (s.chunks > 1) hipLaunchKernelGGL((ScanGradStatesKernel<T, NPL, true>), dim3(static_cast<unsigned>(blocks)), dim3(256), 0, AsStream(stream), p);
+                else hipLaunchKernelGGL((ScanGradStatesKernel<T, NPL, false>), dim3(static_cast<unsigned>(blocks)), dim3(256), 0, AsStream(stream), p);
                 CheckLaunch(what.c_str());
                 hipLaunchKernelGGL((SelectiveScanGradKernel<T, NPL>), dim3(static_cast<unsigned>(blocks)), dim3(256), 0, AsStream(stream), p);
                 CheckLaunch(what.c_str());
@@ -356,7 +447,7 @@ int hipcx_selective_scan_grad(const hipcx_array* u, const hipcx_array* delta, co
         });
         const int64_t columns = static_cast<int64_t>(s.channels) * (s.states + 2);
         if (columns == 0) return;
-        hipLaunchKernelGGL(ScanChannelSumKernel, dim3(static_cast<unsigned>((columns + 63) / 64)), dim3(256), 0, AsStream(stream), p.channel_parts, s.batch, s.channels, s.states,
+        hipLaunchKernelGGL(ScanChannelSumKernel, dim3(static_cast<unsigned>((columns + 63) / 64)), dim3(256), 0, AsStream(stream), p.channel_parts, s.batch * s.chunks, s.channels, s.states,
                            floats(ga), floats(gd), floats(gdelta_bias));
         CheckLaunch(what.c_str());
     });
