@@ -14,238 +14,288 @@ struct ConvArgs {
     SequenceLengths lengths;
     int64_t batch, length, channels;
     int64_t first;        // the launch's first thread
-    int pieces, chunks;   // of 16 bytes of a row, of rows
+    int pieces, chunks;   // of a row's channels, of rows
     int rows;             // to a chunk, taps - 1 at least where there is more than one
     int piece_bits;       // gradients: log2 of the pieces that a workgroup spans
     int silu;
 };
 
-template <typename T>
+// E channels of a row, in one access at any address.
+template <typename T, int E>
 struct __attribute__((packed, aligned(alignof(T)))) Piece {
-    static constexpr int kSize = 16 / sizeof(T);
-    T v[kSize];
+    T v[E];
 };
-
-// `n` channels of a row, all of them in one access.
-template <typename T>
-__device__ __forceinline__ Piece<T> LoadPiece(const T* p, int n) {
-    if (n >= Piece<T>::kSize) return *reinterpret_cast<const Piece<T>*>(p);
-    Piece<T> v{};
-#pragma unroll
-    for (int e = 0; e < Piece<T>::kSize; ++e) {
-        if (e < n) v.v[e] = p[e];
-    }
-    return v;
-}
-template <typename T>
-__device__ __forceinline__ void StorePiece(T* p, const Piece<T>& v, int n) {
-    if (n >= Piece<T>::kSize) {
-        *reinterpret_cast<Piece<T>*>(p) = v;
-        return;
-    }
-#pragma unroll
-    for (int e = 0; e < Piece<T>::kSize; ++e) {
-        if (e < n) p[e] = v.v[e];
-    }
-}
 
 template <typename T>
 __device__ __forceinline__ T* RowOf(const SequenceRows& r, int64_t b, int64_t row, int64_t channel) {
     return static_cast<T*>(r.data) + b * r.batch + row * r.row + channel;
 }
 
-// Row `i` of the state and x behind it.
-template <typename T, int K>
-__device__ __forceinline__ Piece<T> InputRow(const ConvArgs& p, int64_t b, int64_t i, int64_t channel, int n) {
-    if (i >= K - 1) return LoadPiece(RowOf<T>(p.x, b, i - (K - 1), channel), n);
-    if (p.state.data == nullptr) return Piece<T>{};
-    return LoadPiece(RowOf<T>(p.state, b, i, channel), n);
-}
+// A thread's part: E channels of a chunk of a sequence.  The last E channels of a row overlap those of the thread before where E does not divide the row, by `skip`:
+// both compute these and store the same values, unless the state may have been moved forward under this one's reads, whose stores of them are left out then.
+template <typename T, int K, int E>
+struct ConvPart {
+    using P = Piece<T, E>;
+    const ConvArgs& p;
+    int64_t b, t0, channel, len, end;
+    int skip;
+    float w[E][K], bias[E];
 
-template <typename T, int K>
-struct Filter {
-    T w[Piece<T>::kSize][K];
-    T b[Piece<T>::kSize];
-    __device__ __forceinline__ Filter(const ConvArgs& p, int64_t channel, int n) {
-        const T* const from = static_cast<const T*>(p.w) + channel * K;
-        const T* const bias = static_cast<const T*>(p.b);
+    __device__ __forceinline__ ConvPart(const ConvArgs& args, int64_t sequence, int64_t row, int64_t piece)
+        : p(args), b(sequence), t0(row), channel(std::min(piece * E, args.channels - E)), len(LengthOf(args.lengths, sequence, args.length)),
+          end(std::min(row + args.rows, args.length)), skip(static_cast<int>(piece * E - channel)) {
+        const Piece<T, E * K> all = *reinterpret_cast<const Piece<T, E * K>*>(static_cast<const T*>(p.w) + channel * K);
+        P of_bias{};
+        if (p.b != nullptr) of_bias = *reinterpret_cast<const P*>(static_cast<const T*>(p.b) + channel);
 #pragma unroll
-        for (int e = 0; e < Piece<T>::kSize; ++e) {
+        for (int i = 0; i < E * K; ++i) w[i / K][i % K] = static_cast<float>(all.v[i]);
 #pragma unroll
-            for (int k = 0; k < K; ++k) w[e][k] = e < n ? from[e * K + k] : static_cast<T>(0);
-            b[e] = bias != nullptr && e < n ? bias[channel + e] : static_cast<T>(0);
+        for (int e = 0; e < E; ++e) bias[e] = static_cast<float>(of_bias.v[e]);
+    }
+    __device__ __forceinline__ P Load(const SequenceRows& r, int64_t row) const { return *reinterpret_cast<const P*>(RowOf<T>(r, b, row, channel)); }
+    __device__ __forceinline__ void Store(const SequenceRows& r, int64_t row, const P& v) const { *reinterpret_cast<P*>(RowOf<T>(r, b, row, channel)) = v; }
+    __device__ __forceinline__ void StoreOwn(const SequenceRows& r, int64_t row, const P& v) const {
+        T* const to = RowOf<T>(r, b, row, channel);
+        if (skip == 0) {
+            *reinterpret_cast<P*>(to) = v;
+        } else {
+#pragma unroll
+            for (int e = 1; e < E; ++e) {
+                if (e >= skip) to[e] = v.v[e];
+            }
+        }
+    }
+    // Row `i` of the state and x behind it.
+    __device__ __forceinline__ P Input(int64_t i) const {
+        P v{};
+        if (i >= K - 1) v = Load(p.x, i - (K - 1));
+        else if (p.state.data != nullptr) v = Load(p.state, i);
+        return v;
+    }
+    // The taps - 1 rows before the chunk's first.
+    template <int N>
+    __device__ __forceinline__ void Before(P (&window)[N]) const {
+#pragma unroll
+        for (int j = 0; j < K - 1; ++j) {
+            window[j] = P{};
+            if (t0 + j < len + K - 1) window[j] = Input(t0 + j);
         }
     }
     // The sum of `window`'s rows `at` to at + K - 1, in 32 bits.
     template <int N>
-    __device__ __forceinline__ float Sum(const Piece<T> (&window)[N], int at, int e) const {
-        float s = static_cast<float>(b[e]);
+    __device__ __forceinline__ float Sum(const P (&window)[N], int at, int e) const {
+        float s = bias[e];
 #pragma unroll
-        for (int k = 0; k < K; ++k) s = __builtin_fmaf(static_cast<float>(w[e][k]), static_cast<float>(window[at + k].v[e]), s);
+        for (int k = 0; k < K; ++k) s = __builtin_fmaf(static_cast<float>(window[at + k].v[e]), w[e][k], s);
         return s;
     }
 };
 
-constexpr int kAhead = 8;  // rows whose loads are issued together
+constexpr int kAhead = 4;      // rows whose loads are issued together
+constexpr int kFewestRows = 8; // to a chunk, taps - 1 at least
 
-template <typename T, int K>
-__global__ __launch_bounds__(256) void CausalConvKernel(ConvArgs p) {
-    constexpr int E = Piece<T>::kSize;
+template <typename T, int K, int E>
+__global__ __launch_bounds__(256, K <= 4 ? 4 : 2) void CausalConvKernel(ConvArgs p) {
+    using P = Piece<T, E>;
     const int64_t index = p.first + static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
     if (index >= p.batch * p.chunks * p.pieces) return;
     const unsigned line = static_cast<unsigned>(index) / static_cast<unsigned>(p.pieces), piece = static_cast<unsigned>(index) % static_cast<unsigned>(p.pieces);
-    const int64_t b = line / static_cast<unsigned>(p.chunks), t0 = static_cast<int64_t>(line % static_cast<unsigned>(p.chunks)) * p.rows, channel = static_cast<int64_t>(piece) * E;
-    const int n = static_cast<int>(std::min<int64_t>(E, p.channels - channel));
-    const int64_t len = LengthOf(p.lengths, b, p.length), end = std::min(t0 + p.rows, p.length);
-    const Filter<T, K> f(p, channel, n);
-    Piece<T> window[K - 1 + kAhead];
+    const ConvPart<T, K, E> c(p, line / static_cast<unsigned>(p.chunks), static_cast<int64_t>(line % static_cast<unsigned>(p.chunks)) * p.rows, piece);
+    const int64_t stop = std::min(c.end, c.len);
+    P window[K - 1 + kAhead];
+    c.Before(window);
+    const auto row = [&](int64_t t, int j, auto own) __attribute__((always_inline)) {
+        P y;
 #pragma unroll
-    for (int j = 0; j < K - 1; ++j) window[j] = t0 + j < len + K - 1 ? InputRow<T, K>(p, b, t0 + j, channel, n) : Piece<T>{};
-    for (int64_t t = t0; t < end; t += kAhead) {
+        for (int e = 0; e < E; ++e) {
+            const float s = c.Sum(window, j, e);
+            y.v[e] = static_cast<T>(p.silu != 0 ? s * LogisticOf(s) : s);
+        }
+        if constexpr (decltype(own)::value) c.StoreOwn(p.y, t, y);
+        else c.Store(p.y, t, y);
+    };
+    int64_t t = c.t0;
+    // up to kAhead rows: a chunk's first ones and its last ones
+    const auto edge = [&]() __attribute__((always_inline)) {
 #pragma unroll
         for (int j = 0; j < kAhead; ++j) {
-            window[K - 1 + j] = Piece<T>{};
-            if (t + j < len && t + j < end) window[K - 1 + j] = LoadPiece(RowOf<T>(p.x, b, t + j, channel), n);
+            P v{};
+            if (t + j < stop) v = c.Load(p.x, t + j);
+            window[K - 1 + j] = v;
         }
 #pragma unroll
         for (int j = 0; j < kAhead; ++j) {
-            if (t + j >= end) break;
-            Piece<T> y{};
-            if (t + j < len) {
-#pragma unroll
-                for (int e = 0; e < E; ++e) {
-                    const float s = f.Sum(window, j, e);
-                    y.v[e] = static_cast<T>(p.silu != 0 ? s * LogisticOf(s) : s);
-                }
-            }
-            StorePiece(RowOf<T>(p.y, b, t + j, channel), y, n);
+            if (t + j >= stop) break;
+            row(t + j, j, std::true_type{});
         }
 #pragma unroll
         for (int j = 0; j < K - 1; ++j) window[j] = window[kAhead + j];
+        t += kAhead;
+    };
+    edge();
+    for (; t + kAhead <= stop; t += kAhead) {
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j) window[K - 1 + j] = c.Load(p.x, t + j);
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j) row(t + j, j, std::false_type{});
+#pragma unroll
+        for (int j = 0; j < K - 1; ++j) window[j] = window[kAhead + j];
     }
-    // new_state may be state: the only thread that reads these channels of it moves its rows forward, the first one first
-    if (t0 == 0) {
-        for (int j = 0; j < K - 1; ++j) StorePiece(RowOf<T>(p.new_state, b, j, channel), InputRow<T, K>(p, b, len + j, channel, n), n);
+    if (t < stop) edge();
+    for (t = std::max(c.t0, c.len); t < c.end; ++t) c.Store(p.y, t, P{});
+    if (c.t0 == 0) {  // new_state may be state: this thread alone reads and writes these channels of it, all of them before it writes any
+        P last[K];
+#pragma unroll
+        for (int j = 0; j < K - 1; ++j) last[j] = c.Input(c.len + j);
+#pragma unroll
+        for (int j = 0; j < K - 1; ++j) c.StoreOwn(p.new_state, j, last[j]);
     }
 }
 
 // gp = gy act'(sum) where a row counts, else 0.  The gradient of input row i (state and x behind it) is w[k] gp[i - k] summed over the taps: a thread
 // goes through its rows and taps - 1 more, computes every sum again from x, and is done with input row i as soon as it has gp[i].
-template <typename T, int K>
-__global__ __launch_bounds__(256) void CausalConvGradKernel(ConvArgs p) {
-    constexpr int E = Piece<T>::kSize, kRows = 4;
+template <typename T, int K, int E>
+__global__ __launch_bounds__(256, K <= 4 ? 4 : 2) void CausalConvGradKernel(ConvArgs p) {
+    using P = Piece<T, E>;
+    constexpr int kRows = 4;
     __shared__ float sums[256 * E];
     const int span = 1 << p.piece_bits, lines = 256 >> p.piece_bits;
     const unsigned piece_blocks = (static_cast<unsigned>(p.pieces) + span - 1) >> p.piece_bits;
     const unsigned part = blockIdx.x / piece_blocks, piece_block = blockIdx.x % piece_blocks;
     const int64_t piece = static_cast<int64_t>(piece_block) * span + (threadIdx.x & (span - 1));
     const int64_t line = static_cast<int64_t>(part) * lines + (threadIdx.x >> p.piece_bits);
-    const int64_t b = line / p.chunks, t0 = line % p.chunks * p.rows, channel = piece * E;
     float gw[E][K] = {}, gb[E] = {};
-    if (piece < p.pieces && b < p.batch) {
-        const int n = static_cast<int>(std::min<int64_t>(E, p.channels - channel));
-        const int64_t len = LengthOf(p.lengths, b, p.length), end = std::min(t0 + p.rows, p.length);
-        const Filter<T, K> f(p, channel, n);
-        Piece<T> window[K - 1 + kRows];
+    int skip = 0;
+    if (piece < p.pieces && line < p.batch * p.chunks) {
+        const ConvPart<T, K, E> c(p, line / p.chunks, line % p.chunks * p.rows, piece);
+        skip = c.skip;
+        P window[K - 1 + kRows], gy[kRows];
         float gp[K - 1 + kRows][E] = {};
+        c.Before(window);
+        // row j of the window: gp, and the row's share of the sums over rows
+        const auto slope = [&](int j, bool own) __attribute__((always_inline)) {
 #pragma unroll
-        for (int j = 0; j < K - 1; ++j) window[j] = t0 + j < len + K - 1 ? InputRow<T, K>(p, b, t0 + j, channel, n) : Piece<T>{};
-        for (int64_t t = t0; t < end + K - 1; t += kRows) {
-            Piece<T> gy[kRows];
+            for (int e = 0; e < E; ++e) {
+                float g = static_cast<float>(gy[j].v[e]);
+                if (p.silu != 0) {
+                    const float s = c.Sum(window, j, e), l = LogisticOf(s);
+                    g *= l * __builtin_fmaf(s, 1.f - l, 1.f);
+                }
+                gp[K - 1 + j][e] = g;
+                if (own) {
+                    gb[e] += g;
 #pragma unroll
-            for (int j = 0; j < kRows; ++j) {
-                window[K - 1 + j] = gy[j] = Piece<T>{};
-                if (t + j < len && t + j < end + K - 1) {
-                    window[K - 1 + j] = LoadPiece(RowOf<T>(p.x, b, t + j, channel), n);
-                    gy[j] = LoadPiece(RowOf<T>(p.gy, b, t + j, channel), n);
+                    for (int k = 0; k < K; ++k) gw[e][k] = __builtin_fmaf(static_cast<float>(window[j + k].v[e]), g, gw[e][k]);
                 }
             }
+        };
+        const auto of_input = [&](int j, const P& last) __attribute__((always_inline)) {
+            P g;
 #pragma unroll
-            for (int j = 0; j < kRows; ++j) {
-                const int64_t row = t + j;
+            for (int e = 0; e < E; ++e) {
+                float s = static_cast<float>(last.v[e]);
 #pragma unroll
-                for (int e = 0; e < E; ++e) {
-                    float g = 0.f;
-                    if (row < len) {
-                        g = static_cast<float>(gy[j].v[e]);
-                        if (p.silu != 0) {
-                            const float s = f.Sum(window, j, e), l = LogisticOf(s);
-                            g *= l * __builtin_fmaf(s, 1.f - l, 1.f);
-                        }
-                    }
-                    gp[K - 1 + j][e] = g;
-                    if (row < end && row < len) {
-                        gb[e] += g;
-#pragma unroll
-                        for (int k = 0; k < K; ++k) gw[e][k] = __builtin_fmaf(g, static_cast<float>(window[j + k].v[e]), gw[e][k]);
-                    }
-                }
-                const bool of_state = row < K - 1;  // t0 is 0 there, or the row belongs to the chunk before
-                if (row < end + K - 1 && row >= (t0 == 0 ? 0 : t0 + K - 1) && (!of_state || p.gstate.data != nullptr)) {
-                    Piece<T> g{}, last{};
-                    const bool ends = p.gnew.data != nullptr && row >= len && row < len + K - 1;
-                    if (ends) last = LoadPiece(RowOf<T>(p.gnew, b, row - len, channel), n);
-#pragma unroll
-                    for (int e = 0; e < E; ++e) {
-                        float s = static_cast<float>(last.v[e]);
-#pragma unroll
-                        for (int k = 0; k < K; ++k) s = __builtin_fmaf(static_cast<float>(f.w[e][k]), gp[K - 1 + j - k][e], s);
-                        g.v[e] = static_cast<T>(s);
-                    }
-                    StorePiece(of_state ? RowOf<T>(p.gstate, b, row, channel) : RowOf<T>(p.gx, b, row - (K - 1), channel), g, n);
-                }
+                for (int k = 0; k < K; ++k) s = __builtin_fmaf(c.w[e][k], gp[K - 1 + j - k][e], s);
+                g.v[e] = static_cast<T>(s);
             }
+            return g;
+        };
+        const auto shift = [&](auto by) __attribute__((always_inline)) {
+            constexpr int kBy = decltype(by)::value;
 #pragma unroll
             for (int j = 0; j < K - 1; ++j) {
-                window[j] = window[kRows + j];
+                window[j] = window[kBy + j];
 #pragma unroll
-                for (int e = 0; e < E; ++e) gp[j][e] = gp[kRows + j][e];
+                for (int e = 0; e < E; ++e) gp[j][e] = gp[kBy + j][e];
             }
+        };
+        // row by row where a sequence or a chunk begins or ends
+        const auto single = [&](int64_t t) __attribute__((always_inline)) {
+            const bool counts = t < c.len;
+            P x{}, g{};
+            if (counts) x = c.Load(p.x, t), g = c.Load(p.gy, t);
+            window[K - 1] = x, gy[0] = g;
+            slope(0, counts && t < c.end);
+#pragma unroll
+            for (int e = 0; e < E; ++e) gp[K - 1][e] = counts ? gp[K - 1][e] : 0.f;  // (whatever the rows before have made of the sum)
+            const bool of_state = t < K - 1;  // of the first chunk: what comes before a later one's rows belongs to the chunk before
+            if ((c.t0 == 0 || t >= c.t0 + K - 1) && (!of_state || p.gstate.data != nullptr)) {
+                P last{};
+                if (p.gnew.data != nullptr && t >= c.len && t < c.len + K - 1) last = c.Load(p.gnew, t - c.len);
+                if (of_state) c.Store(p.gstate, t, of_input(0, last));
+                else c.Store(p.gx, t - (K - 1), of_input(0, last));
+            }
+            shift(std::integral_constant<int, 1>{});
+        };
+        int64_t t = c.t0;
+        for (const int64_t stop = std::min(c.t0, c.end) + K - 1; t < stop; ++t) single(t);
+        for (const int64_t stop = std::min(c.end, c.len); t + kRows <= stop; t += kRows) {
+#pragma unroll
+            for (int j = 0; j < kRows; ++j) window[K - 1 + j] = c.Load(p.x, t + j), gy[j] = c.Load(p.gy, t + j);
+#pragma unroll
+            for (int j = 0; j < kRows; ++j) {
+                slope(j, true);
+                c.Store(p.gx, t + j - (K - 1), of_input(j, P{}));
+            }
+            shift(std::integral_constant<int, kRows>{});
         }
+        for (; t < c.end + K - 1; ++t) single(t);
     }
     // the lines of a workgroup are added up one after another, the same way every time
 #pragma unroll
     for (int k = 0; k <= K; ++k) {
         __syncthreads();
 #pragma unroll
-        for (int e = 0; e < E; ++e) sums[threadIdx.x * E + e] = k < K ? gw[e][k < K ? k : 0] : gb[e];
+        for (int e = 0; e < E; ++e) {
+            if (e >= skip) sums[threadIdx.x * E + e - skip] = k < K ? gw[e][k < K ? k : 0] : gb[e];
+        }
         __syncthreads();
-        for (int c = threadIdx.x; c < span * E; c += 256) {
-            const int64_t at = static_cast<int64_t>(piece_block) * span * E + c;
+        for (int i = threadIdx.x; i < span * E; i += 256) {
+            const int64_t at = static_cast<int64_t>(piece_block) * span * E + i;
             if (at >= p.channels) continue;
             float s = 0.f;
-            for (int i = 0; i < lines; ++i) s += sums[i * span * E + c];
+            for (int j = 0; j < lines; ++j) s += sums[j * span * E + i];
             p.parts[(static_cast<int64_t>(part) * (K + 1) + k) * p.channels + at] = s;
         }
     }
 }
 
-// A column of partial sums to a thread, four threads to a column.
+// Columns of partial sums, eight threads to a column.
 template <typename T>
 __global__ __launch_bounds__(256) void CausalConvSumKernel(const float* parts, int64_t n_parts, int64_t channels, int taps, T* gw, T* gb) {
-    __shared__ float sums[256];
-    const int64_t width = (taps + 1) * channels, c = static_cast<int64_t>(blockIdx.x) * 64 + (threadIdx.x & 63);
+    __shared__ float sums[8][32];
+    const int64_t width = (taps + 1) * channels, c = static_cast<int64_t>(blockIdx.x) * 32 + (threadIdx.x & 31);
+    const int slice = static_cast<int>(threadIdx.x) >> 5;
     float s = 0.f;
     if (c < width) {
-        for (int64_t i = threadIdx.x >> 6; i < n_parts; i += 4) s += parts[i * width + c];
+#pragma unroll 8
+        for (int64_t i = slice; i < n_parts; i += 8) s += parts[i * width + c];
     }
-    sums[threadIdx.x] = s;
+    sums[slice][threadIdx.x & 31] = s;
     __syncthreads();
-    if (threadIdx.x >= 64 || c >= width) return;
-    const float all = (sums[threadIdx.x] + sums[threadIdx.x + 64]) + (sums[threadIdx.x + 128] + sums[threadIdx.x + 192]);
+    if (slice != 0 || c >= width) return;
+    float all = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) all += sums[i][threadIdx.x];
     const int64_t k = c / channels, channel = c % channels;
     if (k < taps) gw[channel * taps + k] = static_cast<T>(all);
     else if (gb != nullptr) gb[channel] = static_cast<T>(all);
 }
 
-// Rows to a chunk: `most`, or the fewest powers of two of it that leave every compute unit four waves, down to the rows whose loads are issued together.
-int ChunkRows(int64_t length, int64_t lines, int most) {
-    int rows = most;
-    while (rows > kAhead && lines * ((length + rows - 1) / rows) < int64_t{NumCUs()} * 1024) rows /= 2;
+// Rows to a chunk: 32, or 16 or 8 where that leaves a compute unit fewer than 16 waves.  A chunk reads taps - 1 rows of the one before again, mostly from the caches.
+// us, 32 and 64 rows: 16 x 2048 x 4096 float16 109, 114; its gradients at 8 x 2048 x 2048, with the forward call, 84, 87.
+int ChunkRows(int64_t length, int64_t lines) {
+    int rows = 32;
+    while (rows > kFewestRows && lines * ((length + rows - 1) / rows) < int64_t{NumCUs()} * 1024) rows /= 2;
     return rows;
 }
 
-constexpr int kGradRows = 64;
+// Channels to a thread: 16 bytes, and four of either type for the gradients, whose sums over rows and windows fill the registers; one where a row has fewer.
+int ConvChannels(const hipcx_array* x) {
+    const int64_t each = 16 / ItemSize(x->dtype);
+    return x->shape[2] >= each ? static_cast<int>(each) : 1;
+}
+int GradChannels(int64_t channels) { return channels >= 4 ? 4 : 1; }
 
 int GradPieceBits(int64_t pieces) {
     int bits = 0;
@@ -254,17 +304,13 @@ int GradPieceBits(int64_t pieces) {
 }
 
 struct ConvSizes {
-    int64_t batch, length, channels, taps, pieces;
-    ConvSizes(const hipcx_array* x, const hipcx_array* w) : batch(x->shape[0]), length(x->shape[1]), channels(x->shape[2]), taps(w->shape[1]) {
-        const int64_t each = 16 / ItemSize(x->dtype);
-        pieces = (channels + each - 1) / each;
-    }
-    int64_t GradChunks() const {
-        const int rows = ChunkRows(length, batch * pieces, kGradRows);
-        return std::max<int64_t>(1, (length + rows - 1) / rows);
-    }
+    int64_t batch, length, channels, taps;
+    ConvSizes(const hipcx_array* x, const hipcx_array* w) : batch(x->shape[0]), length(x->shape[1]), channels(x->shape[2]), taps(w->shape[1]) {}
+    int64_t GradPieces() const { return (channels + GradChannels(channels) - 1) / GradChannels(channels); }
+    int GradRows() const { return ChunkRows(length, batch * GradPieces()); }
+    int64_t GradChunks() const { return std::max<int64_t>(1, (length + GradRows() - 1) / GradRows()); }
     int64_t GradParts() const {
-        const int lines = 256 >> GradPieceBits(pieces);
+        const int lines = 256 >> GradPieceBits(GradPieces());
         return (batch * GradChunks() + lines - 1) / lines;
     }
 };
@@ -325,15 +371,17 @@ int hipcx_causal_conv(const hipcx_array* x, const hipcx_array* w, const hipcx_ar
         p.w = w->data, p.b = b != nullptr ? b->data : nullptr;
         p.batch = s.batch, p.length = s.length, p.channels = s.channels, p.silu = activation;
         if (s.batch == 0 || s.channels == 0) return;
-        p.rows = ChunkRows(s.length, s.batch * s.pieces, 32);
-        const int64_t chunks = std::max<int64_t>(1, (s.length + p.rows - 1) / p.rows), threads = s.batch * chunks * s.pieces;
+        const int64_t each = ConvChannels(x), pieces = (s.channels + each - 1) / each;
+        p.rows = ChunkRows(s.length, s.batch * pieces);
+        const int64_t chunks = std::max<int64_t>(1, (s.length + p.rows - 1) / p.rows), threads = s.batch * chunks * pieces;
         HIPCX_REQUIRE(threads < (int64_t{1} << 31), HIPCX_NOT_IMPLEMENTED_ERROR, "causal_conv: too many elements");
-        p.pieces = static_cast<int>(s.pieces), p.chunks = static_cast<int>(chunks);
+        p.pieces = static_cast<int>(pieces), p.chunks = static_cast<int>(chunks);
         VisitConv(x->dtype, s.taps, [&](auto tag, auto taps) {
             using T = typename decltype(tag)::type;
             ForLaunches(threads, [&](dim3 grid, int64_t first) {
                 p.first = first;
-                hipLaunchKernelGGL((CausalConvKernel<T, decltype(taps)::value>), grid, dim3(256), 0, AsStream(stream), p);
+                if (each == 1) hipLaunchKernelGGL((CausalConvKernel<T, decltype(taps)::value, 1>), grid, dim3(256), 0, AsStream(stream), p);
+                else hipLaunchKernelGGL((CausalConvKernel<T, decltype(taps)::value, 16 / static_cast<int>(sizeof(T))>), grid, dim3(256), 0, AsStream(stream), p);
                 CheckLaunch("causal_conv");
             });
         });
@@ -373,19 +421,22 @@ int hipcx_causal_conv_grad(const hipcx_array* x, const hipcx_array* w, const hip
         HIPCX_REQUIRE(workspace_bytes >= need && (need == 0 || workspace != nullptr), HIPCX_CHAINERX_ERROR, "causal_conv_grad: the workspace is too small");
         p.parts = static_cast<float*>(workspace);
         const int64_t parts = s.batch == 0 ? 0 : s.GradParts();
-        p.piece_bits = GradPieceBits(s.pieces);
-        p.pieces = static_cast<int>(s.pieces), p.chunks = static_cast<int>(s.GradChunks());
-        p.rows = ChunkRows(s.length, s.batch * s.pieces, kGradRows);
-        const int64_t blocks = parts * ((s.pieces + (1 << p.piece_bits) - 1) >> p.piece_bits);
+        const int64_t pieces = s.GradPieces();
+        p.piece_bits = GradPieceBits(pieces);
+        p.pieces = static_cast<int>(pieces), p.chunks = static_cast<int>(s.GradChunks());
+        p.rows = s.GradRows();
+        const int64_t blocks = parts * ((pieces + (1 << p.piece_bits) - 1) >> p.piece_bits);
         HIPCX_REQUIRE(blocks <= kBlocksPerLaunch, HIPCX_NOT_IMPLEMENTED_ERROR, "causal_conv_grad: too many elements");
         VisitConv(x->dtype, s.taps, [&](auto tag, auto taps) {
             using T = typename decltype(tag)::type;
             if (blocks != 0) {
-                hipLaunchKernelGGL((CausalConvGradKernel<T, decltype(taps)::value>), dim3(static_cast<unsigned>(blocks)), dim3(256), 0, AsStream(stream), p);
+                const dim3 grid(static_cast<unsigned>(blocks));
+                if (GradChannels(s.channels) == 1) hipLaunchKernelGGL((CausalConvGradKernel<T, decltype(taps)::value, 1>), grid, dim3(256), 0, AsStream(stream), p);
+                else hipLaunchKernelGGL((CausalConvGradKernel<T, decltype(taps)::value, 4>), grid, dim3(256), 0, AsStream(stream), p);
                 CheckLaunch("causal_conv_grad");
             }
             const int64_t columns = (s.taps + 1) * s.channels;
-            hipLaunchKernelGGL(CausalConvSumKernel<T>, dim3(static_cast<unsigned>((columns + 63) / 64)), dim3(256), 0, AsStream(stream), p.parts, parts, s.channels,
+            hipLaunchKernelGGL(CausalConvSumKernel<T>, dim3(static_cast<unsigned>((columns + 31) / 32)), dim3(256), 0, AsStream(stream), p.parts, parts, s.channels,
                                static_cast<int>(s.taps), static_cast<T*>(gw->data), static_cast<T*>(gb != nullptr ? gb->data : nullptr));
             CheckLaunch("causal_conv_grad");
         });
