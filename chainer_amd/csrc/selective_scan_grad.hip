@@ -11,7 +11,7 @@ struct ScanGradArgs {
     SequenceRows gy, gu, gdelta, gz;
     const float* gnew;  // gradient of the new state, or null
     float* gstate;      // or null
-    float* states;      // [batch][tiles][channels][states]: where each tile starts, of a chunk that starts from zeros
+    float* states;      // [batch][tiles][channels][4 * NPL]: where each tile starts, of a chunk that starts from zeros
     float* passed;      // [batch][tiles][channels]: dt summed over the chunk's rows before the tile
     float* shared_parts;   // [batch][length][blocks][2][states]: gb and gc by workgroups along the channels
     float* channel_parts;  // [batch * chunks][channels][states + 2]: ga, gd, gbias
@@ -74,15 +74,15 @@ __global__ __launch_bounds__(256) void ScanGradStatesKernel(ScanGradArgs pg) {
     const int64_t len = LengthOf(p.lengths, at.b, p.length);
     const int64_t t0 = static_cast<int64_t>(at.chunk) * p.chunk_rows, last = std::min(std::min(t0 + p.chunk_rows, p.length), len);
     const int n0 = at.q * NPL;
-    const int64_t per_tile = static_cast<int64_t>(p.channels) * p.states;
+    const int64_t per_tile = static_cast<int64_t>(p.channels) * NP;
     float a[NPL], h[NPL], start[NPL], decay[NPL];
     LoadStates<NPL>(p.a + static_cast<int64_t>(at.channel) * p.states, n0, p.states, a);
 #pragma unroll
     for (int i = 0; i < NPL; ++i) a[i] *= kLog2E, h[i] = start[i] = 0.f, decay[i] = 1.f;
     const float bias = p.bias != nullptr ? p.bias[at.channel] : 0.f;
     const bool gated = CHUNKS && p.z.data != nullptr;
-    float* const states = pg.states + (at.b * pg.tiles * p.channels + at.channel) * p.states;
-    float* const passed = pg.passed + at.b * pg.tiles * p.channels + at.channel;
+    const int64_t first_tile = (at.b * pg.tiles + t0 / kTile) * p.channels + at.channel;
+    float *states = pg.states + first_tile * NP + n0, *passed = pg.passed + first_tile;
     TileRows<T, kScanTile> us(p.u, at, t0), ds(p.delta, at, t0), zs(p.z, at, t0), gs(pg.gy, at, t0);
     TileShared<T, NPL, kScanTile, CHUNKS ? 2 : 1> shared(p, at, t0);
     const auto fetch_rows = [&](int rows, auto whole) __attribute__((always_inline)) {
@@ -115,10 +115,13 @@ __global__ __launch_bounds__(256) void ScanGradStatesKernel(ScanGradArgs pg) {
         fetch(t + kScanTile);
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
-            if (4 * g % kTile == 0 && t + 4 * g < last && at.inside) {
-                const int64_t tile = (t + 4 * g) / kTile;
-                StoreStates<NPL>(states + tile * per_tile, n0, p.states, h);
-                if (at.q == 0) passed[tile * p.channels] = all_steps;
+            if (4 * g % kTile == 0) {  // unconditionally: a branch costs half the waves; lanes that stand for no channel write what the channel's own do
+                LaneStates<NPL> tile_start;
+#pragma unroll
+                for (int i = 0; i < NPL; ++i) tile_start.v[i] = h[i];
+                *reinterpret_cast<LaneStates<NPL>*>(states) = tile_start;
+                *passed = all_steps;
+                states += per_tile, passed += p.channels;
             }
             float four = dt[g] + QuadSwap1(dt[g]);
             four += QuadSwap2(four);
@@ -140,6 +143,7 @@ __global__ __launch_bounds__(256) void ScanGradStatesKernel(ScanGradArgs pg) {
             step(std::integral_constant<int, 1>{});
             step(std::integral_constant<int, 2>{});
             step(std::integral_constant<int, 3>{});
+            __builtin_amdgcn_sched_barrier(0);  // (else the tile's b and c are all read at once, for half the waves)
         }
     }
     if (!CHUNKS || !at.inside) return;
@@ -151,7 +155,7 @@ __global__ __launch_bounds__(256) void ScanGradStatesKernel(ScanGradArgs pg) {
 
 // A chunk from its last tile to its first: the tile's states again, in registers, from those that it starts from, and the gradients.
 template <typename T, int NPL>
-__global__ __launch_bounds__(256, 2) void SelectiveScanGradKernel(ScanGradArgs pg) {
+__global__ __launch_bounds__(256) void SelectiveScanGradKernel(ScanGradArgs pg) {
     const ScanArgs& p = pg.s;
     constexpr int NP = 4 * NPL, kTile = kGradTile<NPL>, kGroups = kTile / 4;
     __shared__ float bs[2][kTile][NP], cs[2][kTile][NP], sums[2][4][kTile][2][NP];
@@ -184,7 +188,7 @@ __global__ __launch_bounds__(256, 2) void SelectiveScanGradKernel(ScanGradArgs p
             for (int i = 0; i < NPL; ++i) q[i] = __builtin_fmaf(__builtin_amdgcn_exp2f(dt * a[i]), q[i], from[i]);
         }
     }
-    const float* const states = pg.states + (at.b * pg.tiles * p.channels + at.channel) * p.states;
+    const float* const states = pg.states + (at.b * pg.tiles * p.channels + at.channel) * NP + n0;
     const float* const passed = pg.passed + at.b * pg.tiles * p.channels + at.channel;
     const unsigned of_channels = blockIdx.x % static_cast<unsigned>(p.blocks);
     float gd = 0.f, gbias = 0.f;
@@ -204,7 +208,9 @@ __global__ __launch_bounds__(256, 2) void SelectiveScanGradKernel(ScanGradArgs p
         if (at.inside) {
             if (t + kTile <= last) fetch_rows(kTile, std::true_type{});
             else fetch_rows(static_cast<int>(last - t), std::false_type{});
-            LoadStates<NPL>(states + t / kTile * per_chunk, n0, p.states, next);
+            const LaneStates<NPL> start = *reinterpret_cast<const LaneStates<NPL>*>(states + t / kTile * p.channels * NP);
+#pragma unroll
+            for (int i = 0; i < NPL; ++i) next[i] = start.v[i];
             next_passed = passed[t / kTile * p.channels];
         }
         shared.template Fetch<false>(static_cast<int>(std::min<int64_t>(last - t, kTile)));
@@ -221,7 +227,7 @@ __global__ __launch_bounds__(256, 2) void SelectiveScanGradKernel(ScanGradArgs p
         const int rows = static_cast<int>(std::min<int64_t>(last - t, kTile)), own_rows = at.inside ? rows : 0;
         float u[kGroups], dt[kGroups], x[kGroups], g0[kGroups], gy[kGroups], slope[kGroups], z[kGroups];
         ScanSteps(p, us, ds, at.q, own_rows, bias, dt, x);
-        float h[kTile + 1][NPL], e[kTile][NPL];
+        float h[kTile + 1][NPL], e[kTile][NPL], gz[kGroups] = {}, gu[kGroups], gdelta[kGroups];
 #pragma unroll
         for (int g = 0; g < kGroups; ++g) {
             u[g] = us.Held(g), g0[g] = gy[g] = gys.Held(g), z[g] = zs.Held(g);
@@ -252,7 +258,7 @@ __global__ __launch_bounds__(256, 2) void SelectiveScanGradKernel(ScanGradArgs p
             step(std::integral_constant<int, 3>{});
             if (gated) {
                 const float y0 = __builtin_fmaf(d, u[g], QuadTransposedSum(y, at.q)), l = LogisticOf(z[g]);
-                if (4 * g + at.q < own_rows) gzs[g] = static_cast<T>(gy[g] * y0 * l * __builtin_fmaf(z[g], 1.f - l, 1.f));
+                gz[g] = gy[g] * y0 * l * __builtin_fmaf(z[g], 1.f - l, 1.f);
             }
         }
 #pragma unroll
@@ -280,19 +286,21 @@ __global__ __launch_bounds__(256, 2) void SelectiveScanGradKernel(ScanGradArgs p
             step(std::integral_constant<int, 1>{});
             step(std::integral_constant<int, 0>{});
             const float qb_sum = QuadTransposedSum(qb, at.q), xa_sum = QuadTransposedSum(xa, at.q) * (1.f / kLog2E);
-            const float gdelta = __builtin_fmaf(u[g], qb_sum, xa_sum) * slope[g];
-            if (4 * g + at.q < own_rows) {
-                gbias += gdelta;
-                gd = __builtin_fmaf(g0[g], u[g], gd);
-                gus[g] = static_cast<T>(__builtin_fmaf(d, g0[g], dt[g] * qb_sum));
-                gds[g] = static_cast<T>(gdelta);
-            }
+            gdelta[g] = __builtin_fmaf(u[g], qb_sum, xa_sum) * slope[g];
+            gu[g] = __builtin_fmaf(d, g0[g], dt[g] * qb_sum);
+            gbias += 4 * g + at.q < own_rows ? gdelta[g] : 0.f;
+            gd = __builtin_fmaf(g0[g], u[g], gd);
             float sum_b[NPL], sum_c[NPL];
             SumOverChannels<NPL>(of_b, sum_b);
             SumOverChannels<NPL>(of_c, sum_c);
-            if (((lane >> 2) & 3) == 0) {
 #pragma unroll
-                for (int i = 0; i < NPL; ++i) sums[buffer][wave][4 * g + (lane >> 4)][0][n0 + i] = sum_b[i], sums[buffer][wave][4 * g + (lane >> 4)][1][n0 + i] = sum_c[i];
+            for (int i = 0; i < NPL; ++i) sums[buffer][wave][4 * g + (lane >> 4)][(lane >> 2) & 1][n0 + i] = (lane & 4) == 0 ? sum_b[i] : sum_c[i];
+        }
+#pragma unroll
+        for (int g = 0; g < kGroups; ++g) {  // (the stores together: branches between the groups would keep the compiler from mixing them)
+            if (4 * g + at.q < own_rows) {
+                gus[g] = static_cast<T>(gu[g]), gds[g] = static_cast<T>(gdelta[g]);
+                if (gated) gzs[g] = static_cast<T>(gz[g]);
             }
         }
         gus.Move(-1), gds.Move(-1), gzs.Move(-1);
@@ -362,10 +370,15 @@ __global__ __launch_bounds__(256) void ScanChannelSumKernel(const float* parts, 
 
 int GradTileOf(int states) { return states <= 8 ? 16 : states <= 16 ? 8 : 4; }
 
+int PaddedStates(int states) { return states <= 4 ? 4 : states <= 8 ? 8 : states <= 16 ? 16 : states <= 32 ? 32 : 64; }
+
+// Of a sequence, in whole tiles of the run that makes their states.
+int64_t GradTiles(const ScanArgs& p) { return (p.length + kScanTile - 1) / kScanTile * (kScanTile / GradTileOf(p.states)); }
+
 struct GradWorkspace {
     int64_t states, passed, shared, channels, ends, steps;  // floats
     explicit GradWorkspace(const ScanArgs& p)
-        : states(p.batch * ((p.length + GradTileOf(p.states) - 1) / GradTileOf(p.states)) * p.channels * p.states), passed(states / p.states), shared(p.batch * p.length * p.blocks * 2 * p.states),
+        : states(p.batch * GradTiles(p) * p.channels * PaddedStates(p.states)), passed(states / PaddedStates(p.states)), shared(p.batch * p.length * p.blocks * 2 * p.states),
           channels(p.batch * p.chunks * p.channels * (p.states + 2)), ends(0), steps(0) {
         if (p.chunks > 1) ends = p.batch * p.chunks * p.channels * p.states, steps = p.batch * p.chunks * p.channels;
     }
@@ -425,7 +438,7 @@ int hipcx_selective_scan_grad(const hipcx_array* u, const hipcx_array* delta, co
         HIPCX_REQUIRE(workspace_bytes >= need && (need == 0 || workspace != nullptr), HIPCX_CHAINERX_ERROR, what + ": the workspace is too small");
         p.states = static_cast<float*>(workspace), p.passed = p.states + w.states, p.shared_parts = p.passed + w.passed, p.channel_parts = p.shared_parts + w.shared;
         p.s.ends = p.channel_parts + w.channels, p.starts = p.s.ends + w.ends, p.s.steps = p.starts + w.ends;
-        p.tiles = DivUp(s.length, GradTileOf(s.states));
+        p.tiles = static_cast<int>(GradTiles(s));
         const int64_t blocks = s.batch * s.chunks * s.blocks;
         HIPCX_REQUIRE(blocks <= kBlocksPerLaunch, HIPCX_NOT_IMPLEMENTED_ERROR, what + ": too many elements");
         VisitScan(u->dtype, s.states, [&](auto tag, auto share) {
