@@ -408,12 +408,13 @@ def lstm_lm_input(seed=5, batch=128, seq=35, vocab=10000):
     return _rng(seed + 1000).integers(0, vocab, (batch, seq)).astype(np.int32)
 
 
-def lstm_lm_forward(F, p, ids, zeros, take_mode=None, fused=False, step=None):
+def lstm_lm_forward(F, p, ids, zeros, take_mode=None, fused=False, step=None, dropout=None):
     """Runs the sequence; returns log-probabilities of the last step and the final (h, c) of both layers.
     ``zeros(shape, dtype)`` makes the initial state on the same backend as ``F``.  ``step``: a layer's time step is one call of
     ``F.lstm_step``, in which float16 gates are not rounded, instead of two of ``F.linear``, ``F.add`` and the cell's; None: where ``F``
     has that routine, unless ``fused`` asks for a cell.  ``fused`` calls ``F.lstm_fused`` and ``F.log_softmax_fused``, which run the
-    kernels that ``F.lstm`` and ``F.log_softmax`` of this backend run for these arrays."""
+    kernels that ``F.lstm`` and ``F.log_softmax`` of this backend run for these arrays.  ``dropout``: (ratio, key) of ``F.dropout`` before either layer and the output
+    layer, as the example trains (examples/ptb/train_ptb.py:28-50); time step t's three are the sites 3 t to 3 t + 2."""
     if step is None:
         step = hasattr(F, 'lstm_step') and not fused
     lstm = F.lstm_fused if fused else F.lstm
@@ -427,11 +428,15 @@ def lstm_lm_forward(F, p, ids, zeros, take_mode=None, fused=False, step=None):
     for t in range(seq):
         x = F.take(p['embed'], ids[:, t], 0, take_mode)
         for li, layer in enumerate(p['layers']):
+            if dropout is not None:
+                x = F.dropout(x, dropout[0], dropout[1], site=3 * t + li)
             if step:
                 hs[li], cs[li] = F.lstm_step(cs[li], x, layer['up_w'], layer['up_b'], hs[li], layer['lat_w'])
             else:
                 gates = F.add(F.linear(x, layer['up_w'], layer['up_b']), F.linear(hs[li], layer['lat_w']))
                 hs[li], cs[li] = lstm(cs[li], gates)
             x = hs[li]
+        if dropout is not None:
+            x = F.dropout(x, dropout[0], dropout[1], site=3 * t + 2)
         y = F.linear(x, p['out_w'], p['out_b'])
     return log_softmax(y, 1), hs, cs

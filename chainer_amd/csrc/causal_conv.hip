@@ -133,6 +133,7 @@ __global__ __launch_bounds__(256, K <= 4 ? 4 : 2) void CausalConvKernel(ConvArgs
         t += kAhead;
     };
     edge();
+    if (K - 1 > kAhead && t < stop) edge();  // all rows whose sums take the state's in
     for (; t + kAhead <= stop; t += kAhead) {
 #pragma unroll
         for (int j = 0; j < kAhead; ++j) window[K - 1 + j] = c.Load(p.x, t + j);

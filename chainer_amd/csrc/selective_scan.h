@@ -128,7 +128,7 @@ struct TileRows {
 #pragma unroll
         for (int g = 0; g < kGroups; ++g) held[g] = static_cast<T>(0);
     }
-    __device__ __forceinline__ T& operator[](int g) const { return *reinterpret_cast<T*>(base + (offset + static_cast<unsigned>(g * group))); }
+    __device__ __forceinline__ T& operator[](int g) const { return *reinterpret_cast<T*>(base + (offset + static_cast<unsigned>(g) * static_cast<unsigned>(group))); }
     // A lane's rows of the tile, all of them or those before `rows`.
     template <bool WHOLE>
     __device__ __forceinline__ void Fetch(int q, int rows) {

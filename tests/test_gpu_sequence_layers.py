@@ -133,9 +133,10 @@ def test_causal_conv(chx, sizes, dtype):
 
 
 @pytest.mark.parametrize('dtype', ['float16', 'float32'])
-def test_causal_conv_pieces_and_tokens(chx, dtype):
+@pytest.mark.parametrize('channels,taps', [(19, 4), (1301, 8), (8, 7), (3, 8), (67, 2)])
+def test_causal_conv_pieces_and_tokens(chx, channels, taps, dtype):
     """A sequence in pieces and token by token, the state moved forward in place, is the sequence at once, bit for bit."""
-    c = conv_case(3, 50, 19, 4, dtype)
+    c = conv_case(3, 50, channels, taps, dtype)
     w, b = up(chx, c['w']), up(chx, c['b'])
     whole, last = chx.causal_conv(up(chx, c['x']), w, b, state=up(chx, c['state']), activation='silu')
     state, ys, t = chx.array(c['state']), [], 0
@@ -146,7 +147,7 @@ def test_causal_conv_pieces_and_tokens(chx, dtype):
         t += n
     assert t == 50
     assert np.array_equal(np.concatenate(ys, 1), whole.get()) and np.array_equal(state.get(), last.get())
-    assert np.array_equal(last.get(), c['x'][:, -3:])
+    assert np.array_equal(last.get(), c['x'][:, 51 - taps:])
 
 
 def test_causal_conv_empty(chx):
@@ -158,6 +159,18 @@ def test_causal_conv_empty(chx):
         assert gx.shape == shape and not gw.get().any() and not gb.get().any()
         if shape[1] == 0:
             assert np.array_equal(gstate.get(), c['gnew'])
+
+
+def test_causal_conv_beyond_2_31_elements(chx):
+    """Rows whose place in memory takes more than 32 bits, with the window of the last ones."""
+    length, channels = (1 << 20) + 5, 2056
+    x = chx.zeros((1, length, channels), 'float16')
+    c = conv_case(1, 40, channels, 4, 'float16')
+    chx.routines._copy_into(x[:, length - 40:], chx.array(c['x']))
+    w, b = chx.array(c['w']), chx.array(c['b'])
+    y, new = chx.causal_conv(x, w, b, activation='silu')
+    short, short_new = chx.causal_conv(chx.array(c['x']), w, b, state=chx.zeros((1, 3, channels), 'float16'), activation='silu')
+    assert np.array_equal(y[:, length - 40:].get(), short.get()) and np.array_equal(new.get(), short_new.get())
 
 
 # ---------------------------------------------------------------------------------------------
@@ -277,6 +290,54 @@ def test_selective_scan_of_steps_that_forget_and_that_do_not_move(chx):
     ref.assert_within(y.get()[:, rows], want[:, rows], size[:, rows], 21 * 60 + 60, 'y')
     ref.assert_within(new.get(), want_new, new_size, 21 * 60 + 60, 'state')
     assert not np.isnan(y.get()[:, 3]).any() and not y.get()[:, 4].any()
+
+
+def test_selective_scan_of_sequences_far_apart(chx):
+    """Sequences and rows whose distance in memory takes more than 31 bits."""
+    c, more, _ = scan_case(2, 40, 70, 16, None, 'float16')
+    dev = scan_on_device(chx, c, None, True)
+    gy = up(chx, more['gy'])
+    want, want_new = chx.selective_scan(**dev)
+    grads = chx.selective_scan_grad(gy=gy, **dev)
+    batch, row = 1 << 32, (1 << 26) - 2  # bytes
+    buffer = chx._array.alloc_bytes(batch + 40 * row + 4096)
+    for i, k in enumerate(('u', 'delta', 'z')):
+        far = chx.ndarray(buffer, 512 * i, (2, 40, 70), (batch, row, 2), np.dtype('float16'))
+        chx.routines._copy_into(far, dev[k])
+        dev[k] = far
+    got, new = chx.selective_scan(**dev)
+    assert np.array_equal(got.get(), want.get()) and np.array_equal(new.get(), want_new.get())
+    for a, b in zip(chx.selective_scan_grad(gy=gy, **dev), grads):
+        assert (a is None) == (b is None) and (a is None or np.array_equal(a.get(), b.get()))
+
+
+@pytest.mark.parametrize('seed', range(10))
+def test_layers_of_drawn_sizes(chx, seed):
+    rng = np.random.default_rng(1000 + seed)
+    groups = int(rng.choice([1, 1, 2, 3]))
+    batch, length, per = int(rng.integers(1, 9)), int(np.exp(rng.uniform(0, 5.5))), int(np.exp(rng.uniform(0, 4.5)))
+    dtype, states, ragged = str(rng.choice(['float16', 'float32'])), int(rng.integers(1, 65)), bool(rng.random() < 0.5)
+    sizes = (batch, length, per * groups, states, groups)
+    c, more, lengths = scan_case(*sizes, dtype, seed=seed, ragged=ragged)
+    dev = scan_on_device(chx, c, lengths, True)
+    y, new = chx.selective_scan(**dev)
+    (want, want_new), (size, new_size), n = ref.selective_scan(delta_softplus=True, lengths=lengths, **c)
+    ref.assert_within(y.get(), want, size, n, '%s %s' % (sizes, dtype))
+    ref.assert_within(new.get(), want_new, new_size, n, '%s %s state' % (sizes, dtype))
+    grads = chx.selective_scan_grad(gy=apart(chx, more['gy']), gnew_state=up(chx, more['gnew']), **dev)
+    wants, sizes_of, n = ref.selective_scan_grad(gy=more['gy'], gnew=more['gnew'], delta_softplus=True, lengths=lengths, **c)
+    for k, got in grads._asdict().items():
+        ref.assert_within(got.get(), wants[k].reshape(got.shape), sizes_of[k].reshape(got.shape), n, '%s %s: %s' % (sizes, dtype, k))
+    taps = int(rng.integers(1, 9))
+    c = conv_case(batch, length, per * groups, taps, dtype, seed=seed, ragged=ragged)
+    x, w, b, state, ends = apart(chx, c['x']), up(chx, c['w']), up(chx, c['b']), up(chx, c['state']), up(chx, c['lengths'])
+    y, new = chx.causal_conv(x, w, b, state=state, lengths=ends, activation='silu')
+    want, size, want_new = ref.causal_conv(c['x'], c['w'], c['b'], c['state'], c['lengths'], 'silu')
+    ref.assert_within(y.get(), want, size, 1, 'conv %s %s' % (sizes, taps))
+    assert np.array_equal(new.get(), want_new.astype(dtype))
+    grads = chx.causal_conv_grad(x, w, b, apart(chx, c['gy']), state=state, lengths=ends, activation='silu', gnew_state=up(chx, c['gnew']))
+    for got, want, size in zip(grads, *ref.causal_conv_grad(c['x'], c['w'], c['b'], c['gy'], c['state'], c['lengths'], 'silu', c['gnew'])):
+        ref.assert_within(got.get(), want, size, 1, 'conv %s %s gradients' % (sizes, taps))
 
 
 # ---------------------------------------------------------------------------------------------
@@ -426,3 +487,29 @@ def test_strides_that_repeat_and_run_backwards(chx):
     cc['x'] = np.ascontiguousarray(np.broadcast_to(cc['x'][:1, ::-1], cc['x'].shape))
     want, size, _ = ref.causal_conv(cc['x'], cc['w'])
     ref.assert_within(chx.causal_conv(x, chx.array(cc['w']))[0].get(), want, size, 1, 'conv')
+
+
+def test_language_model_with_dropout(chx):
+    """The language model's forward pass with dropout before its layers, step by step against the oracle and masks in Python's integers."""
+    from chainer_amd import configs as cfg
+    from oracle import native as oracle
+
+    class WithDropout(object):
+        dropout = staticmethod(lambda x, ratio, key, site: ref.dropout(x, ratio, key, site).astype(x.dtype))
+
+        def __getattr__(self, name):
+            return getattr(oracle, name)
+
+    p, ids = cfg.lstm_lm_params(vocab=50, units=20), cfg.lstm_lm_input(batch=3, seq=4, vocab=50)
+    want, want_h, want_c = cfg.lstm_lm_forward(WithDropout(), p, ids, np.zeros, step=False, dropout=(0.5, KEY))
+    plain, _, _ = cfg.lstm_lm_forward(oracle, p, ids, np.zeros, step=False)
+    dev, key = cfg.tree_map(chx.array, p), up(chx, KEY)
+    for step in (None, False):
+        got, h, c = cfg.lstm_lm_forward(chx, dev, chx.array(ids), chx.zeros, step=step, dropout=(0.5, key))
+        for a, b in zip([got] + h + c, [want] + want_h + want_c):
+            # sums of 20 products of |weights| <= 0.05 through four steps: some dozens of roundings of values of at most 5
+            np.testing.assert_allclose(a.get(), b, rtol=0, atol=64 * 2.0 ** -24 * 5)
+        assert np.abs(got.get() - plain).max() > 1e-4
+        none, _, _ = cfg.lstm_lm_forward(chx, dev, chx.array(ids), chx.zeros, step=step, dropout=(0.0, key))
+        same, _, _ = cfg.lstm_lm_forward(chx, dev, chx.array(ids), chx.zeros, step=step)
+        assert np.array_equal(none.get(), same.get())

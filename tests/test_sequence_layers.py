@@ -160,6 +160,10 @@ def test_selective_scan_limits():
         refused(name, missing, *scan_arguments(grad=grad, a=described((6, 0))))
         refused(name, dimension, *scan_arguments(grad=grad, groups=4))  # of 6 channels
         refused(name, dimension, *scan_arguments(grad=grad, groups=0))
+        for far in (1 << 28, -(1 << 28)):  # bytes from a row to the next
+            for k in ('u', 'delta', 'z'):
+                refused(name, missing, *scan_arguments(grad=grad, **{k: described((2, 6, 6), F32, [24, far, 4])}))
+        refused(name, missing, *scan_arguments(grad=grad, c=described((2, 6, 4), F32, [24, 1 << 28, 4])))
     refused('hipcx_selective_scan', plain, *scan_arguments(y=None))
     refused('hipcx_selective_scan', plain, *scan_arguments(new_state=None))
     refused('hipcx_selective_scan', dtype, *scan_arguments(new_state=described((2, 6, 4), F16)))
@@ -169,6 +173,8 @@ def test_selective_scan_limits():
         refused('hipcx_selective_scan_grad', plain, *scan_arguments(grad=True, **{name: None}))
     refused('hipcx_selective_scan_grad', plain, *scan_arguments(grad=True, size=64))
     refused('hipcx_selective_scan_grad', plain, *scan_arguments(grad=True, workspace=None))
+    refused('hipcx_selective_scan', missing, *scan_arguments(y=described((2, 6, 6), F32, [24, 1 << 28, 4])))
+    refused('hipcx_selective_scan_grad', missing, *scan_arguments(grad=True, gu=described((2, 6, 6), F32, [24, 1 << 28, 4])))
     refused('hipcx_selective_scan_grad', dimension, *scan_arguments(grad=True, gb=described((2, 6, 4), F32, [200, 32, 4])))
     refused('hipcx_selective_scan_grad', dtype, *scan_arguments(grad=True, ga=described((6, 4), F16)))
     refused('hipcx_selective_scan_grad', dimension, *scan_arguments(grad=True, gstate=described((2, 4, 6))))
