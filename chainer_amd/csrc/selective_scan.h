@@ -93,6 +93,28 @@ __device__ __forceinline__ void StoreStates(float* p, int n0, int all, const flo
     }
 }
 
+// s = exp(sum of dt) s + what the chunk adds, for `n` chunks one after another, `next` chunks apart (1 or -1): a state from the sequence's start to a chunk, or its gradient
+// from the end back to one.  `adds` [chunk][per_chunk] and `steps` [chunk][channels] are read four chunks at a time.
+template <int NPL>
+__device__ __forceinline__ void ThroughChunks(float (&s)[NPL], const float (&a)[NPL], const float* adds, const float* steps, int n, int next, int64_t per_chunk, int64_t channels,
+                                              int n0, int states) {
+    for (int j = 0; j < n; j += 4) {
+        float add[4][NPL], dt[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const int64_t at = static_cast<int64_t>(j + k < n ? j + k : n - 1) * next;
+            LoadStates<NPL>(adds + at * per_chunk, n0, states, add[k]);
+            dt[k] = steps[at * channels];
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            if (j + k >= n) break;
+#pragma unroll
+            for (int i = 0; i < NPL; ++i) s[i] = __builtin_fmaf(__builtin_amdgcn_exp2f(dt[k] * a[i]), s[i], add[k][i]);
+        }
+    }
+}
+
 // Where a thread stands: its sequence, chunk, channel and lane of the quad.
 struct ScanPlace {
     int64_t b;

@@ -1,6 +1,8 @@
 // The selective scan: whole sequences, and one row of each.
 #include "selective_scan.h"
 
+#include <cmath>
+
 namespace hipcx {
 namespace {
 
@@ -32,13 +34,7 @@ __global__ __launch_bounds__(256) void SelectiveScanKernel(ScanArgs p) {
         }
     } else {
         LoadStates<NPL>(ends, n0, p.states, h);
-        for (int j = 0; j < at.chunk; ++j) {
-            float end[NPL];
-            LoadStates<NPL>(ends + (j + 1) * per_chunk, n0, p.states, end);
-            const float dt = steps[static_cast<int64_t>(j) * p.channels];
-#pragma unroll
-            for (int i = 0; i < NPL; ++i) h[i] = __builtin_fmaf(__builtin_amdgcn_exp2f(dt * a[i]), h[i], end[i]);
-        }
+        ThroughChunks<NPL>(h, a, ends + per_chunk, steps, at.chunk, 1, per_chunk, p.channels, n0, p.states);
     }
     float all_steps = 0.f;
     const float bias = p.bias != nullptr ? p.bias[at.channel] : 0.f, d = p.d != nullptr ? p.d[at.channel] : 0.f;
@@ -54,8 +50,9 @@ __global__ __launch_bounds__(256) void SelectiveScanKernel(ScanArgs p) {
         us.Move(1), ds.Move(1), zs.Move(1), shared.Move(1);
     };
     // `rows` of the tile at t, all 16 of them or fewer
-    const auto run = [&](int64_t t, int buffer, const float (&u)[4], const float (&z)[4], const float (&dt)[4], auto whole) __attribute__((always_inline)) {
+    const auto run = [&](int64_t t, int buffer, const float (&u)[4], const float (&gate)[4], const float (&dt)[4], auto whole) __attribute__((always_inline)) {
         constexpr bool kWhole = decltype(whole)::value;
+        float y[4];
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
             const float x = dt[g] * u[g];
@@ -77,11 +74,16 @@ __global__ __launch_bounds__(256) void SelectiveScanKernel(ScanArgs p) {
             step(std::integral_constant<int, 2>{});
             step(std::integral_constant<int, 3>{});
             if constexpr (!ENDS) {
-                float y = __builtin_fmaf(d, u[g], QuadTransposedSum(sums, at.q));
-                if (gated) y *= z[g] * LogisticOf(z[g]);
-                if (at.inside && (kWhole || t + 4 * g + at.q < last)) ys[g] = static_cast<T>(y);
+                y[g] = __builtin_fmaf(d, u[g], QuadTransposedSum(sums, at.q)) * gate[g];
             }
-            __builtin_amdgcn_sched_barrier(0);
+        }
+        if constexpr (!ENDS) {
+            if (at.inside) {
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {
+                    if (kWhole || t + 4 * g + at.q < last) ys[g] = static_cast<T>(y[g]);
+                }
+            }
         }
     };
     const auto fetch_tile = [&](int64_t t) {
@@ -94,20 +96,24 @@ __global__ __launch_bounds__(256) void SelectiveScanKernel(ScanArgs p) {
         shared.template Stage<0>(bs[buffer]);
         if constexpr (!ENDS) shared.template Stage<1>(cs[buffer]);
         __syncthreads();
-        float u[4], dt[4], z[4];
+        float u[4], dt[4], gate[4];
 #pragma unroll
-        for (int g = 0; g < 4; ++g) {
-            u[g] = us.Held(g), z[g] = zs.Held(g);
-            const float raw = ds.Held(g) + bias;
-            dt[g] = p.softplus != 0 ? SoftplusOf(raw) : raw;
+        for (int g = 0; g < 4; ++g) u[g] = us.Held(g), dt[g] = ds.Held(g) + bias, gate[g] = 1.f;
+        if (p.softplus != 0) {
+#pragma unroll
+            for (int g = 0; g < 4; ++g) dt[g] = SoftplusOf(dt[g]);
+        }
+        if (gated) {
+#pragma unroll
+            for (int g = 0; g < 4; ++g) gate[g] = zs.Held(g) * LogisticOf(zs.Held(g));
         }
         fetch_tile(t + kScanTile);
         if (t + kScanTile <= last) {
-            run(t, buffer, u, z, dt, std::true_type{});
+            run(t, buffer, u, gate, dt, std::true_type{});
         } else {
 #pragma unroll
             for (int g = 0; g < 4; ++g) dt[g] = t + 4 * g + at.q < last ? dt[g] : 0.f;
-            run(t, buffer, u, z, dt, std::false_type{});
+            run(t, buffer, u, gate, dt, std::false_type{});
         }
         ys.Move(1);
         if constexpr (ENDS) all_steps += (dt[0] + dt[1]) + (dt[2] + dt[3]);
@@ -177,10 +183,16 @@ __global__ __launch_bounds__(256) void ScanTokenKernel(ScanArgs p, int64_t first
 
 }  // namespace
 
+// us, forward, 16384 rows of 512 channels in 64, 128, 256 chunks: 102, 101, 147; of 64 channels in 64, 128, 256: 77, 67, 85; 4096 rows of 64 channels in 32, 64, 128: 42, 36, 46: a
+// chunk goes through those before it, so that as many chunks as a chunk has rows are the best, less what a tile's 16 rows round off.  2048 rows, 2048 channels: 16 sequences (two
+// workgroups to a compute unit) whole 404, in four chunks 469; 8 sequences whole 462, in 8 chunks 248; 4 sequences for 4, 8, 12 workgroups to a compute unit 142, 134, 141.
 void CutScan(ScanArgs* p, int enough, int each, int least) {
     const int64_t tiles = DivUp(p->length, kScanTile), lines = p->batch * DivUp(p->channels, kScanChannels);
     int64_t chunks = 1;
-    if (lines > 0 && lines < int64_t{NumCUs()} * enough) chunks = std::max<int64_t>(1, std::min<int64_t>(int64_t{NumCUs()} * each / lines, tiles / least));
+    if (lines > 0 && lines < int64_t{NumCUs()} * enough) {
+        chunks = std::min({int64_t{NumCUs()} * each / lines, tiles / least, static_cast<int64_t>(std::sqrt(static_cast<double>(p->length)))});
+        chunks = std::max<int64_t>(chunks, 1);
+    }
     const int64_t to_chunk = std::max<int64_t>(1, (tiles + chunks - 1) / chunks);
     p->chunk_rows = static_cast<int>(to_chunk) * kScanTile;
     p->chunks = static_cast<int>(std::max<int64_t>(1, (tiles + to_chunk - 1) / to_chunk));
@@ -257,7 +269,7 @@ size_t hipcx_selective_scan_workspace_size(const hipcx_array* u, const hipcx_arr
     if (u == nullptr || a == nullptr || u->ndim != 3 || a->ndim != 2 || u->shape[0] < 0 || u->shape[1] < 0 || u->shape[2] < 0) return 0;
     ScanArgs p{};
     p.batch = u->shape[0], p.length = u->shape[1], p.channels = static_cast<int>(u->shape[2]), p.states = static_cast<int>(a->shape[1]);
-    CutScan(&p, 4, 8, 2);
+    CutScan(&p, 2, 8, 2);
     return ScanWorkspace(p).Bytes();
 }
 
@@ -274,7 +286,7 @@ int hipcx_selective_scan(const hipcx_array* u, const hipcx_array* delta, const h
         HIPCX_REQUIRE(std::abs(y->strides[1]) < kMaxScanRow * ItemSize(y->dtype), HIPCX_NOT_IMPLEMENTED_ERROR, what + ": rows 2^26 elements apart or more");
         p.y = RowsOf(y, "y"), p.new_state = static_cast<float*>(new_state->data);
         if (p.batch == 0 || p.channels == 0) return;
-        CutScan(&p, 4, 8, 2);
+        CutScan(&p, 2, 8, 2);
         const ScanWorkspace w(p);
         HIPCX_REQUIRE(workspace_bytes >= w.Bytes() && (w.Bytes() == 0 || workspace != nullptr), HIPCX_CHAINERX_ERROR, what + ": the workspace is too small");
         p.ends = static_cast<float*>(workspace), p.steps = p.ends + w.ends;

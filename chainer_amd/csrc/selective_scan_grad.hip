@@ -172,21 +172,10 @@ __global__ __launch_bounds__(256) void SelectiveScanGradKernel(ScanGradArgs pg) 
     const int64_t first_line = at.b * p.chunks * p.channels + at.channel;  // of the first chunk
     if (at.inside) {  // a lane that stands for no channel keeps zeros: it adds nothing to the sums over channels
         if (p.state != nullptr) LoadStates<NPL>(p.state + of_state, n0, p.states, first);
-        for (int j = 0; j < at.chunk; ++j) {
-            float from[NPL];
-            LoadStates<NPL>(p.ends + first_line * p.states + j * per_chunk, n0, p.states, from);
-            const float dt = p.steps[first_line + static_cast<int64_t>(j) * p.channels];
-#pragma unroll
-            for (int i = 0; i < NPL; ++i) first[i] = __builtin_fmaf(__builtin_amdgcn_exp2f(dt * a[i]), first[i], from[i]);
-        }
+        ThroughChunks<NPL>(first, a, p.ends + first_line * p.states, p.steps + first_line, at.chunk, 1, per_chunk, p.channels, n0, p.states);
         if (pg.gnew != nullptr) LoadStates<NPL>(pg.gnew + of_state, n0, p.states, q);
-        for (int j = p.chunks - 1; j > at.chunk; --j) {
-            float from[NPL];
-            LoadStates<NPL>(pg.starts + first_line * p.states + j * per_chunk, n0, p.states, from);
-            const float dt = p.steps[first_line + static_cast<int64_t>(j) * p.channels];
-#pragma unroll
-            for (int i = 0; i < NPL; ++i) q[i] = __builtin_fmaf(__builtin_amdgcn_exp2f(dt * a[i]), q[i], from[i]);
-        }
+        const int64_t last_line = first_line + static_cast<int64_t>(p.chunks - 1) * p.channels;
+        ThroughChunks<NPL>(q, a, pg.starts + last_line * p.states, p.steps + last_line, p.chunks - 1 - at.chunk, -1, per_chunk, p.channels, n0, p.states);
     }
     const float* const states = pg.states + (at.b * pg.tiles * p.channels + at.channel) * NP + n0;
     const float* const passed = pg.passed + at.b * pg.tiles * p.channels + at.channel;
