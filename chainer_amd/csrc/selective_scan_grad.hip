@@ -56,9 +56,14 @@ template <typename T, int ROWS>
 __device__ __forceinline__ void ScanSteps(const ScanArgs& p, const TileRows<T, ROWS>& us, const TileRows<T, ROWS>& ds, int q, int rows, float bias, float (&dt)[ROWS / 4],
                                           float (&x)[ROWS / 4]) {
 #pragma unroll
+    for (int g = 0; g < ROWS / 4; ++g) dt[g] = ds.Held(g) + bias;
+    if (p.softplus != 0) {
+#pragma unroll
+        for (int g = 0; g < ROWS / 4; ++g) dt[g] = SoftplusOf(dt[g]);
+    }
+#pragma unroll
     for (int g = 0; g < ROWS / 4; ++g) {
-        const float raw = ds.Held(g) + bias;
-        dt[g] = 4 * g + q < rows ? (p.softplus != 0 ? SoftplusOf(raw) : raw) : 0.f;
+        dt[g] = 4 * g + q < rows ? dt[g] : 0.f;
         x[g] = dt[g] * us.Held(g);
     }
 }
@@ -214,14 +219,23 @@ __global__ __launch_bounds__(256) void SelectiveScanGradKernel(ScanGradArgs pg) 
     }
     for (int64_t t = top; t >= t0; t -= kTile, buffer ^= 1) {
         const int rows = static_cast<int>(std::min<int64_t>(last - t, kTile)), own_rows = at.inside ? rows : 0;
-        float u[kGroups], dt[kGroups], x[kGroups], g0[kGroups], gy[kGroups], slope[kGroups], z[kGroups];
+        float u[kGroups], dt[kGroups], x[kGroups], g0[kGroups], slope[kGroups];
         ScanSteps(p, us, ds, at.q, own_rows, bias, dt, x);
-        float h[kTile + 1][NPL], e[kTile][NPL], gz[kGroups] = {}, gu[kGroups], gdelta[kGroups];
+        float h[kTile + 1][NPL], e[kTile][NPL], gz[kGroups], gu[kGroups], gdelta[kGroups];
+        float of_y[kGroups];  // gz is the sum over states times this
 #pragma unroll
-        for (int g = 0; g < kGroups; ++g) {
-            u[g] = us.Held(g), g0[g] = gy[g] = gys.Held(g), z[g] = zs.Held(g);
-            slope[g] = p.softplus != 0 ? LogisticOf(ds.Held(g) + bias) : 1.f;
-            if (gated) g0[g] *= z[g] * LogisticOf(z[g]);
+        for (int g = 0; g < kGroups; ++g) u[g] = us.Held(g), g0[g] = gys.Held(g), slope[g] = 1.f, of_y[g] = 0.f;
+        if (p.softplus != 0) {
+#pragma unroll
+            for (int g = 0; g < kGroups; ++g) slope[g] = LogisticOf(ds.Held(g) + bias);
+        }
+        if (gated) {
+#pragma unroll
+            for (int g = 0; g < kGroups; ++g) {
+                const float z = zs.Held(g), l = LogisticOf(z);
+                of_y[g] = g0[g] * l * __builtin_fmaf(z, 1.f - l, 1.f);
+                g0[g] *= z * l;
+            }
         }
 #pragma unroll
         for (int i = 0; i < NPL; ++i) h[0][i] = __builtin_fmaf(__builtin_amdgcn_exp2f(next_passed * a[i]), first[i], next[i]);
@@ -245,10 +259,7 @@ __global__ __launch_bounds__(256) void SelectiveScanGradKernel(ScanGradArgs pg) 
             step(std::integral_constant<int, 1>{});
             step(std::integral_constant<int, 2>{});
             step(std::integral_constant<int, 3>{});
-            if (gated) {
-                const float y0 = __builtin_fmaf(d, u[g], QuadTransposedSum(y, at.q)), l = LogisticOf(z[g]);
-                gz[g] = gy[g] * y0 * l * __builtin_fmaf(z[g], 1.f - l, 1.f);
-            }
+            gz[g] = of_y[g] * __builtin_fmaf(d, u[g], QuadTransposedSum(y, at.q));
         }
 #pragma unroll
         for (int g = kGroups - 1; g >= 0; --g) {
