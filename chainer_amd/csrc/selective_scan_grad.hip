@@ -331,22 +331,26 @@ __global__ __launch_bounds__(256) void SelectiveScanGradKernel(ScanGradArgs pg) 
     if (at.q == 0) parts[p.states] = gd, parts[p.states + 1] = gbias;
 }
 
-// gb and gc: the workgroups along a group's channels added up, an element to a thread.
+// gb and gc: the workgroups along a group's channels added up.  A workgroup takes as many rows as it has threads for, an element to a thread.
 template <typename T>
 __global__ __launch_bounds__(256) void ScanSharedSumKernel(const float* parts, SequenceLengths lengths, int64_t batch, int64_t length, int groups, int group_blocks, int states,
                                                           T* gb, T* gc, int64_t first) {
-    const int64_t index = first + static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-    const int n = static_cast<int>(index % states);
-    const int64_t rest = index / states;
-    const int of = static_cast<int>(rest % 2), group = static_cast<int>(rest / 2 % groups);
-    const int64_t line = rest / 2 / groups;
-    if (line >= batch * length) return;
+    const int width = 2 * states, rows = 256 / width, row = static_cast<int>(threadIdx.x) / width, within = static_cast<int>(threadIdx.x) - row * width;
+    const int64_t at = (first + blockIdx.x) * rows + row;  // a sequence's row, a group
+    if (row >= rows || at >= batch * length * groups) return;
     float s = 0.f;
-    if (line % length < LengthOf(lengths, line / length, length)) {
-        const float* const from = parts + (((line * groups + group) * group_blocks) * 2 + of) * states + n;
-        for (int i = 0; i < group_blocks; ++i) s += from[static_cast<int64_t>(i) * 2 * states];
+    bool counts = true;
+    if (lengths.data != nullptr) {
+        const int64_t line = at / groups;
+        counts = line % length < LengthOf(lengths, line / length, length);
     }
-    (of == 0 ? gb : gc)[(line * groups + group) * states + n] = static_cast<T>(s);
+    if (counts) {
+        const float* const from = parts + at * group_blocks * width + within;
+#pragma unroll 8
+        for (int i = 0; i < group_blocks; ++i) s += from[static_cast<int64_t>(i) * width];
+    }
+    const bool of_b = within < states;
+    (of_b ? gb : gc)[at * states + (of_b ? within : within - states)] = static_cast<T>(s);
 }
 
 // ga, gd and gbias: the sequences and chunks added up, four threads to a column.
@@ -452,11 +456,13 @@ int hipcx_selective_scan_grad(const hipcx_array* u, const hipcx_array* delta, co
                 CheckLaunch(what.c_str());
             }
             const int groups = b->ndim == 4 ? static_cast<int>(b->shape[2]) : 1;
-            ForLaunches(s.batch * s.length * groups * 2 * s.states, [&](dim3 grid, int64_t first) {
+            const int64_t per_block = 256 / (2 * s.states), sum_blocks = (s.batch * s.length * groups + per_block - 1) / per_block;
+            for (int64_t from = 0; from < sum_blocks; from += kBlocksPerLaunch) {
+                const dim3 grid(static_cast<unsigned>(std::min(sum_blocks - from, kBlocksPerLaunch)));
                 hipLaunchKernelGGL(ScanSharedSumKernel<T>, grid, dim3(256), 0, AsStream(stream), p.shared_parts, s.lengths, s.batch, s.length, groups, s.group_blocks,
-                                   s.states, static_cast<T*>(gb->data), static_cast<T*>(gc->data), first);
+                                   s.states, static_cast<T*>(gb->data), static_cast<T*>(gc->data), from);
                 CheckLaunch(what.c_str());
-            });
+            }
         });
         const int64_t columns = static_cast<int64_t>(s.channels) * (s.states + 2);
         if (columns == 0) return;
