@@ -91,6 +91,9 @@ struct ConvPart {
     }
 };
 
+// Bound by memory: x read once and y written once, beside taps - 1 rows of the chunk before.  A thread keeps its window in registers and walks down the rows of 16 bytes of
+// channels, kAhead of whose loads are in flight.  A batch of 16 x 2048 x 4096 float16, four taps, SiLU: 109 us, 4.9 TB/s; with sequences half as long on average 90.  kAhead of 8:
+// 110 and 94.  One token of 1300 channels 4.8 us, a launch and two trips to memory.
 constexpr int kAhead = 4;      // rows whose loads are issued together
 constexpr int kFewestRows = 8; // to a chunk, taps - 1 at least
 
@@ -154,7 +157,9 @@ __global__ __launch_bounds__(256, K <= 4 ? 4 : 2) void CausalConvKernel(ConvArgs
 }
 
 // gp = gy act'(sum) where a row counts, else 0.  The gradient of input row i (state and x behind it) is w[k] gp[i - k] summed over the taps: a thread
-// goes through its rows and taps - 1 more, computes every sum again from x, and is done with input row i as soon as it has gp[i].
+// goes through its rows and taps - 1 more, computes every sum again from x, and is done with input row i as soon as it has gp[i].  Bound by memory, x and gy in and gx out:
+// 8 x 2048 x 2048 float16 49 us, 4.1 TB/s, of float32 89 us, 4.5.  Registers decide: 128 of them, four waves, where the compiler has no reason to hold more (blocks of
+// rows with masks instead of single ones at the ends: 150 to 180, 62 to 69 us; held to 128 it spills in the rows, 300 to 490).
 template <typename T, int K, int E>
 __global__ __launch_bounds__(256, K <= 4 ? 4 : 2) void CausalConvGradKernel(ConvArgs p) {
     using P = Piece<T, E>;

@@ -440,7 +440,8 @@ int hipcx_softmax_cross_entropy(const hipcx_array* x, const hipcx_array* t, cons
 /* ---- layers of a recurrent block: additions to the reference, whose links are LSTM, GRU and RNN (chainer/links/rnn) ----
  * Arrays are [batch, time, ...] and may be parts of wider ones: the last axis is dense, the others have any strides.  `lengths` (int32 or int64 [batch], or
  * NULL): the rows that each sequence of a padded batch has, taken as 0 or as all rows where they lie outside; later rows are not looked at and give zeros, and the
- * new state is the one behind the sequence's last row (the given one, of a sequence without rows).  A state that is NULL is zeros.  new_state may be state. */
+ * new state is the one behind the sequence's last row (the given one, of a sequence without rows).  A state that is NULL is zeros.  Results share
+ * no memory with each other or with the inputs, but for new_state, which may be state. */
 enum hipcx_activation { HIPCX_ACTIVATION_NONE = 0, HIPCX_ACTIVATION_SILU = 1 };
 
 /* hipcx_dropout: Dropout (chainer/functions/noise/dropout.py, y = x * mask / (1 - ratio)) whose mask is drawn from the counter-based generator
@@ -469,7 +470,7 @@ int hipcx_causal_conv_grad(const hipcx_array* x, const hipcx_array* w, const hip
  *   with dt = delta + delta_bias, or log(1 + exp(delta + delta_bias)) with delta_softplus; h[-1] is `state`, new_state the last h; d and delta_bias (zeros) and z (no gate)
  *   may be NULL.  u, delta, z, y [batch, time, channels]; b, c [batch, time, states] or [batch, time, groups, states], a group for channels / groups neighbours:
  *   float16 or float32.  a [channels, states], d, delta_bias [channels], state, new_state [batch, channels, states]: float32, C-contiguous.  1 to 64 states, of
- *   float32.
+ *   float32; rows less than 2^26 elements apart.
  * hipcx_selective_scan_grad: the gradients of all that was given, from gy and gnew_state (or NULL, zeros); gz goes with z, gd, gdelta_bias and gstate may be NULL.
  *   ga, gb, gc, gd, gdelta_bias, gnew_state and gstate are C-contiguous.  The states are computed again; sums run in float32 in an order that depends on the sizes
  *   alone. */
