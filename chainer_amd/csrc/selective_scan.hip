@@ -10,12 +10,13 @@ namespace {
 // h -> exp(a * sum of dt) h + what the chunk makes of zeros.  So ENDS runs the chunks but the last from zeros, without outputs, and the second launch runs all of them
 // from the states that it puts together on the way.  Rows go by in tiles of 16, whose b and c lie in LDS; a lane reads u, delta and z of every fourth row
 // of its channel, prepares dt, dt u and the gate once, and hands them to the quad's other lanes.
-// Bound by the vector units.  A state costs a row an exponential (8 cycles of a wave) and four instructions of 4 cycles: 82 us for 16384 rows of 2048 channels and 16 states, four
-// times what their memory traffic takes at 4.9 TB/s (55).  Beside a row's 20 instructions on states there are 17, for softplus, the gate, the sum over the quad, loads and
+// Bound by the vector units.  A state costs a row an exponential (8 cycles of a wave) and four instructions of 4 cycles: 82 us for 16384 rows of 2048 channels and 16 states,
+// whose memory traffic takes 55 at 4.9 TB/s.  Beside a row's 20 instructions on states there are 17, for softplus, the gate, the sum over the quad, loads and
 // LDS.  32 sequences of 2048 rows and channels, float16: 590 to 630 us, 170 to 185 cycles a row of 16 channels, 77 % of the issue slots taken.  One sequence of 16384 rows: 118 us from zeros,
-// 165 to 195 with outputs.  Four lanes to a channel: one would leave a quarter of the waves, and what they share is done once either way.
+// 160 to 195 with outputs.  Four lanes to a channel: one would leave a quarter of the waves, and what they share is done once either way.
+// Five waves to a SIMD (at 96 registers; the compiler would take 104): 282 -> 276 us for that sequence, 626 -> 640 for the 32, which fill four.
 template <typename T, int NPL, bool ENDS>
-__global__ __launch_bounds__(256) void SelectiveScanKernel(ScanArgs p) {
+__global__ __launch_bounds__(256, NPL <= 4 ? 5 : 1) void SelectiveScanKernel(ScanArgs p) {
     constexpr int NP = 4 * NPL;
     __shared__ float bs[2][kScanTile][NP], cs[ENDS ? 1 : 2][ENDS ? 1 : kScanTile][NP];
     const ScanPlace at(p, blockIdx.x, ENDS ? p.chunks - 1 : p.chunks);
