@@ -236,6 +236,9 @@ void VisitScan(int dtype, int states, F&& f) {
     else visit(Tag<float>{});
 }
 
+// [batch, time, ...] as TileRows reads it; of a single row, whatever its stride says of the next.
+SequenceRows ScanRowsOf(const hipcx_array* a, const std::string& what);
+
 // Cuts the time axis into chunks of `least` tiles or more, for `each` workgroups to a compute unit, where sequences and channels alone do not give it `enough`.
 void CutScan(ScanArgs* p, int enough, int each, int least);
 

@@ -217,6 +217,13 @@ struct ScanWorkspace {
 
 }  // namespace
 
+SequenceRows ScanRowsOf(const hipcx_array* a, const std::string& what) {
+    SequenceRows r = RowsOf(a, what.c_str());
+    if (a != nullptr && a->shape[1] <= 1) r.row = 0;
+    HIPCX_REQUIRE(std::abs(r.row) < kMaxScanRow, HIPCX_NOT_IMPLEMENTED_ERROR, what + ": rows 2^26 elements apart or more");
+    return r;
+}
+
 ScanArgs DescribeScan(const std::string& what, const hipcx_array* u, const hipcx_array* delta, const hipcx_array* a, const hipcx_array* b, const hipcx_array* c,
                       const hipcx_array* d, const hipcx_array* z, const hipcx_array* delta_bias, int delta_softplus, const hipcx_array* state,
                       const hipcx_array* lengths) {
@@ -246,15 +253,12 @@ ScanArgs DescribeScan(const std::string& what, const hipcx_array* u, const hipcx
     RequireShape(state, {batch, channels, states}, HIPCX_FLOAT32, what + ": state");
     for (const hipcx_array* s : {a, d, delta_bias, state}) RequireDense(s, what + ": a, d, delta_bias and state");
     ScanArgs p{};
-    for (const hipcx_array* s : {u, delta, z, b, c}) {
-        HIPCX_REQUIRE(s == nullptr || std::abs(s->strides[1]) < kMaxScanRow * ItemSize(s->dtype), HIPCX_NOT_IMPLEMENTED_ERROR, what + ": rows 2^26 elements apart or more");
-    }
-    p.u = RowsOf(u, "u"), p.delta = RowsOf(delta, "delta"), p.z = RowsOf(z, "z");
+    p.u = ScanRowsOf(u, what + ": u"), p.delta = ScanRowsOf(delta, what + ": delta"), p.z = ScanRowsOf(z, what + ": z");
     const auto shared = [&](const hipcx_array* s, const char* name) {
-        const SequenceRows r = RowsOf(s, name);
+        const SequenceRows r = ScanRowsOf(s, what + name);
         return ScanShared{r.data, r.batch, r.row, s->ndim == 4 ? s->strides[2] / ItemSize(s->dtype) : 0};
     };
-    p.b = shared(b, "b"), p.c = shared(c, "c");
+    p.b = shared(b, ": b"), p.c = shared(c, ": c");
     const auto floats = [](const hipcx_array* s) { return s != nullptr ? static_cast<const float*>(s->data) : nullptr; };
     p.a = floats(a), p.d = floats(d), p.bias = floats(delta_bias), p.state = floats(state);
     p.lengths = LengthsOf(lengths, batch, what);
@@ -289,8 +293,7 @@ int hipcx_selective_scan(const hipcx_array* u, const hipcx_array* delta, const h
         RequireShape(y, {p.batch, p.length, p.channels}, u->dtype, what + ": y");
         RequireShape(new_state, {p.batch, p.channels, p.states}, HIPCX_FLOAT32, what + ": new_state");
         RequireDense(new_state, what + ": new_state");
-        HIPCX_REQUIRE(std::abs(y->strides[1]) < kMaxScanRow * ItemSize(y->dtype), HIPCX_NOT_IMPLEMENTED_ERROR, what + ": rows 2^26 elements apart or more");
-        p.y = RowsOf(y, "y"), p.new_state = static_cast<float*>(new_state->data);
+        p.y = ScanRowsOf(y, what + ": y"), p.new_state = static_cast<float*>(new_state->data);
         if (p.batch == 0 || p.channels == 0) return;
         CutScan(&p, 2, 8, 2);
         const ScanWorkspace w(p);

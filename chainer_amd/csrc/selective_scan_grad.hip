@@ -435,10 +435,7 @@ int hipcx_selective_scan_grad(const hipcx_array* u, const hipcx_array* delta, co
         for (const hipcx_array* x : {gd, gdelta_bias}) RequireShape(x, {s.channels}, HIPCX_FLOAT32, what + ": gd and gdelta_bias");
         for (const hipcx_array* x : {gnew_state, gstate}) RequireShape(x, {s.batch, s.channels, s.states}, HIPCX_FLOAT32, what + ": gnew_state and gstate");
         for (const hipcx_array* x : {ga, gb, gc, gd, gdelta_bias, gnew_state, gstate}) RequireDense(x, what + ": ga, gb, gc, gd, gdelta_bias, gnew_state and gstate");
-        for (const hipcx_array* x : {gy, gu, gdelta, gz}) {
-            HIPCX_REQUIRE(x == nullptr || std::abs(x->strides[1]) < kMaxScanRow * ItemSize(x->dtype), HIPCX_NOT_IMPLEMENTED_ERROR, what + ": rows 2^26 elements apart or more");
-        }
-        p.gy = RowsOf(gy, "gy"), p.gu = RowsOf(gu, "gu"), p.gdelta = RowsOf(gdelta, "gdelta"), p.gz = RowsOf(gz, "gz");
+        p.gy = ScanRowsOf(gy, what + ": gy"), p.gu = ScanRowsOf(gu, what + ": gu"), p.gdelta = ScanRowsOf(gdelta, what + ": gdelta"), p.gz = ScanRowsOf(gz, what + ": gz");
         const auto floats = [](const hipcx_array* x) { return x != nullptr ? static_cast<float*>(x->data) : nullptr; };
         p.gnew = floats(gnew_state), p.gstate = floats(gstate);
         CutScanGrad(&p.s);

@@ -311,6 +311,20 @@ def test_selective_scan_of_sequences_far_apart(chx):
         assert (a is None) == (b is None) and (a is None or np.array_equal(a.get(), b.get()))
 
 
+def test_selective_scan_of_a_single_row_of_any_stride(chx):
+    """A unit axis' stride says nothing."""
+    c, more, _ = scan_case(2, 1, 70, 16, None, 'float16')
+    dev, gy = scan_on_device(chx, c, None, True), up(chx, more['gy'])
+    want, want_new = chx.selective_scan(**dev)
+    grads = chx.selective_scan_grad(gy=gy, **dev)
+    for far in (1 << 40, -(1 << 40), 0):
+        odd = dict(dev, **{k: chx.ndarray(dev[k]._buf, dev[k]._offset, dev[k].shape, (dev[k].strides[0], far, 2), dev[k].dtype) for k in ('u', 'delta', 'z', 'b', 'c')})
+        got, new = chx.selective_scan(**odd)
+        assert np.array_equal(got.get(), want.get()) and np.array_equal(new.get(), want_new.get())
+        for a, b in zip(chx.selective_scan_grad(gy=gy, **odd), grads):
+            assert (a is None) == (b is None) and (a is None or np.array_equal(a.get(), b.get()))
+
+
 @pytest.mark.parametrize('seed', range(10))
 def test_layers_of_drawn_sizes(chx, seed):
     rng = np.random.default_rng(1000 + seed)
