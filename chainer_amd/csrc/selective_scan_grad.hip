@@ -336,45 +336,55 @@ __global__ __launch_bounds__(256) void SelectiveScanGradKernel(ScanGradArgs pg) 
     if (at.q == 0) parts[p.states] = gd, parts[p.states + 1] = gbias;
 }
 
-// gb and gc: the workgroups along a group's channels added up.  A workgroup takes as many rows as it has threads for, an element to a thread.
-template <typename T>
-__global__ __launch_bounds__(256) void ScanSharedSumKernel(const float* parts, SequenceLengths lengths, int64_t batch, int64_t length, int groups, int group_blocks, int states,
-                                                          T* gb, T* gc, int64_t first) {
-    const int width = 2 * states, rows = 256 / width, row = static_cast<int>(threadIdx.x) / width, within = static_cast<int>(threadIdx.x) - row * width;
-    const int64_t at = (first + blockIdx.x) * rows + row;  // a sequence's row, a group
-    if (row >= rows || at >= batch * length * groups) return;
-    float s = 0.f;
-    bool counts = true;
-    if (lengths.data != nullptr) {
-        const int64_t line = at / groups;
-        counts = line % length < LengthOf(lengths, line / length, length);
-    }
-    if (counts) {
-        const float* const from = parts + at * group_blocks * width + within;
-#pragma unroll 8
-        for (int i = 0; i < group_blocks; ++i) s += from[static_cast<int64_t>(i) * width];
-    }
-    const bool of_b = within < states;
-    (of_b ? gb : gc)[at * states + (of_b ? within : within - states)] = static_cast<T>(s);
-}
+struct ScanSumArgs {
+    const float *shared, *channel;  // parts of gb and gc, of ga, gd and gbias
+    SequenceLengths lengths;
+    int64_t batch, length, shared_blocks, channel_parts, channels;
+    int groups, group_blocks, states;
+    void *gb, *gc;
+    float *ga, *gd, *gbias;  // gd and gbias: or null
+    int64_t first;           // the launch's first workgroup
+};
 
-// ga, gd and gbias: the sequences and chunks added up, four threads to a column.
-__global__ __launch_bounds__(256) void ScanChannelSumKernel(const float* parts, int64_t n_parts, int64_t channels, int states, float* ga, float* gd, float* gbias) {
+// Both kinds of partial sums in one launch.  gb and gc: the workgroups along a group's channels, as many rows to a workgroup as it has threads for, an element to a thread.  Behind them ga, gd and
+// gbias: the sequences and chunks, four threads to a column.
+template <typename T>
+__global__ __launch_bounds__(256) void ScanSumKernel(ScanSumArgs p) {
     __shared__ float sums[256];
-    const int64_t width = channels * (states + 2), at = static_cast<int64_t>(blockIdx.x) * 64 + (threadIdx.x & 63);
+    const int64_t block = p.first + blockIdx.x;
     float s = 0.f;
+    if (block < p.shared_blocks) {
+        const int width = 2 * p.states, rows = 256 / width, row = static_cast<int>(threadIdx.x) / width, within = static_cast<int>(threadIdx.x) - row * width;
+        const int64_t at = block * rows + row;  // a sequence's row, a group
+        if (row >= rows || at >= p.batch * p.length * p.groups) return;
+        bool counts = true;
+        if (p.lengths.data != nullptr) {
+            const int64_t line = at / p.groups;
+            counts = line % p.length < LengthOf(p.lengths, line / p.length, p.length);
+        }
+        if (counts) {
+            const float* const from = p.shared + at * p.group_blocks * width + within;
+#pragma unroll 8
+            for (int i = 0; i < p.group_blocks; ++i) s += from[static_cast<int64_t>(i) * width];
+        }
+        const bool of_b = within < p.states;
+        static_cast<T*>(of_b ? p.gb : p.gc)[at * p.states + (of_b ? within : within - p.states)] = static_cast<T>(s);
+        return;
+    }
+    const int64_t width = p.channels * (p.states + 2), at = (block - p.shared_blocks) * 64 + (threadIdx.x & 63);
     if (at < width) {
-        for (int64_t i = threadIdx.x >> 6; i < n_parts; i += 4) s += parts[i * width + at];
+#pragma unroll 4
+        for (int64_t i = threadIdx.x >> 6; i < p.channel_parts; i += 4) s += p.channel[i * width + at];
     }
     sums[threadIdx.x] = s;
     __syncthreads();
     if (threadIdx.x >= 64 || at >= width) return;
     const float all = (sums[threadIdx.x] + sums[threadIdx.x + 64]) + (sums[threadIdx.x + 128] + sums[threadIdx.x + 192]);
-    const int64_t channel = at / (states + 2);
-    const int n = static_cast<int>(at % (states + 2));
-    if (n < states) ga[channel * states + n] = all;
-    else if (n == states && gd != nullptr) gd[channel] = all;
-    else if (n > states && gbias != nullptr) gbias[channel] = all;
+    const int64_t channel = at / (p.states + 2);
+    const int n = static_cast<int>(at % (p.states + 2));
+    if (n < p.states) p.ga[channel * p.states + n] = all;
+    else if (n == p.states && p.gd != nullptr) p.gd[channel] = all;
+    else if (n > p.states && p.gbias != nullptr) p.gbias[channel] = all;
 }
 
 int GradTileOf(int states) { return states <= 8 ? 16 : states <= 16 ? 8 : 4; }
@@ -457,20 +467,19 @@ int hipcx_selective_scan_grad(const hipcx_array* u, const hipcx_array* delta, co
                 hipLaunchKernelGGL((SelectiveScanGradKernel<T, NPL>), dim3(static_cast<unsigned>(blocks)), dim3(256), 0, AsStream(stream), p);
                 CheckLaunch(what.c_str());
             }
-            const int groups = b->ndim == 4 ? static_cast<int>(b->shape[2]) : 1;
-            const int64_t per_block = 256 / (2 * s.states), sum_blocks = (s.batch * s.length * groups + per_block - 1) / per_block;
-            for (int64_t from = 0; from < sum_blocks; from += kBlocksPerLaunch) {
-                const dim3 grid(static_cast<unsigned>(std::min(sum_blocks - from, kBlocksPerLaunch)));
-                hipLaunchKernelGGL(ScanSharedSumKernel<T>, grid, dim3(256), 0, AsStream(stream), p.shared_parts, s.lengths, s.batch, s.length, groups, s.group_blocks,
-                                   s.states, static_cast<T*>(gb->data), static_cast<T*>(gc->data), from);
+            ScanSumArgs q{};
+            q.shared = p.shared_parts, q.channel = p.channel_parts, q.lengths = s.lengths;
+            q.batch = s.batch, q.length = s.length, q.channel_parts = s.batch * s.chunks, q.channels = s.channels;
+            q.groups = b->ndim == 4 ? static_cast<int>(b->shape[2]) : 1, q.group_blocks = s.group_blocks, q.states = s.states;
+            q.gb = gb->data, q.gc = gc->data, q.ga = floats(ga), q.gd = floats(gd), q.gbias = floats(gdelta_bias);
+            const int64_t rows = 256 / (2 * s.states);
+            q.shared_blocks = (s.batch * s.length * q.groups + rows - 1) / rows;
+            const int64_t sum_blocks = q.shared_blocks + (static_cast<int64_t>(s.channels) * (s.states + 2) + 63) / 64;
+            for (; q.first < sum_blocks; q.first += kBlocksPerLaunch) {
+                hipLaunchKernelGGL(ScanSumKernel<T>, dim3(static_cast<unsigned>(std::min(sum_blocks - q.first, kBlocksPerLaunch))), dim3(256), 0, AsStream(stream), q);
                 CheckLaunch(what.c_str());
             }
         });
-        const int64_t columns = static_cast<int64_t>(s.channels) * (s.states + 2);
-        if (columns == 0) return;
-        hipLaunchKernelGGL(ScanChannelSumKernel, dim3(static_cast<unsigned>((columns + 63) / 64)), dim3(256), 0, AsStream(stream), p.channel_parts, s.batch * s.chunks, s.channels, s.states,
-                           floats(ga), floats(gd), floats(gdelta_bias));
-        CheckLaunch(what.c_str());
     });
 }
 
