@@ -74,11 +74,10 @@ __device__ __forceinline__ void ScanSteps(const ScanArgs& p, const TileRows<T, R
 // exponential a tile instead of a run through the rows (444 -> 425 us in all).  Stored in every tile without a condition: in a branch they cost a third of the waves (152 registers for
 // 97, 137 us for 115 at 4 x 2048 rows of 2048 channels).  Bound by the vector units: seven instructions and an exponential a state, 44 instructions a row, 63 % of the issue slots.
 template <typename T, int NPL, bool CHUNKS>
-__global__ __launch_bounds__(256) void ScanGradStatesKernel(ScanGradArgs pg) {
+__device__ __forceinline__ void MakeTileStates(const ScanGradArgs& pg, const ScanPlace& at) {
     const ScanArgs& p = pg.s;
     constexpr int NP = 4 * NPL, kTile = kGradTile<NPL>;
     __shared__ float bs[2][kScanTile][NP], cs[CHUNKS ? 2 : 1][CHUNKS ? kScanTile : 1][NP];
-    const ScanPlace at(p, blockIdx.x, p.chunks);
     const int64_t len = LengthOf(p.lengths, at.b, p.length);
     const int64_t t0 = static_cast<int64_t>(at.chunk) * p.chunk_rows, last = std::min(std::min(t0 + p.chunk_rows, p.length), len);
     const int n0 = at.q * NPL;
@@ -160,16 +159,23 @@ __global__ __launch_bounds__(256) void ScanGradStatesKernel(ScanGradArgs pg) {
     if (at.q == 0) p.steps[line] = all_steps;
 }
 
-// A chunk from its last tile to its first: the tile's states again, in registers, from those that it starts from, and the gradients.
+template <typename T, int NPL, bool CHUNKS>
+__global__ __launch_bounds__(256) void ScanGradStatesKernel(ScanGradArgs pg) {
+    MakeTileStates<T, NPL, CHUNKS>(pg, ScanPlace(pg.s, blockIdx.x, pg.s.chunks));
+}
+
+// A chunk from its last tile to its first: the tile's states again, in registers, from those that it starts from, and the gradients.  STATES: sequences are whole, and their tiles'
+// states are made here too.
 // Bound by the vector units: 13 instructions and an exponential a state, the sums over channels (of two numbers a state and row; 18 % of the issue slots), 109 a row, 72 % of the issue slots at
 // two waves to a SIMD.  4 x 2048 rows of 2048 channels of 16 states, float16: 275 to 305 us; 32 sequences 1870 to 2060.  Tiles of 8 rows: 16 keep twice the states and decays, which
 // leaves one wave (588 us in all for 462), and held to three waves by fewer registers it spills (1140).  One barrier a tile, with LDS for two.
-template <typename T, int NPL>
+template <typename T, int NPL, bool STATES>
 __global__ __launch_bounds__(256) void SelectiveScanGradKernel(ScanGradArgs pg) {
     const ScanArgs& p = pg.s;
     constexpr int NP = 4 * NPL, kTile = kGradTile<NPL>, kGroups = kTile / 4;
     __shared__ float bs[2][kTile][NP], cs[2][kTile][NP], sums[2][4][kTile][2][NP];
     const ScanPlace at(p, blockIdx.x, p.chunks);
+    if constexpr (STATES) MakeTileStates<T, NPL, false>(pg, at);  // every thread reads what it has written itself
     const int64_t len = LengthOf(p.lengths, at.b, p.length);
     const int64_t t0 = static_cast<int64_t>(at.chunk) * p.chunk_rows, end = std::min(t0 + p.chunk_rows, p.length), last = std::min(end, len);
     const int n0 = at.q * NPL, lane = static_cast<int>(threadIdx.x) & 63, wave = static_cast<int>(threadIdx.x) >> 6;
@@ -461,10 +467,17 @@ int hipcx_selective_scan_grad(const hipcx_array* u, const hipcx_array* delta, co
             using T = typename decltype(tag)::type;
             constexpr int NPL = decltype(share)::value;
             if (blocks != 0) {
-                if (s.chunks > 1) hipLaunchKernelGGL((ScanGradStatesKernel<T, NPL, true>), dim3(static_cast<unsigned>(blocks)), dim3(256), 0, AsStream(stream), p);
-                else hipLaunchKernelGGL((ScanGradStatesKernel<T, NPL, false>), dim3(static_cast<unsigned>(blocks)), dim3(256), 0, AsStream(stream), p);
-                CheckLaunch(what.c_str());
-                hipLaunchKernelGGL((SelectiveScanGradKernel<T, NPL>), dim3(static_cast<unsigned>(blocks)), dim3(256), 0, AsStream(stream), p);
+                const dim3 grid(static_cast<unsigned>(blocks));
+                // Few whole sequences: a launch less counts for more than the tiles' states at the other kernel's waves.  us, two launches and one: 4 x 16 rows of 64 channels 51.5, 48.7,
+                // 20 x 35 of 650 51.8, 50.0; 128 x 35 of 650 and 8 states 97.7, 100.7, 32 x 2048 of 2048 3276, 3465.
+                if (s.chunks == 1 && blocks <= NumCUs()) {
+                    hipLaunchKernelGGL((SelectiveScanGradKernel<T, NPL, true>), grid, dim3(256), 0, AsStream(stream), p);
+                } else {
+                    if (s.chunks > 1) hipLaunchKernelGGL((ScanGradStatesKernel<T, NPL, true>), grid, dim3(256), 0, AsStream(stream), p);
+                    else hipLaunchKernelGGL((ScanGradStatesKernel<T, NPL, false>), grid, dim3(256), 0, AsStream(stream), p);
+                    CheckLaunch(what.c_str());
+                    hipLaunchKernelGGL((SelectiveScanGradKernel<T, NPL, false>), grid, dim3(256), 0, AsStream(stream), p);
+                }
                 CheckLaunch(what.c_str());
             }
             ScanSumArgs q{};

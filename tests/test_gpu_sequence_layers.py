@@ -245,6 +245,13 @@ def test_selective_scan_grad(chx, sizes, dtype):
 
 
 @pytest.mark.parametrize('dtype', ['float16', 'float32'])
+@pytest.mark.parametrize('sizes', [(300, 18, 5, 16, None), (260, 9, 6, 3, 2), (131, 21, 190, 24, 1), (258, 17, 3, 64, None)])
+def test_selective_scan_grad_many_short(chx, sizes, dtype):
+    """More workgroups than compute units, whole sequences each: the tiles' states come from a launch of their own."""
+    test_selective_scan_grad(chx, sizes, dtype)
+
+
+@pytest.mark.parametrize('dtype', ['float16', 'float32'])
 @pytest.mark.parametrize('channels,states', [(19, 16), (33, 6), (4, 64)])
 def test_selective_scan_pieces_and_tokens(chx, channels, states, dtype):
     """A sequence in pieces and token by token, the state moved forward in place, is the sequence at once."""
