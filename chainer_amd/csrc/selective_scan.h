@@ -3,6 +3,8 @@
 // for every sequence and channel; dt = delta + bias, or softplus of it.  b and c belong to a group of channels.
 #pragma once
 
+#include <cfloat>
+
 #include "sequence.h"
 
 namespace hipcx {
@@ -76,6 +78,16 @@ __device__ __forceinline__ void LoadStates(const float* p, int n0, int all, floa
     } else {
 #pragma unroll
         for (int i = 0; i < NPL; ++i) v[i] = n0 + i < all ? p[n0 + i] : 0.f;
+    }
+}
+// Exponents to base 2 of a step of 1.  -inf (a = -exp(a_log) overflows to it) as the lowest number: rows without a step, behind a sequence's last, multiply by exp(0) then, not by NaN.
+template <int NPL>
+__device__ __forceinline__ void LoadExponents(const float* p, int n0, int all, float (&a)[NPL]) {
+    LoadStates<NPL>(p, n0, all, a);
+#pragma unroll
+    for (int i = 0; i < NPL; ++i) {
+        a[i] *= kLog2E;
+        a[i] = a[i] < -FLT_MAX ? -FLT_MAX : a[i];  // (NaN stays)
     }
 }
 template <int NPL>

@@ -24,9 +24,9 @@ __global__ __launch_bounds__(256, NPL <= 4 ? 5 : 1) void SelectiveScanKernel(Sca
     const int64_t t0 = static_cast<int64_t>(at.chunk) * p.chunk_rows, end = std::min(t0 + p.chunk_rows, p.length), last = std::min(end, len);
     const int n0 = at.q * NPL;
     float a[NPL], h[NPL];
-    LoadStates<NPL>(p.a + static_cast<int64_t>(at.channel) * p.states, n0, p.states, a);
+    LoadExponents<NPL>(p.a + static_cast<int64_t>(at.channel) * p.states, n0, p.states, a);
 #pragma unroll
-    for (int i = 0; i < NPL; ++i) a[i] *= kLog2E, h[i] = 0.f;
+    for (int i = 0; i < NPL; ++i) h[i] = 0.f;
     const int64_t of_state = (at.b * p.channels + at.channel) * p.states, per_chunk = static_cast<int64_t>(p.channels) * p.states;
     float* const ends = p.ends + (at.b * p.chunks * p.channels + at.channel) * p.states;
     const float* const steps = p.steps + at.b * (p.chunks - 1) * p.channels + at.channel;
@@ -144,7 +144,7 @@ __global__ __launch_bounds__(256) void ScanTokenKernel(ScanArgs p, int64_t first
     const int channel = static_cast<int>(line % p.channels), group = channel / p.group_channels, n0 = (static_cast<int>(threadIdx.x) & 3) * NPL;
     float h[V][NPL], a[NPL], bs[V][NPL], cs[V][NPL], u[V], raw[V], z[V];
     bool counts[V];
-    LoadStates<NPL>(p.a + static_cast<int64_t>(channel) * p.states, n0, p.states, a);
+    LoadExponents<NPL>(p.a + static_cast<int64_t>(channel) * p.states, n0, p.states, a);
     const float bias = p.bias != nullptr ? p.bias[channel] : 0.f, d = p.d != nullptr ? p.d[channel] : 0.f;
 #pragma unroll
     for (int v = 0; v < V; ++v) {
@@ -171,7 +171,7 @@ __global__ __launch_bounds__(256) void ScanTokenKernel(ScanArgs p, int64_t first
         float sum = 0.f;
 #pragma unroll
         for (int i = 0; i < NPL; ++i) {
-            const float next = __builtin_fmaf(x, bs[v][i], __builtin_amdgcn_exp2f(dt * (a[i] * kLog2E)) * h[v][i]);
+            const float next = __builtin_fmaf(x, bs[v][i], __builtin_amdgcn_exp2f(dt * a[i]) * h[v][i]);
             h[v][i] = counts[v] ? next : h[v][i];
             sum = n0 + i < p.states ? __builtin_fmaf(cs[v][i], next, sum) : sum;
         }

@@ -83,9 +83,9 @@ __device__ __forceinline__ void MakeTileStates(const ScanGradArgs& pg, const Sca
     const int n0 = at.q * NPL;
     const int64_t per_tile = static_cast<int64_t>(p.channels) * NP;
     float a[NPL], h[NPL], start[NPL], decay[NPL];
-    LoadStates<NPL>(p.a + static_cast<int64_t>(at.channel) * p.states, n0, p.states, a);
+    LoadExponents<NPL>(p.a + static_cast<int64_t>(at.channel) * p.states, n0, p.states, a);
 #pragma unroll
-    for (int i = 0; i < NPL; ++i) a[i] *= kLog2E, h[i] = start[i] = 0.f, decay[i] = 1.f;
+    for (int i = 0; i < NPL; ++i) h[i] = start[i] = 0.f, decay[i] = 1.f;
     const float bias = p.bias != nullptr ? p.bias[at.channel] : 0.f;
     const bool gated = CHUNKS && p.z.data != nullptr;
     const int64_t first_tile = (at.b * pg.tiles + t0 / kTile) * p.channels + at.channel;
@@ -181,9 +181,9 @@ __global__ __launch_bounds__(256) void SelectiveScanGradKernel(ScanGradArgs pg) 
     const int n0 = at.q * NPL, lane = static_cast<int>(threadIdx.x) & 63, wave = static_cast<int>(threadIdx.x) >> 6;
     const int64_t of_state = (at.b * p.channels + at.channel) * p.states, per_chunk = static_cast<int64_t>(p.channels) * p.states;
     float a[NPL], q[NPL], ga[NPL], first[NPL];  // first: the state that the chunk starts from
-    LoadStates<NPL>(p.a + static_cast<int64_t>(at.channel) * p.states, n0, p.states, a);
+    LoadExponents<NPL>(p.a + static_cast<int64_t>(at.channel) * p.states, n0, p.states, a);
 #pragma unroll
-    for (int i = 0; i < NPL; ++i) a[i] *= kLog2E, q[i] = ga[i] = first[i] = 0.f;
+    for (int i = 0; i < NPL; ++i) q[i] = ga[i] = first[i] = 0.f;
     const float bias = p.bias != nullptr ? p.bias[at.channel] : 0.f, d = p.d != nullptr ? p.d[at.channel] : 0.f;
     const int64_t first_line = at.b * p.chunks * p.channels + at.channel;  // of the first chunk
     if (at.inside) {  // a lane that stands for no channel keeps zeros: it adds nothing to the sums over channels

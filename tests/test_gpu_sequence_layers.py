@@ -251,6 +251,33 @@ def test_selective_scan_grad_many_short(chx, sizes, dtype):
     test_selective_scan_grad(chx, sizes, dtype)
 
 
+@pytest.mark.parametrize('batch,length,ragged', [(2, 1, False), (3, 21, False), (3, 150, True), (1, 300, False), (300, 5, False)])
+def test_selective_scan_forgetting_states(chx, batch, length, ragged):
+    """A state whose decay is exp(-inf), what a = -exp(a_log) overflows to, holds its last row alone: rows and chunks behind the last one change nothing."""
+    c, more, lengths = scan_case(batch, length, 9, 16, None, 'float32', seed=1, ragged=ragged)
+    c['a'][3], c['a'][:, 5], c['a'][7, 2] = -np.inf, -np.inf, -3e38
+    finite = dict(c, a=np.maximum(c['a'], np.float32(-1e30)))  # the same decays, 0, and no product of 0 and inf; every step is above 1e-4
+    results = []
+    for v in (c, finite):
+        dev = scan_on_device(chx, v, lengths, True)
+        y, new = chx.selective_scan(**dev)
+        grads = chx.selective_scan_grad(gy=apart(chx, more['gy']), gnew_state=up(chx, more['gnew']), **dev)
+        results.append(dict(grads._asdict(), y=y, new=new))
+    for k, got in results[0].items():
+        assert np.isfinite(got.get()).all(), k
+        assert np.array_equal(got.get(), results[1][k].get()), k
+    ends = ref.ends_of(lengths, batch, length)
+    for b in range(batch):
+        if ends[b] == 0:
+            assert np.array_equal(new.get()[b], c['state'][b])
+            continue
+        t = ends[b] - 1
+        raw = c['delta'][b, t].astype(np.float64) + c['delta_bias']
+        want = np.log1p(np.exp(raw)) * c['u'][b, t] * c['b'][b, t, 5]
+        # the softplus 9 and its argument's |raw|, as in the plain form's bound; two products, and a sum with 0
+        assert (np.abs(new.get()[b, :, 5] - want) <= (12 + np.abs(raw)) * ref.U32 * np.abs(want)).all()
+
+
 @pytest.mark.parametrize('dtype', ['float16', 'float32'])
 @pytest.mark.parametrize('channels,states', [(19, 16), (33, 6), (4, 64)])
 def test_selective_scan_pieces_and_tokens(chx, channels, states, dtype):
