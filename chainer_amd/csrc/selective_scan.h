@@ -70,20 +70,21 @@ struct __attribute__((packed, aligned(4))) LaneStates {
     float v[NPL];
 };
 template <int NPL>
-__device__ __forceinline__ void LoadStates(const float* p, int n0, int all, float (&v)[NPL]) {
+__device__ __forceinline__ void LoadStates(const float* p, int n0, int all, float (&v)[NPL], float padding = 0.f) {
     if (n0 + NPL <= all) {
         const LaneStates<NPL> s = *reinterpret_cast<const LaneStates<NPL>*>(p + n0);
 #pragma unroll
         for (int i = 0; i < NPL; ++i) v[i] = s.v[i];
     } else {
 #pragma unroll
-        for (int i = 0; i < NPL; ++i) v[i] = n0 + i < all ? p[n0 + i] : 0.f;
+        for (int i = 0; i < NPL; ++i) v[i] = n0 + i < all ? p[n0 + i] : padding;
     }
 }
 // Exponents to base 2 of a step of 1.  -inf (a = -exp(a_log) overflows to it) as the lowest number: rows without a step, behind a sequence's last, multiply by exp(0) then, not by NaN.
+// The padding's is next to 0 and below it: a finite step multiplies it by 2^-6 to 2^6, and an infinite one by 0, where exp(inf * 0) would make NaN of it and of the sums over states.
 template <int NPL>
 __device__ __forceinline__ void LoadExponents(const float* p, int n0, int all, float (&a)[NPL]) {
-    LoadStates<NPL>(p, n0, all, a);
+    LoadStates<NPL>(p, n0, all, a, -FLT_MIN);
 #pragma unroll
     for (int i = 0; i < NPL; ++i) {
         a[i] *= kLog2E;
@@ -103,6 +104,21 @@ __device__ __forceinline__ void StoreStates(float* p, int n0, int all, const flo
             if (n0 + i < all) p[n0 + i] = v[i];
         }
     }
+}
+
+// Fewer states than four lanes have room for, in a way that leaves no padding: a lane that has not enough of its own takes the last NPL states, one that has none takes the first ones, and a
+// state that is there several times counts by a fraction.  (More than two lanes have states of their own unless NPL is 1.)
+template <int NPL>
+__device__ __forceinline__ int FirstOfLane(int lane, int all) {
+    const int n0 = lane * NPL;
+    if (n0 < all) return n0 + NPL <= all ? n0 : all - NPL;
+    return NPL == 1 && all > 1 ? n0 - all : 0;
+}
+template <int NPL>
+__device__ __forceinline__ float ShareOf(int n, int all) {
+    if (NPL == 1) return all == 1 ? 0.25f : n < 4 - all ? 0.5f : 1.f;
+    const bool of_first = all <= 3 * NPL && n < NPL, of_last = n >= all - NPL && n < all / NPL * NPL && all % NPL != 0;
+    return of_first || of_last ? 0.5f : 1.f;
 }
 
 // s = exp(sum of dt) s + what the chunk adds, for `n` chunks one after another, `next` chunks apart (1 or -1): a state from the sequence's start to a chunk, or its gradient
@@ -181,19 +197,21 @@ struct TileRows {
 };
 constexpr int64_t kMaxScanRow = int64_t{1} << 26;  // elements from one row to the next: a tile and the channels fit those 32 bits
 
-// A tile of b, or of b and c, on its way to LDS: workgroups of 256 threads take an element each, or a few.
-template <typename T, int NPL, int ROWS, int PARTS>
+// A tile of b, or of b and c, on its way to LDS: workgroups of 256 threads take an element each, or a few.  REPEATS: states as FirstOfLane() deals them out, c times their share.
+template <typename T, int NPL, int ROWS, int PARTS, bool REPEATS = false>
 struct TileShared {
     static constexpr int kNP = 4 * NPL, kEach = (ROWS * kNP + 255) / 256;
     const T* from[PARTS][kEach];
     int64_t step[PARTS];
     bool is_state[kEach];
+    float share[kEach];
     T held[PARTS][kEach];
     __device__ __forceinline__ TileShared(const ScanArgs& p, const ScanPlace& at, int64_t t) {
 #pragma unroll
         for (int i = 0; i < kEach; ++i) {
-            const int e = i * 256 + static_cast<int>(threadIdx.x), r = e / kNP, n = e % kNP;
+            const int e = i * 256 + static_cast<int>(threadIdx.x), r = e / kNP, n = REPEATS ? FirstOfLane<NPL>(e % kNP / NPL, p.states) + e % NPL : e % kNP;
             is_state[i] = r < ROWS && n < p.states;
+            if constexpr (REPEATS) share[i] = ShareOf<NPL>(n, p.states);
 #pragma unroll
             for (int k = 0; k < PARTS; ++k) {
                 const ScanShared& s = k == 0 ? p.b : p.c;
@@ -228,7 +246,7 @@ struct TileShared {
 #pragma unroll
         for (int i = 0; i < kEach; ++i) {
             const int e = i * 256 + static_cast<int>(threadIdx.x);
-            if (e < ROWS * kNP) to[e / kNP][e % kNP] = static_cast<float>(held[K][i]);
+            if (e < ROWS * kNP) to[e / kNP][e % kNP] = REPEATS && K == 1 ? static_cast<float>(held[K][i]) * share[i] : static_cast<float>(held[K][i]);
         }
     }
 };

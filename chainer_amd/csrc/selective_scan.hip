@@ -6,6 +6,10 @@
 namespace hipcx {
 namespace {
 
+// Waves to a SIMD that the registers leave room for without spills in the rows.
+template <typename T, int NPL>
+constexpr int kScanWaves = NPL == 1 ? (sizeof(T) == 4 ? 7 : 6) : NPL <= 4 ? 5 : NPL == 8 ? 4 : 3;
+
 // A workgroup's part of the sequence: 64 channels, a chunk of rows.  Chunks that come after others need the state there, and a state goes through a chunk linearly:
 // h -> exp(a * sum of dt) h + what the chunk makes of zeros.  So ENDS runs the chunks but the last from zeros, without outputs, and the second launch runs all of them
 // from the states that it puts together on the way.  Rows go by in tiles of 16, whose b and c lie in LDS; a lane reads u, delta and z of every fourth row
@@ -15,14 +19,16 @@ namespace {
 // LDS.  32 sequences of 2048 rows and channels, float16: 590 to 630 us, 170 to 185 cycles a row of 16 channels, 77 % of the issue slots taken.  One sequence of 16384 rows: 118 us from zeros,
 // 160 to 195 with outputs.  Four lanes to a channel: one would leave a quarter of the waves, and what they share is done once either way.
 // Five waves to a SIMD (at 96 registers; the compiler would take 104): 282 -> 276 us for that sequence, 626 -> 640 for the 32, which fill four.
-template <typename T, int NPL, bool ENDS>
-__global__ __launch_bounds__(256, NPL <= 4 ? 5 : 1) void SelectiveScanKernel(ScanArgs p) {
+// REPEATS: fewer than 4 * NPL states, some of them twice.  Zeros in the room that is left, b = c = 0, become NaN where dt u is infinite, and with them sums that the states make infinite; to
+// leave them out of the sums takes a selection a state and row, and registers (48 states, 20 x 35 rows of 650 channels: 19.3 -> 21.6 us), while whole lanes of states are read at once.
+template <typename T, int NPL, bool ENDS, bool REPEATS>
+__global__ __launch_bounds__(256, (kScanWaves<T, NPL>)) void SelectiveScanKernel(ScanArgs p) {
     constexpr int NP = 4 * NPL;
     __shared__ float bs[2][kScanTile][NP], cs[ENDS ? 1 : 2][ENDS ? 1 : kScanTile][NP];
     const ScanPlace at(p, blockIdx.x, ENDS ? p.chunks - 1 : p.chunks);
     const int64_t len = LengthOf(p.lengths, at.b, p.length);
     const int64_t t0 = static_cast<int64_t>(at.chunk) * p.chunk_rows, end = std::min(t0 + p.chunk_rows, p.length), last = std::min(end, len);
-    const int n0 = at.q * NPL;
+    const int place = at.q * NPL, n0 = REPEATS ? FirstOfLane<NPL>(at.q, p.states) : place;  // the lane's states in LDS, and in memory
     float a[NPL], h[NPL];
     LoadExponents<NPL>(p.a + static_cast<int64_t>(at.channel) * p.states, n0, p.states, a);
 #pragma unroll
@@ -44,7 +50,7 @@ __global__ __launch_bounds__(256, NPL <= 4 ? 5 : 1) void SelectiveScanKernel(Sca
     float all_steps = 0.f;
     const float bias = p.bias != nullptr ? p.bias[at.channel] : 0.f, d = p.d != nullptr ? p.d[at.channel] : 0.f;
     TileRows<T, kScanTile> us(p.u, at, t0), ds(p.delta, at, t0), zs(p.z, at, t0), ys(p.y, at, t0);
-    TileShared<T, NPL, kScanTile, ENDS ? 1 : 2> shared(p, at, t0);
+    TileShared<T, NPL, kScanTile, ENDS ? 1 : 2, REPEATS> shared(p, at, t0);
     const bool gated = !ENDS && p.z.data != nullptr;
     const auto fetch = [&](int rows, auto whole) __attribute__((always_inline)) {
         constexpr bool kWhole = decltype(whole)::value;
@@ -69,8 +75,8 @@ __global__ __launch_bounds__(256, NPL <= 4 ? 5 : 1) void SelectiveScanKernel(Sca
 #pragma unroll
                 for (int i = 0; i < NPL; ++i) {
                     const float e = __builtin_amdgcn_exp2f(dts * a[i]);
-                    h[i] = __builtin_fmaf(xs, bs[buffer][4 * g + S][n0 + i], e * h[i]);
-                    if constexpr (!ENDS) sum = __builtin_fmaf(cs[buffer][4 * g + S][n0 + i], h[i], sum);
+                    h[i] = __builtin_fmaf(xs, bs[buffer][4 * g + S][place + i], e * h[i]);
+                    if constexpr (!ENDS) sum = __builtin_fmaf(cs[buffer][4 * g + S][place + i], h[i], sum);
                 }
                 sums[S] = sum;
             };
@@ -316,10 +322,12 @@ int hipcx_selective_scan(const hipcx_array* u, const hipcx_array* delta, const h
                 return;
             }
             if (p.chunks > 1) {
-                hipLaunchKernelGGL((SelectiveScanKernel<T, NPL, true>), dim3(static_cast<unsigned>(blocks - p.batch * p.blocks)), dim3(256), 0, AsStream(stream), p);
+                hipLaunchKernelGGL((SelectiveScanKernel<T, NPL, true, false>), dim3(static_cast<unsigned>(blocks - p.batch * p.blocks)), dim3(256), 0, AsStream(stream), p);
                 CheckLaunch("selective_scan");
             }
-            hipLaunchKernelGGL((SelectiveScanKernel<T, NPL, false>), dim3(static_cast<unsigned>(blocks)), dim3(256), 0, AsStream(stream), p);
+            const dim3 grid(static_cast<unsigned>(blocks));
+            if (p.states == 4 * NPL) hipLaunchKernelGGL((SelectiveScanKernel<T, NPL, false, false>), grid, dim3(256), 0, AsStream(stream), p);
+            else hipLaunchKernelGGL((SelectiveScanKernel<T, NPL, false, true>), grid, dim3(256), 0, AsStream(stream), p);
             CheckLaunch("selective_scan");
         });
     });
