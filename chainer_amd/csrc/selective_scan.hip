@@ -6,6 +6,33 @@
 namespace hipcx {
 namespace {
 
+// The state that a chunk starts from, which is behind `n` others.  A chunk's decay may leave float32's range where no row's does: nothing times infinity, and infinity times 0, are NaN then,
+// which the rows one by one do not make.  So whoever ends at infinity or NaN, where what made it stays, goes through the chunks once more, by the decay's root twice; a state of 0, and one of
+// infinity that decays, stay what they are.
+template <int NPL>
+__device__ __forceinline__ void StartOfChunk(float (&s)[NPL], const float (&a)[NPL], const float* state, const float* adds, const float* steps, int n, int64_t per_chunk, int64_t channels,
+                                             int n0, int states) {
+    LoadStates<NPL>(state, n0, states, s);
+    ThroughChunks<NPL>(s, a, adds, steps, n, 1, per_chunk, channels, n0, states);
+    bool finite = true;
+#pragma unroll
+    for (int i = 0; i < NPL; ++i) finite = finite && __builtin_fabsf(s[i]) <= FLT_MAX;
+    if (finite) return;
+    LoadStates<NPL>(state, n0, states, s);
+#pragma unroll 1
+    for (int j = 0; j < n; ++j) {
+        float add[NPL];
+        LoadStates<NPL>(adds + j * per_chunk, n0, states, add);
+        const float dt = steps[j * channels];
+#pragma unroll
+        for (int i = 0; i < NPL; ++i) {
+            const float exponent = dt * a[i], root = __builtin_amdgcn_exp2f(0.5f * exponent);
+            const bool stays = s[i] == 0.f || (__builtin_fabsf(s[i]) > FLT_MAX && __builtin_fabsf(exponent) <= FLT_MAX);
+            s[i] = (stays ? s[i] : s[i] * root * root) + add[i];
+        }
+    }
+}
+
 // Waves to a SIMD that the registers leave room for without spills in the rows.
 template <typename T, int NPL>
 constexpr int kScanWaves = NPL == 1 ? (sizeof(T) == 4 ? 7 : 6) : NPL <= 4 ? 5 : NPL == 8 ? 4 : 3;
@@ -44,8 +71,7 @@ __global__ __launch_bounds__(256, (kScanWaves<T, NPL>)) void SelectiveScanKernel
             for (int i = 0; i < NPL; ++i) h[i] = 0.f;
         }
     } else {
-        LoadStates<NPL>(ends, n0, p.states, h);
-        ThroughChunks<NPL>(h, a, ends + per_chunk, steps, at.chunk, 1, per_chunk, p.channels, n0, p.states);
+        StartOfChunk<NPL>(h, a, ends, ends + per_chunk, steps, at.chunk, per_chunk, p.channels, n0, p.states);
     }
     float all_steps = 0.f;
     const float bias = p.bias != nullptr ? p.bias[at.channel] : 0.f, d = p.d != nullptr ? p.d[at.channel] : 0.f;
