@@ -33,9 +33,11 @@ __device__ __forceinline__ void StartOfChunk(float (&s)[NPL], const float (&a)[N
     }
 }
 
-// Waves to a SIMD that the registers leave room for without spills in the rows.
-template <typename T, int NPL>
-constexpr int kScanWaves = NPL == 1 ? (sizeof(T) == 4 ? 7 : 6) : NPL <= 4 ? 5 : NPL == 8 ? 4 : 3;
+// Waves to a SIMD that the registers leave room for without spills in the rows.  9 to 16 states take 97 registers, which is four waves; held to 96, for a fifth, the rows take longer, so
+// that only launches of more than four workgroups to a compute unit are.  us with four (FEW) and five, 16 states, float16: one sequence of 16384 rows and 2048 channels 282, 276,
+// 4 x 2048 x 1024 83.4, 81.1; 16 x 2048 x 2048 397, 425, 32 x 2048 x 2048 632, 646.
+template <typename T, int NPL, bool FEW>
+constexpr int kScanWaves = NPL == 1 ? (sizeof(T) == 4 ? 7 : 6) : NPL <= 4 ? (FEW ? 4 : 5) : NPL == 8 ? 4 : 3;
 
 // A workgroup's part of the sequence: 64 channels, a chunk of rows.  Chunks that come after others need the state there, and a state goes through a chunk linearly:
 // h -> exp(a * sum of dt) h + what the chunk makes of zeros.  So ENDS runs the chunks but the last from zeros, without outputs, and the second launch runs all of them
@@ -45,11 +47,10 @@ constexpr int kScanWaves = NPL == 1 ? (sizeof(T) == 4 ? 7 : 6) : NPL <= 4 ? 5 : 
 // whose memory traffic takes 55 at 4.9 TB/s.  Beside a row's 20 instructions on states there are 17, for softplus, the gate, the sum over the quad, loads and
 // LDS.  32 sequences of 2048 rows and channels, float16: 590 to 630 us, 170 to 185 cycles a row of 16 channels, 77 % of the issue slots taken.  One sequence of 16384 rows: 118 us from zeros,
 // 160 to 195 with outputs.  Four lanes to a channel: one would leave a quarter of the waves, and what they share is done once either way.
-// Five waves to a SIMD (at 96 registers; the compiler would take 104): 282 -> 276 us for that sequence, 626 -> 640 for the 32, which fill four.
 // REPEATS: fewer than 4 * NPL states, some of them twice.  Zeros in the room that is left, b = c = 0, become NaN where dt u is infinite, and with them sums that the states make infinite; to
 // leave them out of the sums takes a selection a state and row, and registers (48 states, 20 x 35 rows of 650 channels: 19.3 -> 21.6 us), while whole lanes of states are read at once.
-template <typename T, int NPL, bool ENDS, bool REPEATS>
-__global__ __launch_bounds__(256, (kScanWaves<T, NPL>)) void SelectiveScanKernel(ScanArgs p) {
+template <typename T, int NPL, bool ENDS, bool REPEATS, bool FEW>
+__global__ __launch_bounds__(256, (kScanWaves<T, NPL, FEW>)) void SelectiveScanKernel(ScanArgs p) {
     constexpr int NP = 4 * NPL;
     __shared__ float bs[2][kScanTile][NP], cs[ENDS ? 1 : 2][ENDS ? 1 : kScanTile][NP];
     const ScanPlace at(p, blockIdx.x, ENDS ? p.chunks - 1 : p.chunks);
@@ -348,12 +349,16 @@ int hipcx_selective_scan(const hipcx_array* u, const hipcx_array* delta, const h
                 return;
             }
             if (p.chunks > 1) {
-                hipLaunchKernelGGL((SelectiveScanKernel<T, NPL, true, false>), dim3(static_cast<unsigned>(blocks - p.batch * p.blocks)), dim3(256), 0, AsStream(stream), p);
+                hipLaunchKernelGGL((SelectiveScanKernel<T, NPL, true, false, false>), dim3(static_cast<unsigned>(blocks - p.batch * p.blocks)), dim3(256), 0, AsStream(stream), p);
                 CheckLaunch("selective_scan");
             }
-            const dim3 grid(static_cast<unsigned>(blocks));
-            if (p.states == 4 * NPL) hipLaunchKernelGGL((SelectiveScanKernel<T, NPL, false, false>), grid, dim3(256), 0, AsStream(stream), p);
-            else hipLaunchKernelGGL((SelectiveScanKernel<T, NPL, false, true>), grid, dim3(256), 0, AsStream(stream), p);
+            const auto launch = [&](auto repeats, auto few) {
+                constexpr bool kRepeats = decltype(repeats)::value, kFew = decltype(few)::value;
+                hipLaunchKernelGGL((SelectiveScanKernel<T, NPL, false, kRepeats, kFew>), dim3(static_cast<unsigned>(blocks)), dim3(256), 0, AsStream(stream), p);
+            };
+            const auto with_states = [&](auto few) { p.states == 4 * NPL ? launch(std::false_type{}, few) : launch(std::true_type{}, few); };
+            if (NPL == 4 && blocks <= int64_t{NumCUs()} * 4) with_states(std::bool_constant<NPL == 4>{});
+            else with_states(std::false_type{});
             CheckLaunch("selective_scan");
         });
     });
