@@ -397,7 +397,7 @@ int hipcx_causal_conv(const hipcx_array* x, const hipcx_array* w, const hipcx_ar
 size_t hipcx_causal_conv_grad_workspace_size(const hipcx_array* x, const hipcx_array* w) {
     if (x == nullptr || w == nullptr || x->ndim != 3 || w->ndim != 2 || (x->dtype != HIPCX_FLOAT16 && x->dtype != HIPCX_FLOAT32)) return 0;
     const ConvSizes s(x, w);
-    if (s.batch <= 0 || s.channels <= 0) return 0;
+    if (s.batch <= 0 || s.channels <= 0 || w->shape[0] != s.channels || s.taps < 1 || s.taps > kMaxTaps) return 0;  // (none for what the call refuses)
     return static_cast<size_t>(s.GradParts() * (s.taps + 1) * s.channels) * sizeof(float);
 }
 

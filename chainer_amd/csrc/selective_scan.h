@@ -195,6 +195,7 @@ struct TileRows {
         asm("" : "+v"(offset));  // else a register for each group's offset is kept from tile to tile
     }
 };
+constexpr int64_t kMaxScanLength = int64_t{1} << 30, kMaxScanChannels = int64_t{1} << 24, kMaxScanStates = 64;
 constexpr int64_t kMaxScanRow = int64_t{1} << 26;  // elements from one row to the next: a tile and the channels fit those 32 bits
 
 // A tile of b, or of b and c, on its way to LDS: workgroups of 256 threads take an element each, or a few.  REPEATS: states as FirstOfLane() deals them out, c times their share.
@@ -271,6 +272,9 @@ SequenceRows ScanRowsOf(const hipcx_array* a, const std::string& what);
 
 // Cuts the time axis into chunks of `least` tiles or more, for `each` workgroups to a compute unit, where sequences and channels alone do not give it `enough`.
 void CutScan(ScanArgs* p, int enough, int each, int least);
+
+// The sizes that workspaces go by; false for what DescribeScan() refuses, which takes none.
+bool ScanSizesOf(const hipcx_array* u, const hipcx_array* a, ScanArgs* p);
 
 // Checks the inputs that the scan and its gradients share and describes them, except for the cut along time.
 ScanArgs DescribeScan(const std::string& what, const hipcx_array* u, const hipcx_array* delta, const hipcx_array* a, const hipcx_array* b, const hipcx_array* c,

@@ -257,6 +257,14 @@ SequenceRows ScanRowsOf(const hipcx_array* a, const std::string& what) {
     return r;
 }
 
+bool ScanSizesOf(const hipcx_array* u, const hipcx_array* a, ScanArgs* p) {
+    if (u == nullptr || a == nullptr || u->ndim != 3 || a->ndim != 2 || a->shape[0] != u->shape[2]) return false;
+    const int64_t batch = u->shape[0], length = u->shape[1], channels = u->shape[2], states = a->shape[1];
+    if (batch < 0 || length < 0 || length >= kMaxScanLength || channels < 0 || channels >= kMaxScanChannels || states < 1 || states > kMaxScanStates) return false;
+    p->batch = batch, p->length = length, p->channels = static_cast<int>(channels), p->states = static_cast<int>(states);
+    return true;
+}
+
 ScanArgs DescribeScan(const std::string& what, const hipcx_array* u, const hipcx_array* delta, const hipcx_array* a, const hipcx_array* b, const hipcx_array* c,
                       const hipcx_array* d, const hipcx_array* z, const hipcx_array* delta_bias, int delta_softplus, const hipcx_array* state,
                       const hipcx_array* lengths) {
@@ -268,10 +276,10 @@ ScanArgs DescribeScan(const std::string& what, const hipcx_array* u, const hipcx
     HIPCX_REQUIRE(u->ndim == 3, HIPCX_DIMENSION_ERROR, what + ": u must be [batch, time, channels], got " + ShapeStr(u));
     HIPCX_REQUIRE(a->ndim == 2 && a->shape[0] == u->shape[2], HIPCX_DIMENSION_ERROR, what + ": a must be [channels, states], got " + ShapeStr(a));
     const int64_t batch = u->shape[0], length = u->shape[1], channels = u->shape[2], states = a->shape[1];
-    HIPCX_REQUIRE(states >= 1 && states <= 64, HIPCX_NOT_IMPLEMENTED_ERROR, what + ": 1 to 64 states, got " + std::to_string(states));
-    HIPCX_REQUIRE(channels < (int64_t{1} << 24), HIPCX_NOT_IMPLEMENTED_ERROR, what + ": 2^24 channels or more");
+    HIPCX_REQUIRE(states >= 1 && states <= kMaxScanStates, HIPCX_NOT_IMPLEMENTED_ERROR, what + ": 1 to 64 states, got " + std::to_string(states));
+    HIPCX_REQUIRE(channels < kMaxScanChannels, HIPCX_NOT_IMPLEMENTED_ERROR, what + ": 2^24 channels or more");
     HIPCX_REQUIRE(b->ndim == 3 || b->ndim == 4, HIPCX_DIMENSION_ERROR, what + ": b must be [batch, time, states] or [batch, time, groups, states], got " + ShapeStr(b));
-    HIPCX_REQUIRE(length < (int64_t{1} << 30), HIPCX_NOT_IMPLEMENTED_ERROR, what + ": 2^30 rows or more");
+    HIPCX_REQUIRE(length < kMaxScanLength, HIPCX_NOT_IMPLEMENTED_ERROR, what + ": 2^30 rows or more");
     const int64_t groups = b->ndim == 4 ? b->shape[2] : 1;
     HIPCX_REQUIRE(groups >= 1 && channels % groups == 0, HIPCX_DIMENSION_ERROR, what + ": the groups of b must divide the channels");
     for (const hipcx_array* s : {b, c}) {
@@ -309,9 +317,8 @@ using namespace hipcx;
 extern "C" {
 
 size_t hipcx_selective_scan_workspace_size(const hipcx_array* u, const hipcx_array* a) {
-    if (u == nullptr || a == nullptr || u->ndim != 3 || a->ndim != 2 || u->shape[0] < 0 || u->shape[1] < 0 || u->shape[2] < 0) return 0;
     ScanArgs p{};
-    p.batch = u->shape[0], p.length = u->shape[1], p.channels = static_cast<int>(u->shape[2]), p.states = static_cast<int>(a->shape[1]);
+    if (!ScanSizesOf(u, a, &p)) return 0;
     CutScan(&p, 2, 8, 2);
     return ScanWorkspace(p).Bytes();
 }

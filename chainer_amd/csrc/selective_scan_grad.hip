@@ -420,12 +420,12 @@ using namespace hipcx;
 extern "C" {
 
 size_t hipcx_selective_scan_grad_workspace_size(const hipcx_array* u, const hipcx_array* a, const hipcx_array* b) {
-    if (u == nullptr || a == nullptr || b == nullptr || u->ndim != 3 || a->ndim != 2 || (b->ndim != 3 && b->ndim != 4)) return 0;
     ScanArgs p{};
+    if (!ScanSizesOf(u, a, &p) || b == nullptr || (b->ndim != 3 && b->ndim != 4)) return 0;
     const int64_t groups = b->ndim == 4 ? b->shape[2] : 1;
-    if (groups < 1 || u->shape[0] <= 0 || u->shape[2] <= 0 || u->shape[2] % groups != 0) return 0;
-    p.batch = u->shape[0], p.length = u->shape[1], p.channels = static_cast<int>(u->shape[2]), p.states = static_cast<int>(a->shape[1]);
-    p.blocks = static_cast<int>(groups) * DivUp(u->shape[2] / groups, kScanChannels);
+    if (b->shape[0] != p.batch || b->shape[1] != p.length || b->shape[b->ndim - 1] != p.states || groups < 1 || p.channels % groups != 0) return 0;
+    if (p.batch == 0 || p.channels == 0) return 0;
+    p.blocks = static_cast<int>(groups) * DivUp(p.channels / groups, kScanChannels);
     CutScanGrad(&p);
     return GradWorkspace(p).Bytes();
 }
