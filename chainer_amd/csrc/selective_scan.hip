@@ -44,9 +44,9 @@ constexpr int kScanWaves = NPL == 1 ? (sizeof(T) == 4 ? 7 : 6) : NPL <= 4 ? (FEW
 // from the states that it puts together on the way.  Rows go by in tiles of 16, whose b and c lie in LDS; a lane reads u, delta and z of every fourth row
 // of its channel, prepares dt, dt u and the gate once, and hands them to the quad's other lanes.
 // Bound by the vector units.  A state costs a row an exponential (8 cycles of a wave) and four instructions of 4 cycles: 82 us for 16384 rows of 2048 channels and 16 states,
-// whose memory traffic takes 55 at 4.9 TB/s.  Beside a row's 20 instructions on states there are 17, for softplus, the gate, the sum over the quad, loads and
-// LDS.  32 sequences of 2048 rows and channels, float16: 590 to 630 us, 170 to 185 cycles a row of 16 channels, 77 % of the issue slots taken.  One sequence of 16384 rows: 118 us from zeros,
-// 160 to 195 with outputs.  Four lanes to a channel: one would leave a quarter of the waves, and what they share is done once either way.
+// whose memory traffic takes 46 at 5.8 TB/s.  Beside a row's 20 instructions on states there are 17, for softplus, the gate, the sum over the quad, loads and
+// LDS.  32 sequences of 2048 rows and channels, float16: 630 us, 185 cycles a row of 16 channels, 77 % of the issue slots taken.  One sequence of 16384 rows: 275, of which two fifths from
+// zeros.  Four lanes to a channel: one would leave a quarter of the waves, and what they share is done once either way.
 // REPEATS: fewer than 4 * NPL states, some of them twice.  Zeros in the room that is left, b = c = 0, become NaN where dt u is infinite, and with them sums that the states make infinite; to
 // leave them out of the sums takes a selection a state and row, and registers (48 states, 20 x 35 rows of 650 channels: 19.3 -> 21.6 us), while whole lanes of states are read at once.
 template <typename T, int NPL, bool ENDS, bool REPEATS, bool FEW>
@@ -168,7 +168,7 @@ __global__ __launch_bounds__(256, (kScanWaves<T, NPL, FEW>)) void SelectiveScanK
     if (at.chunk == p.chunks - 1) StoreStates<NPL>(p.new_state + of_state, n0, p.states, h);
 }
 
-// One row of each of V sequences: what a token costs is its states, read and written once: 128 x 4096 channels of 16 states in 16 to 17 us, 4.3 TB/s, and 256 in 30, 4.8.  The kernel
+// One row of each of V sequences: what a token costs is its states, read and written once: 128 x 4096 channels of 16 states in 17 us, 4.1 TB/s, and 256 in 27.5, 5.2.  The kernel
 // above, whose threads start with tiles and LDS, takes 43 us for the first.  Four threads to a channel, each with a quarter of the states.
 template <typename T, int NPL, int V>
 __global__ __launch_bounds__(256) void ScanTokenKernel(ScanArgs p, int64_t first) {
@@ -345,8 +345,8 @@ int hipcx_selective_scan(const hipcx_array* u, const hipcx_array* delta, const h
             using T = typename decltype(tag)::type;
             constexpr int NPL = decltype(share)::value;
             if (p.length == 1) {
-                // Two sequences to a thread where that leaves a compute unit 16 waves: 128 x 4096 channels of 16 states, float16, 21.0 us with one, 19.0 with two, 19.0
-                // with four; 256 x 4096 31.9, 30.0, 32.9; 128 x 4096 of 64 states 83, 79, 99.
+                // Two sequences to a thread where that leaves a compute unit 16 waves.  us a call, with the host's part, of one, two and four: 128 x 4096 channels of 16
+                // states, float16, 21.0, 19.0, 19.0; 256 x 4096 31.9, 30.0, 32.9; 128 x 4096 of 64 states 83, 79, 99.
                 const bool two = p.batch / 2 * p.channels * 4 >= int64_t{NumCUs()} * 1024;
                 ForLaunches((two ? (p.batch + 1) / 2 : p.batch) * p.channels * 4, [&](dim3 grid, int64_t first) {
                     if (two) hipLaunchKernelGGL((ScanTokenKernel<T, NPL, 2>), grid, dim3(256), 0, AsStream(stream), p, first);

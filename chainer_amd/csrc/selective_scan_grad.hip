@@ -19,7 +19,8 @@ struct ScanGradArgs {
     int tiles;             // of a sequence
 };
 
-// Rows whose states a lane keeps in registers on the way back: 64 states.
+// Rows whose states a lane keeps in registers on the way back: 64 states.  Those of 33 to 64 states take 256 registers and some 110 of the accumulators', with 3 to 6 spilled there, and leave one
+// wave to a SIMD: 1.09 ms for 4 x 2048 rows of 2048 channels and 64 states, 2.7 times as long as 32.
 template <int NPL>
 constexpr int kGradTile = NPL <= 2 ? 16 : NPL == 4 ? 8 : 4;
 
@@ -167,7 +168,7 @@ __global__ __launch_bounds__(256) void ScanGradStatesKernel(ScanGradArgs pg) {
 // A chunk from its last tile to its first: the tile's states again, in registers, from those that it starts from, and the gradients.  STATES: sequences are whole, and their tiles'
 // states are made here too.
 // Bound by the vector units: 13 instructions and an exponential a state, the sums over channels (of two numbers a state and row; 18 % of the issue slots), 109 a row, 72 % of the issue slots at
-// two waves to a SIMD.  4 x 2048 rows of 2048 channels of 16 states, float16: 275 to 305 us; 32 sequences 1870 to 2060.  Tiles of 8 rows: 16 keep twice the states and decays, which
+// two waves to a SIMD.  4 x 2048 rows of 2048 channels of 16 states, float16: 271 us; 32 sequences 2040.  Tiles of 8 rows: 16 keep twice the states and decays, which
 // leaves one wave (588 us in all for 462), and held to three waves by fewer registers it spills (1140).  One barrier a tile, with LDS for two.
 template <typename T, int NPL, bool STATES>
 __global__ __launch_bounds__(256) void SelectiveScanGradKernel(ScanGradArgs pg) {

@@ -470,10 +470,12 @@ int hipcx_causal_conv_grad(const hipcx_array* x, const hipcx_array* w, const hip
  *   with dt = delta + delta_bias, or log(1 + exp(delta + delta_bias)) with delta_softplus; h[-1] is `state`, new_state the last h; d and delta_bias (zeros) and z (no gate)
  *   may be NULL.  u, delta, z, y [batch, time, channels]; b, c [batch, time, states] or [batch, time, groups, states], a group for channels / groups neighbours:
  *   float16 or float32.  a [channels, states], d, delta_bias [channels], state, new_state [batch, channels, states]: float32, C-contiguous.  1 to 64 states, of
- *   float32; rows less than 2^26 elements apart.
+ *   float32; rows less than 2^26 elements apart.  Infinite inputs and states go through as the formulas say; states that do not decay (dt a > 0) may.
  * hipcx_selective_scan_grad: the gradients of all that was given, from gy and gnew_state (or NULL, zeros); gz goes with z, gd, gdelta_bias and gstate may be NULL.
  *   ga, gb, gc, gd, gdelta_bias, gnew_state and gstate are C-contiguous.  The states are computed again; sums run in float32 in an order that depends on the sizes
- *   alone. */
+ *   alone.  The workspace holds the states that tiles of rows start from and partial sums: some 1, 3, 9, 34 or 68 bytes a row and channel with up to 4, 8, 16, 32 or 64 states,
+ *   and states / 8 more (4 x 2048 rows of 2048 channels, 16 states: 190 MB; 64 states: 1.3 GB).  Gradients may be NaN where the formulas make them infinite, and where the
+ *   decays of states that grow leave float32's range. */
 size_t hipcx_selective_scan_workspace_size(const hipcx_array* u, const hipcx_array* a);
 int hipcx_selective_scan(const hipcx_array* u, const hipcx_array* delta, const hipcx_array* a, const hipcx_array* b, const hipcx_array* c,
                          const hipcx_array* d, const hipcx_array* z, const hipcx_array* delta_bias, int delta_softplus, const hipcx_array* state,
