@@ -78,7 +78,7 @@ __global__ __launch_bounds__(256, (kScanWaves<T, NPL, FEW>)) void SelectiveScanK
     const float bias = p.bias != nullptr ? p.bias[at.channel] : 0.f, d = p.d != nullptr ? p.d[at.channel] : 0.f;
     TileRows<T, kScanTile> us(p.u, at, t0), ds(p.delta, at, t0), zs(p.z, at, t0), ys(p.y, at, t0);
     TileShared<T, NPL, kScanTile, ENDS ? 1 : 2, REPEATS> shared(p, at, t0);
-    const bool gated = !ENDS && p.z.data != nullptr;
+    const bool gated = !ENDS && p.z.data != nullptr, skips = p.d != nullptr;  // (0 times an infinite u would be NaN)
     const auto fetch = [&](int rows, auto whole) __attribute__((always_inline)) {
         constexpr bool kWhole = decltype(whole)::value;
         us.template Fetch<kWhole>(at.q, rows);
@@ -112,7 +112,7 @@ __global__ __launch_bounds__(256, (kScanWaves<T, NPL, FEW>)) void SelectiveScanK
             step(std::integral_constant<int, 2>{});
             step(std::integral_constant<int, 3>{});
             if constexpr (!ENDS) {
-                y[g] = __builtin_fmaf(d, u[g], QuadTransposedSum(sums, at.q)) * gate[g];
+                y[g] = __builtin_fmaf(d, skips ? u[g] : 0.f, QuadTransposedSum(sums, at.q)) * gate[g];
             }
         }
         if constexpr (!ENDS) {
@@ -212,7 +212,7 @@ __global__ __launch_bounds__(256) void ScanTokenKernel(ScanArgs p, int64_t first
         sum += QuadSwap2(sum);
         const int64_t b = b0 + v;
         if (n0 == 0) {
-            float y = __builtin_fmaf(d, u[v], sum);
+            float y = __builtin_fmaf(d, p.d != nullptr ? u[v] : 0.f, sum);  // (0 times an infinite u would be NaN)
             if (p.z.data != nullptr) y *= z[v] * LogisticOf(z[v]);
             static_cast<T*>(p.y.data)[b * p.y.batch + channel] = static_cast<T>(counts[v] ? y : 0.f);
         }

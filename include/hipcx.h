@@ -467,8 +467,8 @@ int hipcx_causal_conv_grad(const hipcx_array* x, const hipcx_array* w, const hip
 
 /* hipcx_selective_scan: for every sequence, channel and state n
  *     h[t][n] = exp(dt[t] a[n]) h[t-1][n] + dt[t] u[t] b[t][n],   y[t] = (sum over n of c[t][n] h[t][n] + d u[t]) z[t] / (1 + exp(-z[t]))
- *   with dt = delta + delta_bias, or log(1 + exp(delta + delta_bias)) with delta_softplus; h[-1] is `state`, new_state the last h; d and delta_bias (zeros) and z (no gate)
- *   may be NULL.  u, delta, z, y [batch, time, channels]; b, c [batch, time, states] or [batch, time, groups, states], a group for channels / groups neighbours:
+ *   with dt = delta + delta_bias, or log(1 + exp(delta + delta_bias)) with delta_softplus; h[-1] is `state`, new_state the last h; d (no such term), delta_bias
+ *   (zeros) and z (no gate) may be NULL.  u, delta, z, y [batch, time, channels]; b, c [batch, time, states] or [batch, time, groups, states], a group for channels / groups neighbours:
  *   float16 or float32.  a [channels, states], d, delta_bias [channels], state, new_state [batch, channels, states]: float32, C-contiguous.  1 to 64 states, of
  *   float32; rows less than 2^26 elements apart.  Infinite inputs and states go through as the formulas say; states that do not decay (dt a > 0) may.
  * hipcx_selective_scan_grad: the gradients of all that was given, from gy and gnew_state (or NULL, zeros); gz goes with z, gd, gdelta_bias and gstate may be NULL.

@@ -62,6 +62,24 @@ def test_infinite_inputs(chx, states, length, dtype):
     assert_same_kinds(new, token_new, 'state of tokens')
 
 
+@pytest.mark.parametrize('length', [1, 40, 300])
+@pytest.mark.parametrize('states', [1, 5, 16])
+def test_infinite_inputs_without_a_skip(chx, states, length):
+    """Without `d` an infinite u counts by its states alone."""
+    c = case(1, length, 21, states, 'float32', seed=3)
+    c['a'] /= 4
+    del c['d']
+    row = length // 2
+    c['u'][0, row, 2] = np.inf
+    y, new = (v.get() for v in chx.selective_scan(**on_device(chx, c)))
+    want = np.zeros(y.shape, bool)
+    want[0, row:, 2] = True
+    assert np.array_equal(np.isposinf(y), want) and not np.isnan(y).any()
+    token_y, token_new = by_tokens(chx, c)
+    assert_same_kinds(y, token_y, 'tokens')
+    assert_same_kinds(new, token_new, 'state of tokens')
+
+
 @pytest.mark.parametrize('states', [1, 5, 16, 24])
 def test_infinite_steps_leave_the_gradients_before_them(chx, states):
     """Behind a step without end nothing is left of the state, so that it takes no part in the gradients of the rows before: those are the gradients without it."""
