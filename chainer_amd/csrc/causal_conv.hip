@@ -94,7 +94,7 @@ struct ConvPart {
 // Bound by memory: x read once and y written once, beside taps - 1 rows of the chunk before.  A thread keeps its window in registers and walks down the rows of 16 bytes of
 // channels, kAhead of whose loads are in flight.  A batch of 16 x 2048 x 4096 float16, four taps, SiLU: 107 us, 5.0 TB/s; with sequences half as long on average 89.  kAhead of 8:
 // 110 and 94.  One token of 1300 channels 4.8 us, a launch and two trips to memory.  float16 windows of five taps take 146 registers (three waves), of six to eight 176 to 235 (two), and
-// bound those by latency: 8 x 2048 x 2048 31 us with four taps, 33, 39, 43 and 45 with five to eight; float32 46 to 51.
+// bound those by latency: 8 x 2048 x 2048 31 us with four taps, 35, 39, 43 and 46 with five to eight; float32 46 to 50.
 constexpr int kAhead = 4;      // rows whose loads are issued together
 constexpr int kFewestRows = 8; // to a chunk, taps - 1 at least
 
@@ -159,9 +159,9 @@ __global__ __launch_bounds__(256, K <= 4 ? 4 : 2) void CausalConvKernel(ConvArgs
 
 // gp = gy act'(sum) where a row counts, else 0.  The gradient of input row i (state and x behind it) is w[k] gp[i - k] summed over the taps: a thread
 // goes through its rows and taps - 1 more, computes every sum again from x, and is done with input row i as soon as it has gp[i].  Bound by memory, x and gy in and gx out:
-// 8 x 2048 x 2048 float16 50 to 54 us, 3.7 to 4.1 TB/s, of float32 87 us, 4.6.  Registers decide: 124 to 128 of them with four taps, four waves (4 spilled outside the rows in
+// 8 x 2048 x 2048 float16 50 to 55 us, 3.7 to 4.0 TB/s, of float32 87 us, 4.6.  Registers decide: 124 to 128 of them with four taps, four waves (4 spilled outside the rows in
 // float16), where the compiler has no reason to hold more (blocks of rows with masks instead of single ones at the ends: 150 to 180, 62 to 69 us; held to 128 it spills in the rows, 300 to
-// 490).  Five and six taps take 142 to 166, three waves, seven and eight 180 to 210, two: 64, 73, 88 and 96 us in float16, 100, 111, 110 and 117 in float32.
+// 490).  Five and six taps take 142 to 166, three waves, seven and eight 180 to 210, two: 64, 73, 88 and 97 us in float16, 100, 112, 110 and 117 in float32.
 template <typename T, int K, int E>
 __global__ __launch_bounds__(256, K <= 4 ? 4 : 2) void CausalConvGradKernel(ConvArgs p) {
     using P = Piece<T, E>;

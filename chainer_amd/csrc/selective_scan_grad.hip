@@ -73,7 +73,7 @@ __device__ __forceinline__ void ScanSteps(const ScanArgs& p, const TileRows<T, R
 // of g0 c times the decay since the chunk began, which runs forwards too.  CHUNKS: there is more than one, else the last two are not needed.
 // Tiles' states as they come out of zeros, so that they are there before the state that the chunk starts from is known: the next launch adds exp(a * sum of dt) times it, an
 // exponential a tile instead of a run through the rows (444 -> 425 us in all).  Stored in every tile without a condition: in a branch they cost a third of the waves (152 registers for
-// 97, 137 us for 115 at 4 x 2048 rows of 2048 channels).  Bound by the vector units: seven instructions and an exponential a state, 44 instructions a row, 63 % of the issue slots.
+// 97, 137 us for 115 at 4 x 2048 rows of 2048 channels).  Bound by the vector units: seven instructions and an exponential a state, 44 instructions a row, 77 % of the issue slots.
 template <typename T, int NPL, bool CHUNKS>
 __device__ __forceinline__ void MakeTileStates(const ScanGradArgs& pg, const ScanPlace& at) {
     const ScanArgs& p = pg.s;
@@ -167,7 +167,7 @@ __global__ __launch_bounds__(256) void ScanGradStatesKernel(ScanGradArgs pg) {
 
 // A chunk from its last tile to its first: the tile's states again, in registers, from those that it starts from, and the gradients.  STATES: sequences are whole, and their tiles'
 // states are made here too.
-// Bound by the vector units: 13 instructions and an exponential a state, the sums over channels (of two numbers a state and row; 18 % of the issue slots), 109 a row, 72 % of the issue slots at
+// Bound by the vector units: 13 instructions and an exponential a state, the sums over channels (of two numbers a state and row; 18 % of the issue slots), 104 a row, 73 % of the issue slots at
 // two waves to a SIMD.  4 x 2048 rows of 2048 channels of 16 states, float16: 271 us; 32 sequences 2040.  Tiles of 8 rows: 16 keep twice the states and decays, which
 // leaves one wave (588 us in all for 462), and held to three waves by fewer registers it spills (1140).  One barrier a tile, with LDS for two.
 template <typename T, int NPL, bool STATES>
