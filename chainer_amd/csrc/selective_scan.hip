@@ -45,8 +45,8 @@ constexpr int kScanWaves = NPL == 1 ? (sizeof(T) == 4 ? 7 : 6) : NPL <= 4 ? (FEW
 // of its channel, prepares dt, dt u and the gate once, and hands them to the quad's other lanes.
 // Bound by the vector units.  A state costs a row an exponential (8 cycles of a wave) and four instructions of 4 cycles: 82 us for 16384 rows of 2048 channels and 16 states,
 // whose memory traffic takes 46 at 5.8 TB/s.  Beside a row's 20 instructions on states there are 17, for softplus, the gate, the sum over the quad, loads and
-// LDS.  32 sequences of 2048 rows and channels, float16: 630 us, 185 cycles a row of 16 channels.  In chunks 76 % of the issue slots are taken from zeros, 80 % with outputs.  One sequence of 16384 rows: 275, of which two fifths from
-// zeros.  Four lanes to a channel: one would leave a quarter of the waves, and what they share is done once either way.
+// LDS.  32 sequences of 2048 rows and channels, float16: 630 us, 185 cycles a row of 16 channels.  One sequence of 16384 rows: 275, of which two fifths from zeros; 76 % of the issue slots
+// are taken there, 80 % with outputs.  Four lanes to a channel: one would leave a quarter of the waves, and what they share is done once either way.
 // REPEATS: fewer than 4 * NPL states, some of them twice.  Zeros in the room that is left, b = c = 0, become NaN where dt u is infinite, and with them sums that the states make infinite; to
 // leave them out of the sums takes a selection a state and row, and registers (48 states, 20 x 35 rows of 650 channels: 19.3 -> 21.6 us), while whole lanes of states are read at once.
 template <typename T, int NPL, bool ENDS, bool REPEATS, bool FEW>

@@ -81,6 +81,29 @@ def test_infinite_inputs_without_a_skip(chx, states, length):
 
 
 @pytest.mark.parametrize('states', [1, 5, 16, 24])
+def test_infinite_inputs_leave_the_gradients_before_them(chx, states):
+    length, row = 300, 150
+    c = case(1, length, 21, states, 'float32', seed=4)
+    c['a'] /= 4
+    gy = np.random.default_rng(5).standard_normal(c['u'].shape).astype(np.float32)
+    want = chx.selective_scan_grad(gy=chx.array(gy), **on_device(chx, c))
+    c['u'][0, row, 7] = np.inf
+    got = chx.selective_scan_grad(gy=chx.array(gy), **on_device(chx, c))
+    others = np.arange(21) != 7
+    for k in ('u', 'delta', 'z'):
+        a, b = getattr(got, k).get(), getattr(want, k).get()
+        assert np.array_equal(a[:, :row], b[:, :row]) and np.array_equal(a[..., others], b[..., others]) and np.isfinite(b).all(), k
+    for k in ('b', 'c'):
+        a, b = getattr(got, k).get(), getattr(want, k).get()
+        assert np.array_equal(a[:, :row], b[:, :row]), k
+    assert np.array_equal(got.u.get(), want.u.get())  # of which the states are no part
+    assert np.array_equal(got.state.get(), want.state.get())
+    for k in ('a', 'd', 'delta_bias'):
+        a, b = getattr(got, k), getattr(want, k)
+        assert (a is None) == (b is None) and (a is None or np.array_equal(a.get()[others], b.get()[others])), k
+
+
+@pytest.mark.parametrize('states', [1, 5, 16, 24])
 def test_infinite_steps_leave_the_gradients_before_them(chx, states):
     """Behind a step without end nothing is left of the state, so that it takes no part in the gradients of the rows before: those are the gradients without it."""
     length, row = 90, 50

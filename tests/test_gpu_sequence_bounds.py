@@ -81,3 +81,21 @@ def test_causal_conv_of_one_sequence_that_ends_inside(chx, sizes, activation, dt
     for name, got, want, size in zip(('gx', 'gw', 'gb', 'gstate'), grads, *ref.causal_conv_grad(c['x'], c['w'], c['b'], c['gy'], c['state'], lengths, activation, c['gnew'])):
         assert want.any() or taps == 1
         ref.assert_within(got.get(), want, size, 1, name)
+
+
+@pytest.mark.parametrize('groups', [None, 2])
+@pytest.mark.parametrize('states', range(1, 65))
+def test_selective_scan_of_every_number_of_states(chx, states, groups):
+    """Lanes that have not enough states for themselves: whole and padded, moved forward in place, in chunks."""
+    for i, length in enumerate((21, 100)):
+        c, _, _ = scan_case(3, length, 6, states, groups, 'float32', seed=states + i)
+        lengths = ends_inside(3, length, states)
+        outside = ~ref.inside(ref.ends_of(lengths, 3, length), length)[..., 0]
+        for k in ('u', 'delta', 'b', 'c', 'z'):
+            c[k][outside] = np.nan
+        state = chx.array(c['state'])
+        y, new = chx.selective_scan(**dict(scan_on_device(chx, c, lengths, True), state=state, out_state=state))
+        wants = bounds.selective_scan(c, True, lengths)
+        assert new is state
+        bounds.assert_close(y.get(), *wants['y'], 'y')
+        bounds.assert_close(new.get(), *wants['state'], 'state')
