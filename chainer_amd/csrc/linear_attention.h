@@ -1,0 +1,184 @@
+// What linear attention and its gradients share.
+//   S[t] = exp(g[t]) S[t-1] + k[t] v[t]^T,  y[t] = scale q[t] S[t]
+// for every sequence and head, S being a matrix [keys, values] and g the logarithm of the decay.
+//
+// The gradients are passes of the same form with the arrays in other places, two of them from the last row to the first:
+//   gq = scale S gy         is the pass of (gy, v, k) over the states' transposes,
+//   R[t] = exp(g[t+1]) R[t+1] + scale q[t] gy[t]^T,  gk = R v, gv = R^T k  are passes backwards of (v, gy, q) and (k, q, gy),
+//   gg[t] = <exp(g[t]) S[t-1], R[t]> = sum over u >= t of (q[u] gq[u] - k[u] gk[u]) and what the rows behind have of it.
+// So one kernel does all of them (AttendRun).
+#pragma once
+
+#include "sequence.h"
+
+namespace hipcx {
+
+// Rows of [batch, time, head, element] whose last axis is dense; strides in elements.  `share` neighbouring heads read one.
+struct AttendRows {
+    void* data;
+    int64_t batch, row, head;
+    int share;
+};
+
+// Matrices [batch and head][segment][i][j]; strides in elements.
+struct AttendStates {
+    float* data;  // null: zeros, or not asked for
+    int64_t head, segment, i, j;
+};
+
+// One pass: y[t] = out_scale sum over s of weight(t, s) kv_scale (q[t] k[s]) v[s] and the state that a segment begins with.
+struct AttendRun {
+    AttendRows q, k, v, y;
+    AttendRows dot;        // rows like y's, whose products with y are wanted
+    float* dots;           // [batch][head][length][2 blocks], or null
+    AttendStates start, last;
+    AttendStates other;    // the state's gradients behind each segment, whose products with the state there are wanted
+    float* ends;           // [batch][head][segment][blocks], or null
+    float* decays;         // [batch][head][segment]: a segment's own, of states alone
+    float kv_scale, out_scale;
+    int keys, values;      // extents of q and k, and of v and y
+    int first, blocks;     // of kAttendColumns columns of v
+    int back;              // from the last row to the first; the state decays by the row that follows
+    int wide;              // y is float32
+    int decay_last;        // `last` takes the first row's decay too
+};
+
+struct AttendArgs {
+    AttendRun run[3];
+    int runs, blocks;      // blocks of all runs
+    const float* decay;    // null: none
+    int64_t decay_batch, decay_row, decay_head;
+    SequenceLengths lengths;
+    int64_t batch, length, segment_rows;
+    int heads, segments;
+};
+
+constexpr int kAttendTile = 64;      // rows that are taken at once
+constexpr int kAttendColumns = 64;   // columns of v to a workgroup
+constexpr int kMaxAttend = 256;      // keys, values
+
+typedef float attend16_t __attribute__((ext_vector_type(16)));
+typedef float attend4_t __attribute__((ext_vector_type(4)));
+
+template <typename T, int N>
+struct __attribute__((packed, aligned(alignof(T)))) AttendPiece {
+    T v[N];
+};
+
+// N elements of a row from `at` on, zeros from `end` on.
+template <typename T, int N>
+__device__ __forceinline__ AttendPiece<T, N> AttendLoad(const T* row, int at, int end) {
+    AttendPiece<T, N> r{};
+    if (at + N <= end) {
+        r = *reinterpret_cast<const AttendPiece<T, N>*>(row + at);
+    } else {
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+            if (at + e < end) r.v[e] = row[at + e];
+        }
+    }
+    return r;
+}
+
+// The log decay that takes the state to row t of a pass, in powers of two.  -infinity, a state that ends, is held at a number that no product of decays brings back.
+__device__ __forceinline__ double AttendDecay(const AttendArgs& p, int64_t b, int h, int64_t t) {
+    if (p.decay == nullptr) return 0;
+    const double g = static_cast<double>(p.decay[b * p.decay_batch + t * p.decay_row + h * p.decay_head]) * 1.4426950408889634;
+    return g < -0x1p20 ? -0x1p20 : g;
+}
+
+// The decays of a tile's rows, summed up from its first: as a float and what the float leaves out, so that differences are as good as a float's for any sum.
+struct AttendDecays {
+    float high[kAttendTile], low[kAttendTile];
+    float end[kAttendTile];  // from a row to the tile's end, as a factor, times kv_scale
+    float step[kAttendTile]; // a row's own, as a factor
+    float all;               // the tile's
+    double sum;              // the tile's, in powers of two
+};
+
+__device__ __forceinline__ double ShflUpDouble(double v, int o) {
+    const uint64_t b = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = __shfl_up(static_cast<uint32_t>(b), o), hi = __shfl_up(static_cast<uint32_t>(b >> 32), o);
+    return __builtin_bit_cast(double, static_cast<uint64_t>(hi) << 32 | lo);
+}
+__device__ __forceinline__ double ShflDouble(double v, int lane) {
+    const uint64_t b = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = __shfl(static_cast<uint32_t>(b), lane), hi = __shfl(static_cast<uint32_t>(b >> 32), lane);
+    return __builtin_bit_cast(double, static_cast<uint64_t>(hi) << 32 | lo);
+}
+
+// By one wave, a lane to a row; g in powers of two, 0 for rows that are not there.
+__device__ __forceinline__ void SumDecays(AttendDecays* to, double g, float kv_scale) {
+    const int lane = threadIdx.x % 64;
+    double sum = g;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const double before = ShflUpDouble(sum, o);
+        if (lane >= o) sum += before;
+    }
+    const double all = ShflDouble(sum, 63);
+    const float high = static_cast<float>(sum);
+    to->high[lane] = high, to->low[lane] = static_cast<float>(sum - high);
+    to->end[lane] = __builtin_amdgcn_exp2f(static_cast<float>(all - sum)) * kv_scale;
+    to->step[lane] = __builtin_amdgcn_exp2f(static_cast<float>(g));
+    if (lane == 0) to->all = __builtin_amdgcn_exp2f(static_cast<float>(all)), to->sum = all;
+}
+
+// Rows of a segment: [first, end) of the sequence's.
+struct AttendSpan {
+    int64_t first, end, whole;  // whole: the end of the segment's rows in the padded batch
+    __device__ __forceinline__ AttendSpan(const AttendArgs& p, int64_t length, int segment) {
+        first = segment * p.segment_rows;
+        whole = first + p.segment_rows < p.length ? first + p.segment_rows : p.length;
+        end = whole < length ? whole : length;
+        end = end < first ? first : end;
+    }
+};
+
+// The row of the sequence that a pass takes as its row r of the segment, and the row whose decay takes the state there (-1: none).
+__device__ __forceinline__ int64_t AttendRowOf(const AttendSpan& s, int back, int64_t r) { return back ? s.end - 1 - r : s.first + r; }
+__device__ __forceinline__ double AttendStep(const AttendArgs& p, const AttendRun& run, const AttendSpan& s, int64_t b, int h, int64_t length, int64_t r) {
+    const int64_t t = AttendRowOf(s, run.back, r);
+    if (!run.back) return AttendDecay(p, b, h, t);
+    return t + 1 < length ? AttendDecay(p, b, h, t + 1) : 0;
+}
+
+// How the time axis is cut: segments of whole tiles, so that about two workgroups to a compute unit have work.
+inline void CutAttend(AttendArgs* p, int64_t blocks) {
+    const int64_t tiles = (p->length + kAttendTile - 1) / kAttendTile;
+    const int64_t each = std::max<int64_t>(1, p->batch * p->heads * blocks), wanted = 2 * int64_t{NumCUs()};
+    int64_t segments = std::min<int64_t>((wanted + each - 1) / each, tiles / 4);
+    if (segments < 2) segments = 1;
+    p->segment_rows = std::max<int64_t>(1, (tiles + segments - 1) / segments) * kAttendTile;
+    p->segments = static_cast<int>(std::max<int64_t>(1, (p->length + p->segment_rows - 1) / p->segment_rows));
+}
+
+// The sizes and arrays that the entries check alike.
+struct AttendCall {
+    AttendArgs p{};
+    AttendRows q, k, v;
+    int keys, values, key_heads;
+    const float* state;
+};
+bool AttendSizesOf(const hipcx_array* q, const hipcx_array* v, AttendCall* c);
+AttendCall DescribeAttend(const std::string& what, const hipcx_array* q, const hipcx_array* k, const hipcx_array* v, const hipcx_array* log_decay, double scale,
+                          const hipcx_array* state, const hipcx_array* lengths);
+// [batch, time, heads, width] with a dense last axis.
+AttendRows DescribeAttendRows(const hipcx_array* a, const AttendCall& c, int64_t heads, int64_t width, int dtype, const std::string& what);
+// [batch, heads, keys, values], or its transposes.
+inline AttendStates AttendStatesOf(const float* data, int keys, int values, bool transposed) {
+    const int64_t head = static_cast<int64_t>(keys) * values;
+    return transposed ? AttendStates{const_cast<float*>(data), head, 0, 1, values} : AttendStates{const_cast<float*>(data), head, 0, values, 1};
+}
+// The segments' states of a pass in a workspace, [batch and head][segment][i][j].
+inline AttendStates AttendSegments(float* data, const AttendArgs& p, int keys, int values) {
+    const int64_t each = static_cast<int64_t>(keys) * values;
+    return {data, each * p.segments, each, values, 1};
+}
+inline int AttendBlocks(int values) { return (values + kAttendColumns - 1) / kAttendColumns; }
+
+void LaunchAttend(const AttendArgs& p, int dtype, bool states_alone, hipStream_t stream);
+// What segments add to a state of zeros (`last` of a pass of states alone) becomes the state that they start from, in the order of the pass.
+void LaunchAttendStarts(const AttendArgs& p, int run, const AttendStates& initial, hipStream_t stream);
+
+}  // namespace hipcx

@@ -207,5 +207,10 @@ HOST_FN(CausalConv);
 HOST_FN(CausalConvGrad);
 HOST_FN(SelectiveScan);
 HOST_FN(SelectiveScanGrad);
+HOST_FN(LinearAttention);
+HOST_FN(LinearAttentionGrad);
+HOST_FN(LayerNorm);              // training.cc
+HOST_FN(LayerNormGrad);
+HOST_FN(AdamWUpdate);
 
 }  // namespace host

@@ -1407,6 +1407,11 @@ PyMethodDef kRoutines[] = {
         ROUTINE("causal_conv_grad", CausalConvGrad, nullptr),
         ROUTINE("selective_scan", SelectiveScan, nullptr),
         ROUTINE("selective_scan_grad", SelectiveScanGrad, nullptr),
+        ROUTINE("linear_attention", LinearAttention, nullptr),
+        ROUTINE("linear_attention_grad", LinearAttentionGrad, nullptr),
+        ROUTINE("layer_norm", LayerNorm, nullptr),
+        ROUTINE("layer_norm_grad", LayerNormGrad, nullptr),
+        ROUTINE("adamw_update", AdamWUpdate, nullptr),
         {nullptr, nullptr, 0, nullptr}};
 
 }  // namespace host

@@ -1,4 +1,5 @@
-// chainer_amd._host: the routines of sequence.h's kernels -- dropout, the causal convolution and the selective scan -- over the C ABI.
+// chainer_amd._host: the routines of sequence.h's kernels -- dropout, the causal convolution, the selective scan and linear attention -- over the C ABI.
+#include <cmath>
 #include <vector>
 
 #include "host.h"
@@ -163,6 +164,62 @@ HOST_FN(SelectiveScanGrad) {
                                          gdelta.d(), ga.d(), gb.d(), gc.d(), gd.d(), gz.d(), gbias.d(), gstate.d(), scratch.ptr, scratch.bytes, stream);
     });
     return Pack({&gu, &gdelta, &ga, &gb, &gc, &gd, &gz, &gbias, &gstate});
+    HOST_CATCH(nullptr);
+}
+
+namespace {
+
+double ScaleOf(PyObject* x, const Array* q) {
+    if (!Given(x)) return 1 / std::sqrt(static_cast<double>(q->d.shape[3] > 0 ? q->d.shape[3] : 1));
+    const double v = PyFloat_AsDouble(x);
+    if (v == -1.0 && PyErr_Occurred()) throw PyError();
+    return v;
+}
+
+}  // namespace
+
+HOST_FN(LinearAttention) {
+    HOST_TRY;
+    HOST_ARGS("linear_attention", 3, "q", "k", "v", "log_decay", "scale", "state", "lengths", "out_state");
+    Array *queries = AsArray(arg[0], "q"), *values = AsArray(arg[2], "v");
+    RequireAxes(queries, 4, "q");
+    RequireAxes(values, 4, "v");
+    Ref q = DenseRows(queries), k = DenseRows(AsArray(arg[1], "k")), v = DenseRows(values);
+    Array* const decay = Optional(arg[3], "log_decay");
+    const double scale = ScaleOf(arg[4], queries);
+    Ref state = ContiguousOrNone(Optional(arg[5], "state"));
+    Array* const lengths = Optional(arg[6], "lengths");
+    const int64_t of_state[4] = {queries->d.shape[0], values->d.shape[2], queries->d.shape[3], values->d.shape[3]};
+    Ref new_state = Given(arg[7]) ? NewRef(AsArray(arg[7], "out_state")) : Empty(4, of_state, HIPCX_FLOAT32);
+    Ref y = EmptyLike(values, values->d.dtype);
+    Workspace scratch(hipcx_linear_attention_workspace_size(q.d(), v.d()));
+    void* stream = Stream();
+    Call([&] {
+        return hipcx_linear_attention(q.d(), k.d(), v.d(), Descriptor(decay), scale, state.d(), Descriptor(lengths), y.d(), new_state.d(), scratch.ptr, scratch.bytes, stream);
+    });
+    return Pack({&y, &new_state});
+    HOST_CATCH(nullptr);
+}
+
+// (gq, gk, gv, glog_decay, gstate); None for what is not given
+HOST_FN(LinearAttentionGrad) {
+    HOST_TRY;
+    HOST_ARGS("linear_attention_grad", 4, "q", "k", "v", "gy", "log_decay", "scale", "state", "lengths", "gnew_state");
+    Array *queries = AsArray(arg[0], "q"), *keys = AsArray(arg[1], "k"), *values = AsArray(arg[2], "v");
+    RequireAxes(queries, 4, "q");
+    RequireAxes(values, 4, "v");
+    Ref q = DenseRows(queries), k = DenseRows(keys), v = DenseRows(values), gy = DenseRows(AsArray(arg[3], "gy"));
+    Array *const decay = Optional(arg[4], "log_decay"), *const first = Optional(arg[6], "state"), *const lengths = Optional(arg[7], "lengths");
+    const double scale = ScaleOf(arg[5], queries);
+    Ref state = ContiguousOrNone(first), gnew = ContiguousOrNone(Optional(arg[8], "gnew_state"));
+    Ref gq = EmptyLikeOrNone(queries), gk = EmptyLikeOrNone(keys), gv = EmptyLikeOrNone(values), gdecay = EmptyLikeOrNone(decay), gstate = EmptyLikeOrNone(first);
+    Workspace scratch(hipcx_linear_attention_grad_workspace_size(q.d(), v.d(), Descriptor(decay)));
+    void* stream = Stream();
+    Call([&] {
+        return hipcx_linear_attention_grad(q.d(), k.d(), v.d(), Descriptor(decay), scale, state.d(), Descriptor(lengths), gy.d(), gnew.d(), gq.d(), gk.d(), gv.d(), gdecay.d(),
+                                           gstate.d(), scratch.ptr, scratch.bytes, stream);
+    });
+    return Pack({&gq, &gk, &gv, &gdecay, &gstate});
     HOST_CATCH(nullptr);
 }
 

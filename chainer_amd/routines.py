@@ -1278,6 +1278,41 @@ def batch_norm_relu_grad(x, gamma, beta, gout, state, axis=None):
     return batch_norm_grad(x, gamma, if_less_else(b, 0, 0, gout), state, axis)
 
 
+LayerNormState = collections.namedtuple('LayerNormState', ['mean', 'inv_std', 'beta_dtype'])
+
+
+def layer_norm(x, gamma=None, beta=None, eps=2e-5):
+    """F.layer_normalization (chainer/functions/normalization/layer_normalization.py) over the last axis in one kernel: (x - mean) * inv_std * gamma + beta, for any number of axes
+    before it.  ``gamma``, ``beta`` [columns]: ones and zeros if not given, of x's dtype or, for float16, of float32.  Returns (y, state) with the state that ``layer_norm_grad`` takes."""
+    y, mean, inv_std = _host.layer_norm(x, gamma, beta, eps)
+    return y, LayerNormState(mean, inv_std, None if beta is None else beta.dtype)
+
+
+def layer_norm_grad(x, gamma, gout, state):
+    """The gradients (gx, ggamma, gbeta) of ``layer_norm``; None for a ``gamma`` or ``beta`` that was not given."""
+    return _host.layer_norm_grad(x, gamma, gout, *state)
+
+
+AdamWState = collections.namedtuple('AdamWState', ['m', 'v', 'm_scale', 'v_scale', 'master'])
+
+
+def adamw_state(param, bits=32, master=False):
+    """The state that ``adamw_update`` starts a parameter with: zeros in 32 bits or in 8, and for ``master`` a float32 copy of a float16 parameter, which is updated in its place."""
+    if bits not in (8, 32):
+        raise _lib.ChainerxError('adamw_state: states have 8 or 32 bits, got %r' % (bits,))
+    blocks = -(-_prod(param.shape) // 256)
+    dtype, scales = ('uint8', [zeros((blocks,)), zeros((blocks,))]) if bits == 8 else ('float32', [None, None])
+    return AdamWState(zeros(param.shape, dtype), zeros(param.shape, dtype), *scales, param.astype('float32') if master and param.dtype != numpy.dtype('float32') else None)
+
+
+def adamw_update(params, grads, states, t, alpha=0.001, beta1=0.9, beta2=0.999, eps=1e-8, eta=1.0, weight_decay_rate=0.0, seed=0):
+    """A step of AdamW (chainer/optimizers/adam.py: AdamRule with weight_decay_rate) of many parameters in place: m += (1 - beta1) * (g - m), v += (1 - beta2) * (g * g - v),
+    p -= eta * (alpha * sqrt(1 - beta2 ** t) / (1 - beta1 ** t) * m / (sqrt(v) + eps) + weight_decay_rate * p), in one launch for up to 48 arrays of a kind.  ``states``: one from
+    ``adamw_state`` for every parameter, of 8 bits for some and of 32 for others as wanted.  ``t``: the step, from 1 on, or an int64 array of one element, so that a captured graph
+    goes on to the next.  ``seed``: of the numbers by which states in 8 bits are rounded; they depend on it, on t, and on a parameter's place in the list."""
+    _host.adamw_update(params, grads, states, t, alpha, beta1, beta2, eps, eta, weight_decay_rate, seed)
+
+
 def add_relu_grad(x, g1, g2):
     """if_less_else(x, 0, 0, add(g1, g2)), the gradient of relu(x) where two of its uses meet, in one kernel call where the arrays are alike."""
     direct = _host.add_relu_grad_direct(x, g1, g2)
@@ -1760,7 +1795,7 @@ def n_step_birnn(n_layers, hx, ws, bs, xs, activation='tanh', kernel=False):
 
 
 # ---------------------------------------------------------------------------------------------
-# layers of a recurrent block that the reference has no kernels for: the causal convolution, the selective scan, dropout
+# layers of a recurrent block that the reference has no kernels for: the causal convolution, the selective scan, linear attention, dropout
 # ---------------------------------------------------------------------------------------------
 def dropout(x, ratio, key, site=0, residual=None):
     """Dropout (chainer/functions/noise/dropout.py): ``x`` scaled by 1 / (1 - ratio) where it is kept, else 0, plus ``residual``, in one kernel.  The mask is
@@ -1799,6 +1834,23 @@ SelectiveScanGradients = collections.namedtuple('SelectiveScanGradients', ['u', 
 def selective_scan_grad(u, delta, a, b, c, gy, d=None, z=None, delta_bias=None, delta_softplus=False, state=None, lengths=None, gnew_state=None):
     """The gradients of ``selective_scan`` from those of its results, by name; None for what is not given.  The states are computed again."""
     return SelectiveScanGradients(*_host.selective_scan_grad(u, delta, a, b, c, gy, d, z, delta_bias, delta_softplus, state, lengths, gnew_state))
+
+
+def linear_attention(q, k, v, log_decay=None, scale=None, state=None, lengths=None, out_state=None):
+    """A recurrent layer whose state is a matrix for each head that decays and gathers keys and values: S[t] = exp(log_decay[t]) * S[t - 1] + outer(k[t], v[t]) and
+    y[t] = scale * (q[t] @ S[t]).  q, k [batch, time, key heads, keys], v [batch, time, heads, values]: float16 or float32, up to 256 keys and values; neighbouring heads of v
+    share one of q and k where these have fewer.  ``log_decay``: float32 [heads] or [batch, time, heads] (0: nothing decays); ``scale``: 1 / sqrt(keys) if not given; ``state``: float32
+    [batch, heads, keys, values] (zeros); ``lengths``: the rows of each sequence of a padded batch.  Returns (y, new state); the next token or piece of the sequence is a call with that
+    state.  ``out_state``: where to put it, the state itself for one."""
+    return _host.linear_attention(q, k, v, log_decay, scale, state, lengths, out_state)
+
+
+LinearAttentionGradients = collections.namedtuple('LinearAttentionGradients', ['q', 'k', 'v', 'log_decay', 'state'])
+
+
+def linear_attention_grad(q, k, v, gy, log_decay=None, scale=None, state=None, lengths=None, gnew_state=None):
+    """The gradients of ``linear_attention`` from those of its results, by name; None for what is not given.  The states are computed again."""
+    return LinearAttentionGradients(*_host.linear_attention_grad(q, k, v, gy, log_decay, scale, state, lengths, gnew_state))
 
 
 def softmax_cross_entropy(x, t):

@@ -194,6 +194,19 @@ int hipcx_copy_many(const hipcx_array* const* as, const hipcx_array* const* outs
  * the difference like MultiplyASKernel and SubtractKernel (CX/kernels/arithmetic.h), float16 and float32 arrays in one launch for up to 112 of them.  No out may
  * overlap another array of the call. */
 int hipcx_update_many(const hipcx_array* const* xs, const hipcx_array* const* gs, hipcx_scalar scale, const hipcx_array* const* outs, int n, void* stream);
+/* hipcx_adamw_many: a step of AdamW (chainer/optimizers/adam.py: AdamRule with weight_decay_rate) of n parameters in place, in one launch for up to 48 arrays of a kind:
+ *     m += (1 - beta1) (g - m),  v += (1 - beta2) (g^2 - v),  p -= eta (alpha sqrt(1 - beta2^t) / (1 - beta1^t) m / (sqrt(v) + eps) + weight_decay_rate p)
+ *   in float32, every operation rounded.  params: float16 or float32; grads: of the parameter's dtype or float32; ms, vs: float32, or both uint8, states in 8 bits: m's and sqrt(v)'s codes,
+ *   with m_scales and v_scales, float32 [size / 256 rounded up], the power of two that no value of a block of 256 exceeds (states of zeros: all zeros).  A code c of m stands for (8 + c % 8)
+ *   2^(c / 8 % 16 - 18) of the scale, c % 8 2^-17 where c / 8 % 16 is 0, minus that from 128 on; one of sqrt(v) for (8 + c % 8) 2^(c / 8 - 34), or c 2^-33 below 8.  Values go to one of their two
+ *   neighbours at random in proportion, but sqrt(v) > 0 never to 0: 16 bits each for m and v of element e of array i from Philox4x32-10's word e % 4 for counter {e / 4, i, low and high half of t}
+ *   and key {low and high half of seed}.  A block that holds what is not finite, or more than 2^100, becomes NaN.  masters: float32 copies of float16 parameters, updated in
+ *   their place, of which the parameters are roundings; NULL for those that have none.  m_scales[i], v_scales[i]: NULL for states in 32 bits.  t: the step, from 1 on, or t_array, int64
+ *   of one element in device memory, so that a captured graph takes another one's.  All arrays C-contiguous, of up to 2^33 elements; those that are written share no memory with any other. */
+int hipcx_adamw_many(const hipcx_array* const* params, const hipcx_array* const* grads, const hipcx_array* const* ms, const hipcx_array* const* vs,
+                     const hipcx_array* const* m_scales, const hipcx_array* const* v_scales, const hipcx_array* const* masters, int n, int64_t t,
+                     const hipcx_array* t_array, double alpha, double beta1, double beta2, double eps, double eta, double weight_decay_rate, int64_t seed,
+                     void* stream);
 int hipcx_fill(const hipcx_array* out, hipcx_scalar value, void* stream);                         /* FillKernel misc.h:9 */
 int hipcx_arange(hipcx_scalar start, hipcx_scalar step, const hipcx_array* out, void* stream);    /* ArangeKernel creation.h:11 */
 
@@ -488,6 +501,39 @@ int hipcx_selective_scan_grad(const hipcx_array* u, const hipcx_array* delta, co
                               const hipcx_array* gdelta, const hipcx_array* ga, const hipcx_array* gb, const hipcx_array* gc, const hipcx_array* gd,
                               const hipcx_array* gz, const hipcx_array* gdelta_bias, const hipcx_array* gstate, void* workspace, size_t workspace_bytes,
                               void* stream);
+
+/* hipcx_linear_attention: for every sequence and head a matrix S [keys, values] that decays and gathers keys and values,
+ *     S[t] = exp(g[t]) S[t-1] + k[t] v[t]^T,   y[t] = scale q[t] S[t]
+ *   with S[-1] `state` and new_state the last S.  q, k [batch, time, key heads, keys], v, y [batch, time, heads, values]: float16 or float32, with heads a multiple of key heads,
+ *   heads / key heads neighbours of which share a head of q and k; 1 to 256 keys and values.  log_decay: g, float32 [heads], [batch, time, heads] or NULL (0), of any strides;
+ *   -infinity ends what was gathered.  state, new_state: float32 [batch, heads, keys, values], C-contiguous.  Up to eight rows go one after another; longer ones in tiles of 64 as matrix
+ *   products, and where sequences and heads are few the time axis is cut into segments whose states take the workspace.  Products and sums of float32 run in float32; float16 inputs are
+ *   taken as they are, what is computed from them in two parts of float16 (22 bits), summed in float32.  Infinities and what is not a number reach the rows that the formulas say, but a decay
+ *   that leaves float32's range makes an infinity NaN rather than leaving it one.
+ * hipcx_linear_attention_grad: from gy and gnew_state (or NULL, zeros) the gradients of q, k, v, and of log_decay (in its shape, C-contiguous) and state (C-contiguous), which may be NULL.
+ *   Those of log_decay are differences of q gq and k gk summed up from the last row of a segment, in 64 bits.  All sums run in an order that depends on the sizes alone.  The workspace holds, for
+ *   key heads that are shared, every head's gradients of q and k in float32, with log_decay some 16 bytes a row, head and 64 keys, and where time is cut two states a segment and head. */
+size_t hipcx_linear_attention_workspace_size(const hipcx_array* q, const hipcx_array* v);
+int hipcx_linear_attention(const hipcx_array* q, const hipcx_array* k, const hipcx_array* v, const hipcx_array* log_decay, double scale,
+                           const hipcx_array* state, const hipcx_array* lengths, const hipcx_array* y, const hipcx_array* new_state, void* workspace,
+                           size_t workspace_bytes, void* stream);
+size_t hipcx_linear_attention_grad_workspace_size(const hipcx_array* q, const hipcx_array* v, const hipcx_array* log_decay);
+int hipcx_linear_attention_grad(const hipcx_array* q, const hipcx_array* k, const hipcx_array* v, const hipcx_array* log_decay, double scale,
+                                const hipcx_array* state, const hipcx_array* lengths, const hipcx_array* gy, const hipcx_array* gnew_state,
+                                const hipcx_array* gq, const hipcx_array* gk, const hipcx_array* gv, const hipcx_array* glog_decay, const hipcx_array* gstate,
+                                void* workspace, size_t workspace_bytes, void* stream);
+
+/* hipcx_layer_norm: F.layer_normalization (chainer/functions/normalization/layer_normalization.py; the reference composes it of some ten kernels): rows, the last axis, brought to mean 0 and
+ *   variance 1, y = (x - mean) inv_std gamma + beta with inv_std = 1 / sqrt(var + eps) and var the mean square of what is off the mean.  x [..., columns] of a floating dtype, its rows dense and
+ *   equally far apart; y like x, C-contiguous; gamma and beta [columns], each may be NULL (ones, zeros), of x's dtype or float32 where x is float16; mean and inv_std: the
+ *   state that the gradient takes, x's shape without its last axis, float32 (float64 for float64), C-contiguous.  Rows of any length but 0; computed in float32 (float64), rounded
+ *   once.  y may be x.
+ * hipcx_layer_norm_grad: gx and, where asked for, ggamma and gbeta, sums over rows in float32 and then in 64 bits, in an order that the sizes and the device's compute units decide. */
+int hipcx_layer_norm(const hipcx_array* x, const hipcx_array* gamma, const hipcx_array* beta, double eps, const hipcx_array* y, const hipcx_array* mean,
+                     const hipcx_array* inv_std, void* stream);
+size_t hipcx_layer_norm_grad_workspace_size(const hipcx_array* x);
+int hipcx_layer_norm_grad(const hipcx_array* x, const hipcx_array* gamma, const hipcx_array* gy, const hipcx_array* mean, const hipcx_array* inv_std,
+                          const hipcx_array* gx, const hipcx_array* ggamma, const hipcx_array* gbeta, void* workspace, size_t workspace_bytes, void* stream);
 
 /* Measurement aid (no counterpart in the reference): between start and stop every implicit-GEMM launch made by
  * hipcx_dot / hipcx_conv from the calling process is bracketed by a pair of HIP events on its stream.  stop waits for them
