@@ -89,7 +89,7 @@ __device__ __forceinline__ double AttendDecay(const AttendArgs& p, int64_t b, in
 
 // The decays of a tile's rows, summed up from its first: as a float and what the float leaves out, so that differences are as good as a float's for any sum.
 struct AttendDecays {
-    float high[kAttendTile], low[kAttendTile];
+    alignas(16) float high[kAttendTile], low[kAttendTile];
     float end[kAttendTile];  // from a row to the tile's end, as a factor, times kv_scale
     float step[kAttendTile]; // a row's own, as a factor
     float all;               // the tile's
@@ -107,19 +107,29 @@ __device__ __forceinline__ double ShflDouble(double v, int lane) {
     return __builtin_bit_cast(double, static_cast<uint64_t>(hi) << 32 | lo);
 }
 
-// By one wave, a lane to a row; g in powers of two, 0 for rows that are not there.
-__device__ __forceinline__ void SumDecays(AttendDecays* to, double g, float kv_scale) {
+// Adds the value that a DPP move brings from another lane of the rows in ROWS, nothing elsewhere.
+template <int MOVE, int ROWS>
+__device__ __forceinline__ double AddMoved(double v) {
+    const uint64_t b = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = __builtin_amdgcn_update_dpp(0, static_cast<int>(b), MOVE, ROWS, 0xf, false), hi = __builtin_amdgcn_update_dpp(0, static_cast<int>(b >> 32), MOVE, ROWS, 0xf, false);
+    return v + __builtin_bit_cast(double, static_cast<uint64_t>(hi) << 32 | lo);
+}
+
+// By one wave, a lane to a row, of which `here` are there; g in powers of two, 0 for the others.
+__device__ __forceinline__ void SumDecays(AttendDecays* to, double g, int here, float kv_scale) {
     const int lane = threadIdx.x % 64;
-    double sum = g;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const double before = ShflUpDouble(sum, o);
-        if (lane >= o) sum += before;
-    }
-    const double all = ShflDouble(sum, 63);
+    double sum = AddMoved<0x111, 0xf>(g);  // from 1, 2, 4 and 8 lanes before in the row of 16, then from the rows' last lanes
+    sum = AddMoved<0x112, 0xf>(sum);
+    sum = AddMoved<0x114, 0xf>(sum);
+    sum = AddMoved<0x118, 0xf>(sum);
+    sum = AddMoved<0x142, 0xa>(sum);
+    sum = AddMoved<0x143, 0xc>(sum);
+    const uint64_t b = __builtin_bit_cast(uint64_t, sum);
+    const double all = __builtin_bit_cast(double, static_cast<uint64_t>(static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(b >> 32), 63))) << 32 |
+                                                      static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(b), 63)));
     const float high = static_cast<float>(sum);
     to->high[lane] = high, to->low[lane] = static_cast<float>(sum - high);
-    to->end[lane] = __builtin_amdgcn_exp2f(static_cast<float>(all - sum)) * kv_scale;
+    to->end[lane] = lane < here ? __builtin_amdgcn_exp2f(static_cast<float>(all - sum)) * kv_scale : 0.f;
     to->step[lane] = __builtin_amdgcn_exp2f(static_cast<float>(g));
     if (lane == 0) to->all = __builtin_amdgcn_exp2f(static_cast<float>(all)), to->sum = all;
 }
@@ -178,6 +188,7 @@ inline AttendStates AttendSegments(float* data, const AttendArgs& p, int keys, i
 inline int AttendBlocks(int values) { return (values + kAttendColumns - 1) / kAttendColumns; }
 
 void LaunchAttend(const AttendArgs& p, int dtype, bool states_alone, hipStream_t stream);
+void LaunchAttendHalf(const AttendArgs& p, int keys, bool states_alone, hipStream_t stream);  // float16
 // What segments add to a state of zeros (`last` of a pass of states alone) becomes the state that they start from, in the order of the pass.
 void LaunchAttendStarts(const AttendArgs& p, int run, const AttendStates& initial, hipStream_t stream);
 

@@ -16,8 +16,9 @@ __device__ __forceinline__ float Finite(float v) { return v - v; }  // 0, or not
 // A workgroup of four waves has 64 columns of v: a wave multiplies 32 rows by 32 columns of y, and has half of the keys and 32 columns of S in its accumulators (a copy is in LDS, for the products with q).
 // P stays in registers: as k q^T its column t is a lane, whose rows s are the reduction of the product v^T P.
 // Products run on the float pipe (v_mfma_f32_32x32x2_f32).
-template <typename T, int KD, bool OUT>
+template <int KD, bool OUT>
 __global__ __launch_bounds__(256) void AttendKernel(AttendArgs p) {
+    using T = float;
     constexpr int KP = KD + 4, VB = kAttendColumns, C = kAttendTile, NS = KD / 64;
     extern __shared__ __align__(16) char lds[];
     float* const ks = reinterpret_cast<float*>(lds);      // [C][KP]
@@ -102,7 +103,7 @@ __global__ __launch_bounds__(256) void AttendKernel(AttendArgs p) {
             }
             *reinterpret_cast<attend4_t*>(vs + row * VB + j) = v;
         }
-        if (wave == 0) SumDecays(dec, lane < here ? AttendStep(p, run, span, b, h, length, r0 + lane) : 0, run.kv_scale);
+        if (wave == 0) SumDecays(dec, lane < here ? AttendStep(p, run, span, b, h, length, r0 + lane) : 0, here, run.kv_scale);
         attend4_t q[OUT ? KD / 8 : 1];
         const int t = 32 * tw + l32;  // this lane's row
         if constexpr (OUT) {
@@ -418,20 +419,18 @@ void LaunchAttend(const AttendArgs& p, int dtype, bool states_alone, hipStream_t
     const int64_t turns = states_alone ? p.segments - 1 : p.segments, blocks = p.blocks * p.batch * p.heads * turns;
     HIPCX_REQUIRE(blocks <= kBlocksPerLaunch, HIPCX_NOT_IMPLEMENTED_ERROR, "linear_attention: too many elements");
     if (blocks == 0) return;
-    VisitAttendType(dtype, [&](auto tag) {
-        using T = typename decltype(tag)::type;
-        VisitKeys(keys, [&](auto kd) {
-            constexpr int KD = decltype(kd)::value, kLds = AttendLds<KD>();
-            const dim3 grid(static_cast<unsigned>(blocks));
-            if (states_alone) {
-                EnsureDynamicLds<AttendTag>(reinterpret_cast<const void*>(AttendKernel<T, KD, false>), kLds);
-                hipLaunchKernelGGL((AttendKernel<T, KD, false>), grid, dim3(256), kLds, stream, p);
-            } else {
-                EnsureDynamicLds<AttendTag>(reinterpret_cast<const void*>(AttendKernel<T, KD, true>), kLds);
-                hipLaunchKernelGGL((AttendKernel<T, KD, true>), grid, dim3(256), kLds, stream, p);
-            }
-            CheckLaunch("linear_attention");
-        });
+    if (dtype == HIPCX_FLOAT16) return LaunchAttendHalf(p, keys, states_alone, stream);
+    VisitKeys(keys, [&](auto kd) {
+        constexpr int KD = decltype(kd)::value, kLds = AttendLds<KD>();
+        const dim3 grid(static_cast<unsigned>(blocks));
+        if (states_alone) {
+            EnsureDynamicLds<AttendTag>(reinterpret_cast<const void*>(AttendKernel<KD, false>), kLds);
+            hipLaunchKernelGGL((AttendKernel<KD, false>), grid, dim3(256), kLds, stream, p);
+        } else {
+            EnsureDynamicLds<AttendTag>(reinterpret_cast<const void*>(AttendKernel<KD, true>), kLds);
+            hipLaunchKernelGGL((AttendKernel<KD, true>), grid, dim3(256), kLds, stream, p);
+        }
+        CheckLaunch("linear_attention");
     });
 }
 
