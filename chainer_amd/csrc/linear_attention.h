@@ -80,11 +80,14 @@ __device__ __forceinline__ AttendPiece<T, N> AttendLoad(const T* row, int at, in
     return r;
 }
 
-// The log decay that takes the state to row t of a pass, in powers of two.  -infinity, a state that ends, is held at a number that no product of decays brings back.
-__device__ __forceinline__ double AttendDecay(const AttendArgs& p, int64_t b, int h, int64_t t) {
-    if (p.decay == nullptr) return 0;
-    const double g = static_cast<double>(p.decay[b * p.decay_batch + t * p.decay_row + h * p.decay_head]) * 1.4426950408889634;
+// A log decay in powers of two.  -infinity, a state that ends, is held at a number that no product of decays brings back.
+__device__ __forceinline__ double LogOfDecay(float decay) {
+    const double g = static_cast<double>(decay) * 1.4426950408889634;
     return g < -0x1p20 ? -0x1p20 : g;
+}
+// The one that takes the state to row t of a pass.
+__device__ __forceinline__ double AttendDecay(const AttendArgs& p, int64_t b, int h, int64_t t) {
+    return p.decay != nullptr ? LogOfDecay(p.decay[b * p.decay_batch + t * p.decay_row + h * p.decay_head]) : 0;
 }
 
 // The decays of a tile's rows, summed up from its first: as a float and what the float leaves out, so that differences are as good as a float's for any sum.

@@ -448,12 +448,15 @@ void LaunchAttendStarts(const AttendArgs& p, int which, const AttendStates& init
 
 namespace {
 
+constexpr int64_t kMaxAttendRow = int64_t{1} << 24;  // elements from one row to the next: a tile's offsets have 32 bits
+
 // Rows [batch, time, heads, elements]; a stride along an axis of one says nothing.
 AttendRows AttendRowsOf(const hipcx_array* a, int heads, const std::string& what) {
     const int64_t it = ItemSize(a->dtype);
     HIPCX_REQUIRE(TotalSize(a) == 0 || a->shape[3] == 1 || a->strides[3] == it, HIPCX_DIMENSION_ERROR, what + ": the last axis must be dense");
     for (int i = 0; i < 3; ++i) HIPCX_REQUIRE(a->strides[i] % it == 0 || a->shape[i] <= 1, HIPCX_DIMENSION_ERROR, what + ": strides must be whole elements");
     const auto stride = [&](int i) { return a->shape[i] > 1 ? a->strides[i] / it : 0; };
+    HIPCX_REQUIRE(std::abs(stride(1)) < kMaxAttendRow, HIPCX_NOT_IMPLEMENTED_ERROR, what + ": rows 2^24 elements apart or more");
     return {a->data, stride(0), stride(1), stride(2), heads / static_cast<int>(std::max<int64_t>(1, a->shape[2]))};
 }
 

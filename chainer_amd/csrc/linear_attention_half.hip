@@ -63,11 +63,12 @@ struct AttendHalfLds {
 };
 
 // As AttendKernel (linear_attention.hip): a wave multiplies 32 rows by 32 columns of y, and has half of the keys and 32 columns of the state in its accumulators.
-//   P^T = K Q^T (rows s, a lane to a row t) from float16 as they come; times the weights, brought to float16's range by a power of two for each t, in two parts;
-//   y^T = V^T P^T + S^T Q^T, S in two parts of float16 in LDS, with a power of two for each column and half of the keys;
+//   y^T = S^T Q^T, S in two parts of float16 in LDS, with a power of two for each column and half of the keys;
+//   P^T = K Q^T (rows s, a lane to a row t) from float16 as they come; times the weights, brought to float16's range by a power of two for each t, in two parts; y^T += V^T P^T;
 //   S <- exp(G[63]) S + K^T (exp(G[63] - G) V), V's products in two parts, with a power of two for each column.
 // A reduction over rows s takes them in the order in which accumulators have them, eight to a lane: 4 h + j and 8 + 4 h + j of sixteen, for both operands.
-template <int KD, bool OUT>
+// EVEN: rows of whole pieces of eight elements.  GRAD: what the passes of the gradients have beyond the forward one.
+template <int KD, bool OUT, bool EVEN, bool GRAD>
 __global__ __launch_bounds__(256, KD == 256 ? 1 : 2) void AttendHalfKernel(AttendArgs p) {
     using T = half_t;
     using Lds = AttendHalfLds<KD>;
@@ -85,37 +86,50 @@ __global__ __launch_bounds__(256, KD == 256 ? 1 : 2) void AttendHalfKernel(Atten
     const int bh = id % static_cast<int>(p.batch * p.heads);
     const int segment_turn = id / static_cast<int>(p.batch * p.heads);
     int which = 0;
-    while (which + 1 < p.runs && block >= p.run[which + 1].first) ++which;
-    const AttendRun& run = p.run[which];
-    const int segment = run.back ? p.segments - 1 - segment_turn : segment_turn;
+    if (GRAD) {
+        while (which + 1 < p.runs && block >= p.run[which + 1].first) ++which;
+    }
+    const AttendRun& run = p.run[GRAD ? which : 0];
+    const bool back = GRAD && run.back != 0, wide = GRAD && run.wide != 0, with_dots = GRAD && OUT && run.dots != nullptr;
+    const float kv_scale = GRAD ? run.kv_scale : 1.f;
+    const int segment = back ? p.segments - 1 - segment_turn : segment_turn;
     const int64_t b = bh / p.heads;
     const int h = bh % p.heads;
     const int64_t length = LengthOf(p.lengths, b, p.length);
     const AttendSpan span(p, length, segment);
     const int64_t rows = span.end - span.first;
-    const int keys = run.keys, col0 = (block - run.first) * VB, cols = min(VB, run.values - col0);
+    int keys = run.keys;
+    const int col0 = (block - run.first) * VB, cols = min(VB, run.values - col0);
 
-    const int tid = threadIdx.x, lane = tid % 64, wave = tid / 64, l32 = lane % 32, half = lane / 32;
-    const int tw = wave / 2, dw = wave % 2;
-    const T* const kp = static_cast<const T*>(run.k.data) + b * run.k.batch + (h / run.k.share) * run.k.head;
-    const T* const vp = static_cast<const T*>(run.v.data) + b * run.v.batch + (h / run.v.share) * run.v.head + col0;
-    const T* const qp = OUT ? static_cast<const T*>(run.q.data) + b * run.q.batch + (h / run.q.share) * run.q.head : nullptr;
-    const T* const dp = OUT && run.dots != nullptr ? static_cast<const T*>(run.dot.data) + b * run.dot.batch + (h / run.dot.share) * run.dot.head + col0 : nullptr;
-    const int64_t y0 = OUT ? b * run.y.batch + h * run.y.head + col0 : 0;
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / 64), tw = wave / 2, dw = wave % 2;
+    int lane = tid % 64;
+    // What follows from the lane is found again in every tile: kept over the loop, it would take the registers of what is multiplied.
+    const auto in_tile = [&] { return lane % 32; };
+    const auto upper = [&] { return lane / 32; };
     const int parts = 2 * run.blocks;
-    float* const dots = OUT && run.dots != nullptr ? run.dots + static_cast<int64_t>(bh) * p.length * parts + (block - run.first) * 2 : nullptr;
+    const auto dots = [&] { return run.dots + static_cast<int64_t>(bh) * p.length * parts + (block - run.first) * 2; };
 
-    const auto state_row = [&](int n, int r) { return KD / 2 * tw + 32 * n + 8 * (r / 4) + 4 * half + r % 4; };
-    const int state_col = 32 * dw + l32;
+    const auto state_row = [&](int n, int r) { return KD / 2 * tw + 32 * n + 8 * (r / 4) + 4 * upper() + r % 4; };
+    const auto state_col = [&] { return 32 * dw + in_tile(); };
     attend16_t s[NS];
 #pragma unroll
     for (int n = 0; n < NS; ++n) {
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
-            const int i = state_row(n, r);
-            s[n][r] = OUT && run.start.data != nullptr && i < keys && state_col < cols
-                          ? run.start.data[bh * run.start.head + segment * run.start.segment + i * run.start.i + (col0 + state_col) * run.start.j]
-                          : 0.f;
+            s[n][r] = 0;
+        }
+    }
+    // elements that are not there are read as the last ones: all loads go out at once
+    const auto state_at = [&](const AttendStates& of, int n, int r) {
+        const int i = state_row(n, r);
+        const float v = of.data[bh * of.head + segment * of.segment + min(i, keys - 1) * of.i + (col0 + min(state_col(), cols - 1)) * of.j];
+        return i < keys && state_col() < cols ? v : 0.f;
+    };
+    if (OUT && run.start.data != nullptr) {
+#pragma unroll
+        for (int n = 0; n < NS; ++n) {
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s[n][r] = state_at(run.start, n, r);
         }
     }
     const auto keep_state = [&] {
@@ -127,7 +141,7 @@ __global__ __launch_bounds__(256, KD == 256 ? 1 : 2) void AttendHalfKernel(Atten
         }
         most = fmaxf(most, __shfl_xor(most, 32));
         const Scale scale(most);
-        if (half == 0) scales[tw * VB + state_col] = scale.out;
+        if (upper() == 0) scales[tw * VB + state_col()] = scale.out;
 #pragma unroll
         for (int n = 0; n < NS; ++n) {
 #pragma unroll
@@ -135,7 +149,7 @@ __global__ __launch_bounds__(256, KD == 256 ? 1 : 2) void AttendHalfKernel(Atten
                 const float v[4] = {s[n][4 * g] * scale.in, s[n][4 * g + 1] * scale.in, s[n][4 * g + 2] * scale.in, s[n][4 * g + 3] * scale.in};
                 attend_half4_t hi, lo;
                 Split(v, &hi, &lo);
-                const int at = state_col * Lds::kStatePitch + state_row(n, 4 * g) * 2;
+                const int at = state_col() * Lds::kStatePitch + state_row(n, 4 * g) * 2;
                 *reinterpret_cast<attend_half4_t*>(high_copy + at) = hi;
                 *reinterpret_cast<attend_half4_t*>(low_copy + at) = lo;
             }
@@ -143,65 +157,60 @@ __global__ __launch_bounds__(256, KD == 256 ? 1 : 2) void AttendHalfKernel(Atten
     };
     if (OUT) keep_state();
 
-    // A tile's rows on their way: pieces of eight elements of k and of v, and this lane's row of q.  Rows that are not there are the last one again; columns that are not there are zeros that
-    // stay in LDS.
+    // A tile's rows on their way: pieces of eight elements of k and of v.  Rows that are not there are the last one again; columns that are not there are zeros that stay in LDS.  Rows lie less
+    // than 2^24 elements apart, so that a tile's are within 32 bits of its first.
     const int key_row = tid / (KD / 8), key_col = tid % (KD / 8) * 8, value_row = tid / (VB / 8), value_col = tid % (VB / 8) * 8;
-    const bool even = keys % 8 == 0 && cols % 8 == 0;
-    const int t = 32 * tw + l32;  // this lane's row of a tile
-    attend_half8_t k_next[NK], v_next[NV], q_next[OUT ? NQ : 1];
-    double g_next = 0;
-    const auto load = [&](int64_t r0) {
-        const auto at = [&](int64_t r) { return AttendRowOf(span, run.back, r0 + r < rows ? r0 + r : rows - 1); };
-        if (even) {
+    const auto own_row = [&] { return 32 * tw + in_tile(); };  // of a tile
+    const int way = back ? -1 : 1;
+    const int64_t row0 = back ? span.end - 1 : span.first;
+    const T* kp = static_cast<const T*>(run.k.data) + b * run.k.batch + (h / run.k.share) * run.k.head + row0 * run.k.row;
+    const T* vp = static_cast<const T*>(run.v.data) + b * run.v.batch + (h / run.v.share) * run.v.head + row0 * run.v.row + col0;
+    const T* qp = OUT ? static_cast<const T*>(run.q.data) + b * run.q.batch + (h / run.q.share) * run.q.head + row0 * run.q.row : nullptr;
+    const int k_row = way * static_cast<int>(run.k.row), v_row = way * static_cast<int>(run.v.row), q_row = OUT ? way * static_cast<int>(run.q.row) : 0;
+    // of y and the rows that its products are wanted with, too
+    char* yp = OUT ? static_cast<char*>(run.y.data) + (b * run.y.batch + h * run.y.head + row0 * run.y.row + col0) * (wide ? 4 : 2) : nullptr;
+    const int y_row = OUT ? way * static_cast<int>(run.y.row) * (wide ? 4 : 2) : 0;
+    const T* dp = with_dots ? static_cast<const T*>(run.dot.data) + b * run.dot.batch + (h / run.dot.share) * run.dot.head + row0 * run.dot.row + col0 : nullptr;
+    const int d_row = with_dots ? way * static_cast<int>(run.dot.row) : 0;
+    const float* gp = p.decay != nullptr ? p.decay + b * p.decay_batch + h * p.decay_head + (row0 + (back ? 1 : 0)) * p.decay_row : nullptr;
+    const int64_t g_row = way * p.decay_row;
+    const int64_t g_rows = back && span.end == length ? 1 : 0;  // the first row has no decay: none follows it
+    attend_half8_t k_next[NK], v_next[NV], q[OUT ? NQ : 1];
+    const auto piece_at = [&](const T* row, int col, int end) {
+        AttendPiece<T, 8> piece;
+        if constexpr (EVEN) piece = *reinterpret_cast<const AttendPiece<T, 8>*>(row + (col < end ? col : 0));
+        else piece = AttendLoad<T, 8>(row, col, end);
+        attend_half8_t v;
 #pragma unroll
-            for (int n = 0; n < NK; ++n) {
-                const AttendPiece<T, 8> piece = *reinterpret_cast<const AttendPiece<T, 8>*>(kp + at(key_row + n * (2048 / KD)) * run.k.row + (key_col < keys ? key_col : 0));
-#pragma unroll
-                for (int e = 0; e < 8; ++e) k_next[n][e] = piece.v[e];
-            }
-#pragma unroll
-            for (int n = 0; n < NV; ++n) {
-                const AttendPiece<T, 8> piece = *reinterpret_cast<const AttendPiece<T, 8>*>(vp + at(value_row + n * 32) * run.v.row + (value_col < cols ? value_col : 0));
-#pragma unroll
-                for (int e = 0; e < 8; ++e) v_next[n][e] = piece.v[e];
-            }
-            if constexpr (OUT) {
-                const T* const q = qp + at(t) * run.q.row;
-#pragma unroll
-                for (int m = 0; m < NQ; ++m) {
-                    const int i = 16 * m + 8 * half;
-                    const AttendPiece<T, 8> piece = *reinterpret_cast<const AttendPiece<T, 8>*>(q + (i < keys ? i : 0));
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) q_next[m][e] = piece.v[e];
-                }
-            }
-        } else {
-#pragma unroll
-            for (int n = 0; n < NK; ++n) {
-                const AttendPiece<T, 8> piece = AttendLoad<T, 8>(kp + at(key_row + n * (2048 / KD)) * run.k.row, key_col, keys);
-#pragma unroll
-                for (int e = 0; e < 8; ++e) k_next[n][e] = piece.v[e];
-            }
-#pragma unroll
-            for (int n = 0; n < NV; ++n) {
-                const AttendPiece<T, 8> piece = AttendLoad<T, 8>(vp + at(value_row + n * 32) * run.v.row, value_col, cols);
-#pragma unroll
-                for (int e = 0; e < 8; ++e) v_next[n][e] = piece.v[e];
-            }
-            if constexpr (OUT) {
-                const T* const q = qp + at(t) * run.q.row;
-#pragma unroll
-                for (int m = 0; m < NQ; ++m) {
-                    const AttendPiece<T, 8> piece = AttendLoad<T, 8>(q, 16 * m + 8 * half, keys);
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) q_next[m][e] = piece.v[e];
-                }
-            }
-        }
-        g_next = r0 + lane < rows ? AttendStep(p, run, span, b, h, length, r0 + lane) : 0;
+        for (int e = 0; e < 8; ++e) v[e] = piece.v[e];
+        return v;
     };
-    const auto sum_next = [&](int64_t r0, AttendDecays* to) { SumDecays(to, g_next, static_cast<int>(rows - r0 < C ? rows - r0 : C), run.kv_scale); };
-    if (even) {
+    const auto load = [&](int64_t r0) {  // k and v; at the tile's first row
+        const int last = static_cast<int>(rows - r0 < C ? rows - r0 : C) - 1;
+#pragma unroll
+        for (int n = 0; n < NK; ++n) k_next[n] = piece_at(kp + min(key_row + n * (2048 / KD), last) * k_row, key_col, keys);
+#pragma unroll
+        for (int n = 0; n < NV; ++n) v_next[n] = piece_at(vp + min(value_row + n * 32, last) * v_row, value_col, cols);
+        kp += static_cast<int64_t>(k_row) * C, vp += static_cast<int64_t>(v_row) * C;
+    };
+    const auto load_q = [&](int64_t r0) {
+        if constexpr (OUT) {
+            const T* const at = qp + min(own_row(), static_cast<int>(rows - r0 < C ? rows - r0 : C) - 1) * q_row;
+#pragma unroll
+            for (int m = 0; m < NQ; ++m) q[m] = piece_at(at, 16 * m + 8 * upper(), keys);
+            qp += static_cast<int64_t>(q_row) * C;
+        }
+    };
+    float g_next = 0;
+    const auto load_decays = [&](int64_t r0) {  // of a row that is there; sum_next takes those that count
+        const int64_t r = r0 + lane < rows ? r0 + lane : rows - 1;
+        if (gp != nullptr) g_next = gp[(r < g_rows ? g_rows : r) * g_row * (rows > g_rows ? 1 : 0)];
+    };
+    const auto sum_next = [&](int64_t r0, AttendDecays* to) {  // by one wave
+        const int here = static_cast<int>(rows - r0 < C ? rows - r0 : C);
+        SumDecays(to, gp != nullptr && lane < here && r0 + lane >= g_rows ? LogOfDecay(g_next) : 0, here, kv_scale);
+    };
+    if (EVEN) {
 #pragma unroll
         for (int n = 0; n < NK; ++n) {
             if (key_col >= keys) *reinterpret_cast<attend_half8_t*>(ks + (key_row + n * (2048 / KD)) * Lds::kKeyPitch + key_col * 2) = attend_half8_t{};
@@ -214,131 +223,126 @@ __global__ __launch_bounds__(256, KD == 256 ? 1 : 2) void AttendHalfKernel(Atten
     if (tid == 0) odd[0] = odd[1] = 0;
     if (rows > 0) {
         load(0);
-        if (wave == 0) sum_next(0, decays);
+        load_q(0);
+        if (wave == 3) load_decays(0), sum_next(0, decays);
     }
     double passed = 0;  // log decay of the tiles so far
-    // where a lane reads blocks of 4 x 16: rows 4 half and on, columns of its 32
-    const int turned_row = 4 * half + lane % 16 / 4, turned_col = (lane / 16 % 2 * 16 + lane % 4 * 4) * 2;
+    // where a lane reads blocks of 4 x 16: rows 4 upper() and on, columns of its 32
+    const auto turned_row = [&] { return 4 * upper() + lane % 16 / 4; };
+    const auto turned_col = [&] { return (lane / 16 % 2 * 16 + lane % 4 * 4) * 2; };
 
     int turn = 0;
+    int64_t r0 = 0;
     __syncthreads();  // the flags
-    for (int64_t r0 = 0; r0 < rows; r0 += C, turn ^= 1) {
-        const int here = static_cast<int>(rows - r0 < C ? rows - r0 : C);
+    for (; r0 < rows; r0 += C, turn ^= 1) {
+        asm volatile("" : "+v"(lane));
+        asm volatile("" : "+s"(keys));
         const AttendDecays* const dec = decays + turn;
-        attend_half8_t q[OUT ? NQ : 1];
         // (the last tile's rows of k and v have been read by all)
 #pragma unroll
         for (int n = 0; n < NK; ++n) {
-            if (!even || key_col < keys) *reinterpret_cast<attend_half8_t*>(ks + (key_row + n * (2048 / KD)) * Lds::kKeyPitch + key_col * 2) = k_next[n];
+            if (!EVEN || key_col < keys) *reinterpret_cast<attend_half8_t*>(ks + (key_row + n * (2048 / KD)) * Lds::kKeyPitch + key_col * 2) = k_next[n];
         }
         attend_half8_t finite{};
 #pragma unroll
         for (int n = 0; n < NV; ++n) {
-            if (!even || value_col < cols) *reinterpret_cast<attend_half8_t*>(vs + (value_row + n * 32) * Lds::kValuePitch + value_col * 2) = v_next[n];
+            if (!EVEN || value_col < cols) *reinterpret_cast<attend_half8_t*>(vs + (value_row + n * 32) * Lds::kValuePitch + value_col * 2) = v_next[n];
             finite += v_next[n] - v_next[n];
         }
         if constexpr (OUT) {
             const T all = finite[0] + finite[1] + finite[2] + finite[3] + finite[4] + finite[5] + finite[6] + finite[7];
             if (all != 0) odd[turn] = 1;
-#pragma unroll
-            for (int m = 0; m < NQ; ++m) q[m] = q_next[m];
         }
         __syncthreads();
         passed += dec->sum;
+        // An infinity of a later row, times P's zeros, would reach earlier ones: the rest goes row by row.
+        if (OUT && odd[turn] != 0) break;
         const bool more = r0 + C < rows;
-        if (more) load(r0 + C);
-        if (OUT && odd[turn] != 0) {
-            // An infinity of a later row, times P's zeros, would reach earlier ones: row by row instead, on a copy of the state in 32 bits in the place of the others.
-            float* const ss = reinterpret_cast<float*>(high_copy);  // [KD][VB]
-#pragma unroll
-            for (int n = 0; n < NS; ++n) {
-#pragma unroll
-                for (int r = 0; r < 16; ++r) ss[state_row(n, r) * VB + state_col] = s[n][r];
-            }
-            if (wave == 0 && more) sum_next(r0 + C, decays + (turn ^ 1));
-            if (tid == 0) odd[turn ^ 1] = 0;
-            __syncthreads();
-            const int j = lane;
-            for (int r = 0; r < here; ++r) {
-                const int64_t row = AttendRowOf(span, run.back, r0 + r);
-                const float step = dec->step[r], v = static_cast<float>(*reinterpret_cast<const T*>(vs + r * Lds::kValuePitch + j * 2)) * run.kv_scale;
-                float y = 0;
-                for (int i = wave * (KD / 4); i < (wave + 1) * (KD / 4); ++i) {
-                    const float now = ss[i * VB + j] * step + static_cast<float>(*reinterpret_cast<const T*>(ks + r * Lds::kKeyPitch + i * 2)) * v;
-                    ss[i * VB + j] = now;
-                    if (i < keys) y += static_cast<float>(qp[row * run.q.row + i]) * now;
-                }
-                sums[wave * VB + j] = y;
-                __syncthreads();
-                if (wave == 0) {
-                    y = (sums[j] + sums[VB + j] + sums[2 * VB + j] + sums[3 * VB + j]) * run.out_scale;
-                    if (j < cols) {
-                        if (run.wide) static_cast<float*>(run.y.data)[y0 + row * run.y.row + j] = y;
-                        else static_cast<T*>(run.y.data)[y0 + row * run.y.row + j] = static_cast<T>(y);
-                    }
-                    if (dots != nullptr) {
-                        float dot = j < cols ? y * static_cast<float>(dp[row * run.dot.row + j]) : 0.f;
-#pragma unroll
-                        for (int o = 1; o < 32; o <<= 1) dot += __shfl_xor(dot, o);
-                        if (l32 == 0) dots[row * parts + half] = dot;
-                    }
-                }
-                __syncthreads();
-            }
-#pragma unroll
-            for (int n = 0; n < NS; ++n) {
-#pragma unroll
-                for (int r = 0; r < 16; ++r) s[n][r] = ss[state_row(n, r) * VB + state_col];
-            }
-            __syncthreads();
-            keep_state();
-            continue;
+        if (more) {
+            load(r0 + C);
+            if (wave == 3) load_decays(r0 + C);
         }
-        // this wave's columns of v, for the products with P and with k: rows 16 u + ... of step u
         attend_half8_t v[C / 16];
+        const auto read_v = [&] {  // this wave's columns, for the products with P and with k: rows 16 u + ... of step u
 #pragma unroll
-        for (int u = 0; u < C / 16; ++u) {
-            const char* const at = vs + (16 * u + turned_row) * Lds::kValuePitch + dw * 64 + turned_col;
-            v[u] = Join(ReadTurned(at), ReadTurned(at + 8 * Lds::kValuePitch));
-        }
+            for (int u = 0; u < C / 16; ++u) {
+                const char* const at = vs + (16 * u + turned_row()) * Lds::kValuePitch + dw * 64 + turned_col();
+                v[u] = Join(ReadTurned(at), ReadTurned(at + 8 * Lds::kValuePitch));
+            }
+        };
         if constexpr (OUT) {
-            attend16_t a[2]{}, of_state[2]{};
+            attend16_t y;
+            attend16_t a[2]{};
+            const float high = dec->high[own_row()], low = dec->low[own_row()];
+            {
+                attend16_t of_state[2]{};
+                const int at = state_col() * Lds::kStatePitch + 16 * upper();
+                attend_half8_t part[2][2];
+                const auto read = [&](int m, attend_half8_t (&to)[2]) {
+                    to[0] = *reinterpret_cast<const attend_half8_t*>(low_copy + at + 32 * m);
+                    to[1] = *reinterpret_cast<const attend_half8_t*>(high_copy + at + 32 * m);
+                };
+                read(0, part[0]);
+#pragma unroll
+                for (int m = 0; m < NQ; ++m) {  // reads of the next step under the products of this one
+                    if (m + 1 < NQ) read(m + 1, part[m % 2 ^ 1]);
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) of_state[m / (NQ / 2)] = Mfma(part[m % 2][i], q[m], of_state[m / (NQ / 2)]);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+                const float from_start = __builtin_amdgcn_exp2f(high + low) * run.out_scale;
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {
+                    const int j = 32 * dw + 8 * g + 4 * upper();
+                    const attend4_t first = *reinterpret_cast<const attend4_t*>(scales + j), second = *reinterpret_cast<const attend4_t*>(scales + VB + j);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) y[4 * g + e] = __builtin_fmaf(of_state[0][4 * g + e], first[e], of_state[1][4 * g + e] * second[e]) * from_start;
+                }
+            }
+            __builtin_amdgcn_sched_barrier(0);  // (the products with the state need as many registers as those with k)
 #pragma unroll
             for (int sb = 0; sb < 2; ++sb) {
                 if (sb > tw) continue;
-                const char* const at = ks + (32 * sb + l32) * Lds::kKeyPitch + 16 * half;
+                const char* const at = ks + (32 * sb + in_tile()) * Lds::kKeyPitch + 16 * upper();
+                attend_half8_t part[2][2];
+                const auto read = [&](int m, attend_half8_t (&to)[2]) {
 #pragma unroll
-                for (int m = 0; m < NQ; ++m) a[sb] = Mfma(*reinterpret_cast<const attend_half8_t*>(at + 32 * m), q[m], a[sb]);
-            }
-            {
-                const int at = state_col * Lds::kStatePitch + 16 * half;
+                    for (int i = 0; i < 2; ++i) to[i] = *reinterpret_cast<const attend_half8_t*>(at + 32 * (m + i));
+                };
+                read(0, part[0]);
 #pragma unroll
-                for (int m = 0; m < NQ; ++m) {
-                    attend16_t& to = of_state[m / (NQ / 2)];
-                    to = Mfma(*reinterpret_cast<const attend_half8_t*>(low_copy + at + 32 * m), q[m], to);
-                    to = Mfma(*reinterpret_cast<const attend_half8_t*>(high_copy + at + 32 * m), q[m], to);
+                for (int m = 0; m < NQ; m += 2) {
+                    if (m + 2 < NQ) read(m + 2, part[m / 2 % 2 ^ 1]);
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) a[sb] = Mfma(part[m / 2 % 2][i], q[m + i], a[sb]);
+                    __builtin_amdgcn_sched_barrier(0);
                 }
             }
             if (wave == 3 && more) sum_next(r0 + C, decays + (turn ^ 1));
             if (tid == 0) odd[turn ^ 1] = 0;
-            const float high = dec->high[t], low = dec->low[t];
             float most = 0;
+            const int own = in_tile() - 4 * upper();  // of this lane's 32 rows, how far its own is behind its half's
 #pragma unroll
             for (int sb = 0; sb < 2; ++sb) {
                 if (sb > tw) continue;
 #pragma unroll
                 for (int g = 0; g < 4; ++g) {
-                    const int first = 32 * sb + 8 * g + 4 * half;
+                    const int first = 32 * sb + 8 * g + 4 * upper();
                     const attend4_t highs = *reinterpret_cast<const attend4_t*>(dec->high + first), lows = *reinterpret_cast<const attend4_t*>(dec->low + first);
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const float weighted = a[sb][4 * g + e] * __builtin_amdgcn_exp2f((high - highs[e]) + (low - lows[e]));
-                        a[sb][4 * g + e] = first + e <= t ? weighted : 0.f;
-                        most = fmaxf(most, fabsf(a[sb][4 * g + e]));
-                    }
+                    for (int e = 0; e < 4; ++e) a[sb][4 * g + e] *= __builtin_amdgcn_exp2f((high - highs[e]) + (low - lows[e]));
                 }
+                __builtin_amdgcn_sched_barrier(0);
+                if (sb == tw) {
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) a[sb][r] = 8 * (r / 4) + r % 4 <= own ? a[sb][r] : 0.f;
+                }
+#pragma unroll
+                for (int r = 0; r < 16; ++r) most = fmaxf(most, fabsf(a[sb][r]));
             }
             const Scale scale(fmaxf(most, __shfl_xor(most, 32)));
+            __builtin_amdgcn_sched_barrier(0);
+            read_v();
             attend16_t of_rows{};
 #pragma unroll
             for (int sb = 0; sb < 2; ++sb) {
@@ -354,56 +358,62 @@ __global__ __launch_bounds__(256, KD == 256 ? 1 : 2) void AttendHalfKernel(Atten
                     of_rows = Mfma(v[2 * sb + u], hi, of_rows);
                 }
             }
-            const float from_start = __builtin_amdgcn_exp2f(high + low) * run.out_scale, from_rows = scale.out * run.kv_scale * run.out_scale;
-            const int64_t row = AttendRowOf(span, run.back, r0 + t);
+            const float from_rows = scale.out * kv_scale * run.out_scale;
+            char* const to = yp + static_cast<int64_t>(own_row()) * y_row;
+            const bool live = r0 + own_row() < rows;
             float dot = 0;
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
-                const int j = 32 * dw + 8 * g + 4 * half;
-                const attend4_t first = *reinterpret_cast<const attend4_t*>(scales + j), second = *reinterpret_cast<const attend4_t*>(scales + VB + j);
-                AttendPiece<float, 4> y;
+                const int j = 32 * dw + 8 * g + 4 * upper();
+                AttendPiece<float, 4> out;
 #pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    y.v[e] = __builtin_fmaf(__builtin_fmaf(of_state[0][4 * g + e], first[e], of_state[1][4 * g + e] * second[e]), from_start, of_rows[4 * g + e] * from_rows);
-                if (t >= here) continue;
-                if (dots != nullptr) {
-                    const AttendPiece<T, 4> with = AttendLoad<T, 4>(dp + row * run.dot.row, j, cols);
+                for (int e = 0; e < 4; ++e) out.v[e] = __builtin_fmaf(of_rows[4 * g + e], from_rows, y[4 * g + e]);
+                if (!live) continue;
+                if (with_dots) {
+                    AttendPiece<T, 4> with{};
+                    const T* const row = dp + static_cast<int64_t>(own_row()) * d_row;
+                    if (!EVEN) with = AttendLoad<T, 4>(row, j, cols);
+                    else if (j < cols) with = *reinterpret_cast<const AttendPiece<T, 4>*>(row + j);
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) dot += j + e < cols ? y.v[e] * static_cast<float>(with.v[e]) : 0.f;
+                    for (int e = 0; e < 4; ++e) dot += j + e < cols ? out.v[e] * static_cast<float>(with.v[e]) : 0.f;
                 }
-                const int64_t to = y0 + row * run.y.row + j;
-                if (j + 4 <= cols) {
-                    if (run.wide) {
-                        *reinterpret_cast<AttendPiece<float, 4>*>(static_cast<float*>(run.y.data) + to) = y;
+                if (EVEN ? j < cols : j + 4 <= cols) {
+                    if (wide) {
+                        *reinterpret_cast<AttendPiece<float, 4>*>(to + j * 4) = out;
                     } else {
                         AttendPiece<T, 4> o;
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) o.v[e] = static_cast<T>(y.v[e]);
-                        *reinterpret_cast<AttendPiece<T, 4>*>(static_cast<T*>(run.y.data) + to) = o;
+                        for (int e = 0; e < 4; ++e) o.v[e] = static_cast<T>(out.v[e]);
+                        *reinterpret_cast<AttendPiece<T, 4>*>(to + j * 2) = o;
                     }
-                } else {
+                } else if (!EVEN) {
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         if (j + e >= cols) continue;
-                        if (run.wide) static_cast<float*>(run.y.data)[to + e] = y.v[e];
-                        else static_cast<T*>(run.y.data)[to + e] = static_cast<T>(y.v[e]);
+                        if (wide) reinterpret_cast<float*>(to)[j + e] = out.v[e];
+                        else reinterpret_cast<T*>(to)[j + e] = static_cast<T>(out.v[e]);
                     }
                 }
             }
-            if (dots != nullptr) {
+            if (with_dots) {
                 dot += __shfl_xor(dot, 32);
-                if (half == 0 && t < here) dots[row * parts + dw] = dot;
+                if (upper() == 0 && live) dots()[(row0 + way * (r0 + own_row())) * parts + dw] = dot;
+                dp += static_cast<int64_t>(d_row) * C;
             }
+            yp += static_cast<int64_t>(y_row) * C;
         } else {
+            read_v();
             if (wave == 3 && more) sum_next(r0 + C, decays + (turn ^ 1));
         }
+        __builtin_amdgcn_sched_barrier(0);
+        if (more) load_q(r0 + C);
         // v times its rows' weights, in two parts
         float w[C / 16][8], most = 0;
 #pragma unroll
         for (int u = 0; u < C / 16; ++u) {
 #pragma unroll
             for (int g = 0; g < 2; ++g) {
-                const attend4_t end = *reinterpret_cast<const attend4_t*>(dec->end + 16 * u + 8 * g + 4 * half);
+                const attend4_t end = *reinterpret_cast<const attend4_t*>(dec->end + 16 * u + 8 * g + 4 * upper());
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     w[u][4 * g + e] = static_cast<float>(v[u][4 * g + e]) * end[e];
@@ -413,18 +423,29 @@ __global__ __launch_bounds__(256, KD == 256 ? 1 : 2) void AttendHalfKernel(Atten
         }
         const Scale scale(fmaxf(most, __shfl_xor(most, 32)));
         attend16_t add[NS]{};
+        {
+            attend_half8_t k[2][NS];
+            const auto read = [&](int u, attend_half8_t (&to)[NS]) {
 #pragma unroll
-        for (int u = 0; u < C / 16; ++u) {
+                for (int n = 0; n < NS; ++n) {
+                    const char* const at = ks + (16 * u + turned_row()) * Lds::kKeyPitch + (KD / 2 * tw + 32 * n) * 2 + turned_col();
+                    to[n] = Join(ReadTurned(at), ReadTurned(at + 8 * Lds::kKeyPitch));
+                }
+            };
+            read(0, k[0]);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) w[u][e] *= scale.in;
-            attend_half8_t hi, lo;
-            Split(w[u], &hi, &lo);
+            for (int u = 0; u < C / 16; ++u) {
+                if (u + 1 < C / 16) read(u + 1, k[u % 2 ^ 1]);
 #pragma unroll
-            for (int n = 0; n < NS; ++n) {
-                const char* const at = ks + (16 * u + turned_row) * Lds::kKeyPitch + (KD / 2 * tw + 32 * n) * 2 + turned_col;
-                const attend_half8_t k = Join(ReadTurned(at), ReadTurned(at + 8 * Lds::kKeyPitch));
-                add[n] = Mfma(k, lo, add[n]);
-                add[n] = Mfma(k, hi, add[n]);
+                for (int e = 0; e < 8; ++e) w[u][e] *= scale.in;
+                attend_half8_t hi, lo;
+                Split(w[u], &hi, &lo);
+#pragma unroll
+                for (int n = 0; n < NS; ++n) {
+                    add[n] = Mfma(k[u % 2][n], lo, add[n]);
+                    add[n] = Mfma(k[u % 2][n], hi, add[n]);
+                }
+                __builtin_amdgcn_sched_barrier(0);
             }
         }
         const float all = dec->all;
@@ -437,6 +458,53 @@ __global__ __launch_bounds__(256, KD == 256 ? 1 : 2) void AttendHalfKernel(Atten
         if (OUT) keep_state();
     }
 
+    if (OUT && r0 < rows) {
+        // row by row, on a copy of the state in 32 bits in the place of the others
+        float* const ss = reinterpret_cast<float*>(high_copy);  // [KD][VB]
+#pragma unroll
+        for (int n = 0; n < NS; ++n) {
+#pragma unroll
+            for (int r = 0; r < 16; ++r) ss[state_row(n, r) * VB + state_col()] = s[n][r];
+        }
+        __syncthreads();
+        const int j = lane;
+        for (; r0 < rows; ++r0) {
+            const int64_t row = row0 + way * r0;
+            const T* const k = static_cast<const T*>(run.k.data) + b * run.k.batch + (h / run.k.share) * run.k.head + row * run.k.row;
+            const T* const x = static_cast<const T*>(run.q.data) + b * run.q.batch + (h / run.q.share) * run.q.head + row * run.q.row;
+            const T* const of_v = static_cast<const T*>(run.v.data) + b * run.v.batch + (h / run.v.share) * run.v.head + row * run.v.row + col0;
+            const float step = gp != nullptr && r0 >= g_rows ? __builtin_amdgcn_exp2f(static_cast<float>(LogOfDecay(gp[r0 * g_row]))) : 1.f, v = j < cols ? static_cast<float>(of_v[j]) * kv_scale : 0.f;
+            float y = 0;
+            for (int i = wave * (KD / 4); i < (wave + 1) * (KD / 4) && i < keys; ++i) {
+                const float now = ss[i * VB + j] * step + static_cast<float>(k[i]) * v;
+                ss[i * VB + j] = now;
+                y += static_cast<float>(x[i]) * now;
+            }
+            sums[wave * VB + j] = y;
+            __syncthreads();
+            if (wave == 0) {
+                y = (sums[j] + sums[VB + j] + sums[2 * VB + j] + sums[3 * VB + j]) * run.out_scale;
+                const int64_t to = b * run.y.batch + h * run.y.head + row * run.y.row + col0 + j;
+                if (j < cols) {
+                    if (wide) static_cast<float*>(run.y.data)[to] = y;
+                    else static_cast<T*>(run.y.data)[to] = static_cast<T>(y);
+                }
+                if (with_dots) {
+                    float dot = 0;
+                    if (j < cols) dot = y * static_cast<float>((static_cast<const T*>(run.dot.data) + b * run.dot.batch + (h / run.dot.share) * run.dot.head + row * run.dot.row + col0)[j]);
+#pragma unroll
+                    for (int o = 1; o < 32; o <<= 1) dot += __shfl_xor(dot, o);
+                    if (in_tile() == 0) dots()[row * parts + upper()] = dot;
+                }
+            }
+            __syncthreads();
+        }
+#pragma unroll
+        for (int n = 0; n < NS; ++n) {
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s[n][r] = ss[state_row(n, r) * VB + state_col()];
+        }
+    }
     if constexpr (!OUT) {
         float* const to = run.last.data + bh * run.last.head + segment * run.last.segment;
 #pragma unroll
@@ -444,7 +512,7 @@ __global__ __launch_bounds__(256, KD == 256 ? 1 : 2) void AttendHalfKernel(Atten
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
                 const int i = state_row(n, r);
-                if (i < keys && state_col < cols) to[i * run.last.i + (col0 + state_col) * run.last.j] = s[n][r];
+                if (i < keys && state_col() < cols) to[i * run.last.i + (col0 + state_col()) * run.last.j] = s[n][r];
             }
         }
         if (tid == 0 && block == run.first) run.decays[static_cast<int64_t>(bh) * p.segments + segment] = __builtin_amdgcn_exp2f(static_cast<float>(passed));
@@ -453,11 +521,11 @@ __global__ __launch_bounds__(256, KD == 256 ? 1 : 2) void AttendHalfKernel(Atten
     // rows behind the sequence's end
     for (int64_t row = (span.end > span.first ? span.end : span.first) + wave; row < span.whole; row += 4) {
         if (lane >= cols) continue;
-        const int64_t to = y0 + row * run.y.row + lane;
-        if (run.wide) static_cast<float*>(run.y.data)[to] = 0.f;
+        const int64_t to = b * run.y.batch + h * run.y.head + row * run.y.row + col0 + lane;
+        if (wide) static_cast<float*>(run.y.data)[to] = 0.f;
         else static_cast<T*>(run.y.data)[to] = static_cast<T>(0);
     }
-    if (run.ends != nullptr) {
+    if (GRAD && run.ends != nullptr) {
         // <state behind the segment, its gradient there>, the waves' parts added up in the same order always
         float dot = 0;
         if (run.other.data != nullptr) {
@@ -465,9 +533,8 @@ __global__ __launch_bounds__(256, KD == 256 ? 1 : 2) void AttendHalfKernel(Atten
             for (int n = 0; n < NS; ++n) {
 #pragma unroll
                 for (int r = 0; r < 16; ++r) {
-                    const int i = state_row(n, r);
-                    if (i < keys && state_col < cols)
-                        dot += s[n][r] * run.other.data[bh * run.other.head + segment * run.other.segment + i * run.other.i + (col0 + state_col) * run.other.j];
+                    const float other = state_at(run.other, n, r);
+                    dot += state_row(n, r) < keys && state_col() < cols ? s[n][r] * other : 0.f;
                 }
             }
         }
@@ -482,14 +549,14 @@ __global__ __launch_bounds__(256, KD == 256 ? 1 : 2) void AttendHalfKernel(Atten
         }
     }
     if (run.last.data != nullptr && segment_turn == p.segments - 1) {
-        const float more = run.decay_last && length > 0 ? __builtin_amdgcn_exp2f(static_cast<float>(AttendDecay(p, b, h, 0))) : 1.f;
+        const float more = GRAD && run.decay_last && length > 0 ? __builtin_amdgcn_exp2f(static_cast<float>(AttendDecay(p, b, h, 0))) : 1.f;
         float* const to = run.last.data + bh * run.last.head;
 #pragma unroll
         for (int n = 0; n < NS; ++n) {
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
                 const int i = state_row(n, r);
-                if (i < keys && state_col < cols) to[i * run.last.i + (col0 + state_col) * run.last.j] = s[n][r] * more;
+                if (i < keys && state_col() < cols) to[i * run.last.i + (col0 + state_col()) * run.last.j] = s[n][r] * more;
             }
         }
     }
@@ -499,17 +566,19 @@ __global__ __launch_bounds__(256, KD == 256 ? 1 : 2) void AttendHalfKernel(Atten
 
 void LaunchAttendHalf(const AttendArgs& p, int keys, bool states_alone, hipStream_t stream) {
     const int64_t blocks = p.blocks * p.batch * p.heads * (states_alone ? p.segments - 1 : p.segments);
+    bool even = true;
+    for (int i = 0; i < p.runs; ++i) even = even && p.run[i].keys % 8 == 0 && p.run[i].values % 8 == 0;
     const auto launch = [&](auto kd) {
-        constexpr int KD = decltype(kd)::value, kLds = AttendHalfLds<KD>::kBytes;
-        const dim3 grid(static_cast<unsigned>(blocks));
-        if (states_alone) {
-            EnsureDynamicLds<AttendHalfTag>(reinterpret_cast<const void*>(AttendHalfKernel<KD, false>), kLds);
-            hipLaunchKernelGGL((AttendHalfKernel<KD, false>), grid, dim3(256), kLds, stream, p);
-        } else {
-            EnsureDynamicLds<AttendHalfTag>(reinterpret_cast<const void*>(AttendHalfKernel<KD, true>), kLds);
-            hipLaunchKernelGGL((AttendHalfKernel<KD, true>), grid, dim3(256), kLds, stream, p);
-        }
-        CheckLaunch("linear_attention");
+        const auto kernel = [&](auto out, auto whole, auto grad) {
+            constexpr int KD = decltype(kd)::value, kLds = AttendHalfLds<KD>::kBytes;
+            void (*const k)(AttendArgs) = AttendHalfKernel<KD, decltype(out)::value, decltype(whole)::value, decltype(grad)::value>;
+            EnsureDynamicLds<AttendHalfTag>(reinterpret_cast<const void*>(k), kLds);
+            hipLaunchKernelGGL(k, dim3(static_cast<unsigned>(blocks)), dim3(256), kLds, stream, p);
+            CheckLaunch("linear_attention");
+        };
+        const auto whole = [&](auto out, auto grad) { even ? kernel(out, std::true_type{}, grad) : kernel(out, std::false_type{}, grad); };
+        if (states_alone) p.runs > 1 ? whole(std::false_type{}, std::true_type{}) : whole(std::false_type{}, std::false_type{});
+        else p.runs > 1 ? whole(std::true_type{}, std::true_type{}) : whole(std::true_type{}, std::false_type{});
     };
     if (keys <= 64) launch(std::integral_constant<int, 64>{});
     else if (keys <= 128) launch(std::integral_constant<int, 128>{});
