@@ -30,7 +30,7 @@ struct AttendStates {
 struct AttendRun {
     AttendRows q, k, v, y;
     AttendRows dot;        // rows like y's, whose products with y are wanted
-    float* dots;           // [batch][head][length][2 blocks], or null
+    float* dots;           // [batch][head][blocks][length], or null
     AttendStates start, last;
     AttendStates other;    // the state's gradients behind each segment, whose products with the state there are wanted
     float* ends;           // [batch][head][segment][blocks], or null
@@ -51,7 +51,14 @@ struct AttendArgs {
     SequenceLengths lengths;
     int64_t batch, length, segment_rows;
     int heads, segments;
+    int groups;            // of workgroups, all blocks of one head's segment, and the launch holds them eight times, rounded up
 };
+
+// The workgroup's number among those that have work, or -1: workgroups go to the eight chips in turn, and the blocks of a head's segment, which read the same rows, belong on one.
+__device__ __forceinline__ int AttendNumber(const AttendArgs& p) {
+    const int chip = static_cast<int>(blockIdx.x % 8), turn = static_cast<int>(blockIdx.x / 8), group = turn / p.blocks * 8 + chip;
+    return group < p.groups ? group * p.blocks + turn % p.blocks : -1;
+}
 
 constexpr int kAttendTile = 64;      // rows that are taken at once
 constexpr int kAttendColumns = 64;   // columns of v to a workgroup
@@ -94,6 +101,7 @@ __device__ __forceinline__ double AttendDecay(const AttendArgs& p, int64_t b, in
 struct AttendDecays {
     alignas(16) float high[kAttendTile], low[kAttendTile];
     float end[kAttendTile];  // from a row to the tile's end, as a factor, times kv_scale
+    float near[kAttendTile]; // from a row to the last of its sixteen, as a factor
     float step[kAttendTile]; // a row's own, as a factor
     float all;               // the tile's
     double sum;              // the tile's, in powers of two
@@ -118,6 +126,14 @@ __device__ __forceinline__ double AddMoved(double v) {
     return v + __builtin_bit_cast(double, static_cast<uint64_t>(hi) << 32 | lo);
 }
 
+// The value of lane L of a row of 16 lanes.
+template <int L>
+__device__ __forceinline__ double OfLaneInRow(double v) {
+    const uint64_t b = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = __builtin_amdgcn_mov_dpp(static_cast<int>(b), 0x150 + L, 0xf, 0xf, true), hi = __builtin_amdgcn_mov_dpp(static_cast<int>(b >> 32), 0x150 + L, 0xf, 0xf, true);
+    return __builtin_bit_cast(double, static_cast<uint64_t>(hi) << 32 | lo);
+}
+
 // By one wave, a lane to a row, of which `here` are there; g in powers of two, 0 for the others.
 __device__ __forceinline__ void SumDecays(AttendDecays* to, double g, int here, float kv_scale) {
     const int lane = threadIdx.x % 64;
@@ -133,6 +149,7 @@ __device__ __forceinline__ void SumDecays(AttendDecays* to, double g, int here, 
     const float high = static_cast<float>(sum);
     to->high[lane] = high, to->low[lane] = static_cast<float>(sum - high);
     to->end[lane] = lane < here ? __builtin_amdgcn_exp2f(static_cast<float>(all - sum)) * kv_scale : 0.f;
+    to->near[lane] = __builtin_amdgcn_exp2f(static_cast<float>(OfLaneInRow<15>(sum) - sum));
     to->step[lane] = __builtin_amdgcn_exp2f(static_cast<float>(g));
     if (lane == 0) to->all = __builtin_amdgcn_exp2f(static_cast<float>(all)), to->sum = all;
 }
@@ -191,7 +208,7 @@ inline AttendStates AttendSegments(float* data, const AttendArgs& p, int keys, i
 inline int AttendBlocks(int values) { return (values + kAttendColumns - 1) / kAttendColumns; }
 
 void LaunchAttend(const AttendArgs& p, int dtype, bool states_alone, hipStream_t stream);
-void LaunchAttendHalf(const AttendArgs& p, int keys, bool states_alone, hipStream_t stream);  // float16
+void LaunchAttendHalf(const AttendArgs& p, int keys, int64_t blocks, bool states_alone, hipStream_t stream);  // float16
 // What segments add to a state of zeros (`last` of a pass of states alone) becomes the state that they start from, in the order of the pass.
 void LaunchAttendStarts(const AttendArgs& p, int run, const AttendStates& initial, hipStream_t stream);
 

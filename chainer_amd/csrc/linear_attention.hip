@@ -28,7 +28,8 @@ __global__ __launch_bounds__(256) void AttendKernel(AttendArgs p) {
     AttendDecays* const dec = reinterpret_cast<AttendDecays*>(red + 4 * VB);
     int* const odd = reinterpret_cast<int*>(dec + 1);     // v has infinities or what is not a number
 
-    int id = static_cast<int>(blockIdx.x);
+    int id = AttendNumber(p);
+    if (id < 0) return;
     const int block = id % p.blocks;
     id /= p.blocks;
     const int bh = id % static_cast<int>(p.batch * p.heads);
@@ -51,8 +52,7 @@ __global__ __launch_bounds__(256) void AttendKernel(AttendArgs p) {
     const T* const qp = OUT ? static_cast<const T*>(run.q.data) + b * run.q.batch + (h / run.q.share) * run.q.head : nullptr;
     const T* const dp = OUT && run.dots != nullptr ? static_cast<const T*>(run.dot.data) + b * run.dot.batch + (h / run.dot.share) * run.dot.head + col0 : nullptr;
     const int64_t y0 = OUT ? b * run.y.batch + h * run.y.head + col0 : 0;
-    const int parts = 2 * run.blocks;
-    float* const dots = OUT && run.dots != nullptr ? run.dots + static_cast<int64_t>(bh) * p.length * parts + (block - run.first) * 2 : nullptr;
+    float* const dots = OUT && run.dots != nullptr ? run.dots + (static_cast<int64_t>(bh) * run.blocks + block - run.first) * p.length : nullptr;
 
     // element r of a state's accumulator n: row i, column j of the workgroup's
     const auto state_row = [&](int n, int r) { return KD / 2 * tw + 32 * n + 8 * (r / 4) + 4 * half + r % 4; };
@@ -142,8 +142,8 @@ __global__ __launch_bounds__(256) void AttendKernel(AttendArgs p) {
                     if (dots != nullptr) {
                         float dot = j < cols ? y * static_cast<float>(dp[row * run.dot.row + j]) : 0.f;
 #pragma unroll
-                        for (int o = 1; o < 32; o <<= 1) dot += __shfl_xor(dot, o);
-                        if (l32 == 0) dots[row * parts + half] = dot;
+                        for (int o = 1; o < 64; o <<= 1) dot += __shfl_xor(dot, o);
+                        if (lane == 0) dots[row] = dot;
                     }
                 }
                 __syncthreads();
@@ -220,11 +220,12 @@ __global__ __launch_bounds__(256) void AttendKernel(AttendArgs p) {
                     }
                 }
             }
-            if (dots != nullptr) {
+            if (dots != nullptr) {  // the two halves of the columns meet in LDS
                 dot += __shfl_xor(dot, 32);
-                if (half == 0 && t < here) dots[row * parts + dw] = dot;
+                if (half == 0 && dw == 1) red[t] = dot;
             }
             __syncthreads();  // the copy of the state has been read
+            if (dots != nullptr && half == 0 && dw == 0 && t < here) dots[row] = dot + red[t];
         }
         const float all = dec->all;
 #pragma unroll
@@ -413,13 +414,15 @@ void VisitAttendType(int dtype, F&& f) {
 
 }  // namespace
 
-void LaunchAttend(const AttendArgs& p, int dtype, bool states_alone, hipStream_t stream) {
+void LaunchAttend(const AttendArgs& args, int dtype, bool states_alone, hipStream_t stream) {
+    AttendArgs p = args;
     int keys = 0;
     for (int i = 0; i < p.runs; ++i) keys = std::max(keys, p.run[i].keys);
-    const int64_t turns = states_alone ? p.segments - 1 : p.segments, blocks = p.blocks * p.batch * p.heads * turns;
+    const int64_t turns = states_alone ? p.segments - 1 : p.segments, groups = p.batch * p.heads * turns, blocks = (groups + 7) / 8 * 8 * p.blocks;
     HIPCX_REQUIRE(blocks <= kBlocksPerLaunch, HIPCX_NOT_IMPLEMENTED_ERROR, "linear_attention: too many elements");
     if (blocks == 0) return;
-    if (dtype == HIPCX_FLOAT16) return LaunchAttendHalf(p, keys, states_alone, stream);
+    p.groups = static_cast<int>(groups);
+    if (dtype == HIPCX_FLOAT16) return LaunchAttendHalf(p, keys, blocks, states_alone, stream);
     VisitKeys(keys, [&](auto kd) {
         constexpr int KD = decltype(kd)::value, kLds = AttendLds<KD>();
         const dim3 grid(static_cast<unsigned>(blocks));

@@ -7,13 +7,13 @@ namespace hipcx {
 namespace {
 
 struct AttendDecayArgs {
-    const float *of_q, *of_k;  // [batch][head][length][parts]: parts of q gq and k gk
+    const float *of_q, *of_k;  // [batch][head][blocks][length]: parts of q gq and k gk
     const float* ends;         // [batch][head][segment][blocks]: what the rows behind a segment have of the decays in it
     float* out;                // [batch][length][head], or null
     double* totals;            // [batch][head][segment], or null
     SequenceLengths lengths;
     int64_t length, segment_rows;
-    int parts, blocks, heads, segments;
+    int blocks, heads, segments;
 };
 
 // gg[t] = sum over u >= t of (q[u] gq[u] - k[u] gk[u]): sums from a segment's last row to its first, in 64 bits, on top of what lies behind the segment.
@@ -30,8 +30,7 @@ __global__ __launch_bounds__(256) void AttendDecayKernel(AttendDecayArgs p) {
         const int64_t t = last - 1 - tid;
         double sum = 0;
         if (t >= first) {
-            const float *q = p.of_q + (bh * p.length + t) * p.parts, *k = p.of_k + (bh * p.length + t) * p.parts;
-            for (int i = 0; i < p.parts; ++i) sum += static_cast<double>(q[i]) - k[i];
+            for (int i = 0; i < p.blocks; ++i) sum += static_cast<double>(p.of_q[(bh * p.blocks + i) * p.length + t]) - p.of_k[(bh * p.blocks + i) * p.length + t];
         }
 #pragma unroll
         for (int o = 1; o < 64; o <<= 1) {
@@ -104,7 +103,7 @@ struct GradWorkspace {
         const int64_t bh = p.batch * p.heads, each = static_cast<int64_t>(c.keys) * c.values, blocks = AttendBlocks(c.keys);
         states = Take(p.segments > 1 ? bh * p.segments * each : 0), gradients = Take(p.segments > 1 ? bh * p.segments * each : 0);
         decays = Take(p.segments > 1 ? 2 * bh * p.segments : 0);
-        of_q = Take(of_decays ? bh * p.length * 2 * blocks : 0), of_k = Take(of_decays ? bh * p.length * 2 * blocks : 0);
+        of_q = Take(of_decays ? bh * p.length * blocks : 0), of_k = Take(of_decays ? bh * p.length * blocks : 0);
         ends = Take(of_decays ? bh * p.segments * blocks : 0), totals = Take(of_heads ? bh * p.segments * 2 : 0);
         const int64_t shared = c.key_heads < p.heads ? bh * p.length * c.keys : 0;
         gq = Take(shared), gk = Take(shared);
@@ -217,7 +216,7 @@ int hipcx_linear_attention_grad(const hipcx_array* q, const hipcx_array* k, cons
                 AttendDecayArgs d{};
                 d.of_q = floats(w.of_q), d.of_k = floats(w.of_k), d.ends = floats(w.ends);
                 d.lengths = p.lengths, d.length = p.length, d.segment_rows = p.segment_rows, d.heads = p.heads, d.segments = p.segments;
-                d.blocks = AttendBlocks(c.keys), d.parts = 2 * d.blocks;
+                d.blocks = AttendBlocks(c.keys);
                 if (of_heads) d.totals = reinterpret_cast<double*>(ws + w.totals);
                 else d.out = static_cast<float*>(glog_decay->data);
                 HIPCX_REQUIRE(bh * p.segments <= kBlocksPerLaunch, HIPCX_NOT_IMPLEMENTED_ERROR, what + ": too many elements");

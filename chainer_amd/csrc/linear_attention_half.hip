@@ -27,29 +27,20 @@ struct Scale {
     }
 };
 
-// Eight values of at most 2^15 as the sum of two float16: 22 bits of those from 2^-14 on.
-__device__ __forceinline__ void Split(const float (&v)[8], attend_half8_t* high, attend_half8_t* low) {
-    attend_half8_t h, l;
+// Values of at most 2^15 as the sum of two float16: 22 bits of those from 2^-14 on.  `minus`: -1, which the compiler is not to know, so that the difference is one instruction that takes a
+// float16 as it is.
+template <int N>
+__device__ __forceinline__ void Split(const float (&v)[N], float minus, _Float16 __attribute__((ext_vector_type(N)))* high, _Float16 __attribute__((ext_vector_type(N)))* low) {
 #pragma unroll
-    for (int e = 0; e < 8; e += 2) {
+    for (int e = 0; e < N; e += 2) {
         const auto hi = __builtin_amdgcn_cvt_pkrtz(v[e], v[e + 1]);
-        const auto lo = __builtin_amdgcn_cvt_pkrtz(__builtin_fmaf(static_cast<float>(hi[0]), -1.f, v[e]), __builtin_fmaf(static_cast<float>(hi[1]), -1.f, v[e + 1]));
-        h[e] = hi[0], h[e + 1] = hi[1], l[e] = lo[0], l[e + 1] = lo[1];
+        const auto lo = __builtin_amdgcn_cvt_pkrtz(__builtin_fmaf(static_cast<float>(hi[0]), minus, v[e]), __builtin_fmaf(static_cast<float>(hi[1]), minus, v[e + 1]));
+        (*high)[e] = hi[0], (*high)[e + 1] = hi[1], (*low)[e] = lo[0], (*low)[e + 1] = lo[1];
     }
-    *high = h, *low = l;
-}
-__device__ __forceinline__ void Split(const float (&v)[4], attend_half4_t* high, attend_half4_t* low) {
-    attend_half4_t h, l;
-#pragma unroll
-    for (int e = 0; e < 4; e += 2) {
-        const auto hi = __builtin_amdgcn_cvt_pkrtz(v[e], v[e + 1]);
-        const auto lo = __builtin_amdgcn_cvt_pkrtz(__builtin_fmaf(static_cast<float>(hi[0]), -1.f, v[e]), __builtin_fmaf(static_cast<float>(hi[1]), -1.f, v[e + 1]));
-        h[e] = hi[0], h[e + 1] = hi[1], l[e] = lo[0], l[e + 1] = lo[1];
-    }
-    *high = h, *low = l;
 }
 
 __device__ __forceinline__ attend16_t Mfma(attend_half8_t a, attend_half8_t b, attend16_t c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ attend4_t Mfma(attend_half8_t a, attend_half8_t b, attend4_t c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
 
 // LDS of a workgroup, in bytes.  Rows' pitches keep the banks apart: of k, read by rows (32 of them, 16 bytes each) and in blocks of 4 x 16, 80 bytes more than a multiple of 128; of v, read in
 // such blocks alone, 64 more; of the state's copies, read by rows, 16 more.
@@ -62,17 +53,19 @@ struct AttendHalfLds {
     static_assert(kValues % 16 == 0 && kStates % 16 == 0 && kDecays % 16 == 0 && sizeof(AttendDecays) % 16 == 0, "aligned parts");
 };
 
-// As AttendKernel (linear_attention.hip): a wave multiplies 32 rows by 32 columns of y, and has half of the keys and 32 columns of the state in its accumulators.
+// As AttendKernel (linear_attention.hip), with other shares: a wave has sixteen rows of y with all 64 columns, and half of the keys and 32 columns of the state in its accumulators.
 //   y^T = S^T Q^T, S in two parts of float16 in LDS, with a power of two for each column and half of the keys;
 //   P^T = K Q^T (rows s, a lane to a row t) from float16 as they come; times the weights, brought to float16's range by a power of two for each t, in two parts; y^T += V^T P^T;
 //   S <- exp(G[63]) S + K^T (exp(G[63] - G) V), V's products in two parts, with a power of two for each column.
-// A reduction over rows s takes them in the order in which accumulators have them, eight to a lane: 4 h + j and 8 + 4 h + j of sixteen, for both operands.
+// A reduction over rows s takes them in the order in which accumulators have them, eight to a lane, for both operands: 4 q + j and 16 + 4 q + j of 32 for quarter q of a wave with blocks of
+// 16 x 16, 4 h + j and 8 + 4 h + j of sixteen for half h with blocks of 32 x 32.  (32 rows by 32 columns to a wave have every block of P computed by two waves, which are a third of the
+// vector instructions: 134 us for the pass over 16384 rows of 16 heads of 128.)
 // EVEN: rows of whole pieces of eight elements.  GRAD: what the passes of the gradients have beyond the forward one.
 template <int KD, bool OUT, bool EVEN, bool GRAD>
 __global__ __launch_bounds__(256, KD == 256 ? 1 : 2) void AttendHalfKernel(AttendArgs p) {
     using T = half_t;
     using Lds = AttendHalfLds<KD>;
-    constexpr int VB = kAttendColumns, C = kAttendTile, NS = KD / 64, NK = KD / 32, NV = VB / 32, NQ = KD / 16;
+    constexpr int VB = kAttendColumns, C = kAttendTile, NS = KD / 64, NK = KD / 32, NV = VB / 32, NQ = KD / 32, DB = VB / 16;
     extern __shared__ __align__(16) char lds[];
     char *const ks = lds, *const vs = lds + Lds::kValues, *const high_copy = lds + Lds::kStates, *const low_copy = lds + Lds::kLow;
     float* const scales = reinterpret_cast<float*>(lds + Lds::kScales);  // [2][VB]
@@ -80,7 +73,8 @@ __global__ __launch_bounds__(256, KD == 256 ? 1 : 2) void AttendHalfKernel(Atten
     AttendDecays* const decays = reinterpret_cast<AttendDecays*>(lds + Lds::kDecays);
     int* const odd = reinterpret_cast<int*>(lds + Lds::kOdd);            // v has infinities or what is not a number
 
-    int id = static_cast<int>(blockIdx.x);
+    int id = AttendNumber(p);
+    if (id < 0) return;
     const int block = id % p.blocks;
     id /= p.blocks;
     const int bh = id % static_cast<int>(p.batch * p.heads);
@@ -106,8 +100,7 @@ __global__ __launch_bounds__(256, KD == 256 ? 1 : 2) void AttendHalfKernel(Atten
     // What follows from the lane is found again in every tile: kept over the loop, it would take the registers of what is multiplied.
     const auto in_tile = [&] { return lane % 32; };
     const auto upper = [&] { return lane / 32; };
-    const int parts = 2 * run.blocks;
-    const auto dots = [&] { return run.dots + static_cast<int64_t>(bh) * p.length * parts + (block - run.first) * 2; };
+    const auto dots = [&] { return run.dots + (static_cast<int64_t>(bh) * run.blocks + block - run.first) * p.length; };
 
     const auto state_row = [&](int n, int r) { return KD / 2 * tw + 32 * n + 8 * (r / 4) + 4 * upper() + r % 4; };
     const auto state_col = [&] { return 32 * dw + in_tile(); };
@@ -132,6 +125,8 @@ __global__ __launch_bounds__(256, KD == 256 ? 1 : 2) void AttendHalfKernel(Atten
             for (int r = 0; r < 16; ++r) s[n][r] = state_at(run.start, n, r);
         }
     }
+    float minus = -1;
+    asm volatile("" : "+s"(minus));
     const auto keep_state = [&] {
         float most = 0;
 #pragma unroll
@@ -148,7 +143,7 @@ __global__ __launch_bounds__(256, KD == 256 ? 1 : 2) void AttendHalfKernel(Atten
             for (int g = 0; g < 4; ++g) {
                 const float v[4] = {s[n][4 * g] * scale.in, s[n][4 * g + 1] * scale.in, s[n][4 * g + 2] * scale.in, s[n][4 * g + 3] * scale.in};
                 attend_half4_t hi, lo;
-                Split(v, &hi, &lo);
+                Split<4>(v, minus, &hi, &lo);
                 const int at = state_col() * Lds::kStatePitch + state_row(n, 4 * g) * 2;
                 *reinterpret_cast<attend_half4_t*>(high_copy + at) = hi;
                 *reinterpret_cast<attend_half4_t*>(low_copy + at) = lo;
@@ -160,7 +155,7 @@ __global__ __launch_bounds__(256, KD == 256 ? 1 : 2) void AttendHalfKernel(Atten
     // A tile's rows on their way: pieces of eight elements of k and of v.  Rows that are not there are the last one again; columns that are not there are zeros that stay in LDS.  Rows lie less
     // than 2^24 elements apart, so that a tile's are within 32 bits of its first.
     const int key_row = tid / (KD / 8), key_col = tid % (KD / 8) * 8, value_row = tid / (VB / 8), value_col = tid % (VB / 8) * 8;
-    const auto own_row = [&] { return 32 * tw + in_tile(); };  // of a tile
+    const auto own_row = [&] { return 16 * wave + lane % 16; };  // of a tile
     const int way = back ? -1 : 1;
     const int64_t row0 = back ? span.end - 1 : span.first;
     const T* kp = static_cast<const T*>(run.k.data) + b * run.k.batch + (h / run.k.share) * run.k.head + row0 * run.k.row;
@@ -197,7 +192,7 @@ __global__ __launch_bounds__(256, KD == 256 ? 1 : 2) void AttendHalfKernel(Atten
         if constexpr (OUT) {
             const T* const at = qp + min(own_row(), static_cast<int>(rows - r0 < C ? rows - r0 : C) - 1) * q_row;
 #pragma unroll
-            for (int m = 0; m < NQ; ++m) q[m] = piece_at(at, 16 * m + 8 * upper(), keys);
+            for (int m = 0; m < NQ; ++m) q[m] = piece_at(at, 32 * m + lane / 16 * 8, keys);
             qp += static_cast<int64_t>(q_row) * C;
         }
     };
@@ -224,7 +219,7 @@ __global__ __launch_bounds__(256, KD == 256 ? 1 : 2) void AttendHalfKernel(Atten
     if (rows > 0) {
         load(0);
         load_q(0);
-        if (wave == 3) load_decays(0), sum_next(0, decays);
+        if (wave == 0) load_decays(0), sum_next(0, decays);
     }
     double passed = 0;  // log decay of the tiles so far
     // where a lane reads blocks of 4 x 16: rows 4 upper() and on, columns of its 32
@@ -260,114 +255,107 @@ __global__ __launch_bounds__(256, KD == 256 ? 1 : 2) void AttendHalfKernel(Atten
         const bool more = r0 + C < rows;
         if (more) {
             load(r0 + C);
-            if (wave == 3) load_decays(r0 + C);
+            if (wave == 0) load_decays(r0 + C);
         }
-        attend_half8_t v[C / 16];
-        const auto read_v = [&] {  // this wave's columns, for the products with P and with k: rows 16 u + ... of step u
-#pragma unroll
-            for (int u = 0; u < C / 16; ++u) {
-                const char* const at = vs + (16 * u + turned_row()) * Lds::kValuePitch + dw * 64 + turned_col();
-                v[u] = Join(ReadTurned(at), ReadTurned(at + 8 * Lds::kValuePitch));
-            }
-        };
         if constexpr (OUT) {
-            attend16_t y;
-            attend16_t a[2]{};
+            // this wave's sixteen rows by all columns, in blocks of 16 x 16
+            const int quarter = lane / 16;
             const float high = dec->high[own_row()], low = dec->low[own_row()];
+            attend4_t y[DB];
             {
-                attend16_t of_state[2]{};
-                const int at = state_col() * Lds::kStatePitch + 16 * upper();
-                attend_half8_t part[2][2];
-                const auto read = [&](int m, attend_half8_t (&to)[2]) {
-                    to[0] = *reinterpret_cast<const attend_half8_t*>(low_copy + at + 32 * m);
-                    to[1] = *reinterpret_cast<const attend_half8_t*>(high_copy + at + 32 * m);
+                attend4_t of_state[2][DB]{};
+                const int at = lane % 16 * Lds::kStatePitch + 16 * quarter;
+                attend_half8_t part[2][DB];
+                const auto read = [&](int step, attend_half8_t (&to)[DB]) {  // step 2 m: the low parts, 2 m + 1: the high ones
+                    const char* const from = (step % 2 == 0 ? low_copy : high_copy) + at + 64 * (step / 2);
+#pragma unroll
+                    for (int d = 0; d < DB; ++d) to[d] = *reinterpret_cast<const attend_half8_t*>(from + 16 * d * Lds::kStatePitch);
                 };
                 read(0, part[0]);
 #pragma unroll
-                for (int m = 0; m < NQ; ++m) {  // reads of the next step under the products of this one
-                    if (m + 1 < NQ) read(m + 1, part[m % 2 ^ 1]);
+                for (int step = 0; step < 2 * NQ; ++step) {  // reads of the next step under the products of this one
+                    if (step + 1 < 2 * NQ) read(step + 1, part[step % 2 ^ 1]);
 #pragma unroll
-                    for (int i = 0; i < 2; ++i) of_state[m / (NQ / 2)] = Mfma(part[m % 2][i], q[m], of_state[m / (NQ / 2)]);
+                    for (int d = 0; d < DB; ++d) of_state[step / NQ][d] = Mfma(part[step % 2][d], q[step / 2], of_state[step / NQ][d]);
                     __builtin_amdgcn_sched_barrier(0);
                 }
                 const float from_start = __builtin_amdgcn_exp2f(high + low) * run.out_scale;
 #pragma unroll
-                for (int g = 0; g < 4; ++g) {
-                    const int j = 32 * dw + 8 * g + 4 * upper();
+                for (int d = 0; d < DB; ++d) {
+                    const int j = 16 * d + 4 * quarter;
                     const attend4_t first = *reinterpret_cast<const attend4_t*>(scales + j), second = *reinterpret_cast<const attend4_t*>(scales + VB + j);
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) y[4 * g + e] = __builtin_fmaf(of_state[0][4 * g + e], first[e], of_state[1][4 * g + e] * second[e]) * from_start;
+                    for (int e = 0; e < 4; ++e) y[d][e] = __builtin_fmaf(of_state[0][d][e], first[e], of_state[1][d][e] * second[e]) * from_start;
                 }
             }
             __builtin_amdgcn_sched_barrier(0);  // (the products with the state need as many registers as those with k)
+            attend4_t a[4]{};
+            {
+                const char* const at = ks + lane % 16 * Lds::kKeyPitch + 16 * quarter;
 #pragma unroll
-            for (int sb = 0; sb < 2; ++sb) {
-                if (sb > tw) continue;
-                const char* const at = ks + (32 * sb + in_tile()) * Lds::kKeyPitch + 16 * upper();
-                attend_half8_t part[2][2];
-                const auto read = [&](int m, attend_half8_t (&to)[2]) {
+                for (int sb = 0; sb < 4; ++sb) {
+                    if (sb > wave) continue;
+                    attend_half8_t part[NQ];
 #pragma unroll
-                    for (int i = 0; i < 2; ++i) to[i] = *reinterpret_cast<const attend_half8_t*>(at + 32 * (m + i));
-                };
-                read(0, part[0]);
+                    for (int m = 0; m < NQ; ++m) part[m] = *reinterpret_cast<const attend_half8_t*>(at + 16 * sb * Lds::kKeyPitch + 64 * m);
 #pragma unroll
-                for (int m = 0; m < NQ; m += 2) {
-                    if (m + 2 < NQ) read(m + 2, part[m / 2 % 2 ^ 1]);
-#pragma unroll
-                    for (int i = 0; i < 2; ++i) a[sb] = Mfma(part[m / 2 % 2][i], q[m + i], a[sb]);
-                    __builtin_amdgcn_sched_barrier(0);
+                    for (int m = 0; m < NQ; ++m) a[sb] = Mfma(part[m], q[m], a[sb]);
                 }
             }
-            if (wave == 3 && more) sum_next(r0 + C, decays + (turn ^ 1));
+            if (wave == 0 && more) sum_next(r0 + C, decays + (turn ^ 1));
             if (tid == 0) odd[turn ^ 1] = 0;
-            float most = 0;
-            const int own = in_tile() - 4 * upper();  // of this lane's 32 rows, how far its own is behind its half's
+            // weights: of the sixteen rows that this one is among, exp(G[t] - G[s]); of earlier ones, whose last is l, exp(G[l] - G[s]) here and exp(G[t] - G[l]) with the power of two
+            float most = 0, since[4];
 #pragma unroll
-            for (int sb = 0; sb < 2; ++sb) {
-                if (sb > tw) continue;
-#pragma unroll
-                for (int g = 0; g < 4; ++g) {
-                    const int first = 32 * sb + 8 * g + 4 * upper();
+            for (int sb = 0; sb < 4; ++sb) {
+                if (sb > wave) continue;
+                const int first = 16 * sb + 4 * quarter;
+                if (sb == wave) {
                     const attend4_t highs = *reinterpret_cast<const attend4_t*>(dec->high + first), lows = *reinterpret_cast<const attend4_t*>(dec->low + first);
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) a[sb][4 * g + e] *= __builtin_amdgcn_exp2f((high - highs[e]) + (low - lows[e]));
-                }
-                __builtin_amdgcn_sched_barrier(0);
-                if (sb == tw) {
+                    for (int e = 0; e < 4; ++e) {
+                        const float weighted = a[sb][e] * __builtin_amdgcn_exp2f((high - highs[e]) + (low - lows[e]));
+                        a[sb][e] = 4 * quarter + e <= lane % 16 ? weighted : 0.f;
+                    }
+                    since[sb] = 1;
+                } else {
+                    const attend4_t near = *reinterpret_cast<const attend4_t*>(dec->near + first);
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) a[sb][r] = 8 * (r / 4) + r % 4 <= own ? a[sb][r] : 0.f;
+                    for (int e = 0; e < 4; ++e) a[sb][e] *= near[e];
+                    since[sb] = __builtin_amdgcn_exp2f((high - dec->high[16 * sb + 15]) + (low - dec->low[16 * sb + 15]));
                 }
-#pragma unroll
-                for (int r = 0; r < 16; ++r) most = fmaxf(most, fabsf(a[sb][r]));
+                most = fmaxf(most, fmaxf(fmaxf(fabsf(a[sb][0]), fabsf(a[sb][1])), fmaxf(fabsf(a[sb][2]), fabsf(a[sb][3]))) * since[sb]);
             }
+            most = fmaxf(most, __shfl_xor(most, 16));
             const Scale scale(fmaxf(most, __shfl_xor(most, 32)));
-            __builtin_amdgcn_sched_barrier(0);
-            read_v();
-            attend16_t of_rows{};
+            attend4_t of_rows[DB]{};
 #pragma unroll
-            for (int sb = 0; sb < 2; ++sb) {
-                if (sb > tw) continue;
+            for (int u = 0; u < 2; ++u) {
+                if (2 * u > wave) continue;
+                float w[8];
 #pragma unroll
-                for (int u = 0; u < 2; ++u) {
-                    float w[8];
+                for (int e = 0; e < 8; ++e) w[e] = 2 * u + e / 4 <= wave ? a[2 * u + e / 4][e % 4] * (since[2 * u + e / 4] * scale.in) : 0.f;
+                attend_half8_t hi, lo;
+                Split<8>(w, minus, &hi, &lo);
+                const char* const at = vs + (32 * u + 4 * quarter + lane % 16 / 4) * Lds::kValuePitch + lane % 4 * 8;
+                attend_half8_t v[DB];
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) w[e] = a[sb][8 * u + e] * scale.in;
-                    attend_half8_t hi, lo;
-                    Split(w, &hi, &lo);
-                    of_rows = Mfma(v[2 * sb + u], lo, of_rows);
-                    of_rows = Mfma(v[2 * sb + u], hi, of_rows);
-                }
+                for (int d = 0; d < DB; ++d) v[d] = Join(ReadTurned(at + 32 * d), ReadTurned(at + 16 * Lds::kValuePitch + 32 * d));
+#pragma unroll
+                for (int d = 0; d < DB; ++d) of_rows[d] = Mfma(v[d], lo, of_rows[d]);
+#pragma unroll
+                for (int d = 0; d < DB; ++d) of_rows[d] = Mfma(v[d], hi, of_rows[d]);
             }
             const float from_rows = scale.out * kv_scale * run.out_scale;
             char* const to = yp + static_cast<int64_t>(own_row()) * y_row;
             const bool live = r0 + own_row() < rows;
             float dot = 0;
 #pragma unroll
-            for (int g = 0; g < 4; ++g) {
-                const int j = 32 * dw + 8 * g + 4 * upper();
+            for (int d = 0; d < DB; ++d) {
+                const int j = 16 * d + 4 * quarter;
                 AttendPiece<float, 4> out;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) out.v[e] = __builtin_fmaf(of_rows[4 * g + e], from_rows, y[4 * g + e]);
+                for (int e = 0; e < 4; ++e) out.v[e] = __builtin_fmaf(of_rows[d][e], from_rows, y[d][e]);
                 if (!live) continue;
                 if (with_dots) {
                     AttendPiece<T, 4> with{};
@@ -396,14 +384,20 @@ __global__ __launch_bounds__(256, KD == 256 ? 1 : 2) void AttendHalfKernel(Atten
                 }
             }
             if (with_dots) {
+                dot += __shfl_xor(dot, 16);
                 dot += __shfl_xor(dot, 32);
-                if (upper() == 0 && live) dots()[(row0 + way * (r0 + own_row())) * parts + dw] = dot;
+                if (quarter == 0 && live) dots()[row0 + way * (r0 + own_row())] = dot;
                 dp += static_cast<int64_t>(d_row) * C;
             }
             yp += static_cast<int64_t>(y_row) * C;
         } else {
-            read_v();
-            if (wave == 3 && more) sum_next(r0 + C, decays + (turn ^ 1));
+            if (wave == 0 && more) sum_next(r0 + C, decays + (turn ^ 1));
+        }
+        attend_half8_t v[C / 16];  // this wave's 32 columns: rows 16 u + ... of step u
+#pragma unroll
+        for (int u = 0; u < C / 16; ++u) {
+            const char* const at = vs + (16 * u + turned_row()) * Lds::kValuePitch + dw * 64 + turned_col();
+            v[u] = Join(ReadTurned(at), ReadTurned(at + 8 * Lds::kValuePitch));
         }
         __builtin_amdgcn_sched_barrier(0);
         if (more) load_q(r0 + C);
@@ -416,7 +410,7 @@ __global__ __launch_bounds__(256, KD == 256 ? 1 : 2) void AttendHalfKernel(Atten
                 const attend4_t end = *reinterpret_cast<const attend4_t*>(dec->end + 16 * u + 8 * g + 4 * upper());
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    w[u][4 * g + e] = static_cast<float>(v[u][4 * g + e]) * end[e];
+                    w[u][4 * g + e] = __builtin_fmaf(static_cast<float>(v[u][4 * g + e]), end[e], 0.f);
                     most = fmaxf(most, fabsf(w[u][4 * g + e]));
                 }
             }
@@ -439,7 +433,7 @@ __global__ __launch_bounds__(256, KD == 256 ? 1 : 2) void AttendHalfKernel(Atten
 #pragma unroll
                 for (int e = 0; e < 8; ++e) w[u][e] *= scale.in;
                 attend_half8_t hi, lo;
-                Split(w[u], &hi, &lo);
+                Split<8>(w[u], minus, &hi, &lo);
 #pragma unroll
                 for (int n = 0; n < NS; ++n) {
                     add[n] = Mfma(k[u % 2][n], lo, add[n]);
@@ -493,8 +487,8 @@ __global__ __launch_bounds__(256, KD == 256 ? 1 : 2) void AttendHalfKernel(Atten
                     float dot = 0;
                     if (j < cols) dot = y * static_cast<float>((static_cast<const T*>(run.dot.data) + b * run.dot.batch + (h / run.dot.share) * run.dot.head + row * run.dot.row + col0)[j]);
 #pragma unroll
-                    for (int o = 1; o < 32; o <<= 1) dot += __shfl_xor(dot, o);
-                    if (in_tile() == 0) dots()[row * parts + upper()] = dot;
+                    for (int o = 1; o < 64; o <<= 1) dot += __shfl_xor(dot, o);
+                    if (lane == 0) dots()[row] = dot;
                 }
             }
             __syncthreads();
@@ -564,8 +558,7 @@ __global__ __launch_bounds__(256, KD == 256 ? 1 : 2) void AttendHalfKernel(Atten
 
 }  // namespace
 
-void LaunchAttendHalf(const AttendArgs& p, int keys, bool states_alone, hipStream_t stream) {
-    const int64_t blocks = p.blocks * p.batch * p.heads * (states_alone ? p.segments - 1 : p.segments);
+void LaunchAttendHalf(const AttendArgs& p, int keys, int64_t blocks, bool states_alone, hipStream_t stream) {
     bool even = true;
     for (int i = 0; i < p.runs; ++i) even = even && p.run[i].keys % 8 == 0 && p.run[i].values % 8 == 0;
     const auto launch = [&](auto kd) {
