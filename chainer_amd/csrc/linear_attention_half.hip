@@ -8,6 +8,7 @@ namespace {
 struct AttendHalfTag {};
 
 typedef short attend_short4_t __attribute__((ext_vector_type(4)));
+typedef _Float16 attend_half2_t __attribute__((ext_vector_type(2)));
 typedef _Float16 attend_half4_t __attribute__((ext_vector_type(4)));
 typedef _Float16 attend_half8_t __attribute__((ext_vector_type(8)));
 
@@ -16,6 +17,19 @@ __device__ __forceinline__ attend_half4_t ReadTurned(const char* at) {
     return __builtin_bit_cast(attend_half4_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) attend_short4_t*)at));
 }
 __device__ __forceinline__ attend_half8_t Join(attend_half4_t a, attend_half4_t b) { return attend_half8_t{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]}; }
+
+// The larger of a lane's value and that of the lane 32 or 16 away: two registers exchange halves, or rows of 16 lanes.  (As assembly, with the waits that the vector units' results need: of the
+// builtin's two results the compiler takes the first for both.)
+__device__ __forceinline__ float MaxOver32(float v) {
+    float w = v;
+    asm("s_nop 1\n\tv_permlane32_swap_b32 %0, %1\n\ts_nop 1" : "+v"(v), "+v"(w));
+    return fmaxf(v, w);
+}
+__device__ __forceinline__ float MaxOver16(float v) {
+    float w = v;
+    asm("s_nop 1\n\tv_permlane16_swap_b32 %0, %1\n\ts_nop 1" : "+v"(v), "+v"(w));
+    return fmaxf(v, w);
+}
 
 // The power of two that brings `most`, the largest of some values, to at least 2^14 and below 2^15; and the one that brings them back.
 struct Scale {
@@ -42,11 +56,12 @@ __device__ __forceinline__ void Split(const float (&v)[N], float minus, _Float16
 __device__ __forceinline__ attend16_t Mfma(attend_half8_t a, attend_half8_t b, attend16_t c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
 __device__ __forceinline__ attend4_t Mfma(attend_half8_t a, attend_half8_t b, attend4_t c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
 
-// LDS of a workgroup, in bytes.  Rows' pitches keep the banks apart: of k, read by rows (32 of them, 16 bytes each) and in blocks of 4 x 16, 80 bytes more than a multiple of 128; of v, read in
-// such blocks alone, 64 more; of the state's copies, read by rows, 16 more.
+// LDS of a workgroup, in bytes.  Rows' pitches keep the banks apart.  Clocks of a wave's instruction (eight waves at work), at 128 keys: k and the state's copies read by rows, sixteen rows of 64
+// bytes each, 4.0 with 32 or 96 bytes more than a multiple of 256, 7.9 with 16, 6.6 with 80; v in blocks of 4 x 16, sixteen rows, 2.6 with 32 more than 128, 4.0 with 64; the state's copies
+// written, 8.0 with 32, 5.0 with 16.
 template <int KD>
 struct AttendHalfLds {
-    static constexpr int kKeyPitch = KD * 2 + 80, kValuePitch = kAttendColumns * 2 + 64, kStatePitch = KD * 2 + 16;
+    static constexpr int kKeyPitch = KD * 2 + 96, kValuePitch = kAttendColumns * 2 + 32, kStatePitch = KD * 2 + 32;
     static constexpr int kValues = kAttendTile * kKeyPitch, kStates = kValues + kAttendTile * kValuePitch, kLow = kStates + kAttendColumns * kStatePitch,
                          kScales = kLow + kAttendColumns * kStatePitch, kSums = kScales + 2 * kAttendColumns * 4, kDecays = kSums + 4 * kAttendColumns * 4,
                          kOdd = kDecays + 2 * static_cast<int>(sizeof(AttendDecays)), kBytes = kOdd + 16;
@@ -134,8 +149,7 @@ __global__ __launch_bounds__(256, KD == 256 ? 1 : 2) void AttendHalfKernel(Atten
 #pragma unroll
             for (int r = 0; r < 16; ++r) most = fmaxf(most, fabsf(s[n][r]));
         }
-        most = fmaxf(most, __shfl_xor(most, 32));
-        const Scale scale(most);
+        const Scale scale(MaxOver32(most));
         if (upper() == 0) scales[tw * VB + state_col()] = scale.out;
 #pragma unroll
         for (int n = 0; n < NS; ++n) {
@@ -238,16 +252,14 @@ __global__ __launch_bounds__(256, KD == 256 ? 1 : 2) void AttendHalfKernel(Atten
         for (int n = 0; n < NK; ++n) {
             if (!EVEN || key_col < keys) *reinterpret_cast<attend_half8_t*>(ks + (key_row + n * (2048 / KD)) * Lds::kKeyPitch + key_col * 2) = k_next[n];
         }
-        attend_half8_t finite{};
+        attend_half2_t finite{};  // 0, or not a number
 #pragma unroll
         for (int n = 0; n < NV; ++n) {
             if (!EVEN || value_col < cols) *reinterpret_cast<attend_half8_t*>(vs + (value_row + n * 32) * Lds::kValuePitch + value_col * 2) = v_next[n];
-            finite += v_next[n] - v_next[n];
+#pragma unroll
+            for (int e = 0; e < 8; e += 2) finite = __builtin_elementwise_fma(attend_half2_t{v_next[n][e], v_next[n][e + 1]}, attend_half2_t{}, finite);
         }
-        if constexpr (OUT) {
-            const T all = finite[0] + finite[1] + finite[2] + finite[3] + finite[4] + finite[5] + finite[6] + finite[7];
-            if (all != 0) odd[turn] = 1;
-        }
+        if (OUT && !(finite[0] + finite[1] == 0)) odd[turn] = 1;
         __syncthreads();
         passed += dec->sum;
         // An infinity of a later row, times P's zeros, would reach earlier ones: the rest goes row by row.
@@ -292,14 +304,19 @@ __global__ __launch_bounds__(256, KD == 256 ? 1 : 2) void AttendHalfKernel(Atten
             attend4_t a[4]{};
             {
                 const char* const at = ks + lane % 16 * Lds::kKeyPitch + 16 * quarter;
+                attend_half8_t part[2][NQ];
+                const auto read = [&](int sb, attend_half8_t (&to)[NQ]) {
+#pragma unroll
+                    for (int m = 0; m < NQ; ++m) to[m] = *reinterpret_cast<const attend_half8_t*>(at + 16 * sb * Lds::kKeyPitch + 64 * m);
+                };
+                read(0, part[0]);
 #pragma unroll
                 for (int sb = 0; sb < 4; ++sb) {
                     if (sb > wave) continue;
-                    attend_half8_t part[NQ];
+                    if (sb < 3) read(sb + 1, part[sb % 2 ^ 1]);  // (of the last one, of no use)
 #pragma unroll
-                    for (int m = 0; m < NQ; ++m) part[m] = *reinterpret_cast<const attend_half8_t*>(at + 16 * sb * Lds::kKeyPitch + 64 * m);
-#pragma unroll
-                    for (int m = 0; m < NQ; ++m) a[sb] = Mfma(part[m], q[m], a[sb]);
+                    for (int m = 0; m < NQ; ++m) a[sb] = Mfma(part[sb % 2][m], q[m], a[sb]);
+                    __builtin_amdgcn_sched_barrier(0);
                 }
             }
             if (wave == 0 && more) sum_next(r0 + C, decays + (turn ^ 1));
@@ -326,8 +343,7 @@ __global__ __launch_bounds__(256, KD == 256 ? 1 : 2) void AttendHalfKernel(Atten
                 }
                 most = fmaxf(most, fmaxf(fmaxf(fabsf(a[sb][0]), fabsf(a[sb][1])), fmaxf(fabsf(a[sb][2]), fabsf(a[sb][3]))) * since[sb]);
             }
-            most = fmaxf(most, __shfl_xor(most, 16));
-            const Scale scale(fmaxf(most, __shfl_xor(most, 32)));
+            const Scale scale(MaxOver32(MaxOver16(most)));
             attend4_t of_rows[DB]{};
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
@@ -415,7 +431,7 @@ __global__ __launch_bounds__(256, KD == 256 ? 1 : 2) void AttendHalfKernel(Atten
                 }
             }
         }
-        const Scale scale(fmaxf(most, __shfl_xor(most, 32)));
+        const Scale scale(MaxOver32(most));
         attend16_t add[NS]{};
         {
             attend_half8_t k[2][NS];
