@@ -41,6 +41,9 @@ struct Scale {
     }
 };
 
+__device__ __forceinline__ int ExponentOf(float v) { return (__builtin_bit_cast(int, v) >> 23) - 127; }  // of v >= 0
+__device__ __forceinline__ float Power(int e) { return __builtin_bit_cast(float, (127 + e) << 23); }       // of -126 to 127
+
 // Values of at most 2^15 as the sum of two float16: 22 bits of those from 2^-14 on.  `minus`: -1, which the compiler is not to know, so that the difference is one instruction that takes a
 // float16 as it is.
 template <int N>
@@ -63,24 +66,25 @@ template <int KD>
 struct AttendHalfLds {
     static constexpr int kKeyPitch = KD * 2 + 96, kValuePitch = kAttendColumns * 2 + 32, kStatePitch = KD * 2 + 32;
     static constexpr int kValues = kAttendTile * kKeyPitch, kStates = kValues + kAttendTile * kValuePitch, kLow = kStates + kAttendColumns * kStatePitch,
-                         kScales = kLow + kAttendColumns * kStatePitch, kSums = kScales + 2 * kAttendColumns * 4, kDecays = kSums + 4 * kAttendColumns * 4,
+                         kScales = kLow + kAttendColumns * kStatePitch, kSums = kScales + kAttendColumns * 4, kDecays = kSums + 4 * kAttendColumns * 4,
                          kOdd = kDecays + 2 * static_cast<int>(sizeof(AttendDecays)), kBytes = kOdd + 16;
     static_assert(kValues % 16 == 0 && kStates % 16 == 0 && kDecays % 16 == 0 && sizeof(AttendDecays) % 16 == 0, "aligned parts");
 };
 
-// As AttendKernel (linear_attention.hip), with other shares: a wave has sixteen rows of y with all 64 columns, and half of the keys and 32 columns of the state in its accumulators.
-//   y^T = S^T Q^T, S in two parts of float16 in LDS, with a power of two for each column and half of the keys;
+// As AttendKernel (linear_attention.hip), with other shares: a wave has sixteen rows of y with all 64 columns, and sixteen columns of the state with all keys in its accumulators.
+//   y^T = S^T Q^T, S in two parts of float16 in LDS;
 //   P^T = K Q^T (rows s, a lane to a row t) from float16 as they come; times the weights, brought to float16's range by a power of two for each t, in two parts; y^T += V^T P^T;
-//   S <- exp(G[63]) S + K^T (exp(G[63] - G) V), V's products in two parts, with a power of two for each column.
-// A reduction over rows s takes them in the order in which accumulators have them, eight to a lane, for both operands: 4 q + j and 16 + 4 q + j of 32 for quarter q of a wave with blocks of
-// 16 x 16, 4 h + j and 8 + 4 h + j of sixteen for half h with blocks of 32 x 32.  (32 rows by 32 columns to a wave have every block of P computed by two waves, which are a third of the
-// vector instructions: 134 us for the pass over 16384 rows of 16 heads of 128.)
+//   S <- exp(G[63]) S + K^T (exp(G[63] - G) V), V's products in two parts.
+// S and what is added to it are counted in a power of two for each column (`unit`), which changes when the column's largest element leaves 2^4 to 2^15 of it, so that parts of float16 keep 22
+// bits of anything that counts next to it.
+// A reduction over 32 rows s takes them in the order in which accumulators have them, eight to a lane, for both operands: 4 q + j and 16 + 4 q + j for quarter q of a wave.
+// (32 rows by 32 columns of y to a wave have every block of P computed by two waves; half of the keys by 32 columns of S every product with V.  Vector instructions are what bounds the kernel.)
 // EVEN: rows of whole pieces of eight elements.  GRAD: what the passes of the gradients have beyond the forward one.
 template <int KD, bool OUT, bool EVEN, bool GRAD>
 __global__ __launch_bounds__(256, KD == 256 ? 1 : 2) void AttendHalfKernel(AttendArgs p) {
     using T = half_t;
     using Lds = AttendHalfLds<KD>;
-    constexpr int VB = kAttendColumns, C = kAttendTile, NS = KD / 64, NK = KD / 32, NV = VB / 32, NQ = KD / 32, DB = VB / 16;
+    constexpr int VB = kAttendColumns, C = kAttendTile, NS = KD / 16, NK = KD / 32, NV = VB / 32, NQ = KD / 32, DB = VB / 16;
     extern __shared__ __align__(16) char lds[];
     char *const ks = lds, *const vs = lds + Lds::kValues, *const high_copy = lds + Lds::kStates, *const low_copy = lds + Lds::kLow;
     float* const scales = reinterpret_cast<float*>(lds + Lds::kScales);  // [2][VB]
@@ -110,61 +114,74 @@ __global__ __launch_bounds__(256, KD == 256 ? 1 : 2) void AttendHalfKernel(Atten
     int keys = run.keys;
     const int col0 = (block - run.first) * VB, cols = min(VB, run.values - col0);
 
-    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / 64), tw = wave / 2, dw = wave % 2;
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / 64);
     int lane = tid % 64;
     // What follows from the lane is found again in every tile: kept over the loop, it would take the registers of what is multiplied.
-    const auto in_tile = [&] { return lane % 32; };
-    const auto upper = [&] { return lane / 32; };
     const auto dots = [&] { return run.dots + (static_cast<int64_t>(bh) * run.blocks + block - run.first) * p.length; };
 
-    const auto state_row = [&](int n, int r) { return KD / 2 * tw + 32 * n + 8 * (r / 4) + 4 * upper() + r % 4; };
-    const auto state_col = [&] { return 32 * dw + in_tile(); };
-    attend16_t s[NS];
-#pragma unroll
-    for (int n = 0; n < NS; ++n) {
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-            s[n][r] = 0;
-        }
-    }
-    // elements that are not there are read as the last ones: all loads go out at once
-    const auto state_at = [&](const AttendStates& of, int n, int r) {
-        const int i = state_row(n, r);
-        const float v = of.data[bh * of.head + segment * of.segment + min(i, keys - 1) * of.i + (col0 + min(state_col(), cols - 1)) * of.j];
-        return i < keys && state_col() < cols ? v : 0.f;
-    };
-    if (OUT && run.start.data != nullptr) {
+    const auto state_row = [&](int n, int r) { return 16 * n + lane / 16 * 4 + r; };
+    const auto state_col = [&] { return 16 * wave + lane % 16; };
+    attend4_t s[NS]{};
+    // Elements that are not there are read as the last ones, so that all loads go out at once; the compiler would have each wait for its condition.
+    const auto states_at = [&](const AttendStates& of, attend4_t (&to)[NS]) {
+        const float* const from = of.data + bh * of.head + segment * of.segment + (col0 + min(state_col(), cols - 1)) * of.j;
 #pragma unroll
         for (int n = 0; n < NS; ++n) {
 #pragma unroll
-            for (int r = 0; r < 16; ++r) s[n][r] = state_at(run.start, n, r);
+            for (int r = 0; r < 4; ++r) to[n][r] = from[min(state_row(n, r), keys - 1) * of.i];
         }
-    }
+#pragma unroll
+        for (int n = 0; n < NS; ++n) {
+            asm volatile("" : "+v"(to[n]));
+#pragma unroll
+            for (int r = 0; r < 4; ++r) to[n][r] = state_row(n, r) < keys && state_col() < cols ? to[n][r] : 0.f;
+        }
+    };
     float minus = -1;
     asm volatile("" : "+s"(minus));
-    const auto keep_state = [&] {
-        float most = 0;
+    int unit = 0;    // the state is s times 2^unit
+    float most = 0;  // the largest |s| of the column
+    const auto find_most = [&] {
+        most = 0;
 #pragma unroll
         for (int n = 0; n < NS; ++n) {
 #pragma unroll
-            for (int r = 0; r < 16; ++r) most = fmaxf(most, fabsf(s[n][r]));
+            for (int r = 0; r < 4; ++r) most = fmaxf(most, fabsf(s[n][r]));
         }
-        const Scale scale(MaxOver32(most));
-        if (upper() == 0) scales[tw * VB + state_col()] = scale.out;
+        most = MaxOver32(MaxOver16(most));
+        const bool over = most >= 0x1p15f && most < HUGE_VALF;
+        if (__any(over)) {
+            const int up = over ? min(ExponentOf(most) - 13, 114 - unit) : 0;
+            unit += up;
+            most *= Power(-up);
 #pragma unroll
-        for (int n = 0; n < NS; ++n) {
-#pragma unroll
-            for (int g = 0; g < 4; ++g) {
-                const float v[4] = {s[n][4 * g] * scale.in, s[n][4 * g + 1] * scale.in, s[n][4 * g + 2] * scale.in, s[n][4 * g + 3] * scale.in};
-                attend_half4_t hi, lo;
-                Split<4>(v, minus, &hi, &lo);
-                const int at = state_col() * Lds::kStatePitch + state_row(n, 4 * g) * 2;
-                *reinterpret_cast<attend_half4_t*>(high_copy + at) = hi;
-                *reinterpret_cast<attend_half4_t*>(low_copy + at) = lo;
-            }
+            for (int n = 0; n < NS; ++n) s[n] *= Power(-up);
         }
     };
-    if (OUT) keep_state();
+    const auto keep_state = [&] {
+        if (lane / 16 == 0) scales[state_col()] = Power(unit);
+#pragma unroll
+        for (int n = 0; n < NS; ++n) {
+            const float v[4] = {s[n][0], s[n][1], s[n][2], s[n][3]};
+            attend_half4_t hi, lo;
+            Split<4>(v, minus, &hi, &lo);
+            const int at = state_col() * Lds::kStatePitch + state_row(n, 0) * 2;
+            *reinterpret_cast<attend_half4_t*>(high_copy + at) = hi;
+            *reinterpret_cast<attend_half4_t*>(low_copy + at) = lo;
+        }
+    };
+    if (OUT) {
+        if (run.start.data != nullptr) states_at(run.start, s);
+        find_most();
+        if (most > 0 && most < 0x1p4f) {
+            const int down = max(ExponentOf(most) - 13, -112);
+            unit = down;
+            most *= Power(-down);
+#pragma unroll
+            for (int n = 0; n < NS; ++n) s[n] *= Power(-down);
+        }
+        keep_state();
+    }
 
     // A tile's rows on their way: pieces of eight elements of k and of v.  Rows that are not there are the last one again; columns that are not there are zeros that stay in LDS.  Rows lie less
     // than 2^24 elements apart, so that a tile's are within 32 bits of its first.
@@ -194,6 +211,7 @@ __global__ __launch_bounds__(256, KD == 256 ? 1 : 2) void AttendHalfKernel(Atten
         for (int e = 0; e < 8; ++e) v[e] = piece.v[e];
         return v;
     };
+    // (Behind the last tile every row is the last one: a branch round the loads would have those of the tile before, too, waited for where the two ways meet.)
     const auto load = [&](int64_t r0) {  // k and v; at the tile's first row
         const int last = static_cast<int>(rows - r0 < C ? rows - r0 : C) - 1;
 #pragma unroll
@@ -210,14 +228,16 @@ __global__ __launch_bounds__(256, KD == 256 ? 1 : 2) void AttendHalfKernel(Atten
             qp += static_cast<int64_t>(q_row) * C;
         }
     };
-    float g_next = 0;
-    const auto load_decays = [&](int64_t r0) {  // of a row that is there; sum_next takes those that count
+    // Log decays, by one wave, a lane to a row: summed up a tile ahead, on their way two tiles ahead, so that nothing waits for what was asked for in the same tile.
+    float g_now = 0, g_next = 0;
+    const auto load_decays = [&](int64_t r0) {  // of a row that is there; sum_decays takes those that count
+        if (gp == nullptr) return;
         const int64_t r = r0 + lane < rows ? r0 + lane : rows - 1;
-        if (gp != nullptr) g_next = gp[(r < g_rows ? g_rows : r) * g_row * (rows > g_rows ? 1 : 0)];
+        g_next = gp[(r < g_rows ? g_rows : r) * g_row * (rows > g_rows ? 1 : 0)];
     };
-    const auto sum_next = [&](int64_t r0, AttendDecays* to) {  // by one wave
+    const auto sum_decays = [&](int64_t r0, AttendDecays* to) {
         const int here = static_cast<int>(rows - r0 < C ? rows - r0 : C);
-        SumDecays(to, gp != nullptr && lane < here && r0 + lane >= g_rows ? LogOfDecay(g_next) : 0, here, kv_scale);
+        SumDecays(to, gp != nullptr && lane < here && r0 + lane >= g_rows ? LogOfDecay(g_now) : 0, here, kv_scale);
     };
     if (EVEN) {
 #pragma unroll
@@ -231,15 +251,16 @@ __global__ __launch_bounds__(256, KD == 256 ? 1 : 2) void AttendHalfKernel(Atten
     }
     if (tid == 0) odd[0] = odd[1] = 0;
     if (rows > 0) {
+        if (wave == 0) {
+            load_decays(0);
+            g_now = g_next;
+            load_decays(C);
+        }
         load(0);
         load_q(0);
-        if (wave == 0) load_decays(0), sum_next(0, decays);
+        if (wave == 0) sum_decays(0, decays);
     }
     double passed = 0;  // log decay of the tiles so far
-    // where a lane reads blocks of 4 x 16: rows 4 upper() and on, columns of its 32
-    const auto turned_row = [&] { return 4 * upper() + lane % 16 / 4; };
-    const auto turned_col = [&] { return (lane / 16 % 2 * 16 + lane % 4 * 4) * 2; };
-
     int turn = 0;
     int64_t r0 = 0;
     __syncthreads();  // the flags
@@ -265,17 +286,16 @@ __global__ __launch_bounds__(256, KD == 256 ? 1 : 2) void AttendHalfKernel(Atten
         // An infinity of a later row, times P's zeros, would reach earlier ones: the rest goes row by row.
         if (OUT && odd[turn] != 0) break;
         const bool more = r0 + C < rows;
-        if (more) {
-            load(r0 + C);
-            if (wave == 0) load_decays(r0 + C);
-        }
+        g_now = g_next;
+        if (wave == 0) load_decays(r0 + 2 * C);
+        load(r0 + C);
         if constexpr (OUT) {
             // this wave's sixteen rows by all columns, in blocks of 16 x 16
             const int quarter = lane / 16;
             const float high = dec->high[own_row()], low = dec->low[own_row()];
             attend4_t y[DB];
             {
-                attend4_t of_state[2][DB]{};
+                attend4_t of_state[DB]{};
                 const int at = lane % 16 * Lds::kStatePitch + 16 * quarter;
                 attend_half8_t part[2][DB];
                 const auto read = [&](int step, attend_half8_t (&to)[DB]) {  // step 2 m: the low parts, 2 m + 1: the high ones
@@ -288,16 +308,15 @@ __global__ __launch_bounds__(256, KD == 256 ? 1 : 2) void AttendHalfKernel(Atten
                 for (int step = 0; step < 2 * NQ; ++step) {  // reads of the next step under the products of this one
                     if (step + 1 < 2 * NQ) read(step + 1, part[step % 2 ^ 1]);
 #pragma unroll
-                    for (int d = 0; d < DB; ++d) of_state[step / NQ][d] = Mfma(part[step % 2][d], q[step / 2], of_state[step / NQ][d]);
+                    for (int d = 0; d < DB; ++d) of_state[d] = Mfma(part[step % 2][d], q[step / 2], of_state[d]);
                     __builtin_amdgcn_sched_barrier(0);
                 }
                 const float from_start = __builtin_amdgcn_exp2f(high + low) * run.out_scale;
 #pragma unroll
                 for (int d = 0; d < DB; ++d) {
-                    const int j = 16 * d + 4 * quarter;
-                    const attend4_t first = *reinterpret_cast<const attend4_t*>(scales + j), second = *reinterpret_cast<const attend4_t*>(scales + VB + j);
+                    const attend4_t units = *reinterpret_cast<const attend4_t*>(scales + 16 * d + 4 * quarter);
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) y[d][e] = __builtin_fmaf(of_state[0][d][e], first[e], of_state[1][d][e] * second[e]) * from_start;
+                    for (int e = 0; e < 4; ++e) y[d][e] = of_state[d][e] * units[e] * from_start;
                 }
             }
             __builtin_amdgcn_sched_barrier(0);  // (the products with the state need as many registers as those with k)
@@ -319,10 +338,10 @@ __global__ __launch_bounds__(256, KD == 256 ? 1 : 2) void AttendHalfKernel(Atten
                     __builtin_amdgcn_sched_barrier(0);
                 }
             }
-            if (wave == 0 && more) sum_next(r0 + C, decays + (turn ^ 1));
+            if (wave == 0 && more) sum_decays(r0 + C, decays + (turn ^ 1));
             if (tid == 0) odd[turn ^ 1] = 0;
             // weights: of the sixteen rows that this one is among, exp(G[t] - G[s]); of earlier ones, whose last is l, exp(G[l] - G[s]) here and exp(G[t] - G[l]) with the power of two
-            float most = 0, since[4];
+            float largest = 0, since[4];
 #pragma unroll
             for (int sb = 0; sb < 4; ++sb) {
                 if (sb > wave) continue;
@@ -341,9 +360,9 @@ __global__ __launch_bounds__(256, KD == 256 ? 1 : 2) void AttendHalfKernel(Atten
                     for (int e = 0; e < 4; ++e) a[sb][e] *= near[e];
                     since[sb] = __builtin_amdgcn_exp2f((high - dec->high[16 * sb + 15]) + (low - dec->low[16 * sb + 15]));
                 }
-                most = fmaxf(most, fmaxf(fmaxf(fabsf(a[sb][0]), fabsf(a[sb][1])), fmaxf(fabsf(a[sb][2]), fabsf(a[sb][3]))) * since[sb]);
+                largest = fmaxf(largest, fmaxf(fmaxf(fabsf(a[sb][0]), fabsf(a[sb][1])), fmaxf(fabsf(a[sb][2]), fabsf(a[sb][3]))) * since[sb]);
             }
-            const Scale scale(MaxOver32(MaxOver16(most)));
+            const Scale scale(MaxOver32(MaxOver16(largest)));
             attend4_t of_rows[DB]{};
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
@@ -407,63 +426,62 @@ __global__ __launch_bounds__(256, KD == 256 ? 1 : 2) void AttendHalfKernel(Atten
             }
             yp += static_cast<int64_t>(y_row) * C;
         } else {
-            if (wave == 0 && more) sum_next(r0 + C, decays + (turn ^ 1));
-        }
-        attend_half8_t v[C / 16];  // this wave's 32 columns: rows 16 u + ... of step u
-#pragma unroll
-        for (int u = 0; u < C / 16; ++u) {
-            const char* const at = vs + (16 * u + turned_row()) * Lds::kValuePitch + dw * 64 + turned_col();
-            v[u] = Join(ReadTurned(at), ReadTurned(at + 8 * Lds::kValuePitch));
+            if (wave == 0 && more) sum_decays(r0 + C, decays + (turn ^ 1));
         }
         __builtin_amdgcn_sched_barrier(0);
-        if (more) load_q(r0 + C);
-        // v times its rows' weights, in two parts
-        float w[C / 16][8], most = 0;
-#pragma unroll
-        for (int u = 0; u < C / 16; ++u) {
-#pragma unroll
-            for (int g = 0; g < 2; ++g) {
-                const attend4_t end = *reinterpret_cast<const attend4_t*>(dec->end + 16 * u + 8 * g + 4 * upper());
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    w[u][4 * g + e] = __builtin_fmaf(static_cast<float>(v[u][4 * g + e]), end[e], 0.f);
-                    most = fmaxf(most, fabsf(w[u][4 * g + e]));
-                }
-            }
-        }
-        const Scale scale(MaxOver32(most));
-        attend16_t add[NS]{};
+        load_q(r0 + C);
         {
-            attend_half8_t k[2][NS];
-            const auto read = [&](int u, attend_half8_t (&to)[NS]) {
+            // this wave's columns of v times their rows' weights, in two parts
+            const int block = lane / 16 * 4 + lane % 16 / 4, piece = lane % 4 * 8;
+            const char *const from = vs + block * Lds::kValuePitch + 32 * wave + piece, *const at = ks + block * Lds::kKeyPitch + piece;
+            attend_half8_t k[2][NS / 2];
+            const auto read = [&](int step, attend_half8_t (&to)[NS / 2]) {  // half of the keys of 32 rows
 #pragma unroll
-                for (int n = 0; n < NS; ++n) {
-                    const char* const at = ks + (16 * u + turned_row()) * Lds::kKeyPitch + (KD / 2 * tw + 32 * n) * 2 + turned_col();
-                    to[n] = Join(ReadTurned(at), ReadTurned(at + 8 * Lds::kKeyPitch));
+                for (int n = 0; n < NS / 2; ++n) {
+                    const char* const row = at + 32 * (step / 2) * Lds::kKeyPitch + 32 * (step % 2 * (NS / 2) + n);
+                    to[n] = Join(ReadTurned(row), ReadTurned(row + 16 * Lds::kKeyPitch));
                 }
             };
-            read(0, k[0]);
+            float w[2][8], largest = 0;
 #pragma unroll
-            for (int u = 0; u < C / 16; ++u) {
-                if (u + 1 < C / 16) read(u + 1, k[u % 2 ^ 1]);
+            for (int u = 0; u < 2; ++u) {
+                const attend_half8_t v = Join(ReadTurned(from + 32 * u * Lds::kValuePitch), ReadTurned(from + (32 * u + 16) * Lds::kValuePitch));
 #pragma unroll
-                for (int e = 0; e < 8; ++e) w[u][e] *= scale.in;
-                attend_half8_t hi, lo;
-                Split<8>(w[u], minus, &hi, &lo);
+                for (int g = 0; g < 2; ++g) {
+                    const attend4_t end = *reinterpret_cast<const attend4_t*>(dec->end + 32 * u + 16 * g + lane / 16 * 4);
 #pragma unroll
-                for (int n = 0; n < NS; ++n) {
-                    add[n] = Mfma(k[u % 2][n], lo, add[n]);
-                    add[n] = Mfma(k[u % 2][n], hi, add[n]);
+                    for (int e = 0; e < 4; ++e) {
+                        w[u][4 * g + e] = __builtin_fmaf(static_cast<float>(v[4 * g + e]), end[e], 0.f);
+                        largest = fmaxf(largest, fabsf(w[u][4 * g + e]));
+                    }
                 }
+            }
+            read(0, k[0]);
+            const float all = dec->all, decayed = most * all, added = MaxOver32(MaxOver16(largest)) * Power(-unit);
+            const float size = fmaxf(decayed < HUGE_VALF ? decayed : 0.f, added);
+            int up = 0;
+            if (size >= 0x1p15f || (size < 0x1p4f && size > 0)) up = min(max(ExponentOf(size) - 13, -112 - unit), 114 - unit);
+            unit += up;
+            const float keep = all * Power(-up), in = Power(-unit);
+#pragma unroll
+            for (int n = 0; n < NS; ++n) s[n] *= keep;
+            attend_half8_t hi, lo;
+#pragma unroll
+            for (int step = 0; step < 4; ++step) {
+                if (step + 1 < 4) read(step + 1, k[step % 2 ^ 1]);
+                if (step % 2 == 0) {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) w[step / 2][e] *= in;
+                    Split<8>(w[step / 2], minus, &hi, &lo);
+                }
+#pragma unroll
+                for (int n = 0; n < NS / 2; ++n) s[step % 2 * (NS / 2) + n] = Mfma(k[step % 2][n], lo, s[step % 2 * (NS / 2) + n]);
+#pragma unroll
+                for (int n = 0; n < NS / 2; ++n) s[step % 2 * (NS / 2) + n] = Mfma(k[step % 2][n], hi, s[step % 2 * (NS / 2) + n]);
                 __builtin_amdgcn_sched_barrier(0);
             }
         }
-        const float all = dec->all;
-#pragma unroll
-        for (int n = 0; n < NS; ++n) {
-#pragma unroll
-            for (int r = 0; r < 16; ++r) s[n][r] = __builtin_fmaf(s[n][r], all, add[n][r] * scale.out);
-        }
+        find_most();
         __syncthreads();  // the copies of the state, and the rows of k and v, have been read
         if (OUT) keep_state();
     }
@@ -474,7 +492,7 @@ __global__ __launch_bounds__(256, KD == 256 ? 1 : 2) void AttendHalfKernel(Atten
 #pragma unroll
         for (int n = 0; n < NS; ++n) {
 #pragma unroll
-            for (int r = 0; r < 16; ++r) ss[state_row(n, r) * VB + state_col()] = s[n][r];
+            for (int r = 0; r < 4; ++r) ss[state_row(n, r) * VB + state_col()] = s[n][r] * Power(unit);
         }
         __syncthreads();
         const int j = lane;
@@ -512,17 +530,18 @@ __global__ __launch_bounds__(256, KD == 256 ? 1 : 2) void AttendHalfKernel(Atten
 #pragma unroll
         for (int n = 0; n < NS; ++n) {
 #pragma unroll
-            for (int r = 0; r < 16; ++r) s[n][r] = ss[state_row(n, r) * VB + state_col()];
+            for (int r = 0; r < 4; ++r) s[n][r] = ss[state_row(n, r) * VB + state_col()];
         }
+        unit = 0;
     }
     if constexpr (!OUT) {
         float* const to = run.last.data + bh * run.last.head + segment * run.last.segment;
 #pragma unroll
         for (int n = 0; n < NS; ++n) {
 #pragma unroll
-            for (int r = 0; r < 16; ++r) {
+            for (int r = 0; r < 4; ++r) {
                 const int i = state_row(n, r);
-                if (i < keys && state_col() < cols) to[i * run.last.i + (col0 + state_col()) * run.last.j] = s[n][r];
+                if (i < keys && state_col() < cols) to[i * run.last.i + (col0 + state_col()) * run.last.j] = s[n][r] * Power(unit);
             }
         }
         if (tid == 0 && block == run.first) run.decays[static_cast<int64_t>(bh) * p.segments + segment] = __builtin_amdgcn_exp2f(static_cast<float>(passed));
@@ -539,13 +558,12 @@ __global__ __launch_bounds__(256, KD == 256 ? 1 : 2) void AttendHalfKernel(Atten
         // <state behind the segment, its gradient there>, the waves' parts added up in the same order always
         float dot = 0;
         if (run.other.data != nullptr) {
+            attend4_t other[NS];
+            states_at(run.other, other);
 #pragma unroll
             for (int n = 0; n < NS; ++n) {
 #pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    const float other = state_at(run.other, n, r);
-                    dot += state_row(n, r) < keys && state_col() < cols ? s[n][r] * other : 0.f;
-                }
+                for (int r = 0; r < 4; ++r) dot += state_row(n, r) < keys && state_col() < cols ? s[n][r] * Power(unit) * other[n][r] : 0.f;
             }
         }
 #pragma unroll
@@ -564,9 +582,9 @@ __global__ __launch_bounds__(256, KD == 256 ? 1 : 2) void AttendHalfKernel(Atten
 #pragma unroll
         for (int n = 0; n < NS; ++n) {
 #pragma unroll
-            for (int r = 0; r < 16; ++r) {
+            for (int r = 0; r < 4; ++r) {
                 const int i = state_row(n, r);
-                if (i < keys && state_col() < cols) to[i * run.last.i + (col0 + state_col()) * run.last.j] = s[n][r] * more;
+                if (i < keys && state_col() < cols) to[i * run.last.i + (col0 + state_col()) * run.last.j] = s[n][r] * Power(unit) * more;
             }
         }
     }
