@@ -62,11 +62,11 @@ __device__ __forceinline__ attend4_t Mfma(attend_half8_t a, attend_half8_t b, at
 // LDS of a workgroup, in bytes.  Rows' pitches keep the banks apart.  Clocks of a wave's instruction (eight waves at work), at 128 keys: k and the state's copies read by rows, sixteen rows of 64
 // bytes each, 4.0 with 32 or 96 bytes more than a multiple of 256, 7.9 with 16, 6.6 with 80; v in blocks of 4 x 16, sixteen rows, 2.6 with 32 more than 128, 4.0 with 64; the state's copies
 // written, 8.0 with 32, 5.0 with 16.
-template <int KD>
+template <int KD, bool OUT>
 struct AttendHalfLds {
     static constexpr int kKeyPitch = KD * 2 + 96, kValuePitch = kAttendColumns * 2 + 32, kStatePitch = KD * 2 + 32;
-    static constexpr int kValues = kAttendTile * kKeyPitch, kStates = kValues + kAttendTile * kValuePitch, kLow = kStates + kAttendColumns * kStatePitch,
-                         kScales = kLow + kAttendColumns * kStatePitch, kSums = kScales + kAttendColumns * 4, kDecays = kSums + 4 * kAttendColumns * 4,
+    static constexpr int kValues = kAttendTile * kKeyPitch, kStates = kValues + kAttendTile * kValuePitch,
+                         kLow = kStates + (OUT ? kAttendColumns * kStatePitch : 0), kScales = kLow + (OUT ? kAttendColumns * kStatePitch : 0), kSums = kScales + kAttendColumns * 4, kDecays = kSums + 4 * kAttendColumns * 4,
                          kOdd = kDecays + 2 * static_cast<int>(sizeof(AttendDecays)), kBytes = kOdd + 16;
     static_assert(kValues % 16 == 0 && kStates % 16 == 0 && kDecays % 16 == 0 && sizeof(AttendDecays) % 16 == 0, "aligned parts");
 };
@@ -83,7 +83,7 @@ struct AttendHalfLds {
 template <int KD, bool OUT, bool EVEN, bool GRAD>
 __global__ __launch_bounds__(256, KD == 256 ? 1 : 2) void AttendHalfKernel(AttendArgs p) {
     using T = half_t;
-    using Lds = AttendHalfLds<KD>;
+    using Lds = AttendHalfLds<KD, OUT>;
     constexpr int VB = kAttendColumns, C = kAttendTile, NS = KD / 16, NK = KD / 32, NV = VB / 32, NQ = KD / 32, DB = VB / 16;
     extern __shared__ __align__(16) char lds[];
     char *const ks = lds, *const vs = lds + Lds::kValues, *const high_copy = lds + Lds::kStates, *const low_copy = lds + Lds::kLow;
@@ -287,8 +287,8 @@ __global__ __launch_bounds__(256, KD == 256 ? 1 : 2) void AttendHalfKernel(Atten
         if (OUT && odd[turn] != 0) break;
         const bool more = r0 + C < rows;
         g_now = g_next;
-        if (wave == 0) load_decays(r0 + 2 * C);
         load(r0 + C);
+        if (wave == 0) load_decays(r0 + 2 * C);  // (behind the others: what waits for them must not wait for this one)
         if constexpr (OUT) {
             // this wave's sixteen rows by all columns, in blocks of 16 x 16
             const int quarter = lane / 16;
@@ -597,7 +597,7 @@ void LaunchAttendHalf(const AttendArgs& p, int keys, int64_t blocks, bool states
     for (int i = 0; i < p.runs; ++i) even = even && p.run[i].keys % 8 == 0 && p.run[i].values % 8 == 0;
     const auto launch = [&](auto kd) {
         const auto kernel = [&](auto out, auto whole, auto grad) {
-            constexpr int KD = decltype(kd)::value, kLds = AttendHalfLds<KD>::kBytes;
+            constexpr int KD = decltype(kd)::value, kLds = AttendHalfLds<KD, decltype(out)::value>::kBytes;
             void (*const k)(AttendArgs) = AttendHalfKernel<KD, decltype(out)::value, decltype(whole)::value, decltype(grad)::value>;
             EnsureDynamicLds<AttendHalfTag>(reinterpret_cast<const void*>(k), kLds);
             hipLaunchKernelGGL(k, dim3(static_cast<unsigned>(blocks)), dim3(256), kLds, stream, p);
