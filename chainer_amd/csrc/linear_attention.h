@@ -87,6 +87,38 @@ __device__ __forceinline__ AttendPiece<T, N> AttendLoad(const T* row, int at, in
     return r;
 }
 
+// The same without a branch where the row has N elements at all: a piece that reaches over the row's end is read as far back as it has to be (AttendLoadBack), and its elements move to their places
+// when they are used (AttendMove), so that loads of many pieces are under way together.  `before`: elements of the row in front of `row`.
+template <typename T, int N>
+__device__ __forceinline__ AttendPiece<T, N> AttendLoadBack(const T* row, int at, int end, int before) {
+    if (before + end >= N) return *reinterpret_cast<const AttendPiece<T, N>*>(row + (at < end ? min(at, end - N) : end - N));
+    AttendPiece<T, N> r;
+#pragma unroll
+    for (int e = 0; e < N; ++e) r.v[e] = row[min(at + e, end - 1)];
+    return r;
+}
+template <typename T, int N>
+__device__ __forceinline__ AttendPiece<T, N> AttendMove(AttendPiece<T, N> r, int at, int end, int before) {
+    static_assert(N * sizeof(T) == 16, "four registers");
+    typedef uint32_t registers_t __attribute__((ext_vector_type(4)));
+    const int back = before + end >= N && at < end ? max(0, at + N - end) : 0;
+    registers_t d = __builtin_bit_cast(registers_t, r);
+    if constexpr (sizeof(T) == 2) {
+        const registers_t half{d[0] >> 16 | d[1] << 16, d[1] >> 16 | d[2] << 16, d[2] >> 16 | d[3] << 16, d[3] >> 16};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) d[i] = back & 1 ? half[i] : d[i];
+    }
+    constexpr int one = 4 / sizeof(T);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) d[i] = back & one ? (i < 3 ? d[i + 1] : 0u) : d[i];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) d[i] = back & (2 * one) ? (i < 2 ? d[i + 2] : 0u) : d[i];
+    r = __builtin_bit_cast(AttendPiece<T, N>, d);
+#pragma unroll
+    for (int e = 0; e < N; ++e) r.v[e] = at + e < end ? r.v[e] : static_cast<T>(0);
+    return r;
+}
+
 // A log decay in powers of two.  -infinity, a state that ends, is held at a number that no product of decays brings back.
 __device__ __forceinline__ double LogOfDecay(float decay) {
     const double g = static_cast<double>(decay) * 1.4426950408889634;
@@ -173,13 +205,24 @@ __device__ __forceinline__ double AttendStep(const AttendArgs& p, const AttendRu
     return t + 1 < length ? AttendDecay(p, b, h, t + 1) : 0;
 }
 
-// How the time axis is cut: segments of whole tiles, so that about two workgroups to a compute unit have work.
-inline void CutAttend(AttendArgs* p, int64_t blocks) {
-    const int64_t tiles = (p->length + kAttendTile - 1) / kAttendTile;
-    const int64_t each = std::max<int64_t>(1, p->batch * p->heads * blocks), wanted = 2 * int64_t{NumCUs()};
-    int64_t segments = std::min<int64_t>((wanted + each - 1) / each, tiles / 4);
-    if (segments < 2) segments = 1;
-    p->segment_rows = std::max<int64_t>(1, (tiles + segments - 1) / segments) * kAttendTile;
+// How the time axis is cut: into segments of whole tiles, four at least, of the number that costs least.  Costs are in a tile's time with the compute units full (`resident` workgroups to each):
+// a round of workgroups takes a segment's tiles and three more for what comes before and behind them, six tenths of that where there is a workgroup to a compute unit at most; segments need
+// the states that they start from first, which takes 0.4 of a tile each, and a pass over the states.  `blocks`: workgroups to a head and segment; `states`: those of the states alone.
+inline void CutAttend(AttendArgs* p, int64_t blocks, int64_t states, int64_t resident, int64_t matrix) {
+    const int64_t tiles = (p->length + kAttendTile - 1) / kAttendTile, heads = p->batch * p->heads, units = NumCUs();
+    const auto rounds = [&](int64_t workgroups, int64_t at_once) {
+        const int64_t rest = workgroups % at_once;
+        return static_cast<double>(workgroups / at_once) + (rest == 0 ? 0.0 : rest <= units ? 0.6 : 1.0);
+    };
+    int64_t best = 1;
+    double least = 0;
+    for (int64_t n = 1; n <= std::max<int64_t>(1, std::min<int64_t>(tiles / 4, 64)); ++n) {
+        const int64_t each = (tiles + n - 1) / n;
+        double cost = rounds(heads * blocks * n, units * resident) * static_cast<double>(each + 3);
+        if (n > 1) cost += rounds(heads * states * (n - 1), units * 4) * (0.4 * static_cast<double>(each) + 2) + 1 + static_cast<double>(heads * n * matrix) * 3e-7;
+        if (n == 1 || cost < least) best = n, least = cost;
+    }
+    p->segment_rows = std::max<int64_t>(1, (tiles + best - 1) / best) * kAttendTile;
     p->segments = static_cast<int>(std::max<int64_t>(1, (p->length + p->segment_rows - 1) / p->segment_rows));
 }
 
@@ -187,7 +230,7 @@ inline void CutAttend(AttendArgs* p, int64_t blocks) {
 struct AttendCall {
     AttendArgs p{};
     AttendRows q, k, v;
-    int keys, values, key_heads;
+    int keys, values, key_heads, dtype;
     const float* state;
 };
 bool AttendSizesOf(const hipcx_array* q, const hipcx_array* v, AttendCall* c);
@@ -206,6 +249,9 @@ inline AttendStates AttendSegments(float* data, const AttendArgs& p, int keys, i
     return {data, each * p.segments, each, values, 1};
 }
 inline int AttendBlocks(int values) { return (values + kAttendColumns - 1) / kAttendColumns; }
+
+// Workgroups that a compute unit holds, as LDS lets them.
+inline int64_t AttendResident(int dtype, int keys) { return keys <= 64 ? 3 : keys <= 128 && dtype == HIPCX_FLOAT16 ? 2 : 1; }
 
 void LaunchAttend(const AttendArgs& p, int dtype, bool states_alone, hipStream_t stream);
 void LaunchAttendHalf(const AttendArgs& p, int keys, int64_t blocks, bool states_alone, hipStream_t stream);  // float16

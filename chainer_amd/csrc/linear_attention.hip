@@ -9,24 +9,30 @@ namespace {
 
 struct AttendTag {};
 
-__device__ __forceinline__ float Finite(float v) { return v - v; }  // 0, or not a number
-
 // Tiles of 64 rows, one after another.  With G the decays summed up from the tile's first row and S the state before it,
 //   P[t][s] = exp(G[t] - G[s]) q[t] k[s] for s <= t,  y = P v + exp(G) q S,  S <- exp(G[63]) S + (exp(G[63] - G) k)^T v.
-// A workgroup of four waves has 64 columns of v: a wave multiplies 32 rows by 32 columns of y, and has half of the keys and 32 columns of S in its accumulators (a copy is in LDS, for the products with q).
+// A workgroup of four waves has 64 columns of v: a wave has sixteen rows of y, and sixteen columns of S in its accumulators (a copy is in LDS, turned, for the products with q).
 // P stays in registers: as k q^T its column t is a lane, whose rows s are the reduction of the product v^T P.
-// Products run on the float pipe (v_mfma_f32_32x32x2_f32).
+// Products run on the float pipe (v_mfma_f32_16x16x4_f32), with the reduction's elements in an order that gives a lane four neighbours.
+// EVEN: rows of whole pieces of four elements.  GRAD: what the passes of the gradients have beyond the forward one.
 template <int KD, bool OUT>
-__global__ __launch_bounds__(256) void AttendKernel(AttendArgs p) {
-    using T = float;
-    constexpr int KP = KD + 4, VB = kAttendColumns, C = kAttendTile, NS = KD / 64;
-    extern __shared__ __align__(16) char lds[];
-    float* const ks = reinterpret_cast<float*>(lds);      // [C][KP]
-    float* const vs = ks + C * KP;                        // [C][VB]
-    float* const ss = vs + C * VB;                        // [KD][VB]
-    float* const red = ss + KD * VB;                      // [4][VB]
-    AttendDecays* const dec = reinterpret_cast<AttendDecays*>(red + 4 * VB);
-    int* const odd = reinterpret_cast<int*>(dec + 1);     // v has infinities or what is not a number
+struct AttendLds {
+    static constexpr int kPitch = KD + 4, kValuePitch = kAttendColumns + 4;  // floats; four rows on is sixteen banks on
+    static constexpr int kValues = kAttendTile * kPitch, kStates = kValues + kAttendTile * kValuePitch, kSums = kStates + (OUT ? kAttendColumns * kPitch : 0);
+    static constexpr int kDecays = kSums + 4 * kAttendColumns;
+    static constexpr int kBytes = kDecays * 4 + 2 * static_cast<int>(sizeof(AttendDecays)) + 16;
+};
+
+__device__ __forceinline__ attend4_t Mfma4(float a, float b, attend4_t c) { return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0); }
+
+template <int KD, bool OUT, bool EVEN, bool GRAD>
+__global__ __launch_bounds__(256, KD == 64 ? 3 : 1) void AttendKernel(AttendArgs p) {
+    using Lds = AttendLds<KD, OUT>;
+    constexpr int VB = kAttendColumns, C = kAttendTile, NS = KD / 16, KP = Lds::kPitch, VP = Lds::kValuePitch, DB = VB / 16;
+    extern __shared__ __align__(16) float lds[];
+    float *const ks = lds, *const vs = lds + Lds::kValues, *const ss = lds + Lds::kStates, *const sums = lds + Lds::kSums;  // rows, rows, columns of the state
+    AttendDecays* const decays = reinterpret_cast<AttendDecays*>(lds + Lds::kDecays);
+    int* const odd = reinterpret_cast<int*>(decays + 2);  // v has infinities or what is not a number
 
     int id = AttendNumber(p);
     if (id < 0) return;
@@ -35,222 +41,336 @@ __global__ __launch_bounds__(256) void AttendKernel(AttendArgs p) {
     const int bh = id % static_cast<int>(p.batch * p.heads);
     const int segment_turn = id / static_cast<int>(p.batch * p.heads);
     int which = 0;
-    while (which + 1 < p.runs && block >= p.run[which + 1].first) ++which;
-    const AttendRun& run = p.run[which];
-    const int segment = run.back ? p.segments - 1 - segment_turn : segment_turn;
+    if (GRAD) {
+        while (which + 1 < p.runs && block >= p.run[which + 1].first) ++which;
+    }
+    const AttendRun& run = p.run[GRAD ? which : 0];
+    const bool back = GRAD && run.back != 0, with_dots = GRAD && OUT && run.dots != nullptr;
+    const float kv_scale = GRAD ? run.kv_scale : 1.f;
+    const int segment = back ? p.segments - 1 - segment_turn : segment_turn;
     const int64_t b = bh / p.heads;
     const int h = bh % p.heads;
     const int64_t length = LengthOf(p.lengths, b, p.length);
     const AttendSpan span(p, length, segment);
     const int64_t rows = span.end - span.first;
+    int keys = run.keys;
     const int col0 = (block - run.first) * VB, cols = min(VB, run.values - col0);
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / 64);
+    int lane = tid % 64;
+    float* const dots = with_dots ? run.dots + (static_cast<int64_t>(bh) * run.blocks + block - run.first) * p.length : nullptr;
 
-    const int tid = threadIdx.x, lane = tid % 64, wave = tid / 64, l32 = lane % 32, half = lane / 32;
-    const int tw = wave / 2, dw = wave % 2;
-    const T* const kp = static_cast<const T*>(run.k.data) + b * run.k.batch + (h / run.k.share) * run.k.head;
-    const T* const vp = static_cast<const T*>(run.v.data) + b * run.v.batch + (h / run.v.share) * run.v.head + col0;
-    const T* const qp = OUT ? static_cast<const T*>(run.q.data) + b * run.q.batch + (h / run.q.share) * run.q.head : nullptr;
-    const T* const dp = OUT && run.dots != nullptr ? static_cast<const T*>(run.dot.data) + b * run.dot.batch + (h / run.dot.share) * run.dot.head + col0 : nullptr;
-    const int64_t y0 = OUT ? b * run.y.batch + h * run.y.head + col0 : 0;
-    float* const dots = OUT && run.dots != nullptr ? run.dots + (static_cast<int64_t>(bh) * run.blocks + block - run.first) * p.length : nullptr;
-
-    // element r of a state's accumulator n: row i, column j of the workgroup's
-    const auto state_row = [&](int n, int r) { return KD / 2 * tw + 32 * n + 8 * (r / 4) + 4 * half + r % 4; };
-    const int state_col = 32 * dw + l32;
-    attend16_t s[NS];
-#pragma unroll
-    for (int n = 0; n < NS; ++n) {
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-            const int i = state_row(n, r);
-            s[n][r] = OUT && run.start.data != nullptr && i < run.keys && state_col < cols
-                          ? run.start.data[bh * run.start.head + segment * run.start.segment + i * run.start.i + (col0 + state_col) * run.start.j]
-                          : 0.f;
-        }
-    }
-    const auto keep_state = [&] {
+    const auto state_row = [&](int n, int r) { return 16 * n + lane / 16 * 4 + r; };
+    const auto state_col = [&] { return 16 * wave + lane % 16; };
+    attend4_t s[NS]{};
+    // Elements that are not there are read as the last ones, so that all loads go out at once; the compiler would have each wait for its condition.
+    const auto states_at = [&](const AttendStates& of, attend4_t (&to)[NS]) {
+        const float* const from = of.data + bh * of.head + segment * of.segment + (col0 + min(state_col(), cols - 1)) * of.j;
 #pragma unroll
         for (int n = 0; n < NS; ++n) {
 #pragma unroll
-            for (int r = 0; r < 16; ++r) ss[state_row(n, r) * VB + state_col] = s[n][r];
+            for (int r = 0; r < 4; ++r) to[n][r] = from[min(state_row(n, r), keys - 1) * of.i];
+        }
+#pragma unroll
+        for (int n = 0; n < NS; ++n) {
+            asm volatile("" : "+v"(to[n]));
+#pragma unroll
+            for (int r = 0; r < 4; ++r) to[n][r] = state_row(n, r) < keys && state_col() < cols ? to[n][r] : 0.f;
         }
     };
-    if (OUT) keep_state();
-    double passed = 0;  // log decay of the tiles so far
+    const auto keep_state = [&] {
+#pragma unroll
+        for (int n = 0; n < NS; ++n) *reinterpret_cast<attend4_t*>(ss + state_col() * KP + state_row(n, 0)) = s[n];
+    };
 
-    for (int64_t r0 = 0; r0 < rows; r0 += C) {
-        const int here = static_cast<int>(rows - r0 < C ? rows - r0 : C);
-        if (tid == 0) *odd = 0;
-        __syncthreads();
-        for (int at = tid; at < C * KD / 4; at += 256) {
-            const int row = at / (KD / 4), i = at % (KD / 4) * 4;
-            attend4_t v{0, 0, 0, 0};
-            if (row < here) {
-                const AttendPiece<T, 4> piece = AttendLoad<T, 4>(kp + AttendRowOf(span, run.back, r0 + row) * run.k.row, i, run.keys);
+    // A tile's rows on their way: pieces of four elements.  Rows that are not there are the last one again (their weights are zeros; behind the last tile every row is, since a branch round the loads
+    // would have those of the tile before, too, waited for where the two ways meet); elements that are not there become zeros.  Rows lie less than 2^24 elements apart, so that a tile's are within
+    // 32 bits of its first.
+    constexpr int KR = 1024 / KD, NK = C / KR, NV = C / 16;  // rows of k that are read at once, and times
+    const int key_row = tid / (KD / 4), key_col = tid % (KD / 4) * 4, value_row = tid / 16, value_col = tid % 16 * 4;
+    const auto own_row = [&] { return 16 * wave + lane % 16; };  // of a tile
+    const int way = back ? -1 : 1;
+    const int64_t row0 = back ? span.end - 1 : span.first;
+    const float* kp = static_cast<const float*>(run.k.data) + b * run.k.batch + (h / run.k.share) * run.k.head + row0 * run.k.row;
+    const float* vp = static_cast<const float*>(run.v.data) + b * run.v.batch + (h / run.v.share) * run.v.head + row0 * run.v.row + col0;
+    const float* qp = OUT ? static_cast<const float*>(run.q.data) + b * run.q.batch + (h / run.q.share) * run.q.head + row0 * run.q.row : nullptr;
+    const int k_row = way * static_cast<int>(run.k.row), v_row = way * static_cast<int>(run.v.row), q_row = OUT ? way * static_cast<int>(run.q.row) : 0;
+    float* yp = OUT ? static_cast<float*>(run.y.data) + b * run.y.batch + h * run.y.head + row0 * run.y.row + col0 : nullptr;
+    const int y_row = OUT ? way * static_cast<int>(run.y.row) : 0;
+    const float* dp = with_dots ? static_cast<const float*>(run.dot.data) + b * run.dot.batch + (h / run.dot.share) * run.dot.head + row0 * run.dot.row + col0 : nullptr;
+    const int d_row = with_dots ? way * static_cast<int>(run.dot.row) : 0;
+    const float* gp = p.decay != nullptr ? p.decay + b * p.decay_batch + h * p.decay_head + (row0 + (back ? 1 : 0)) * p.decay_row : nullptr;
+    const int64_t g_row = way * p.decay_row;
+    const int64_t g_rows = back && span.end == length ? 1 : 0;  // the first row has no decay: none follows it
+    AttendPiece<float, 4> k_next[NK], v_next[NV], q_next[OUT ? NS : 1];
+    const auto piece_at = [&](const float* row, int col, int end, int before) {
+        if constexpr (EVEN) return *reinterpret_cast<const AttendPiece<float, 4>*>(row + (col < end ? col : 0));
+        else return AttendLoadBack<float, 4>(row, col, end, before);
+    };
+    const auto moved = [&](const AttendPiece<float, 4>& piece, int col, int end, int before) {
+        attend4_t v;
+        if constexpr (EVEN) {
 #pragma unroll
-                for (int e = 0; e < 4; ++e) v[e] = static_cast<float>(piece.v[e]);
-            }
-            *reinterpret_cast<attend4_t*>(ks + row * KP + i) = v;
-        }
-        for (int at = tid; at < C * VB / 4; at += 256) {
-            const int row = at / (VB / 4), j = at % (VB / 4) * 4;
-            attend4_t v{0, 0, 0, 0};
-            if (row < here) {
-                const AttendPiece<T, 4> piece = AttendLoad<T, 4>(vp + AttendRowOf(span, run.back, r0 + row) * run.v.row, j, cols);
+            for (int e = 0; e < 4; ++e) v[e] = col < end ? piece.v[e] : 0.f;
+        } else {
+            const AttendPiece<float, 4> there = AttendMove<float, 4>(piece, col, end, before);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) v[e] = static_cast<float>(piece.v[e]);
-                if (OUT && Finite(v[0]) + Finite(v[1]) + Finite(v[2]) + Finite(v[3]) != 0) *odd = 1;
-            }
-            *reinterpret_cast<attend4_t*>(vs + row * VB + j) = v;
+            for (int e = 0; e < 4; ++e) v[e] = there.v[e];
         }
-        if (wave == 0) SumDecays(dec, lane < here ? AttendStep(p, run, span, b, h, length, r0 + lane) : 0, here, run.kv_scale);
-        attend4_t q[OUT ? KD / 8 : 1];
-        const int t = 32 * tw + l32;  // this lane's row
+        return v;
+    };
+    const auto load = [&](int64_t r0) {  // k and v; at the tile's first row
+        const int last = static_cast<int>(rows - r0 < C ? rows - r0 : C) - 1;
+#pragma unroll
+        for (int n = 0; n < NK; ++n) k_next[n] = piece_at(kp + min(key_row + n * KR, last) * k_row, key_col, keys, 0);
+#pragma unroll
+        for (int n = 0; n < NV; ++n) v_next[n] = piece_at(vp + min(value_row + n * 16, last) * v_row, value_col, cols, col0);
+        kp += static_cast<int64_t>(k_row) * C, vp += static_cast<int64_t>(v_row) * C;
+    };
+    const auto load_q = [&](int64_t r0) {
         if constexpr (OUT) {
+            const float* const at = qp + min(own_row(), static_cast<int>(rows - r0 < C ? rows - r0 : C) - 1) * q_row;
 #pragma unroll
-            for (int m = 0; m < KD / 8; ++m) {
-                q[m] = attend4_t{0, 0, 0, 0};
-                if (t < here) {
-                    const AttendPiece<T, 4> piece = AttendLoad<T, 4>(qp + AttendRowOf(span, run.back, r0 + t) * run.q.row, 8 * m + 4 * half, run.keys);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) q[m][e] = static_cast<float>(piece.v[e]);
-                }
-            }
+            for (int m = 0; m < NS; ++m) q_next[m] = piece_at(at, 16 * m + lane / 16 * 4, keys, 0);
+            qp += static_cast<int64_t>(q_row) * C;
         }
+    };
+    // Log decays, by one wave, a lane to a row: summed up a tile ahead, on their way two tiles ahead, so that nothing waits for what was asked for in the same tile.
+    float g_now = 0, g_next = 0;
+    const auto load_decays = [&](int64_t r0) {  // of a row that is there; sum_decays takes those that count
+        if (gp == nullptr) return;
+        const int64_t r = r0 + lane < rows ? r0 + lane : rows - 1;
+        g_next = gp[(r < g_rows ? g_rows : r) * g_row * (rows > g_rows ? 1 : 0)];
+    };
+    const auto sum_decays = [&](int64_t r0, AttendDecays* to) {
+        const int here = static_cast<int>(rows - r0 < C ? rows - r0 : C);
+        SumDecays(to, gp != nullptr && lane < here && r0 + lane >= g_rows ? LogOfDecay(g_now) : 0, here, kv_scale);
+    };
+    if (tid == 0) odd[0] = odd[1] = 0;
+    if (rows > 0) {
+        if (wave == 0) {
+            load_decays(0);
+            g_now = g_next;
+            load_decays(C);
+        }
+        load(0);
+        load_q(0);
+        if (wave == 0) sum_decays(0, decays);
+    }
+    if (OUT) {
+        if (run.start.data != nullptr) states_at(run.start, s);
+        keep_state();
+    }
+    double passed = 0;  // log decay of the tiles so far
+    int turn = 0;
+    int64_t r0 = 0;
+    __syncthreads();  // the flags
+    for (; r0 < rows; r0 += C, turn ^= 1) {
+        asm volatile("" : "+v"(lane));  // (what follows from these is found again in every tile, and takes no registers over the loop)
+        asm volatile("" : "+s"(keys));
+        const int quarter = lane / 16;
+        const AttendDecays* const dec = decays + turn;
+        // (the last tile's rows of k and v have been read by all)
+#pragma unroll
+        for (int n = 0; n < NK; ++n) *reinterpret_cast<attend4_t*>(ks + (key_row + n * KR) * KP + key_col) = moved(k_next[n], key_col, keys, 0);
+        float finite = 0;  // or not a number
+#pragma unroll
+        for (int n = 0; n < NV; ++n) {
+            const attend4_t v = moved(v_next[n], value_col, cols, col0);
+            *reinterpret_cast<attend4_t*>(vs + (value_row + n * 16) * VP + value_col) = v;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) finite = __builtin_fmaf(v[e], 0.f, finite);
+        }
+        if (OUT && !(finite == 0)) odd[turn] = 1;
         __syncthreads();
         passed += dec->sum;
-        if (OUT && *odd != 0) {
-            // An infinity of a later row, times P's zeros, would reach earlier ones: row by row instead, on the copy in LDS.
-            const int j = lane;
-            for (int r = 0; r < here; ++r) {
-                const int64_t row = AttendRowOf(span, run.back, r0 + r);
-                const float step = dec->step[r], v = vs[r * VB + j] * run.kv_scale;
-                float y = 0;
-                for (int i = wave * (KD / 4); i < (wave + 1) * (KD / 4); ++i) {
-                    const float now = ss[i * VB + j] * step + ks[r * KP + i] * v;
-                    ss[i * VB + j] = now;
-                    if (i < run.keys) y += static_cast<float>(qp[row * run.q.row + i]) * now;
-                }
-                red[wave * VB + j] = y;
-                __syncthreads();
-                if (wave == 0) {
-                    y = (red[j] + red[VB + j] + red[2 * VB + j] + red[3 * VB + j]) * run.out_scale;
-                    if (j < cols) {
-                        if (run.wide) static_cast<float*>(run.y.data)[y0 + row * run.y.row + j] = y;
-                        else static_cast<T*>(run.y.data)[y0 + row * run.y.row + j] = static_cast<T>(y);
-                    }
-                    if (dots != nullptr) {
-                        float dot = j < cols ? y * static_cast<float>(dp[row * run.dot.row + j]) : 0.f;
-#pragma unroll
-                        for (int o = 1; o < 64; o <<= 1) dot += __shfl_xor(dot, o);
-                        if (lane == 0) dots[row] = dot;
-                    }
-                }
-                __syncthreads();
-            }
-#pragma unroll
-            for (int n = 0; n < NS; ++n) {
-#pragma unroll
-                for (int r = 0; r < 16; ++r) s[n][r] = ss[state_row(n, r) * VB + state_col];
-            }
-            continue;
-        }
+        // An infinity of a later row, times P's zeros, would reach earlier ones: the rest goes row by row.
+        if (OUT && odd[turn] != 0) break;
+        const bool more = r0 + C < rows;
+        g_now = g_next;
+        load(r0 + C);
+        if (wave == 0) load_decays(r0 + 2 * C);  // (behind the others: what waits for them must not wait for this one)
         if constexpr (OUT) {
-            const float high = dec->high[t], low = dec->low[t];
-            attend16_t y{};
+            // this wave's sixteen rows by all columns, in blocks of 16 x 16
+            const float high = dec->high[own_row()], low = dec->low[own_row()];
+            attend4_t q[NS];
 #pragma unroll
-            for (int m = 0; m < KD / 8; ++m) {
+            for (int m = 0; m < NS; ++m) q[m] = moved(q_next[m], 16 * m + 4 * quarter, keys, 0);
+            attend4_t y[DB]{};
+            {
+                const float* const at = ss + lane % 16 * KP + 4 * quarter;
+                attend4_t part[2][DB];
+                const auto read = [&](int m, attend4_t (&to)[DB]) {
 #pragma unroll
-                for (int e = 0; e < 4; ++e) y = __builtin_amdgcn_mfma_f32_32x32x2f32(ss[(8 * m + 4 * half + e) * VB + state_col], q[m][e], y, 0, 0, 0);
+                    for (int d = 0; d < DB; ++d) to[d] = *reinterpret_cast<const attend4_t*>(at + 16 * d * KP + 16 * m);
+                };
+                read(0, part[0]);
+#pragma unroll
+                for (int m = 0; m < NS; ++m) {  // reads of the next step under the products of this one
+                    if (m + 1 < NS) read(m + 1, part[m % 2 ^ 1]);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+#pragma unroll
+                        for (int d = 0; d < DB; ++d) y[d] = Mfma4(part[m % 2][d][e], q[m][e], y[d]);
+                    }
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+                const float from_start = __builtin_amdgcn_exp2f(high + low);
+#pragma unroll
+                for (int d = 0; d < DB; ++d) y[d] *= from_start;
             }
-            const float from_start = __builtin_amdgcn_exp2f(high + low);
+            attend4_t a[4]{};
+            {
+                const float* const at = ks + lane % 16 * KP + 4 * quarter;
 #pragma unroll
-            for (int r = 0; r < 16; ++r) y[r] *= from_start;
-            for (int sb = 0; sb <= tw; ++sb) {  // rows up to this wave's
-                attend16_t a{};
+                for (int m = 0; m < NS; ++m) {
+                    attend4_t part[4];
 #pragma unroll
-                for (int m = 0; m < KD / 8; ++m) {
-                    const attend4_t k = *reinterpret_cast<const attend4_t*>(ks + (32 * sb + l32) * KP + 8 * m + 4 * half);
+                    for (int sb = 0; sb < 4; ++sb) part[sb] = *reinterpret_cast<const attend4_t*>(at + 16 * min(sb, wave) * KP + 16 * m);
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) a = __builtin_amdgcn_mfma_f32_32x32x2f32(k[e], q[m][e], a, 0, 0, 0);
-                }
+                    for (int sb = 0; sb < 4; ++sb) {
+                        if (sb > wave) continue;
 #pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    const int at = 32 * sb + 8 * (r / 4) + 4 * half + r % 4;
-                    const float weight = __builtin_amdgcn_exp2f((high - dec->high[at]) + (low - dec->low[at])) * run.kv_scale;
-                    a[r] = at <= t ? a[r] * weight : 0.f;
-                }
-#pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    const int at = 32 * sb + 8 * (r / 4) + 4 * half + r % 4;
-                    y = __builtin_amdgcn_mfma_f32_32x32x2f32(vs[at * VB + state_col], a[r], y, 0, 0, 0);
+                        for (int e = 0; e < 4; ++e) a[sb] = Mfma4(part[sb][e], q[m][e], a[sb]);
+                    }
                 }
             }
-            const int64_t row = AttendRowOf(span, run.back, r0 + t);
+            load_q(r0 + C);
+            if (wave == 0 && more) sum_decays(r0 + C, decays + (turn ^ 1));
+            if (tid == 0) odd[turn ^ 1] = 0;
+#pragma unroll
+            for (int sb = 0; sb < 4; ++sb) {
+                if (sb > wave) continue;
+                const int first = 16 * sb + 4 * quarter;
+                const attend4_t highs = *reinterpret_cast<const attend4_t*>(dec->high + first), lows = *reinterpret_cast<const attend4_t*>(dec->low + first);
+                float v[DB][4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+#pragma unroll
+                    for (int d = 0; d < DB; ++d) v[d][e] = vs[(first + e) * VP + 16 * d + lane % 16];
+                }
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float weighted = a[sb][e] * (__builtin_amdgcn_exp2f((high - highs[e]) + (low - lows[e])) * kv_scale);
+                    a[sb][e] = first + e <= own_row() ? weighted : 0.f;
+                }
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+#pragma unroll
+                    for (int d = 0; d < DB; ++d) y[d] = Mfma4(v[d][e], a[sb][e], y[d]);
+                }
+            }
+            float* const to = yp + static_cast<int64_t>(own_row()) * y_row;
+            const bool live = r0 + own_row() < rows;
             float dot = 0;
-            if (t < here) {
 #pragma unroll
-                for (int g = 0; g < 4; ++g) {
-                    const int j = 32 * dw + 8 * g + 4 * half;
-                    AttendPiece<float, 4> v;
+            for (int d = 0; d < DB; ++d) {
+                const int j = 16 * d + 4 * quarter;
+                AttendPiece<float, 4> out;
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) v.v[e] = y[4 * g + e] * run.out_scale;
-                    if (dots != nullptr) {
-                        const AttendPiece<T, 4> with = AttendLoad<T, 4>(dp + row * run.dot.row, j, cols);
+                for (int e = 0; e < 4; ++e) out.v[e] = y[d][e] * run.out_scale;
+                if (!live) continue;
+                if (with_dots) {
+                    const float* const row = dp + static_cast<int64_t>(own_row()) * d_row;
+                    AttendPiece<float, 4> with{};
+                    if (!EVEN) with = AttendLoad<float, 4>(row, j, cols);
+                    else if (j < cols) with = *reinterpret_cast<const AttendPiece<float, 4>*>(row + j);
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) dot += j + e < cols ? v.v[e] * static_cast<float>(with.v[e]) : 0.f;
-                    }
-                    const int64_t to = y0 + row * run.y.row + j;
-                    if (j + 4 <= cols) {
-                        if (run.wide) {
-                            *reinterpret_cast<AttendPiece<float, 4>*>(static_cast<float*>(run.y.data) + to) = v;
-                        } else {
-                            AttendPiece<T, 4> o;
+                    for (int e = 0; e < 4; ++e) dot += j + e < cols ? out.v[e] * with.v[e] : 0.f;
+                }
+                if (EVEN ? j < cols : j + 4 <= cols) {
+                    *reinterpret_cast<AttendPiece<float, 4>*>(to + j) = out;
+                } else if (!EVEN) {
 #pragma unroll
-                            for (int e = 0; e < 4; ++e) o.v[e] = static_cast<T>(v.v[e]);
-                            *reinterpret_cast<AttendPiece<T, 4>*>(static_cast<T*>(run.y.data) + to) = o;
-                        }
-                    } else {
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            if (j + e >= cols) continue;
-                            if (run.wide) static_cast<float*>(run.y.data)[to + e] = v.v[e];
-                            else static_cast<T*>(run.y.data)[to + e] = static_cast<T>(v.v[e]);
-                        }
+                    for (int e = 0; e < 4; ++e) {
+                        if (j + e < cols) to[j + e] = out.v[e];
                     }
                 }
             }
-            if (dots != nullptr) {  // the two halves of the columns meet in LDS
+            if (with_dots) {
+                dot += __shfl_xor(dot, 16);
                 dot += __shfl_xor(dot, 32);
-                if (half == 0 && dw == 1) red[t] = dot;
+                if (quarter == 0 && live) dots[row0 + way * (r0 + own_row())] = dot;
+                dp += static_cast<int64_t>(d_row) * C;
             }
-            __syncthreads();  // the copy of the state has been read
-            if (dots != nullptr && half == 0 && dw == 0 && t < here) dots[row] = dot + red[t];
+            yp += static_cast<int64_t>(y_row) * C;
+        } else {
+            if (wave == 0 && more) sum_decays(r0 + C, decays + (turn ^ 1));
         }
-        const float all = dec->all;
+        __builtin_amdgcn_sched_barrier(0);
+        {
+            // this wave's columns of v times their rows' weights
+            const float all = dec->all;
 #pragma unroll
-        for (int n = 0; n < NS; ++n) {
+            for (int n = 0; n < NS; ++n) s[n] *= all;
+            const float *const from = vs + 4 * quarter * VP + state_col(), *const at = ks + 4 * quarter * KP + lane % 16;
+            constexpr int N = NS < 8 ? NS : 8;  // accumulators between the reads
 #pragma unroll
-            for (int r = 0; r < 16; ++r) s[n][r] *= all;
+            for (int sb = 0; sb < 4; ++sb) {
+                const attend4_t end = *reinterpret_cast<const attend4_t*>(dec->end + 16 * sb + 4 * quarter);
+                float v[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[e] = from[(16 * sb + e) * VP] * end[e];
+#pragma unroll
+                for (int n0 = 0; n0 < NS; n0 += N) {
+                    float k[4][N];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+#pragma unroll
+                        for (int n = 0; n < N; ++n) k[e][n] = at[(16 * sb + e) * KP + 16 * (n0 + n)];
+                    }
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+#pragma unroll
+                        for (int n = 0; n < N; ++n) s[n0 + n] = Mfma4(k[e][n], v[e], s[n0 + n]);
+                    }
+                }
+            }
         }
-#pragma unroll 4
-        for (int m = 0; m < C / 2; ++m) {
-            const int at = 2 * m + half;
-            const float v = vs[at * VB + state_col] * dec->end[at];
-#pragma unroll
-            for (int n = 0; n < NS; ++n) s[n] = __builtin_amdgcn_mfma_f32_32x32x2f32(ks[at * KP + KD / 2 * tw + 32 * n + l32], v, s[n], 0, 0, 0);
-        }
+        __syncthreads();  // the copy of the state, and the rows of k and v, have been read
         if (OUT) keep_state();
     }
 
+    if (OUT && r0 < rows) {
+        // row by row, on the copy
+        const int j = lane;
+        for (; r0 < rows; ++r0) {
+            const int64_t row = row0 + way * r0;
+            const float* const k = static_cast<const float*>(run.k.data) + b * run.k.batch + (h / run.k.share) * run.k.head + row * run.k.row;
+            const float* const x = static_cast<const float*>(run.q.data) + b * run.q.batch + (h / run.q.share) * run.q.head + row * run.q.row;
+            const float* const of_v = static_cast<const float*>(run.v.data) + b * run.v.batch + (h / run.v.share) * run.v.head + row * run.v.row + col0;
+            const float step = gp != nullptr && r0 >= g_rows ? __builtin_amdgcn_exp2f(static_cast<float>(LogOfDecay(gp[r0 * g_row]))) : 1.f, v = j < cols ? of_v[j] * kv_scale : 0.f;
+            float y = 0;
+            for (int i = wave * (KD / 4); i < (wave + 1) * (KD / 4) && i < keys; ++i) {
+                const float now = ss[j * KP + i] * step + k[i] * v;
+                ss[j * KP + i] = now;
+                y += x[i] * now;
+            }
+            sums[wave * VB + j] = y;
+            __syncthreads();
+            if (wave == 0) {
+                y = (sums[j] + sums[VB + j] + sums[2 * VB + j] + sums[3 * VB + j]) * run.out_scale;
+                if (j < cols) static_cast<float*>(run.y.data)[b * run.y.batch + h * run.y.head + row * run.y.row + col0 + j] = y;
+                if (with_dots) {
+                    float dot = 0;
+                    if (j < cols) dot = y * (static_cast<const float*>(run.dot.data) + b * run.dot.batch + (h / run.dot.share) * run.dot.head + row * run.dot.row + col0)[j];
+#pragma unroll
+                    for (int o = 1; o < 64; o <<= 1) dot += __shfl_xor(dot, o);
+                    if (lane == 0) dots[row] = dot;
+                }
+            }
+            __syncthreads();
+        }
+#pragma unroll
+        for (int n = 0; n < NS; ++n) s[n] = *reinterpret_cast<const attend4_t*>(ss + state_col() * KP + state_row(n, 0));
+    }
     if constexpr (!OUT) {
         float* const to = run.last.data + bh * run.last.head + segment * run.last.segment;
 #pragma unroll
         for (int n = 0; n < NS; ++n) {
 #pragma unroll
-            for (int r = 0; r < 16; ++r) {
+            for (int r = 0; r < 4; ++r) {
                 const int i = state_row(n, r);
-                if (i < run.keys && state_col < cols) to[i * run.last.i + (col0 + state_col) * run.last.j] = s[n][r];
+                if (i < keys && state_col() < cols) to[i * run.last.i + (col0 + state_col()) * run.last.j] = s[n][r];
             }
         }
         if (tid == 0 && block == run.first) run.decays[static_cast<int64_t>(bh) * p.segments + segment] = __builtin_amdgcn_exp2f(static_cast<float>(passed));
@@ -258,44 +378,39 @@ __global__ __launch_bounds__(256) void AttendKernel(AttendArgs p) {
     }
     // rows behind the sequence's end
     for (int64_t row = (span.end > span.first ? span.end : span.first) + wave; row < span.whole; row += 4) {
-        if (lane >= cols) continue;
-        const int64_t to = y0 + row * run.y.row + lane;
-        if (run.wide) static_cast<float*>(run.y.data)[to] = 0.f;
-        else static_cast<T*>(run.y.data)[to] = static_cast<T>(0);
+        if (lane < cols) static_cast<float*>(run.y.data)[b * run.y.batch + h * run.y.head + row * run.y.row + col0 + lane] = 0.f;
     }
-    if (run.ends != nullptr) {
-        // <state behind the segment, its gradient there>; one wave after another adds its part up in the same order always
+    if (GRAD && run.ends != nullptr) {
+        // <state behind the segment, its gradient there>, the waves' parts added up in the same order always
         float dot = 0;
         if (run.other.data != nullptr) {
+            attend4_t other[NS];
+            states_at(run.other, other);
 #pragma unroll
             for (int n = 0; n < NS; ++n) {
 #pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    const int i = state_row(n, r);
-                    if (i < run.keys && state_col < cols)
-                        dot += s[n][r] * run.other.data[bh * run.other.head + segment * run.other.segment + i * run.other.i + (col0 + state_col) * run.other.j];
-                }
+                for (int r = 0; r < 4; ++r) dot += state_row(n, r) < keys && state_col() < cols ? s[n][r] * other[n][r] : 0.f;
             }
         }
 #pragma unroll
         for (int o = 1; o < 64; o <<= 1) dot += __shfl_xor(dot, o);
         __syncthreads();
-        if (lane == 0) red[wave] = dot;
+        if (lane == 0) sums[wave] = dot;
         __syncthreads();
         if (tid == 0) {
             const float behind = span.end < length ? __builtin_amdgcn_exp2f(static_cast<float>(AttendDecay(p, b, h, span.end))) : 1.f;
-            run.ends[(static_cast<int64_t>(bh) * p.segments + segment) * run.blocks + block - run.first] = (red[0] + red[1] + red[2] + red[3]) * behind;
+            run.ends[(static_cast<int64_t>(bh) * p.segments + segment) * run.blocks + block - run.first] = (sums[0] + sums[1] + sums[2] + sums[3]) * behind;
         }
     }
     if (run.last.data != nullptr && segment_turn == p.segments - 1) {
-        const float more = run.decay_last && length > 0 ? __builtin_amdgcn_exp2f(static_cast<float>(AttendDecay(p, b, h, 0))) : 1.f;
+        const float more = GRAD && run.decay_last && length > 0 ? __builtin_amdgcn_exp2f(static_cast<float>(AttendDecay(p, b, h, 0))) : 1.f;
         float* const to = run.last.data + bh * run.last.head;
 #pragma unroll
         for (int n = 0; n < NS; ++n) {
 #pragma unroll
-            for (int r = 0; r < 16; ++r) {
+            for (int r = 0; r < 4; ++r) {
                 const int i = state_row(n, r);
-                if (i < run.keys && state_col < cols) to[i * run.last.i + (col0 + state_col) * run.last.j] = s[n][r] * more;
+                if (i < keys && state_col() < cols) to[i * run.last.i + (col0 + state_col()) * run.last.j] = s[n][r] * more;
             }
         }
     }
@@ -307,12 +422,21 @@ __global__ __launch_bounds__(256) void AttendStartsKernel(AttendStates at, Atten
     const int i = e / values, j = e % values;
     float* const to = at.data + bh * at.head + i * at.i + j * at.j;
     float now = initial.data != nullptr ? initial.data[bh * initial.head + i * initial.i + j * initial.j] : 0.f;
-    for (int n = 0; n < segments; ++n) {
-        const int segment = back ? segments - 1 - n : n;
-        float* const here = to + segment * at.segment;
-        const float more = n + 1 < segments ? *here : 0.f;
-        *here = now;
-        if (n + 1 < segments) now = __builtin_elementwise_fma(now, decays[static_cast<int64_t>(bh) * segments + segment], more);
+    const float* const decay = decays + static_cast<int64_t>(bh) * segments;
+    constexpr int N = 8;  // segments whose loads go out together
+    for (int n = 0; n < segments; n += N) {
+        float more[N], keep[N];
+#pragma unroll
+        for (int k = 0; k < N; ++k) {  // (the last one's own share and decay have no place to go, and those behind it are it again)
+            const int turn = min(n + k, segments - 2), segment = back ? segments - 1 - turn : turn;
+            more[k] = to[segment * at.segment], keep[k] = decay[segment];
+        }
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+            if (n + k >= segments) continue;
+            to[(back ? segments - 1 - n - k : n + k) * at.segment] = now;
+            now = __builtin_elementwise_fma(now, keep[k], more[k]);
+        }
     }
 }
 
@@ -394,11 +518,6 @@ __global__ __launch_bounds__(256) void AttendTokensKernel(AttendArgs p) {
     }
 }
 
-template <int KD>
-constexpr int AttendLds() {
-    return (kAttendTile * (KD + 4) + kAttendTile * kAttendColumns + KD * kAttendColumns + 4 * kAttendColumns) * 4 + static_cast<int>(sizeof(AttendDecays)) + 16;
-}
-
 template <typename F>
 void VisitKeys(int keys, F&& f) {
     if (keys <= 64) f(std::integral_constant<int, 64>{});
@@ -423,17 +542,19 @@ void LaunchAttend(const AttendArgs& args, int dtype, bool states_alone, hipStrea
     if (blocks == 0) return;
     p.groups = static_cast<int>(groups);
     if (dtype == HIPCX_FLOAT16) return LaunchAttendHalf(p, keys, blocks, states_alone, stream);
+    bool even = true;
+    for (int i = 0; i < p.runs; ++i) even = even && p.run[i].keys % 4 == 0 && p.run[i].values % 4 == 0;
     VisitKeys(keys, [&](auto kd) {
-        constexpr int KD = decltype(kd)::value, kLds = AttendLds<KD>();
-        const dim3 grid(static_cast<unsigned>(blocks));
-        if (states_alone) {
-            EnsureDynamicLds<AttendTag>(reinterpret_cast<const void*>(AttendKernel<KD, false>), kLds);
-            hipLaunchKernelGGL((AttendKernel<KD, false>), grid, dim3(256), kLds, stream, p);
-        } else {
-            EnsureDynamicLds<AttendTag>(reinterpret_cast<const void*>(AttendKernel<KD, true>), kLds);
-            hipLaunchKernelGGL((AttendKernel<KD, true>), grid, dim3(256), kLds, stream, p);
-        }
-        CheckLaunch("linear_attention");
+        const auto kernel = [&](auto out, auto whole, auto grad) {
+            constexpr int KD = decltype(kd)::value, kLds = AttendLds<KD, decltype(out)::value>::kBytes;
+            void (*const k)(AttendArgs) = AttendKernel<KD, decltype(out)::value, decltype(whole)::value, decltype(grad)::value>;
+            EnsureDynamicLds<AttendTag>(reinterpret_cast<const void*>(k), kLds);
+            hipLaunchKernelGGL(k, dim3(static_cast<unsigned>(blocks)), dim3(256), kLds, stream, p);
+            CheckLaunch("linear_attention");
+        };
+        const auto whole = [&](auto out, auto grad) { even ? kernel(out, std::true_type{}, grad) : kernel(out, std::false_type{}, grad); };
+        if (states_alone) p.runs > 1 ? whole(std::false_type{}, std::true_type{}) : whole(std::false_type{}, std::false_type{});
+        else p.runs > 1 ? whole(std::true_type{}, std::true_type{}) : whole(std::true_type{}, std::false_type{});
     });
 }
 
@@ -471,7 +592,7 @@ bool AttendSizesOf(const hipcx_array* q, const hipcx_array* v, AttendCall* c) {
     if (q->shape[0] < 0 || q->shape[1] < 0 || q->shape[1] >= (int64_t{1} << 30) || kh < 1 || h < 1 || h >= (1 << 20) || h % kh != 0) return false;
     if (q->shape[3] < 1 || q->shape[3] > kMaxAttend || v->shape[3] < 1 || v->shape[3] > kMaxAttend || q->shape[0] > kBlocksPerLaunch / h) return false;
     c->p.batch = q->shape[0], c->p.length = q->shape[1], c->p.heads = static_cast<int>(h);
-    c->keys = static_cast<int>(q->shape[3]), c->values = static_cast<int>(v->shape[3]), c->key_heads = static_cast<int>(kh);
+    c->keys = static_cast<int>(q->shape[3]), c->values = static_cast<int>(v->shape[3]), c->key_heads = static_cast<int>(kh), c->dtype = q->dtype;
     return true;
 }
 
@@ -523,7 +644,7 @@ constexpr int kAttendTokens = 8;
 
 void CutForward(AttendCall* c) {
     if (c->p.length <= kAttendTokens) c->p.segments = 1, c->p.segment_rows = kAttendTile;
-    else CutAttend(&c->p, AttendBlocks(c->values));
+    else CutAttend(&c->p, AttendBlocks(c->values), AttendBlocks(c->values), AttendResident(c->dtype, c->keys), static_cast<int64_t>(c->keys) * c->values);
 }
 
 size_t ForwardWorkspace(const AttendCall& c) {

@@ -110,7 +110,10 @@ struct GradWorkspace {
     }
 };
 
-void CutGrad(AttendCall* c) { CutAttend(&c->p, 2 * AttendBlocks(c->keys) + AttendBlocks(c->values)); }
+void CutGrad(AttendCall* c) {
+    const int64_t keys = AttendBlocks(c->keys), values = AttendBlocks(c->values);
+    CutAttend(&c->p, 2 * keys + values, keys + values, AttendResident(c->dtype, std::max(c->keys, c->values)), 2 * static_cast<int64_t>(c->keys) * c->values);
+}
 
 }  // namespace
 }  // namespace hipcx
