@@ -87,36 +87,48 @@ __device__ __forceinline__ AttendPiece<T, N> AttendLoad(const T* row, int at, in
     return r;
 }
 
-// The same without a branch where the row has N elements at all: a piece that reaches over the row's end is read as far back as it has to be (AttendLoadBack), and its elements move to their places
-// when they are used (AttendMove), so that loads of many pieces are under way together.  `before`: elements of the row in front of `row`.
-template <typename T, int N>
-__device__ __forceinline__ AttendPiece<T, N> AttendLoadBack(const T* row, int at, int end, int before) {
-    if (before + end >= N) return *reinterpret_cast<const AttendPiece<T, N>*>(row + (at < end ? min(at, end - N) : end - N));
-    AttendPiece<T, N> r;
+// How the rows of a pass fall into pieces of 16 bytes: all whole; the last one not; rows of less than a piece.
+enum AttendWidths { kAttendWhole, kAttendPart, kAttendNarrow };
+
+// N elements of a row, a piece or less, without a branch, so that the loads of many are under way together: AttendFetch has them, from the row's end back where they reach over the end (a block of
+// columns has at least one and may have others in front of it: where the row has a whole piece, so has what ends at its end), and AttendPlace brings them to their places when they are used.
+template <int WIDTHS, int N, typename T>
+__device__ __forceinline__ AttendPiece<T, N> AttendFetch(const T* row, int at, int end) {
+    if constexpr (WIDTHS == kAttendNarrow) {
+        AttendPiece<T, N> r;
 #pragma unroll
-    for (int e = 0; e < N; ++e) r.v[e] = row[min(at + e, end - 1)];
-    return r;
-}
-template <typename T, int N>
-__device__ __forceinline__ AttendPiece<T, N> AttendMove(AttendPiece<T, N> r, int at, int end, int before) {
-    static_assert(N * sizeof(T) == 16, "four registers");
-    typedef uint32_t registers_t __attribute__((ext_vector_type(4)));
-    const int back = before + end >= N && at < end ? max(0, at + N - end) : 0;
-    registers_t d = __builtin_bit_cast(registers_t, r);
-    if constexpr (sizeof(T) == 2) {
-        const registers_t half{d[0] >> 16 | d[1] << 16, d[1] >> 16 | d[2] << 16, d[2] >> 16 | d[3] << 16, d[3] >> 16};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) d[i] = back & 1 ? half[i] : d[i];
+        for (int e = 0; e < N; ++e) r.v[e] = row[min(at + e, end - 1)];
+        return r;
+    } else {
+        return *reinterpret_cast<const AttendPiece<T, N>*>(row + (WIDTHS == kAttendWhole ? (at < end ? at : 0) : min(at, end - N)));
     }
-    constexpr int one = 4 / sizeof(T);
+}
+template <int WIDTHS, typename T, int N>
+__device__ __forceinline__ AttendPiece<T, N> AttendPlace(AttendPiece<T, N> r, int at, int end) {
+    constexpr int one = 4 / sizeof(T), R = N / one;
+    typedef uint32_t registers_t __attribute__((ext_vector_type(R)));
+    registers_t d = __builtin_bit_cast(registers_t, r);
+    if constexpr (WIDTHS == kAttendPart) {
+        const int back = max(0, at + N - end);
+        if constexpr (sizeof(T) == 2) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) d[i] = back & one ? (i < 3 ? d[i + 1] : 0u) : d[i];
+            for (int i = 0; i < R; ++i) d[i] = back & 1 ? d[i] >> 16 | (i + 1 < R ? d[i + 1] << 16 : 0u) : d[i];
+        }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) d[i] = back & (2 * one) ? (i < 2 ? d[i + 2] : 0u) : d[i];
-    r = __builtin_bit_cast(AttendPiece<T, N>, d);
+        for (int step = 1; step < R; step *= 2) {
 #pragma unroll
-    for (int e = 0; e < N; ++e) r.v[e] = at + e < end ? r.v[e] : static_cast<T>(0);
-    return r;
+            for (int i = 0; i < R; ++i) d[i] = back & (step * one) ? (i + step < R ? d[i + step] : 0u) : d[i];
+        }
+    }
+    if constexpr (WIDTHS == kAttendNarrow) {
+        r = __builtin_bit_cast(AttendPiece<T, N>, d);
+#pragma unroll
+        for (int e = 0; e < N; ++e) r.v[e] = at + e < end ? r.v[e] : static_cast<T>(0);
+        return r;
+    }
+#pragma unroll
+    for (int i = 0; i < R; ++i) d[i] = at < end ? d[i] : 0u;
+    return __builtin_bit_cast(AttendPiece<T, N>, d);
 }
 
 // A log decay in powers of two.  -infinity, a state that ends, is held at a number that no product of decays brings back.
@@ -249,6 +261,22 @@ inline AttendStates AttendSegments(float* data, const AttendArgs& p, int keys, i
     return {data, each * p.segments, each, values, 1};
 }
 inline int AttendBlocks(int values) { return (values + kAttendColumns - 1) / kAttendColumns; }
+
+inline AttendWidths AttendWidthsOf(const AttendArgs& p, int piece) {
+    bool whole = true, narrow = false;
+    for (int i = 0; i < p.runs; ++i) {
+        for (const int width : {p.run[i].keys, p.run[i].values}) whole = whole && width % piece == 0, narrow = narrow || width < piece;
+    }
+    return whole ? kAttendWhole : narrow ? kAttendNarrow : kAttendPart;
+}
+
+// (narrow rows, which are few bytes, have no kernels without what the gradients need)
+template <typename F>
+void VisitWidths(AttendWidths widths, bool grad, F&& f) {
+    if (widths == kAttendNarrow) f(std::integral_constant<int, kAttendNarrow>{}, std::true_type{});
+    else if (widths == kAttendWhole) grad ? f(std::integral_constant<int, kAttendWhole>{}, std::true_type{}) : f(std::integral_constant<int, kAttendWhole>{}, std::false_type{});
+    else grad ? f(std::integral_constant<int, kAttendPart>{}, std::true_type{}) : f(std::integral_constant<int, kAttendPart>{}, std::false_type{});
+}
 
 // Workgroups that a compute unit holds, as LDS lets them.
 inline int64_t AttendResident(int dtype, int keys) { return keys <= 64 ? 3 : keys <= 128 && dtype == HIPCX_FLOAT16 ? 2 : 1; }

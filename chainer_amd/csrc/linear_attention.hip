@@ -14,7 +14,7 @@ struct AttendTag {};
 // A workgroup of four waves has 64 columns of v: a wave has sixteen rows of y, and sixteen columns of S in its accumulators (a copy is in LDS, turned, for the products with q).
 // P stays in registers: as k q^T its column t is a lane, whose rows s are the reduction of the product v^T P.
 // Products run on the float pipe (v_mfma_f32_16x16x4_f32), with the reduction's elements in an order that gives a lane four neighbours.
-// EVEN: rows of whole pieces of four elements.  GRAD: what the passes of the gradients have beyond the forward one.
+// GRAD: what the passes of the gradients have beyond the forward one.
 template <int KD, bool OUT>
 struct AttendLds {
     static constexpr int kPitch = KD + 4, kValuePitch = kAttendColumns + 4;  // floats; four rows on is sixteen banks on
@@ -25,7 +25,7 @@ struct AttendLds {
 
 __device__ __forceinline__ attend4_t Mfma4(float a, float b, attend4_t c) { return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0); }
 
-template <int KD, bool OUT, bool EVEN, bool GRAD>
+template <int KD, bool OUT, int WIDTHS, bool GRAD>
 __global__ __launch_bounds__(256, KD == 64 ? 3 : 1) void AttendKernel(AttendArgs p) {
     using Lds = AttendLds<KD, OUT>;
     constexpr int VB = kAttendColumns, C = kAttendTile, NS = KD / 16, KP = Lds::kPitch, VP = Lds::kValuePitch, DB = VB / 16;
@@ -102,35 +102,23 @@ __global__ __launch_bounds__(256, KD == 64 ? 3 : 1) void AttendKernel(AttendArgs
     const int64_t g_row = way * p.decay_row;
     const int64_t g_rows = back && span.end == length ? 1 : 0;  // the first row has no decay: none follows it
     AttendPiece<float, 4> k_next[NK], v_next[NV], q_next[OUT ? NS : 1];
-    const auto piece_at = [&](const float* row, int col, int end, int before) {
-        if constexpr (EVEN) return *reinterpret_cast<const AttendPiece<float, 4>*>(row + (col < end ? col : 0));
-        else return AttendLoadBack<float, 4>(row, col, end, before);
-    };
-    const auto moved = [&](const AttendPiece<float, 4>& piece, int col, int end, int before) {
-        attend4_t v;
-        if constexpr (EVEN) {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] = col < end ? piece.v[e] : 0.f;
-        } else {
-            const AttendPiece<float, 4> there = AttendMove<float, 4>(piece, col, end, before);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] = there.v[e];
-        }
-        return v;
+    const auto placed = [&](const AttendPiece<float, 4>& piece, int col, int end) {
+        const AttendPiece<float, 4> there = AttendPlace<WIDTHS>(piece, col, end);
+        return attend4_t{there.v[0], there.v[1], there.v[2], there.v[3]};
     };
     const auto load = [&](int64_t r0) {  // k and v; at the tile's first row
         const int last = static_cast<int>(rows - r0 < C ? rows - r0 : C) - 1;
 #pragma unroll
-        for (int n = 0; n < NK; ++n) k_next[n] = piece_at(kp + min(key_row + n * KR, last) * k_row, key_col, keys, 0);
+        for (int n = 0; n < NK; ++n) k_next[n] = AttendFetch<WIDTHS, 4>(kp + min(key_row + n * KR, last) * k_row, key_col, keys);
 #pragma unroll
-        for (int n = 0; n < NV; ++n) v_next[n] = piece_at(vp + min(value_row + n * 16, last) * v_row, value_col, cols, col0);
+        for (int n = 0; n < NV; ++n) v_next[n] = AttendFetch<WIDTHS, 4>(vp + min(value_row + n * 16, last) * v_row, value_col, cols);
         kp += static_cast<int64_t>(k_row) * C, vp += static_cast<int64_t>(v_row) * C;
     };
     const auto load_q = [&](int64_t r0) {
         if constexpr (OUT) {
             const float* const at = qp + min(own_row(), static_cast<int>(rows - r0 < C ? rows - r0 : C) - 1) * q_row;
 #pragma unroll
-            for (int m = 0; m < NS; ++m) q_next[m] = piece_at(at, 16 * m + lane / 16 * 4, keys, 0);
+            for (int m = 0; m < NS; ++m) q_next[m] = AttendFetch<WIDTHS, 4>(at, 16 * m + lane / 16 * 4, keys);
             qp += static_cast<int64_t>(q_row) * C;
         }
     };
@@ -171,11 +159,11 @@ __global__ __launch_bounds__(256, KD == 64 ? 3 : 1) void AttendKernel(AttendArgs
         const AttendDecays* const dec = decays + turn;
         // (the last tile's rows of k and v have been read by all)
 #pragma unroll
-        for (int n = 0; n < NK; ++n) *reinterpret_cast<attend4_t*>(ks + (key_row + n * KR) * KP + key_col) = moved(k_next[n], key_col, keys, 0);
+        for (int n = 0; n < NK; ++n) *reinterpret_cast<attend4_t*>(ks + (key_row + n * KR) * KP + key_col) = placed(k_next[n], key_col, keys);
         float finite = 0;  // or not a number
 #pragma unroll
         for (int n = 0; n < NV; ++n) {
-            const attend4_t v = moved(v_next[n], value_col, cols, col0);
+            const attend4_t v = placed(v_next[n], value_col, cols);
             *reinterpret_cast<attend4_t*>(vs + (value_row + n * 16) * VP + value_col) = v;
 #pragma unroll
             for (int e = 0; e < 4; ++e) finite = __builtin_fmaf(v[e], 0.f, finite);
@@ -194,7 +182,7 @@ __global__ __launch_bounds__(256, KD == 64 ? 3 : 1) void AttendKernel(AttendArgs
             const float high = dec->high[own_row()], low = dec->low[own_row()];
             attend4_t q[NS];
 #pragma unroll
-            for (int m = 0; m < NS; ++m) q[m] = moved(q_next[m], 16 * m + 4 * quarter, keys, 0);
+            for (int m = 0; m < NS; ++m) q[m] = placed(q_next[m], 16 * m + 4 * quarter, keys);
             attend4_t y[DB]{};
             {
                 const float* const at = ss + lane % 16 * KP + 4 * quarter;
@@ -271,15 +259,13 @@ __global__ __launch_bounds__(256, KD == 64 ? 3 : 1) void AttendKernel(AttendArgs
                 if (!live) continue;
                 if (with_dots) {
                     const float* const row = dp + static_cast<int64_t>(own_row()) * d_row;
-                    AttendPiece<float, 4> with{};
-                    if (!EVEN) with = AttendLoad<float, 4>(row, j, cols);
-                    else if (j < cols) with = *reinterpret_cast<const AttendPiece<float, 4>*>(row + j);
+                    const AttendPiece<float, 4> with = AttendPlace<WIDTHS>(AttendFetch<WIDTHS, 4>(row, j, cols), j, cols);
 #pragma unroll
                     for (int e = 0; e < 4; ++e) dot += j + e < cols ? out.v[e] * with.v[e] : 0.f;
                 }
-                if (EVEN ? j < cols : j + 4 <= cols) {
+                if (WIDTHS == kAttendWhole ? j < cols : j + 4 <= cols) {
                     *reinterpret_cast<AttendPiece<float, 4>*>(to + j) = out;
-                } else if (!EVEN) {
+                } else if (WIDTHS != kAttendWhole) {
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         if (j + e < cols) to[j + e] = out.v[e];
@@ -542,19 +528,16 @@ void LaunchAttend(const AttendArgs& args, int dtype, bool states_alone, hipStrea
     if (blocks == 0) return;
     p.groups = static_cast<int>(groups);
     if (dtype == HIPCX_FLOAT16) return LaunchAttendHalf(p, keys, blocks, states_alone, stream);
-    bool even = true;
-    for (int i = 0; i < p.runs; ++i) even = even && p.run[i].keys % 4 == 0 && p.run[i].values % 4 == 0;
+    const AttendWidths widths = AttendWidthsOf(p, 4);
     VisitKeys(keys, [&](auto kd) {
-        const auto kernel = [&](auto out, auto whole, auto grad) {
+        const auto kernel = [&](auto out, auto rows, auto grad) {
             constexpr int KD = decltype(kd)::value, kLds = AttendLds<KD, decltype(out)::value>::kBytes;
-            void (*const k)(AttendArgs) = AttendKernel<KD, decltype(out)::value, decltype(whole)::value, decltype(grad)::value>;
+            void (*const k)(AttendArgs) = AttendKernel<KD, decltype(out)::value, decltype(rows)::value, decltype(grad)::value>;
             EnsureDynamicLds<AttendTag>(reinterpret_cast<const void*>(k), kLds);
             hipLaunchKernelGGL(k, dim3(static_cast<unsigned>(blocks)), dim3(256), kLds, stream, p);
             CheckLaunch("linear_attention");
         };
-        const auto whole = [&](auto out, auto grad) { even ? kernel(out, std::true_type{}, grad) : kernel(out, std::false_type{}, grad); };
-        if (states_alone) p.runs > 1 ? whole(std::false_type{}, std::true_type{}) : whole(std::false_type{}, std::false_type{});
-        else p.runs > 1 ? whole(std::true_type{}, std::true_type{}) : whole(std::true_type{}, std::false_type{});
+        VisitWidths(widths, p.runs > 1, [&](auto rows, auto grad) { states_alone ? kernel(std::false_type{}, rows, grad) : kernel(std::true_type{}, rows, grad); });
     });
 }
 

@@ -79,10 +79,11 @@ struct AttendHalfLds {
 // bits of anything that counts next to it.
 // A reduction over 32 rows s takes them in the order in which accumulators have them, eight to a lane, for both operands: 4 q + j and 16 + 4 q + j for quarter q of a wave.
 // (32 rows by 32 columns of y to a wave have every block of P computed by two waves; half of the keys by 32 columns of S every product with V.  Vector instructions are what bounds the kernel.)
-// EVEN: rows of whole pieces of eight elements.  GRAD: what the passes of the gradients have beyond the forward one.
-template <int KD, bool OUT, bool EVEN, bool GRAD>
+// GRAD: what the passes of the gradients have beyond the forward one.
+template <int KD, bool OUT, int WIDTHS, bool GRAD>
 __global__ __launch_bounds__(256, KD == 256 ? 1 : 2) void AttendHalfKernel(AttendArgs p) {
     using T = half_t;
+    constexpr bool EVEN = WIDTHS == kAttendWhole;
     using Lds = AttendHalfLds<KD, OUT>;
     constexpr int VB = kAttendColumns, C = kAttendTile, NS = KD / 16, NK = KD / 32, NV = VB / 32, NQ = KD / 32, DB = VB / 16;
     extern __shared__ __align__(16) char lds[];
@@ -201,30 +202,24 @@ __global__ __launch_bounds__(256, KD == 256 ? 1 : 2) void AttendHalfKernel(Atten
     const float* gp = p.decay != nullptr ? p.decay + b * p.decay_batch + h * p.decay_head + (row0 + (back ? 1 : 0)) * p.decay_row : nullptr;
     const int64_t g_row = way * p.decay_row;
     const int64_t g_rows = back && span.end == length ? 1 : 0;  // the first row has no decay: none follows it
-    attend_half8_t k_next[NK], v_next[NV], q[OUT ? NQ : 1];
-    const auto piece_at = [&](const T* row, int col, int end) {
-        AttendPiece<T, 8> piece;
-        if constexpr (EVEN) piece = *reinterpret_cast<const AttendPiece<T, 8>*>(row + (col < end ? col : 0));
-        else piece = AttendLoad<T, 8>(row, col, end);
-        attend_half8_t v;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = piece.v[e];
-        return v;
+    AttendPiece<T, 8> k_next[NK], v_next[NV], q_next[OUT ? NQ : 1];
+    const auto placed = [&](const AttendPiece<T, 8>& piece, int col, int end) {  // (where all pieces are whole, zeros behind the columns stay in LDS and in the state)
+        return __builtin_bit_cast(attend_half8_t, EVEN ? piece : AttendPlace<WIDTHS>(piece, col, end));
     };
     // (Behind the last tile every row is the last one: a branch round the loads would have those of the tile before, too, waited for where the two ways meet.)
     const auto load = [&](int64_t r0) {  // k and v; at the tile's first row
         const int last = static_cast<int>(rows - r0 < C ? rows - r0 : C) - 1;
 #pragma unroll
-        for (int n = 0; n < NK; ++n) k_next[n] = piece_at(kp + min(key_row + n * (2048 / KD), last) * k_row, key_col, keys);
+        for (int n = 0; n < NK; ++n) k_next[n] = AttendFetch<WIDTHS, 8>(kp + min(key_row + n * (2048 / KD), last) * k_row, key_col, keys);
 #pragma unroll
-        for (int n = 0; n < NV; ++n) v_next[n] = piece_at(vp + min(value_row + n * 32, last) * v_row, value_col, cols);
+        for (int n = 0; n < NV; ++n) v_next[n] = AttendFetch<WIDTHS, 8>(vp + min(value_row + n * 32, last) * v_row, value_col, cols);
         kp += static_cast<int64_t>(k_row) * C, vp += static_cast<int64_t>(v_row) * C;
     };
     const auto load_q = [&](int64_t r0) {
         if constexpr (OUT) {
             const T* const at = qp + min(own_row(), static_cast<int>(rows - r0 < C ? rows - r0 : C) - 1) * q_row;
 #pragma unroll
-            for (int m = 0; m < NQ; ++m) q[m] = piece_at(at, 32 * m + lane / 16 * 8, keys);
+            for (int m = 0; m < NQ; ++m) q_next[m] = AttendFetch<WIDTHS, 8>(at, 32 * m + lane / 16 * 8, keys);
             qp += static_cast<int64_t>(q_row) * C;
         }
     };
@@ -271,14 +266,15 @@ __global__ __launch_bounds__(256, KD == 256 ? 1 : 2) void AttendHalfKernel(Atten
         // (the last tile's rows of k and v have been read by all)
 #pragma unroll
         for (int n = 0; n < NK; ++n) {
-            if (!EVEN || key_col < keys) *reinterpret_cast<attend_half8_t*>(ks + (key_row + n * (2048 / KD)) * Lds::kKeyPitch + key_col * 2) = k_next[n];
+            if (!EVEN || key_col < keys) *reinterpret_cast<attend_half8_t*>(ks + (key_row + n * (2048 / KD)) * Lds::kKeyPitch + key_col * 2) = placed(k_next[n], key_col, keys);
         }
         attend_half2_t finite{};  // 0, or not a number
 #pragma unroll
         for (int n = 0; n < NV; ++n) {
-            if (!EVEN || value_col < cols) *reinterpret_cast<attend_half8_t*>(vs + (value_row + n * 32) * Lds::kValuePitch + value_col * 2) = v_next[n];
+            const attend_half8_t v = placed(v_next[n], value_col, cols);
+            if (!EVEN || value_col < cols) *reinterpret_cast<attend_half8_t*>(vs + (value_row + n * 32) * Lds::kValuePitch + value_col * 2) = v;
 #pragma unroll
-            for (int e = 0; e < 8; e += 2) finite = __builtin_elementwise_fma(attend_half2_t{v_next[n][e], v_next[n][e + 1]}, attend_half2_t{}, finite);
+            for (int e = 0; e < 8; e += 2) finite = __builtin_elementwise_fma(attend_half2_t{v[e], v[e + 1]}, attend_half2_t{}, finite);
         }
         if (OUT && !(finite[0] + finite[1] == 0)) odd[turn] = 1;
         __syncthreads();
@@ -293,6 +289,9 @@ __global__ __launch_bounds__(256, KD == 256 ? 1 : 2) void AttendHalfKernel(Atten
             // this wave's sixteen rows by all columns, in blocks of 16 x 16
             const int quarter = lane / 16;
             const float high = dec->high[own_row()], low = dec->low[own_row()];
+            attend_half8_t q[NQ];
+#pragma unroll
+            for (int m = 0; m < NQ; ++m) q[m] = placed(q_next[m], 32 * m + 8 * quarter, keys);
             attend4_t y[DB];
             {
                 attend4_t of_state[DB]{};
@@ -393,10 +392,7 @@ __global__ __launch_bounds__(256, KD == 256 ? 1 : 2) void AttendHalfKernel(Atten
                 for (int e = 0; e < 4; ++e) out.v[e] = __builtin_fmaf(of_rows[d][e], from_rows, y[d][e]);
                 if (!live) continue;
                 if (with_dots) {
-                    AttendPiece<T, 4> with{};
-                    const T* const row = dp + static_cast<int64_t>(own_row()) * d_row;
-                    if (!EVEN) with = AttendLoad<T, 4>(row, j, cols);
-                    else if (j < cols) with = *reinterpret_cast<const AttendPiece<T, 4>*>(row + j);
+                    const AttendPiece<T, 4> with = AttendPlace<WIDTHS>(AttendFetch<WIDTHS, 4>(dp + static_cast<int64_t>(own_row()) * d_row, j, cols), j, cols);
 #pragma unroll
                     for (int e = 0; e < 4; ++e) dot += j + e < cols ? out.v[e] * static_cast<float>(with.v[e]) : 0.f;
                 }
@@ -457,12 +453,13 @@ __global__ __launch_bounds__(256, KD == 256 ? 1 : 2) void AttendHalfKernel(Atten
                 }
             }
             read(0, k[0]);
-            const float all = dec->all, decayed = most * all, added = MaxOver32(MaxOver16(largest)) * Power(-unit);
-            const float size = fmaxf(decayed < HUGE_VALF ? decayed : 0.f, added);
+            // (in exponents: what is added may be further from the unit than a float reaches)
+            const float all = dec->all, decayed = most * all, added = MaxOver32(MaxOver16(largest));
+            const int size = max(decayed < HUGE_VALF ? ExponentOf(decayed) : -127, added > 0 ? ExponentOf(added) - unit : -127);
             int up = 0;
-            if (size >= 0x1p15f || (size < 0x1p4f && size > 0)) up = min(max(ExponentOf(size) - 13, -112 - unit), 114 - unit);
+            if (size >= 15 || (size < 4 && size > -127)) up = min(max(max(size - 13, -112 - unit), -112), 114 - unit);
             unit += up;
-            const float keep = all * Power(-up), in = Power(-unit);
+            const float keep = all * Power(max(-up, -126)), in = Power(-unit);
 #pragma unroll
             for (int n = 0; n < NS; ++n) s[n] *= keep;
             attend_half8_t hi, lo;
@@ -593,19 +590,16 @@ __global__ __launch_bounds__(256, KD == 256 ? 1 : 2) void AttendHalfKernel(Atten
 }  // namespace
 
 void LaunchAttendHalf(const AttendArgs& p, int keys, int64_t blocks, bool states_alone, hipStream_t stream) {
-    bool even = true;
-    for (int i = 0; i < p.runs; ++i) even = even && p.run[i].keys % 8 == 0 && p.run[i].values % 8 == 0;
+    const AttendWidths widths = AttendWidthsOf(p, 8);
     const auto launch = [&](auto kd) {
-        const auto kernel = [&](auto out, auto whole, auto grad) {
+        const auto kernel = [&](auto out, auto rows, auto grad) {
             constexpr int KD = decltype(kd)::value, kLds = AttendHalfLds<KD, decltype(out)::value>::kBytes;
-            void (*const k)(AttendArgs) = AttendHalfKernel<KD, decltype(out)::value, decltype(whole)::value, decltype(grad)::value>;
+            void (*const k)(AttendArgs) = AttendHalfKernel<KD, decltype(out)::value, decltype(rows)::value, decltype(grad)::value>;
             EnsureDynamicLds<AttendHalfTag>(reinterpret_cast<const void*>(k), kLds);
             hipLaunchKernelGGL(k, dim3(static_cast<unsigned>(blocks)), dim3(256), kLds, stream, p);
             CheckLaunch("linear_attention");
         };
-        const auto whole = [&](auto out, auto grad) { even ? kernel(out, std::true_type{}, grad) : kernel(out, std::false_type{}, grad); };
-        if (states_alone) p.runs > 1 ? whole(std::false_type{}, std::true_type{}) : whole(std::false_type{}, std::false_type{});
-        else p.runs > 1 ? whole(std::true_type{}, std::true_type{}) : whole(std::true_type{}, std::false_type{});
+        VisitWidths(widths, p.runs > 1, [&](auto rows, auto grad) { states_alone ? kernel(std::false_type{}, rows, grad) : kernel(std::true_type{}, rows, grad); });
     };
     if (keys <= 64) launch(std::integral_constant<int, 64>{});
     else if (keys <= 128) launch(std::integral_constant<int, 128>{});

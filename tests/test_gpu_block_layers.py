@@ -264,6 +264,40 @@ def test_linear_attention_starts_anew_where_nothing_is_kept(chx, length, dtype):
             ref.assert_off(got.get(), wants[name], offs[name], name)
 
 
+@pytest.mark.parametrize('dtype', ['float16', 'float32'])
+@pytest.mark.parametrize('keys,values', [(24, 40), (6, 90), (130, 33)])
+def test_linear_attention_of_the_largest_and_smallest_numbers(chx, keys, values, dtype):
+    """A state that all but vanishes and comes back, one that starts near the type's end, growing and fading by sixteens of powers of two, a scale that takes products far away."""
+    c = attend_case((4, 260, 1, 1, keys, values), dtype)
+    c['log_decay'][:] = -0.01
+    c['state'][0] *= 1e-30
+    c['log_decay'][0, :130] = -0.5                   # 2^-94 of it is left ...
+    c['v'][0, :200] = 0
+    c['v'][0, 200:] *= 8000                          # ... when rows of 2^13 come
+    c['state'][1] *= 1e30
+    c['log_decay'][1, :] = -0.7
+    c['v'][2] *= np.exp2(np.arange(260) // 64 * 6.0 - 12).astype(dtype)[:, None, None]
+    c['log_decay'][2, :] = 0.02                      # (grows)
+    c['k'][3] *= np.exp2(-(np.arange(260) // 64) * 3.0).astype(dtype)[:, None, None]
+    c['log_decay'][3, 128] = -80
+    for scale in (None, 2.0 ** -20, 2.0 ** 12):
+        with np.errstate(over='ignore'):
+            check_attend_outputs(chx, c, scale)
+
+
+def check_attend_outputs(chx, c, scale):
+    more = dict(log_decay=up(chx, c['log_decay']), scale=scale, state=up(chx, c['state']))
+    y, new = chx.linear_attention(*(up(chx, c[k]) for k in ('q', 'k', 'v')), **more)
+    (want, want_new), (off, off_new) = ref.linear_attention(c['q'], c['k'], c['v'], c['log_decay'], scale, c['state'])
+    grads = chx.linear_attention_grad(*(up(chx, c[k]) for k in ('q', 'k', 'v', 'gy')), gnew_state=up(chx, c['gnew']), **more)
+    wants, offs, _ = ref.linear_attention_grad(c['q'], c['k'], c['v'], c['gy'], c['log_decay'], scale, c['state'], None, c['gnew'])
+    for b in range(y.shape[0]):  # (each has its own numbers, and limits that follow from them)
+        ref.assert_off(y.get()[b], want[b], off[b], 'y of %d' % b)
+        ref.assert_off(new.get()[b], want_new[b], off_new[b], 'state of %d' % b)
+        for name, got in grads._asdict().items():
+            ref.assert_off(got.get()[b], wants[name][b], offs[name][b], 'g%s of %d' % (name, b))
+
+
 def test_linear_attention_of_nothing(chx):
     state = np.random.default_rng(0).standard_normal((2, 3, 4, 5)).astype(np.float32)
     z = lambda *s: chx.zeros(s, 'float32')  # noqa: E731
