@@ -209,17 +209,22 @@ __global__ __launch_bounds__(256, KD == 64 ? 3 : 1) void AttendKernel(AttendArgs
             attend4_t a[4]{};
             {
                 const float* const at = ks + lane % 16 * KP + 4 * quarter;
+                attend4_t part[2][4];
+                const auto read = [&](int m, attend4_t (&to)[4]) {
+#pragma unroll
+                    for (int sb = 0; sb < 4; ++sb) to[sb] = *reinterpret_cast<const attend4_t*>(at + 16 * min(sb, wave) * KP + 16 * m);
+                };
+                read(0, part[0]);
 #pragma unroll
                 for (int m = 0; m < NS; ++m) {
-                    attend4_t part[4];
-#pragma unroll
-                    for (int sb = 0; sb < 4; ++sb) part[sb] = *reinterpret_cast<const attend4_t*>(at + 16 * min(sb, wave) * KP + 16 * m);
+                    if (m + 1 < NS) read(m + 1, part[m % 2 ^ 1]);
 #pragma unroll
                     for (int sb = 0; sb < 4; ++sb) {
                         if (sb > wave) continue;
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) a[sb] = Mfma4(part[sb][e], q[m][e], a[sb]);
+                        for (int e = 0; e < 4; ++e) a[sb] = Mfma4(part[m % 2][sb][e], q[m][e], a[sb]);
                     }
+                    __builtin_amdgcn_sched_barrier(0);
                 }
             }
             load_q(r0 + C);
@@ -625,9 +630,9 @@ namespace {
 // Up to so many rows go one after another.
 constexpr int kAttendTokens = 8;
 
-void CutForward(AttendCall* c) {
+void CutForward(AttendCall* c, bool padded) {
     if (c->p.length <= kAttendTokens) c->p.segments = 1, c->p.segment_rows = kAttendTile;
-    else CutAttend(&c->p, AttendBlocks(c->values), AttendBlocks(c->values), AttendResident(c->dtype, c->keys), static_cast<int64_t>(c->keys) * c->values);
+    else CutAttend(&c->p, padded, AttendBlocks(c->values), AttendBlocks(c->values), AttendResident(c->dtype, c->keys), static_cast<int64_t>(c->keys) * c->values);
 }
 
 size_t ForwardWorkspace(const AttendCall& c) {
@@ -645,8 +650,12 @@ extern "C" {
 size_t hipcx_linear_attention_workspace_size(const hipcx_array* q, const hipcx_array* v) {
     AttendCall c;
     if (!AttendSizesOf(q, v, &c)) return 0;
-    CutForward(&c);
-    return ForwardWorkspace(c);
+    size_t bytes = 0;
+    for (const bool padded : {false, true}) {
+        CutForward(&c, padded);
+        bytes = std::max(bytes, ForwardWorkspace(c));
+    }
+    return bytes;
 }
 
 int hipcx_linear_attention(const hipcx_array* q, const hipcx_array* k, const hipcx_array* v, const hipcx_array* log_decay, double scale, const hipcx_array* state,
@@ -660,7 +669,7 @@ int hipcx_linear_attention(const hipcx_array* q, const hipcx_array* k, const hip
         RequireShape(new_state, {p.batch, p.heads, c.keys, c.values}, HIPCX_FLOAT32, what + ": new_state");
         RequireDense(new_state, what + ": new_state");
         if (p.batch == 0) return;
-        CutForward(&c);
+        CutForward(&c, lengths != nullptr);
         HIPCX_REQUIRE(workspace_bytes >= ForwardWorkspace(c) && (ForwardWorkspace(c) == 0 || workspace != nullptr), HIPCX_CHAINERX_ERROR, what + ": the workspace is too small");
         AttendRun& run = p.run[0];
         run.q = c.q, run.k = c.k, run.v = c.v, run.y = to;

@@ -110,9 +110,9 @@ struct GradWorkspace {
     }
 };
 
-void CutGrad(AttendCall* c) {
+void CutGrad(AttendCall* c, bool padded) {
     const int64_t keys = AttendBlocks(c->keys), values = AttendBlocks(c->values);
-    CutAttend(&c->p, 2 * keys + values, keys + values, AttendResident(c->dtype, std::max(c->keys, c->values)), 2 * static_cast<int64_t>(c->keys) * c->values);
+    CutAttend(&c->p, padded, 2 * keys + values, keys + values, AttendResident(c->dtype, std::max(c->keys, c->values)), 2 * static_cast<int64_t>(c->keys) * c->values);
 }
 
 }  // namespace
@@ -125,8 +125,12 @@ extern "C" {
 size_t hipcx_linear_attention_grad_workspace_size(const hipcx_array* q, const hipcx_array* v, const hipcx_array* log_decay) {
     AttendCall c;
     if (!AttendSizesOf(q, v, &c)) return 0;
-    CutGrad(&c);
-    return GradWorkspace(c, log_decay != nullptr, log_decay != nullptr && log_decay->ndim == 1).bytes;
+    size_t bytes = 0;
+    for (const bool padded : {false, true}) {
+        CutGrad(&c, padded);
+        bytes = std::max(bytes, GradWorkspace(c, log_decay != nullptr, log_decay != nullptr && log_decay->ndim == 1).bytes);
+    }
+    return bytes;
 }
 
 int hipcx_linear_attention_grad(const hipcx_array* q, const hipcx_array* k, const hipcx_array* v, const hipcx_array* log_decay, double scale, const hipcx_array* state,
@@ -151,7 +155,7 @@ int hipcx_linear_attention_grad(const hipcx_array* q, const hipcx_array* k, cons
             else RequireShape(glog_decay, {p.batch, p.length, p.heads}, HIPCX_FLOAT32, what + ": glog_decay");
             RequireDense(glog_decay, what + ": glog_decay");
         }
-        CutGrad(&c);
+        CutGrad(&c, lengths != nullptr);
         const bool of_heads = glog_decay != nullptr && glog_decay->ndim == 1;
         const GradWorkspace w(c, log_decay != nullptr, log_decay != nullptr && log_decay->ndim == 1);
         HIPCX_REQUIRE(workspace_bytes >= w.bytes && (w.bytes == 0 || workspace != nullptr), HIPCX_CHAINERX_ERROR, what + ": the workspace is too small");
