@@ -60,36 +60,35 @@ struct __attribute__((packed, aligned(alignof(T)))) Run {
 
 __device__ __forceinline__ float PowerOfTwo(int e) { return __builtin_bit_cast(float, (e + 127) << 23); }
 
-// What a code stands for, as a part of the scale; EXPONENTS powers of two.
+// What a code stands for, as a part of the scale; EXPONENTS powers of two.  Its bits are a float's: of the lowest eighths, which have no power, those of the next ones less their power.
 template <int EXPONENTS>
 __device__ __forceinline__ float PartOf(int code) {
-    const int e = code >> 3, f = code & 7;
-    return e > 0 ? static_cast<float>(8 + f) * PowerOfTwo(e - EXPONENTS - 2) : static_cast<float>(f) * PowerOfTwo(-EXPONENTS - 1);
+    const bool low = code < 8;
+    return __builtin_bit_cast(float, ((low ? code + 8 : code) << 20) + ((128 - EXPONENTS) << 23)) - (low ? PowerOfTwo(2 - EXPONENTS) : 0.f);
 }
 
-// A part of the scale, not negative, as a code; `up` in (0, 1) of a step.
+// A part of the scale, not negative, as a code: `random` of 16 bits and a half, as a part of a step, is added and what is beyond the code's bits cut off.
 template <int EXPONENTS>
-__device__ __forceinline__ int CodeOf(float part, float up) {
-    const int power = max((__builtin_bit_cast(int, part) >> 23) - 127 + EXPONENTS - 1, 1);
-    const int steps = static_cast<int>(floorf(part * PowerOfTwo(EXPONENTS + 2 - power) + up));
-    return min(8 * power + steps - 8, 8 * EXPONENTS - 1);
+__device__ __forceinline__ int CodeOf(float part, uint32_t random) {
+    int code = static_cast<int>((__builtin_bit_cast(uint32_t, part) + (random << 4) + 8) >> 20) - ((128 - EXPONENTS) << 3);
+    if (part < PowerOfTwo(2 - EXPONENTS)) code = static_cast<int>(__builtin_fmaf(part, PowerOfTwo(EXPONENTS + 1), (static_cast<float>(random) + 0.5f) * 0x1p-16f));
+    return min(code, 8 * EXPONENTS - 1);
 }
 
-// The power of two that `top` does not exceed, within 2^-100 and 2^100; not a number where top is not finite or larger.
-__device__ __forceinline__ float ScaleOf(float top) {
-    const int bits = __builtin_bit_cast(int, top);
-    const int e = (bits >> 23) - 127 + ((bits & 0x7fffff) != 0 ? 1 : 0);
-    return top <= 0x1p100f ? PowerOfTwo(max(e, -100)) : __builtin_nanf("");
+// The power of two that `top`, in a float's bits, does not exceed, within 2^-100 and 2^100; not a number where top is not finite or larger.
+__device__ __forceinline__ float ScaleOf(uint32_t top) {
+    const int e = static_cast<int>((top + 0x7fffff) >> 23) - 127;
+    return top <= __builtin_bit_cast(uint32_t, 0x1p100f) ? PowerOfTwo(max(e, -100)) : __builtin_nanf("");
 }
 
-// The largest of 32 neighbours' values; not a number where one is.
-__device__ __forceinline__ float TopOf32(float v) {
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const float w = __shfl_xor(v, o);
-        v = w > v || w != w ? w : v;
-    }
-    return v;
+template <int MOVE>
+__device__ __forceinline__ uint32_t MaxMoved(uint32_t v) {
+    return max(v, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), MOVE, 0xf, 0xf, false)));
+}
+// The largest of 32 neighbours' values, which are not negative, by their bits: those of what is not a number are larger than all others.  Rotations among sixteen lanes, and the sixteen beside them.
+__device__ __forceinline__ uint32_t TopOf32(uint32_t v) {
+    v = MaxMoved<0x121>(MaxMoved<0x122>(MaxMoved<0x124>(MaxMoved<0x128>(v))));
+    return max(v, static_cast<uint32_t>(__shfl_xor(static_cast<int>(v), 16)));
 }
 
 // A pass over memory.  A thread takes eight neighbours, 32 threads a block of states in 8 bits.
@@ -134,7 +133,8 @@ __global__ __launch_bounds__(256) void AdamWKernel(AdamWArgs a) {
         t = *a.t_array;
         step = StepSize(a.alpha, a.beta1, a.beta2, t);
     }
-    float new_m[E], root[E], new_v[E], new_w[E], m_top = 0, root_top = 0;
+    float new_m[E], root[E], new_v[E], new_w[E];
+    uint32_t m_top = 0, root_top = 0;
 #pragma unroll
     for (int e = 0; e < E; ++e) {
         float old_m, old_v;
@@ -152,9 +152,8 @@ __global__ __launch_bounds__(256) void AdamWKernel(AdamWArgs a) {
         root[e] = sqrtf(new_v[e]);
         new_w[e] = weight - (step * (new_m[e] / (root[e] + a.eps)) + a.decay * weight);
         if constexpr (EIGHT) {
-            const float size_m = fabsf(new_m[e]);
-            m_top = size_m > m_top || size_m != size_m ? size_m : m_top;
-            root_top = root[e] > root_top || root[e] != root[e] ? root[e] : root_top;
+            m_top = max(m_top, __builtin_bit_cast(uint32_t, fabsf(new_m[e])));
+            root_top = max(root_top, __builtin_bit_cast(uint32_t, root[e]));
         }
     }
     if constexpr (EIGHT) {
@@ -168,10 +167,9 @@ __global__ __launch_bounds__(256) void AdamWKernel(AdamWArgs a) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const int e = c * 4 + i;
-                const float m_up = (static_cast<float>(word[i] & 0xffff) + 0.5f) * 0x1p-16f, v_up = (static_cast<float>(word[i] >> 16) + 0.5f) * 0x1p-16f;
-                const int code = CodeOf<16>(fabsf(new_m[e]) * m_part, m_up);
+                const int code = CodeOf<16>(fabsf(new_m[e]) * m_part, word[i] & 0xffff);
                 mv.v[e] = static_cast<S>(code | (__builtin_bit_cast(uint32_t, new_m[e]) >> 31 << 7));
-                const int root_code = CodeOf<32>(root[e] * v_part, v_up);
+                const int root_code = CodeOf<32>(root[e] * v_part, word[i] >> 16);
                 vv.v[e] = static_cast<S>(root[e] > 0 ? max(root_code, 1) : root_code);
             }
         }
