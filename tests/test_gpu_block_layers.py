@@ -61,6 +61,21 @@ def test_layer_norm(chx, rows, cols, dtype, params):
                 assert got.dtype == (x.dtype if name == 'gx' else np.dtype(params))
 
 
+@pytest.mark.parametrize('rows,cols,dtype', [(132000, 3, 'float16'), (132001, 40, 'float32'), (33003, 300, 'float16'), (33001, 250, 'float32'), (17001, 600, 'float16'), (4101, 2500, 'float16'),
+                                             (4097, 1700, 'float32'), (2050, 5000, 'float16')])
+def test_layer_norm_of_many_rows(chx, rows, cols, dtype):
+    """So many that a thread takes several at once, the last ones not all there."""
+    x, gamma, beta, gy = norm_case(rows, cols, dtype, 'float32')
+    y, state = chx.layer_norm(up(chx, x), up(chx, gamma), up(chx, beta))
+    want, off = ref.layer_norm(x, gamma, beta, 2e-5)
+    for name, got in (('y', y), ('mean', state.mean), ('inv_std', state.inv_std)):
+        ref.assert_off(got.get(), want[name], off[name], name)
+    grads = chx.layer_norm_grad(up(chx, x), up(chx, gamma), up(chx, gy), state)
+    want, off = ref.layer_norm_grad(x, gamma, gy, 2e-5)
+    for name, got in zip(('gx', 'ggamma', 'gbeta'), grads):
+        ref.assert_off(got.get(), want[name].reshape(got.shape), off[name].reshape(got.shape), name)
+
+
 def test_layer_norm_of_many_axes_and_of_none(chx):
     x, gamma, beta, gy = norm_case(24, 40, 'float32', 'float32')
     want, state = chx.layer_norm(up(chx, x), up(chx, gamma), up(chx, beta))
