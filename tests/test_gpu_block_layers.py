@@ -482,3 +482,239 @@ def test_adamw_refuses_what_would_be_written_twice(chx):
         chx.adamw_update([p], [g, g], [s], 1)
     with pytest.raises(chx.ChainerxError):
         chx.adamw_update([p], [g], [s], 0)
+
+
+# ---------------------------------------------------------------------------------------------
+# long sequences in segments, addresses far apart
+# ---------------------------------------------------------------------------------------------
+@pytest.mark.parametrize('dtype', ['float16', 'float32'])
+@pytest.mark.parametrize('sizes', [(1, 2100, 2, 2, 256, 70), (2, 1500, 4, 4, 100, 130), (3, 900, 2, 1, 50, 50), (1, 1281, 1, 1, 5, 6)])
+def test_linear_attention_of_long_sequences(chx, sizes, dtype):
+    """Time in segments: with states and without, heads that share keys, sequences that end in the first segment, the last, and before any; the state moved forward in place."""
+    for i, (decay, ragged, state, gnew) in enumerate((('heads', False, True, True), ('rows', True, True, False), (None, True, False, True))):
+        c = attend_case(sizes, dtype, seed=i, ragged=ragged, decay=decay)
+        if decay is None:  # (all that there is stays: values that keep the sums in float16's range)
+            c['v'] = c['v'] * np.asarray(0.1, dtype)
+        check_attend(chx, c, lambda a: up(chx, a), None, state, gnew, '%s %s %d' % (sizes, dtype, i))
+    state = up(chx, c['state'])
+    y, new = chx.linear_attention(*(up(chx, c[k]) for k in ('q', 'k', 'v')), state=up(chx, c['state']), lengths=up(chx, c['lengths']))
+    y2, same = chx.linear_attention(*(up(chx, c[k]) for k in ('q', 'k', 'v')), state=state, lengths=up(chx, c['lengths']), out_state=state)
+    assert same is state and np.array_equal(y.get(), y2.get()) and np.array_equal(state.get(), new.get())
+
+
+@pytest.mark.parametrize('dtype', ['float16', 'float32'])
+@pytest.mark.parametrize('length', [4, 90])
+def test_linear_attention_of_sequences_far_apart(chx, length, dtype):
+    """Sequences and rows whose distance in memory takes more than 31 bits, results among them; at 2^24 elements from row to row the call is refused."""
+    c = attend_case((2, length, 2, 1, 16, 24), dtype)
+    dev = {k: up(chx, c[k]) for k in ('q', 'k', 'v', 'gy')}
+    more = dict(log_decay=up(chx, c['log_decay']), state=up(chx, c['state']))
+    want, want_new = chx.linear_attention(dev['q'], dev['k'], dev['v'], **more)
+    grads = chx.linear_attention_grad(dev['q'], dev['k'], dev['v'], dev['gy'], **more)
+    item = np.dtype(dtype).itemsize
+    batch, row = 1 << 33, ((1 << 24) - 3) * item
+    buffer = chx._array.alloc_bytes(batch + length * row + (1 << 16))
+    far = {}
+    for i, k in enumerate(('q', 'k', 'v', 'gy')):
+        far[k] = chx.ndarray(buffer, 8192 * i, c[k].shape, (batch, row, c[k].shape[3] * item + 256, item), np.dtype(dtype))
+        chx.routines._copy_into(far[k], dev[k])
+    y, new = chx.linear_attention(far['q'], far['k'], far['v'], **more)
+    assert np.array_equal(y.get(), want.get()) and np.array_equal(new.get(), want_new.get())
+    for got, w in zip(chx.linear_attention_grad(far['q'], far['k'], far['v'], far['gy'], **more), grads):
+        assert np.array_equal(got.get(), w.get())
+    beyond = chx.ndarray(buffer, 0, c['q'].shape, (batch, item << 24, 512, item), np.dtype(dtype))
+    with pytest.raises(chx.ChainerxNotImplementedError):
+        chx.linear_attention(beyond, far['k'], far['v'])
+
+
+@pytest.mark.parametrize('dtype', ['float16', 'float32'])
+@pytest.mark.parametrize('length', [3, 100])
+def test_linear_attention_of_strides_that_repeat_and_run_backwards(chx, length, dtype):
+    """Inputs broadcast over the batch and read backwards in time, and a single row of any stride."""
+    c = attend_case((3, length, 2, 1, 18, 20), dtype)
+    dev = {k: up(chx, c[k]) for k in ('q', 'k', 'v', 'gy')}
+    for k in ('q', 'k', 'v'):
+        c[k] = np.ascontiguousarray(np.broadcast_to(c[k][:1, ::-1], c[k].shape))
+        dev[k] = dev[k][:1, ::-1].broadcast_to(c[k].shape)
+    dense = [up(chx, c[k]) for k in ('q', 'k', 'v')]
+    views = [dev[k] for k in ('q', 'k', 'v')]
+    for got, want in zip(chx.linear_attention(*views), chx.linear_attention(*dense)):
+        assert np.array_equal(got.get(), want.get())
+    for got, want in zip(chx.linear_attention_grad(*views, dev['gy'])[:3], chx.linear_attention_grad(*dense, dev['gy'])[:3]):
+        assert np.array_equal(got.get(), want.get())
+    q, k, v = (a[:, :1] for a in dense)
+    want = chx.linear_attention(up(chx, q.get()), up(chx, k.get()), up(chx, v.get()))
+    for far in (1 << 40, -(1 << 40), 0):
+        odd = [chx.ndarray(a._buf, a._offset, a.shape, (a.strides[0], far) + a.strides[2:], a.dtype) for a in (q, k, v)]
+        for got, w in zip(chx.linear_attention(*odd), want):
+            assert np.array_equal(got.get(), w.get())
+
+
+# ---------------------------------------------------------------------------------------------
+# the layers together, graphs, streams, threads
+# ---------------------------------------------------------------------------------------------
+NAMES = ('gamma', 'beta', 'in_w', 'out_w')
+
+
+def block_case(rng, units, heads, width, dtype='float32'):
+    n = lambda *s: (rng.standard_normal(s) / np.sqrt(s[-1])).astype(np.float32)  # noqa: E731
+    return {'gamma': 1 + 0.1 * n(units) * units ** 0.5, 'beta': n(units), 'in_w': n(3 * heads * width, units), 'out_w': n(units, heads * width)}
+
+
+def block(chx, p, x, decay, state=None, lengths=None):
+    """layer norm -> linear -> linear attention -> linear, added to what went in; (the result, the state, what the gradients need)."""
+    batch, length, units = x.shape
+    heads, width = decay.shape[-1], p['out_w'].shape[1] // decay.shape[-1]
+    n, stats = chx.layer_norm(x, p['gamma'], p['beta'])
+    rows = n.reshape(batch * length, units)
+    wide = chx.linear(rows, p['in_w']).reshape(batch, length, 3, heads, width)
+    qkv = [wide[:, :, i] for i in range(3)]
+    y, new = chx.linear_attention(*qkv, decay, state=state, lengths=lengths)
+    out = chx.add(chx.linear(y.reshape(batch * length, heads * width), p['out_w']).reshape(x.shape), x)
+    return out, new, (stats, rows, qkv, y)
+
+
+def block_grad(chx, p, x, decay, kept, gout, state=None, lengths=None, gnew=None):
+    """The gradients of the parameters, by name, and those of x and the state."""
+    batch, length, units = x.shape
+    stats, rows, qkv, y = kept
+    g = gout.reshape(batch * length, units)
+    flat = y.reshape(batch * length, -1)
+    grads = {'out_w': chx.dot(g.T, flat)}
+    a = chx.linear_attention_grad(*qkv, chx.dot(g, p['out_w']).reshape(y.shape), decay, state=state, lengths=lengths, gnew_state=gnew)
+    gwide = chx.concatenate([v.reshape(batch * length, -1) for v in (a.q, a.k, a.v)], 1)
+    grads['in_w'] = chx.dot(gwide.T, rows)
+    gx, grads['gamma'], grads['beta'] = chx.layer_norm_grad(x, p['gamma'], chx.dot(gwide, p['in_w']).reshape(x.shape), stats)
+    return grads, chx.add(gx, gout), a.state
+
+
+def plain_block(p, x, decay, state, lengths):
+    heads, width = decay.shape[-1], p['out_w'].shape[1] // decay.shape[-1]
+    n = ref.layer_norm(x, p['gamma'], p['beta'], 2e-5)[0]['y']
+    wide = (n @ p['in_w'].T).reshape(x.shape[:2] + (3, heads, width))
+    (y, new), _ = ref.linear_attention(wide[:, :, 0], wide[:, :, 1], wide[:, :, 2], decay, None, state, lengths)
+    return y.reshape(x.shape[:2] + (-1,)) @ p['out_w'].T + x, new
+
+
+def test_a_block_is_trained_as_its_formulas_say(chx):
+    """Its gradients against differences of the plain forms in 64 bits along random directions, and the step that AdamW takes with them bit by bit."""
+    rng = np.random.default_rng(5)
+    host, x = block_case(rng, 20, 2, 9), rng.standard_normal((3, 70, 20)).astype(np.float32)
+    decay, state, lengths = -np.exp(rng.standard_normal((3, 70, 2)) - 2).astype(np.float32), rng.standard_normal((3, 2, 9, 9)).astype(np.float32), np.array([70, 0, 41])
+    gout, gnew = rng.standard_normal(x.shape).astype(np.float32), rng.standard_normal(state.shape).astype(np.float32)
+    p, dx, dd, ds, dl = {k: up(chx, v) for k, v in host.items()}, up(chx, x), up(chx, decay), up(chx, state), up(chx, lengths)
+    _, _, kept = block(chx, p, dx, dd, ds, dl)
+    grads, gx, gstate = block_grad(chx, p, dx, dd, kept, up(chx, gout), ds, dl, up(chx, gnew))
+
+    def loss(**over):
+        v = {k: over.get(k, a).astype(np.float64) for k, a in dict(host, x=x, state=state).items()}
+        out, new = plain_block(v, v['x'], decay.astype(np.float64), v['state'], lengths)
+        return (out * gout).sum() + (new * gnew).sum()
+
+    for name, base, got in [(k, host[k], grads[k]) for k in NAMES] + [('x', x, gx), ('state', state, gstate)]:
+        along, base, step, got = rng.standard_normal(base.shape), base.astype(np.float64), 1e-4, got.get().astype(np.float64)
+        change = (loss(**{name: base + step * along}) - loss(**{name: base - step * along})) / (2 * step)
+        # differences are exact to step^2; a float32 gradient's elements to some 1e-6 of their size
+        assert abs((got * along).sum() - change) <= 1e-4 * (np.abs(got * along).sum() + 1), name
+    states = [chx.adamw_state(p[k], bits=8 if k.endswith('w') else 32) for k in NAMES]
+    want = []
+    for i, k in enumerate(NAMES):
+        s = states[i]
+        want.append(ref.adamw(host[k].reshape(-1), grads[k].get().reshape(-1), *[None if a is None else a.get().reshape(-1) for a in (s.m, s.v, s.m_scale, s.v_scale)], None, i, 1, 0.01, 0.9, 0.999,
+                              1e-8, 1.0, 0.1, 3))
+    chx.adamw_update([p[k] for k in NAMES], [grads[k] for k in NAMES], states, 1, alpha=0.01, weight_decay_rate=0.1, seed=3)
+    for k, s, w in zip(NAMES, states, want):
+        for got, expected in zip((p[k], s.m, s.v, s.m_scale, s.v_scale), w):
+            assert (got is None) == (expected is None) and (got is None or np.array_equal(got.get().reshape(-1), expected)), k
+
+
+@pytest.mark.parametrize('length', [30, 400])
+def test_a_block_answers_a_prompt_and_then_token_by_token(chx, length):
+    """As a server runs it, a state for each layer, moved forward in place: what the whole sequences give."""
+    rng = np.random.default_rng(6)
+    layers = [{k: up(chx, v) for k, v in block_case(rng, 24, 3, 8).items()} for _ in range(2)]
+    x = rng.standard_normal((3, length, 24)).astype(np.float32)
+    decay = up(chx, np.log1p(-np.exp2(-3.0 - np.arange(3))).astype(np.float32))
+
+    def run(x, states):
+        h = up(chx, x)
+        for i, p in enumerate(layers):
+            h, new, _ = block(chx, p, h, decay, states[i])
+            states[i] = new
+        return h.get()
+
+    want, states = run(x, [None, None]), [None, None]
+    cuts = [0, length - 12, length - 11, length - 10, length - 4, length]
+    got = [run(x[:, a:b], states) for a, b in zip(cuts, cuts[1:])]
+    # sums of some tens of terms in other orders, through two layers that divide by a deviation of order 1: far from any mistake in a row or a state
+    np.testing.assert_allclose(np.concatenate(got, 1), want, rtol=0, atol=1e-4)
+
+
+def test_a_step_replays_in_a_graph(chx):
+    """The block's forward pass, gradients and AdamW's step in a captured graph, replayed between eager steps from the same weights: each replay is the next step."""
+    from chainer_amd import graph
+    rng = np.random.default_rng(9)
+    host, x = block_case(rng, 24, 2, 16), up(chx, rng.standard_normal((2, 700, 24)).astype(np.float32))
+    decay, lengths, gout = up(chx, -np.exp(rng.standard_normal((2, 700, 2)) - 2).astype(np.float32)), up(chx, np.array([700, 333])), up(chx, rng.standard_normal((2, 700, 24)).astype(np.float32))
+    make = lambda: ({k: up(chx, v) for k, v in host.items()}, up(chx, np.array([1], np.int64)))  # noqa: E731
+    (p, t), (q, u) = make(), make()
+    s, r = ([chx.adamw_state(w[k], bits=b) for k, b in zip(NAMES, (32, 32, 8, 8))] for w in (p, q))
+
+    def step(p, s, t):
+        out, new, kept = block(chx, p, x, decay, None, lengths)
+        grads, gx, _ = block_grad(chx, p, x, decay, kept, gout, None, lengths)
+        chx.adamw_update([p[k] for k in NAMES], [grads[k] for k in NAMES], s, t, alpha=0.01, weight_decay_rate=0.1, seed=3)
+        return out, new, gx
+
+    everything = lambda p, s, t: [p[k] for k in NAMES] + [a for state in s for a in state if a is not None] + [t]  # noqa: E731
+    captured = graph.capture(lambda: step(p, s, t))
+    for _ in range(4):
+        for a, b in zip(everything(q, r, u), everything(p, s, t)):  # (the passes before the capture were steps, too)
+            chx.routines._copy_into(a, b)
+        want = [a.get() for a in step(q, r, u)]
+        captured.replay()
+        chx.synchronize()
+        for a, w in zip(captured.result, want):
+            assert np.array_equal(a.get(), w)
+        for a, b in zip(everything(p, s, t), everything(q, r, u)):
+            assert np.array_equal(a.get(), b.get())
+        chx.add(t, chx.array(np.array([1], np.int64)), out=t)  # the next step
+    captured.release()
+
+
+def test_layers_on_two_streams_and_threads_at_once(chx):
+    """Calls at the same time have workspaces of their own, on whatever stream is current where they are made."""
+    import threading
+
+    import torch
+    c = attend_case((2, 1500, 2, 1, 50, 50), 'float16', ragged=True)
+    args = [up(chx, c[k]) for k in ('q', 'k', 'v')]
+    more = dict(log_decay=up(chx, c['log_decay']), lengths=up(chx, c['lengths']))
+    x, gamma, beta, gy = (up(chx, a) for a in norm_case(900, 650, 'float32', 'float32'))
+
+    def everything():
+        y, stats = chx.layer_norm(x, gamma, beta)
+        p = chx.array(np.linspace(-1, 1, 5000, dtype=np.float32))
+        s = chx.adamw_state(p, bits=8)
+        chx.adamw_update([p], [chx.ones((5000,))], [s], 1)
+        return [y] + list(chx.layer_norm_grad(x, gamma, gy, stats)) + list(chx.linear_attention(*args, **more)) + list(chx.linear_attention_grad(*args, up(chx, c['gy']), **more))[:4] + [p, s.v]
+
+    want = [a.get() for a in everything()]
+    chx.synchronize()
+    streams, results = [torch.cuda.Stream() for _ in range(3)], {}
+
+    def work(i):
+        with torch.cuda.stream(streams[i]):
+            results[i] = [everything() for _ in range(3)]
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(3)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for s in streams:
+        s.synchronize()
+    for i in range(3):
+        for r in results[i]:
+            for a, w in zip(r, want):
+                assert np.array_equal(a.get(), w)
