@@ -407,6 +407,7 @@ __global__ __launch_bounds__(256, KD == 64 ? 3 : 1) void AttendKernel(AttendArgs
     }
 }
 
+// An element of a state to a thread.  Bound by memory and its latency, once the segments' loads go out together.
 __global__ __launch_bounds__(256) void AttendStartsKernel(AttendStates at, AttendStates initial, const float* decays, int keys, int values, int segments, int back) {
     const int bh = blockIdx.y, e = blockIdx.x * 256 + threadIdx.x;
     if (e >= keys * values) return;
@@ -432,7 +433,8 @@ __global__ __launch_bounds__(256) void AttendStartsKernel(AttendStates at, Atten
 }
 
 // Few rows, one after another: a workgroup has 64 columns of the state in its registers, four of them and every sixteenth row to a thread.  Bound by the state, read and written once.
-template <typename T, int KD>
+// Rows of the state that are not there are read as the last one; their q and k are zeros.
+template <typename T, int KD, int WIDTHS>
 __global__ __launch_bounds__(256) void AttendTokensKernel(AttendArgs p) {
     constexpr int VB = kAttendColumns, N = KD / 16;
     __shared__ __align__(16) float red[16][VB];
@@ -442,22 +444,35 @@ __global__ __launch_bounds__(256) void AttendTokensKernel(AttendArgs p) {
     const int64_t b = bh / p.heads;
     const int h = bh % p.heads;
     const int64_t length = LengthOf(p.lengths, b, p.length);
-    const int col0 = block * VB, cols = min(VB, run.values - col0);
+    const int col0 = block * VB, cols = min(VB, run.values - col0), keys = run.keys;
     const int tid = threadIdx.x, j = tid % 16 * 4, i0 = tid / 16;
     const T* const kp = static_cast<const T*>(run.k.data) + b * run.k.batch + (h / run.k.share) * run.k.head;
     const T* const vp = static_cast<const T*>(run.v.data) + b * run.v.batch + h * run.v.head + col0;
     const T* const qp = static_cast<const T*>(run.q.data) + b * run.q.batch + (h / run.q.share) * run.q.head;
-    const float* const from = run.start.data != nullptr ? run.start.data + bh * run.start.head + col0 : nullptr;
+    AttendPiece<float, 4> first[N];
+    if (run.start.data != nullptr) {
+        const float* const from = run.start.data + bh * run.start.head + col0;
+#pragma unroll
+        for (int n = 0; n < N; ++n) first[n] = AttendFetch<WIDTHS, 4>(from + min(i0 + 16 * n, keys - 1) * run.start.i, j, cols);
+    }
+    T k[N], q[N];
+    AttendPiece<T, 4> v;
+    float decay = 0;
+    const auto load = [&](int64_t t) {  // a row that is there
+        v = AttendFetch<WIDTHS, 4>(vp + t * run.v.row, j, cols);
+#pragma unroll
+        for (int n = 0; n < N; ++n) k[n] = kp[t * run.k.row + min(i0 + 16 * n, keys - 1)], q[n] = qp[t * run.q.row + min(i0 + 16 * n, keys - 1)];
+        if (p.decay != nullptr) decay = p.decay[b * p.decay_batch + t * p.decay_row + h * p.decay_head];
+    };
+    if (length > 0) load(0);
     attend4_t s[N];
 #pragma unroll
     for (int n = 0; n < N; ++n) {
-        const int i = i0 + 16 * n;
         s[n] = attend4_t{0, 0, 0, 0};
-        if (from != nullptr && i < run.keys) {
-            const AttendPiece<float, 4> piece = AttendLoad<float, 4>(from + i * run.start.i, j, cols);
+        if (run.start.data == nullptr) continue;
+        const AttendPiece<float, 4> piece = AttendPlace<WIDTHS>(first[n], j, cols);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) s[n][e] = piece.v[e];
-        }
+        for (int e = 0; e < 4; ++e) s[n][e] = piece.v[e];
     }
     for (int64_t t = 0; t < p.length; ++t) {
         T* const to = static_cast<T*>(run.y.data) + b * run.y.batch + t * run.y.row + h * run.y.head + col0;
@@ -465,21 +480,20 @@ __global__ __launch_bounds__(256) void AttendTokensKernel(AttendArgs p) {
             if (tid < cols) to[tid] = static_cast<T>(0);
             continue;
         }
-        const float step = __builtin_amdgcn_exp2f(static_cast<float>(AttendDecay(p, b, h, t)));
-        const AttendPiece<T, 4> vv = AttendLoad<T, 4>(vp + t * run.v.row, j, cols);
-        attend4_t v, y{0, 0, 0, 0};
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = static_cast<float>(vv.v[e]);
+        const float step = __builtin_amdgcn_exp2f(static_cast<float>(LogOfDecay(decay)));
+        const AttendPiece<T, 4> vv = AttendPlace<WIDTHS>(v, j, cols);
+        attend4_t y{0, 0, 0, 0};
 #pragma unroll
         for (int n = 0; n < N; ++n) {
-            const int i = i0 + 16 * n;
-            const float k = i < run.keys ? static_cast<float>(kp[t * run.k.row + i]) : 0.f, q = i < run.keys ? static_cast<float>(qp[t * run.q.row + i]) : 0.f;
+            const bool there = i0 + 16 * n < keys;
+            const float ki = there ? static_cast<float>(k[n]) : 0.f, qi = static_cast<float>(q[n]);
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                s[n][e] = __builtin_elementwise_fma(k, v[e], s[n][e] * step);
-                if (i < run.keys) y[e] = __builtin_elementwise_fma(q, s[n][e], y[e]);
+                s[n][e] = __builtin_elementwise_fma(ki, static_cast<float>(vv.v[e]), s[n][e] * step);
+                y[e] = there ? __builtin_elementwise_fma(qi, s[n][e], y[e]) : y[e];
             }
         }
+        if (t + 1 < length) load(t + 1);
         __syncthreads();  // the last row's sums have been read
         *reinterpret_cast<attend4_t*>(&red[i0][j]) = y;
         __syncthreads();
@@ -494,13 +508,13 @@ __global__ __launch_bounds__(256) void AttendTokensKernel(AttendArgs p) {
 #pragma unroll
     for (int n = 0; n < N; ++n) {
         const int i = i0 + 16 * n;
-        if (i >= run.keys) continue;
+        if (i >= keys) continue;
         AttendPiece<float, 4> piece;
 #pragma unroll
         for (int e = 0; e < 4; ++e) piece.v[e] = s[n][e];
         if (j + 4 <= cols) {
             *reinterpret_cast<AttendPiece<float, 4>*>(last + i * run.last.i + j) = piece;
-        } else {
+        } else if (WIDTHS != kAttendWhole) {
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 if (j + e < cols) last[i * run.last.i + j + e] = piece.v[e];
@@ -684,13 +698,16 @@ int hipcx_linear_attention(const hipcx_array* q, const hipcx_array* k, const hip
                 VisitKeys(c.keys, [&](auto kd) {
                     const int64_t blocks = p.blocks * p.batch * p.heads;
                     HIPCX_REQUIRE(blocks <= kBlocksPerLaunch, HIPCX_NOT_IMPLEMENTED_ERROR, what + ": too many elements");
-                    hipLaunchKernelGGL((AttendTokensKernel<T, decltype(kd)::value>), dim3(static_cast<unsigned>(blocks)), dim3(256), 0, AsStream(stream), p);
+                    constexpr int KD = decltype(kd)::value;
+                    void (*const kernel)(AttendArgs) = c.values < 4 ? AttendTokensKernel<T, KD, kAttendNarrow> : c.values % 4 == 0 ? AttendTokensKernel<T, KD, kAttendWhole> : AttendTokensKernel<T, KD, kAttendPart>;
+                    hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, AsStream(stream), p);
                     CheckLaunch("linear_attention");
                 });
             });
             return;
         }
         if (p.segments > 1) {
+            HIPCX_REQUIRE(reinterpret_cast<uintptr_t>(workspace) % 16 == 0, HIPCX_CHAINERX_ERROR, "workspace must be 16-byte aligned");
             const AttendStates starts = AttendSegments(static_cast<float*>(workspace), p, c.keys, c.values);
             run.last = starts, run.decays = starts.data + p.batch * p.heads * starts.head;
             LaunchAttend(p, q->dtype, true, AsStream(stream));

@@ -17,8 +17,9 @@ struct AttendDecayArgs {
 };
 
 // gg[t] = sum over u >= t of (q[u] gq[u] - k[u] gk[u]): sums from a segment's last row to its first, in 64 bits, on top of what lies behind the segment.
-__global__ __launch_bounds__(256) void AttendDecayKernel(AttendDecayArgs p) {
-    __shared__ double waves[4];
+template <int THREADS>
+__global__ __launch_bounds__(THREADS) void AttendDecayKernel(AttendDecayArgs p) {
+    __shared__ double waves[THREADS / 64];
     const int segment = static_cast<int>(blockIdx.x % p.segments);
     const int64_t bh = blockIdx.x / p.segments, b = bh / p.heads;
     const int h = static_cast<int>(bh % p.heads), tid = threadIdx.x, lane = tid % 64;
@@ -26,7 +27,7 @@ __global__ __launch_bounds__(256) void AttendDecayKernel(AttendDecayArgs p) {
     const int64_t whole = first + p.segment_rows < p.length ? first + p.segment_rows : p.length, end = whole < length ? whole : length;
     double behind = 0, total = 0;
     for (int i = 0; i < p.blocks; ++i) behind += p.ends[(bh * p.segments + segment) * p.blocks + i];
-    for (int64_t last = end; last > first; last -= 256) {
+    for (int64_t last = end; last > first; last -= THREADS) {
         const int64_t t = last - 1 - tid;
         double sum = 0;
         if (t >= first) {
@@ -46,10 +47,11 @@ __global__ __launch_bounds__(256) void AttendDecayKernel(AttendDecayArgs p) {
             if (p.out != nullptr) p.out[(b * p.length + t) * p.heads + h] = static_cast<float>(sum);
             total += sum;
         }
-        behind += waves[0] + waves[1] + waves[2] + waves[3];
+#pragma unroll
+        for (int w = 0; w < THREADS / 64; ++w) behind += waves[w];
     }
     if (p.out != nullptr) {
-        for (int64_t t = (end > first ? end : first) + tid; t < whole; t += 256) p.out[(b * p.length + t) * p.heads + h] = 0.f;
+        for (int64_t t = (end > first ? end : first) + tid; t < whole; t += THREADS) p.out[(b * p.length + t) * p.heads + h] = 0.f;
     }
     if (p.totals == nullptr) return;
 #pragma unroll
@@ -60,7 +62,12 @@ __global__ __launch_bounds__(256) void AttendDecayKernel(AttendDecayArgs p) {
     __syncthreads();
     if (lane == 0) waves[tid / 64] = total;
     __syncthreads();
-    if (tid == 0) p.totals[bh * p.segments + segment] = waves[0] + waves[1] + waves[2] + waves[3];
+    if (tid == 0) {
+        total = 0;
+#pragma unroll
+        for (int w = 0; w < THREADS / 64; ++w) total += waves[w];
+        p.totals[bh * p.segments + segment] = total;
+    }
 }
 
 // One decay for all rows of a head: the sum over sequences and segments, a wave to a head.
@@ -160,13 +167,15 @@ int hipcx_linear_attention_grad(const hipcx_array* q, const hipcx_array* k, cons
         const GradWorkspace w(c, log_decay != nullptr, log_decay != nullptr && log_decay->ndim == 1);
         HIPCX_REQUIRE(workspace_bytes >= w.bytes && (w.bytes == 0 || workspace != nullptr), HIPCX_CHAINERX_ERROR, what + ": the workspace is too small");
         HIPCX_REQUIRE(reinterpret_cast<uintptr_t>(workspace) % 16 == 0, HIPCX_CHAINERX_ERROR, "workspace must be 16-byte aligned");
+        const bool shared = c.key_heads < p.heads;
+        HIPCX_REQUIRE(!shared || p.batch * p.length * c.key_heads * c.keys < (int64_t{1} << 31), HIPCX_NOT_IMPLEMENTED_ERROR, what + ": too many elements");
+        HIPCX_REQUIRE(p.batch * p.heads * p.segments <= kBlocksPerLaunch, HIPCX_NOT_IMPLEMENTED_ERROR, what + ": too many elements");
         char* const ws = static_cast<char*>(workspace);
         const auto floats = [&](size_t at) { return reinterpret_cast<float*>(ws + at); };
         const hipStream_t s = AsStream(stream);
         const float* const gnew = gnew_state != nullptr ? static_cast<const float*>(gnew_state->data) : nullptr;
         const int64_t bh = p.batch * p.heads;
         if (bh > 0) {
-            const bool shared = c.key_heads < p.heads;
             const AttendRows wide{nullptr, p.length * p.heads * c.keys, static_cast<int64_t>(p.heads) * c.keys, c.keys, 1};
             const float f_scale = static_cast<float>(scale);
             AttendRun &of_q = p.run[0], &of_k = p.run[1], &of_v = p.run[2];
@@ -211,7 +220,6 @@ int hipcx_linear_attention_grad(const hipcx_array* q, const hipcx_array* k, cons
             LaunchAttend(p, dtype, false, s);
             if (shared && p.length > 0) {
                 const int64_t rows = p.batch * p.length, n = rows * c.key_heads * c.keys;
-                HIPCX_REQUIRE(n < (int64_t{1} << 31), HIPCX_NOT_IMPLEMENTED_ERROR, what + ": too many elements");
                 for (const auto& [at, to] : {std::pair<size_t, const AttendRows*>{w.gq, &to_q}, {w.gk, &to_k}}) {
                     const dim3 grid(static_cast<unsigned>((n + 255) / 256));
                     if (dtype == HIPCX_FLOAT16) hipLaunchKernelGGL((AttendShareKernel<half_t>), grid, dim3(256), 0, s, floats(at), *to, rows, p.length, c.key_heads, p.heads / c.key_heads, c.keys);
@@ -226,8 +234,9 @@ int hipcx_linear_attention_grad(const hipcx_array* q, const hipcx_array* k, cons
                 d.blocks = AttendBlocks(c.keys);
                 if (of_heads) d.totals = reinterpret_cast<double*>(ws + w.totals);
                 else d.out = static_cast<float*>(glog_decay->data);
-                HIPCX_REQUIRE(bh * p.segments <= kBlocksPerLaunch, HIPCX_NOT_IMPLEMENTED_ERROR, what + ": too many elements");
-                hipLaunchKernelGGL(AttendDecayKernel, dim3(static_cast<unsigned>(bh * p.segments)), dim3(256), 0, s, d);
+                // (segments of 2048 rows: 12 us with 256 threads)
+                if (p.segment_rows > 256) hipLaunchKernelGGL(AttendDecayKernel<1024>, dim3(static_cast<unsigned>(bh * p.segments)), dim3(1024), 0, s, d);
+                else hipLaunchKernelGGL(AttendDecayKernel<256>, dim3(static_cast<unsigned>(bh * p.segments)), dim3(256), 0, s, d);
                 CheckLaunch("linear_attention_grad");
             }
         }
