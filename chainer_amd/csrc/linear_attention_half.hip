@@ -285,6 +285,48 @@ __global__ __launch_bounds__(256, KD == 256 ? 1 : 2) void AttendHalfKernel(Atten
         g_now = g_next;
         load(r0 + C);
         if (wave == 0) load_decays(r0 + 2 * C);  // (behind the others: what waits for them must not wait for this one)
+        // This wave's columns of v times their rows' weights, in two parts of the unit that the state will have, and the state in that unit: in pieces, which go between the products with the state.
+        const int block = lane / 16 * 4 + lane % 16 / 4, piece = lane % 4 * 8;
+        attend_half8_t of_v[2], hi[2], lo[2];
+        attend4_t end[2][2];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            const char* const from = vs + (block + 32 * u) * Lds::kValuePitch + 32 * wave + piece;
+            of_v[u] = Join(ReadTurned(from), ReadTurned(from + 16 * Lds::kValuePitch));
+#pragma unroll
+            for (int g = 0; g < 2; ++g) end[u][g] = *reinterpret_cast<const attend4_t*>(dec->end + 32 * u + 16 * g + lane / 16 * 4);
+        }
+        float w[2][8], largest_v = 0, keep = 1, in = 1;
+        const float all = dec->all;
+        constexpr int kPieces = 7;
+        const auto prepare = [&](int at) {
+            if (at < 2) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    w[at][e] = __builtin_fmaf(static_cast<float>(of_v[at][e]), end[at][e / 4][e % 4], 0.f);
+                    largest_v = fmaxf(largest_v, fabsf(w[at][e]));
+                }
+            } else if (at == 2) {
+                // (in exponents: what is added may be further from the unit than a float reaches)
+                const float decayed = most * all, added = MaxOver32(MaxOver16(largest_v));
+                const int size = max(decayed < HUGE_VALF ? ExponentOf(decayed) : -127, added > 0 ? ExponentOf(added) - unit : -127);
+                int up = 0;
+                if (size >= 15 || (size < 4 && size > -127)) up = min(max(max(size - 13, -112 - unit), -112), 114 - unit);
+                unit += up;
+                keep = all * Power(max(-up, -126)), in = Power(-unit);
+            } else if (at < 5) {
+#pragma unroll
+                for (int n = (at - 3) * (NS / 2); n < (at - 2) * (NS / 2); ++n) s[n] *= keep;
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) w[at - 5][e] *= in;
+                Split<8>(w[at - 5], minus, &hi[at - 5], &lo[at - 5]);
+            }
+        };
+        if constexpr (!OUT) {
+#pragma unroll
+            for (int i = 0; i < kPieces; ++i) prepare(i);
+        }
         if constexpr (OUT) {
             // this wave's sixteen rows by all columns, in blocks of 16 x 16
             const int quarter = lane / 16;
@@ -308,6 +350,10 @@ __global__ __launch_bounds__(256, KD == 256 ? 1 : 2) void AttendHalfKernel(Atten
                     if (step + 1 < 2 * NQ) read(step + 1, part[step % 2 ^ 1]);
 #pragma unroll
                     for (int d = 0; d < DB; ++d) of_state[d] = Mfma(part[step % 2][d], q[step / 2], of_state[d]);
+#pragma unroll
+                    for (int i = 0; i < kPieces; ++i) {
+                        if (i * (2 * NQ) / kPieces == step) prepare(i);
+                    }
                     __builtin_amdgcn_sched_barrier(0);
                 }
                 const float from_start = __builtin_amdgcn_exp2f(high + low) * run.out_scale;
@@ -366,19 +412,19 @@ __global__ __launch_bounds__(256, KD == 256 ? 1 : 2) void AttendHalfKernel(Atten
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
                 if (2 * u > wave) continue;
-                float w[8];
+                float weights[8];
 #pragma unroll
-                for (int e = 0; e < 8; ++e) w[e] = 2 * u + e / 4 <= wave ? a[2 * u + e / 4][e % 4] * (since[2 * u + e / 4] * scale.in) : 0.f;
-                attend_half8_t hi, lo;
-                Split<8>(w, minus, &hi, &lo);
+                for (int e = 0; e < 8; ++e) weights[e] = 2 * u + e / 4 <= wave ? a[2 * u + e / 4][e % 4] * (since[2 * u + e / 4] * scale.in) : 0.f;
+                attend_half8_t p_hi, p_lo;
+                Split<8>(weights, minus, &p_hi, &p_lo);
                 const char* const at = vs + (32 * u + 4 * quarter + lane % 16 / 4) * Lds::kValuePitch + lane % 4 * 8;
                 attend_half8_t v[DB];
 #pragma unroll
                 for (int d = 0; d < DB; ++d) v[d] = Join(ReadTurned(at + 32 * d), ReadTurned(at + 16 * Lds::kValuePitch + 32 * d));
 #pragma unroll
-                for (int d = 0; d < DB; ++d) of_rows[d] = Mfma(v[d], lo, of_rows[d]);
+                for (int d = 0; d < DB; ++d) of_rows[d] = Mfma(v[d], p_lo, of_rows[d]);
 #pragma unroll
-                for (int d = 0; d < DB; ++d) of_rows[d] = Mfma(v[d], hi, of_rows[d]);
+                for (int d = 0; d < DB; ++d) of_rows[d] = Mfma(v[d], p_hi, of_rows[d]);
             }
             const float from_rows = scale.out * kv_scale * run.out_scale;
             char* const to = yp + static_cast<int64_t>(own_row()) * y_row;
@@ -427,9 +473,7 @@ __global__ __launch_bounds__(256, KD == 256 ? 1 : 2) void AttendHalfKernel(Atten
         __builtin_amdgcn_sched_barrier(0);
         load_q(r0 + C);
         {
-            // this wave's columns of v times their rows' weights, in two parts
-            const int block = lane / 16 * 4 + lane % 16 / 4, piece = lane % 4 * 8;
-            const char *const from = vs + block * Lds::kValuePitch + 32 * wave + piece, *const at = ks + block * Lds::kKeyPitch + piece;
+            const char* const at = ks + block * Lds::kKeyPitch + piece;
             attend_half8_t k[2][NS / 2];
             const auto read = [&](int step, attend_half8_t (&to)[NS / 2]) {  // half of the keys of 32 rows
 #pragma unroll
@@ -438,43 +482,14 @@ __global__ __launch_bounds__(256, KD == 256 ? 1 : 2) void AttendHalfKernel(Atten
                     to[n] = Join(ReadTurned(row), ReadTurned(row + 16 * Lds::kKeyPitch));
                 }
             };
-            float w[2][8], largest = 0;
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                const attend_half8_t v = Join(ReadTurned(from + 32 * u * Lds::kValuePitch), ReadTurned(from + (32 * u + 16) * Lds::kValuePitch));
-#pragma unroll
-                for (int g = 0; g < 2; ++g) {
-                    const attend4_t end = *reinterpret_cast<const attend4_t*>(dec->end + 32 * u + 16 * g + lane / 16 * 4);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        w[u][4 * g + e] = __builtin_fmaf(static_cast<float>(v[4 * g + e]), end[e], 0.f);
-                        largest = fmaxf(largest, fabsf(w[u][4 * g + e]));
-                    }
-                }
-            }
             read(0, k[0]);
-            // (in exponents: what is added may be further from the unit than a float reaches)
-            const float all = dec->all, decayed = most * all, added = MaxOver32(MaxOver16(largest));
-            const int size = max(decayed < HUGE_VALF ? ExponentOf(decayed) : -127, added > 0 ? ExponentOf(added) - unit : -127);
-            int up = 0;
-            if (size >= 15 || (size < 4 && size > -127)) up = min(max(max(size - 13, -112 - unit), -112), 114 - unit);
-            unit += up;
-            const float keep = all * Power(max(-up, -126)), in = Power(-unit);
-#pragma unroll
-            for (int n = 0; n < NS; ++n) s[n] *= keep;
-            attend_half8_t hi, lo;
 #pragma unroll
             for (int step = 0; step < 4; ++step) {
                 if (step + 1 < 4) read(step + 1, k[step % 2 ^ 1]);
-                if (step % 2 == 0) {
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) w[step / 2][e] *= in;
-                    Split<8>(w[step / 2], minus, &hi, &lo);
-                }
+                for (int n = 0; n < NS / 2; ++n) s[step % 2 * (NS / 2) + n] = Mfma(k[step % 2][n], lo[step / 2], s[step % 2 * (NS / 2) + n]);
 #pragma unroll
-                for (int n = 0; n < NS / 2; ++n) s[step % 2 * (NS / 2) + n] = Mfma(k[step % 2][n], lo, s[step % 2 * (NS / 2) + n]);
-#pragma unroll
-                for (int n = 0; n < NS / 2; ++n) s[step % 2 * (NS / 2) + n] = Mfma(k[step % 2][n], hi, s[step % 2 * (NS / 2) + n]);
+                for (int n = 0; n < NS / 2; ++n) s[step % 2 * (NS / 2) + n] = Mfma(k[step % 2][n], hi[step / 2], s[step % 2 * (NS / 2) + n]);
                 __builtin_amdgcn_sched_barrier(0);
             }
         }
