@@ -111,6 +111,20 @@ def test_layer_norm_of_rows_far_from_zero_and_of_constant_ones(chx):
     assert np.isnan(with_nan[9:12]).all() and np.array_equal(np.delete(with_nan, [9, 10, 11], 0), np.delete(y.get(), [9, 10, 11], 0))
 
 
+@pytest.mark.parametrize('cols', [64, 900, 4096, 40000])
+def test_layer_norm_means_of_float16_are_those_of_its_values(chx, cols):
+    """Differences from a mean with more bits than the values would all be rounded alike, and the mean of 4096 values off by up to 6e-8.
+
+    Exact ones of variance 1 leave what their sum loses: an addition rounds by at most 2^-25 of its result where that is a power of two, by 2^-24 of it at most, with a deviation of half of that.
+    m <= 40 terms one after another in a thread have results of order sqrt(m) at most, and the levels of the tree behind, ten at most, cols / (m 2^l) results of order sqrt(m 2^l):
+    together a deviation of 2^-25 sqrt(cols (m + 10)), so that six of them are below 2^-19.5 sqrt(cols), and cols times less in the mean.  The division and the last addition round the mean."""
+    rng = np.random.default_rng(3)
+    x = rng.standard_normal((50, cols)).astype(np.float16)
+    _, state = chx.layer_norm(up(chx, x))
+    want = x.astype(np.float64).mean(1)
+    assert (np.abs(state.mean.get() - want) <= 2.0 ** -19.5 / cols ** 0.5 + 2.0 ** -23 * np.abs(want)).all()
+
+
 def test_layer_norm_gradients_against_differences(chx):
     """In float64: central differences of sum(y * gy), whose error is h^2 / 6 of the third derivative (of order 1 here) and 2^-53 of the sum (of order 20) over h."""
     x, gamma, beta, gy = norm_case(3, 11, 'float64', 'float64')
