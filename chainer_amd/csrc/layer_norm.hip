@@ -501,7 +501,7 @@ struct NormPlan {
 NormPlan PlanNorm(int64_t cols, int64_t item) {
     if (cols * item < 16) return {16, 0};
     const int64_t pieces = (cols * item + 15) / 16;
-    for (const NormPlan plan : {NormPlan{16, 1}, {16, 2}, {64, 1}, {64, 2}, {64, 3}, {64, 4}, {256, 2}, {256, 4}, {1024, 4}}) {
+    for (const NormPlan plan : {NormPlan{16, 1}, {16, 2}, {64, 1}, {64, 2}, {64, 3}, {64, 4}, {256, 2}, {256, 4}, {1024, 2}, {1024, 4}}) {
         if (pieces <= static_cast<int64_t>(plan.threads) * plan.pieces) return plan;
     }
     return {0, 0};
@@ -513,7 +513,7 @@ void VisitNorm(NormPlan plan, F&& f) {
     const auto visit = [&](auto threads, auto pieces) { f(threads, pieces, std::false_type{}); };
     if (plan.pieces == 0) f(std::integral_constant<int, 16>{}, std::integral_constant<int, 1>{}, std::true_type{});
     else if (plan.threads == 16) plan.pieces == 1 ? visit(std::integral_constant<int, 16>{}, std::integral_constant<int, 1>{}) : visit(std::integral_constant<int, 16>{}, std::integral_constant<int, 2>{});
-    else if (plan.threads == 1024) visit(std::integral_constant<int, 1024>{}, std::integral_constant<int, 4>{});
+    else if (plan.threads == 1024) plan.pieces == 2 ? visit(std::integral_constant<int, 1024>{}, std::integral_constant<int, 2>{}) : visit(std::integral_constant<int, 1024>{}, std::integral_constant<int, 4>{});
     else if (plan.threads == 256) plan.pieces == 2 ? visit(std::integral_constant<int, 256>{}, std::integral_constant<int, 2>{}) : visit(std::integral_constant<int, 256>{}, std::integral_constant<int, 4>{});
     else if (plan.pieces == 1) visit(std::integral_constant<int, 64>{}, std::integral_constant<int, 1>{});
     else if (plan.pieces == 2) visit(std::integral_constant<int, 64>{}, std::integral_constant<int, 2>{});

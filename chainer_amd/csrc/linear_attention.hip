@@ -65,10 +65,18 @@ __global__ __launch_bounds__(256, KD == 64 ? 3 : 1) void AttendKernel(AttendArgs
     // Elements that are not there are read as the last ones, so that all loads go out at once; the compiler would have each wait for its condition.
     const auto states_at = [&](const AttendStates& of, attend4_t (&to)[NS]) {
         const float* const from = of.data + bh * of.head + segment * of.segment + (col0 + min(state_col(), cols - 1)) * of.j;
+        if (of.i == 1 && keys % 4 == 0) {  // (a transpose: a lane's four are neighbours)
 #pragma unroll
-        for (int n = 0; n < NS; ++n) {
+            for (int n = 0; n < NS; ++n) {
+                const AttendPiece<float, 4> four = *reinterpret_cast<const AttendPiece<float, 4>*>(from + min(state_row(n, 0), keys - 4));
+                to[n] = __builtin_bit_cast(attend4_t, four);
+            }
+        } else {
 #pragma unroll
-            for (int r = 0; r < 4; ++r) to[n][r] = from[min(state_row(n, r), keys - 1) * of.i];
+            for (int n = 0; n < NS; ++n) {
+#pragma unroll
+                for (int r = 0; r < 4; ++r) to[n][r] = from[min(state_row(n, r), keys - 1) * of.i];
+            }
         }
 #pragma unroll
         for (int n = 0; n < NS; ++n) {
@@ -177,7 +185,8 @@ __global__ __launch_bounds__(256, KD == 64 ? 3 : 1) void AttendKernel(AttendArgs
         g_now = g_next;
         load(r0 + C);
         if (wave == 0) load_decays(r0 + 2 * C);  // (behind the others: what waits for them must not wait for this one)
-        if constexpr (OUT) {
+        const int here = static_cast<int>(rows - r0 < C ? rows - r0 : C);
+        if (OUT && 16 * wave < here) {
             // this wave's sixteen rows by all columns, in blocks of 16 x 16
             const float high = dec->high[own_row()], low = dec->low[own_row()];
             attend4_t q[NS];
@@ -228,8 +237,6 @@ __global__ __launch_bounds__(256, KD == 64 ? 3 : 1) void AttendKernel(AttendArgs
                 }
             }
             load_q(r0 + C);
-            if (wave == 0 && more) sum_decays(r0 + C, decays + (turn ^ 1));
-            if (tid == 0) odd[turn ^ 1] = 0;
 #pragma unroll
             for (int sb = 0; sb < 4; ++sb) {
                 if (sb > wave) continue;
@@ -284,9 +291,9 @@ __global__ __launch_bounds__(256, KD == 64 ? 3 : 1) void AttendKernel(AttendArgs
                 dp += static_cast<int64_t>(d_row) * C;
             }
             yp += static_cast<int64_t>(y_row) * C;
-        } else {
-            if (wave == 0 && more) sum_decays(r0 + C, decays + (turn ^ 1));
         }
+        if (wave == 0 && more) sum_decays(r0 + C, decays + (turn ^ 1));
+        if (tid == 0) odd[turn ^ 1] = 0;
         __builtin_amdgcn_sched_barrier(0);
         {
             // this wave's columns of v times their rows' weights
@@ -297,6 +304,7 @@ __global__ __launch_bounds__(256, KD == 64 ? 3 : 1) void AttendKernel(AttendArgs
             constexpr int N = NS < 8 ? NS : 8;  // accumulators between the reads
 #pragma unroll
             for (int sb = 0; sb < 4; ++sb) {
+                if (16 * sb >= here) break;
                 const attend4_t end = *reinterpret_cast<const attend4_t*>(dec->end + 16 * sb + 4 * quarter);
                 float v[4];
 #pragma unroll

@@ -126,10 +126,18 @@ __global__ __launch_bounds__(256, KD == 256 ? 1 : 2) void AttendHalfKernel(Atten
     // Elements that are not there are read as the last ones, so that all loads go out at once; the compiler would have each wait for its condition.
     const auto states_at = [&](const AttendStates& of, attend4_t (&to)[NS]) {
         const float* const from = of.data + bh * of.head + segment * of.segment + (col0 + min(state_col(), cols - 1)) * of.j;
+        if (of.i == 1 && keys % 4 == 0) {  // (a transpose: a lane's four are neighbours)
 #pragma unroll
-        for (int n = 0; n < NS; ++n) {
+            for (int n = 0; n < NS; ++n) {
+                const AttendPiece<float, 4> four = *reinterpret_cast<const AttendPiece<float, 4>*>(from + min(state_row(n, 0), keys - 4));
+                to[n] = __builtin_bit_cast(attend4_t, four);
+            }
+        } else {
 #pragma unroll
-            for (int r = 0; r < 4; ++r) to[n][r] = from[min(state_row(n, r), keys - 1) * of.i];
+            for (int n = 0; n < NS; ++n) {
+#pragma unroll
+                for (int r = 0; r < 4; ++r) to[n][r] = from[min(state_row(n, r), keys - 1) * of.i];
+            }
         }
 #pragma unroll
         for (int n = 0; n < NS; ++n) {
@@ -323,11 +331,11 @@ __global__ __launch_bounds__(256, KD == 256 ? 1 : 2) void AttendHalfKernel(Atten
                 Split<8>(w[at - 5], minus, &hi[at - 5], &lo[at - 5]);
             }
         };
-        if constexpr (!OUT) {
+        const int here = static_cast<int>(rows - r0 < C ? rows - r0 : C);
+        if (!OUT || 16 * wave >= here) {
 #pragma unroll
             for (int i = 0; i < kPieces; ++i) prepare(i);
-        }
-        if constexpr (OUT) {
+        } else if constexpr (OUT) {
             // this wave's sixteen rows by all columns, in blocks of 16 x 16
             const int quarter = lane / 16;
             const float high = dec->high[own_row()], low = dec->low[own_row()];
@@ -467,9 +475,8 @@ __global__ __launch_bounds__(256, KD == 256 ? 1 : 2) void AttendHalfKernel(Atten
                 dp += static_cast<int64_t>(d_row) * C;
             }
             yp += static_cast<int64_t>(y_row) * C;
-        } else {
-            if (wave == 0 && more) sum_decays(r0 + C, decays + (turn ^ 1));
         }
+        if (!OUT && wave == 0 && more) sum_decays(r0 + C, decays + (turn ^ 1));
         __builtin_amdgcn_sched_barrier(0);
         load_q(r0 + C);
         {
@@ -485,6 +492,7 @@ __global__ __launch_bounds__(256, KD == 256 ? 1 : 2) void AttendHalfKernel(Atten
             read(0, k[0]);
 #pragma unroll
             for (int step = 0; step < 4; ++step) {
+                if (step == 2 && here <= 32) break;
                 if (step + 1 < 4) read(step + 1, k[step % 2 ^ 1]);
 #pragma unroll
                 for (int n = 0; n < NS / 2; ++n) s[step % 2 * (NS / 2) + n] = Mfma(k[step % 2][n], lo[step / 2], s[step % 2 * (NS / 2) + n]);
