@@ -247,7 +247,7 @@ inline void CutAttend(AttendArgs* p, bool padded, int64_t blocks, int64_t states
 struct AttendCall {
     AttendArgs p{};
     AttendRows q, k, v;
-    int keys, values, key_heads, dtype;
+    int keys, values, key_heads;
     const float* state;
 };
 bool AttendSizesOf(const hipcx_array* q, const hipcx_array* v, AttendCall* c);
@@ -283,8 +283,8 @@ void VisitWidths(AttendWidths widths, bool grad, F&& f) {
     else grad ? f(std::integral_constant<int, kAttendPart>{}, std::true_type{}) : f(std::integral_constant<int, kAttendPart>{}, std::false_type{});
 }
 
-// Workgroups that a compute unit holds, as LDS lets them.
-inline int64_t AttendResident(int dtype, int keys) { return keys <= 64 ? 3 : keys <= 128 && dtype == HIPCX_FLOAT16 ? 2 : 1; }
+// Workgroups that a compute unit holds, as registers and LDS let them.
+inline int64_t AttendResident(int keys) { return keys <= 64 ? 3 : keys <= 128 ? 2 : 1; }
 
 void LaunchAttend(const AttendArgs& p, int dtype, bool states_alone, hipStream_t stream);
 void LaunchAttendHalf(const AttendArgs& p, int keys, int64_t blocks, bool states_alone, hipStream_t stream);  // float16

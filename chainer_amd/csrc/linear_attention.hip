@@ -17,8 +17,13 @@ struct AttendTag {};
 // GRAD: what the passes of the gradients have beyond the forward one.
 template <int KD, bool OUT>
 struct AttendLds {
+    static_assert(kAttendTile == kAttendColumns, "the rows of k and the columns of the state share a place");
     static constexpr int kPitch = KD + 4, kValuePitch = kAttendColumns + 4;  // floats; four rows on is sixteen banks on
-    static constexpr int kValues = kAttendTile * kPitch, kStates = kValues + kAttendTile * kValuePitch, kSums = kStates + (OUT ? kAttendColumns * kPitch : 0);
+    // At 128 keys the copy of the state and the rows of k, as many, take turns in one place, so that two workgroups fit into a compute unit: for two more barriers a tile, 24 x 478 rows of 11 heads
+    // with gradients 898 -> 723 us.  64 keys fit three times either way (20 padded prompts of 777 rows: 94 us, with turns 109), 256 once.
+    static constexpr bool kTurns = KD == 128;
+    static constexpr int kValues = kAttendTile * kPitch, kStates = kTurns ? 0 : kValues + kAttendTile * kValuePitch;
+    static constexpr int kSums = (kTurns ? kValues + kAttendTile * kValuePitch : kStates + (OUT ? kAttendColumns * kPitch : 0));
     static constexpr int kDecays = kSums + 4 * kAttendColumns;
     static constexpr int kBytes = kDecays * 4 + 2 * static_cast<int>(sizeof(AttendDecays)) + 16;
 };
@@ -26,7 +31,7 @@ struct AttendLds {
 __device__ __forceinline__ attend4_t Mfma4(float a, float b, attend4_t c) { return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0); }
 
 template <int KD, bool OUT, int WIDTHS, bool GRAD>
-__global__ __launch_bounds__(256, KD == 64 ? 3 : 1) void AttendKernel(AttendArgs p) {
+__global__ __launch_bounds__(256, KD == 64 ? 3 : KD == 128 ? 2 : 1) void AttendKernel(AttendArgs p) {
     using Lds = AttendLds<KD, OUT>;
     constexpr int VB = kAttendColumns, C = kAttendTile, NS = KD / 16, KP = Lds::kPitch, VP = Lds::kValuePitch, DB = VB / 16;
     extern __shared__ __align__(16) float lds[];
@@ -165,9 +170,10 @@ __global__ __launch_bounds__(256, KD == 64 ? 3 : 1) void AttendKernel(AttendArgs
         asm volatile("" : "+s"(keys));
         const int quarter = lane / 16;
         const AttendDecays* const dec = decays + turn;
-        // (the last tile's rows of k and v have been read by all)
-#pragma unroll
-        for (int n = 0; n < NK; ++n) *reinterpret_cast<attend4_t*>(ks + (key_row + n * KR) * KP + key_col) = placed(k_next[n], key_col, keys);
+        const int here = static_cast<int>(rows - r0 < C ? rows - r0 : C);
+        const bool live = OUT && 16 * wave < here;  // this wave has rows
+        const bool more = r0 + C < rows;
+        // (the last tile's rows of v have been read by all)
         float finite = 0;  // or not a number
 #pragma unroll
         for (int n = 0; n < NV; ++n) {
@@ -177,44 +183,52 @@ __global__ __launch_bounds__(256, KD == 64 ? 3 : 1) void AttendKernel(AttendArgs
             for (int e = 0; e < 4; ++e) finite = __builtin_fmaf(v[e], 0.f, finite);
         }
         if (OUT && !(finite == 0)) odd[turn] = 1;
-        __syncthreads();
+        const auto place_k = [&] {
+#pragma unroll
+            for (int n = 0; n < NK; ++n) *reinterpret_cast<attend4_t*>(ks + (key_row + n * KR) * KP + key_col) = placed(k_next[n], key_col, keys);
+            __syncthreads();
+        };
+        constexpr bool kTurns = OUT && Lds::kTurns;
+        if (!kTurns) place_k();
+        attend4_t q[OUT ? NS : 1], y[DB]{};
+        float high = 0, low = 0;
+        if (live) {
+            // this wave's sixteen rows by all columns, in blocks of 16 x 16
+            high = dec->high[own_row()], low = dec->low[own_row()];
+#pragma unroll
+            for (int m = 0; m < NS; ++m) q[OUT ? m : 0] = placed(q_next[OUT ? m : 0], 16 * m + 4 * quarter, keys);
+            const float* const at = ss + lane % 16 * KP + 4 * quarter;
+            attend4_t part[2][DB];
+            const auto read = [&](int m, attend4_t (&to)[DB]) {
+#pragma unroll
+                for (int d = 0; d < DB; ++d) to[d] = *reinterpret_cast<const attend4_t*>(at + 16 * d * KP + 16 * m);
+            };
+            read(0, part[0]);
+#pragma unroll
+            for (int m = 0; m < NS; ++m) {  // reads of the next step under the products of this one
+                if (m + 1 < NS) read(m + 1, part[m % 2 ^ 1]);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+#pragma unroll
+                    for (int d = 0; d < DB; ++d) y[d] = Mfma4(part[m % 2][d][e], q[OUT ? m : 0][e], y[d]);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            const float from_start = __builtin_amdgcn_exp2f(high + low);
+#pragma unroll
+            for (int d = 0; d < DB; ++d) y[d] *= from_start;
+        }
+        if (kTurns) {
+            __syncthreads();  // the copy of the state has been read
+            place_k();
+        }
         passed += dec->sum;
         // An infinity of a later row, times P's zeros, would reach earlier ones: the rest goes row by row.
         if (OUT && odd[turn] != 0) break;
-        const bool more = r0 + C < rows;
         g_now = g_next;
         load(r0 + C);
         if (wave == 0) load_decays(r0 + 2 * C);  // (behind the others: what waits for them must not wait for this one)
-        const int here = static_cast<int>(rows - r0 < C ? rows - r0 : C);
-        if (OUT && 16 * wave < here) {
-            // this wave's sixteen rows by all columns, in blocks of 16 x 16
-            const float high = dec->high[own_row()], low = dec->low[own_row()];
-            attend4_t q[NS];
-#pragma unroll
-            for (int m = 0; m < NS; ++m) q[m] = placed(q_next[m], 16 * m + 4 * quarter, keys);
-            attend4_t y[DB]{};
-            {
-                const float* const at = ss + lane % 16 * KP + 4 * quarter;
-                attend4_t part[2][DB];
-                const auto read = [&](int m, attend4_t (&to)[DB]) {
-#pragma unroll
-                    for (int d = 0; d < DB; ++d) to[d] = *reinterpret_cast<const attend4_t*>(at + 16 * d * KP + 16 * m);
-                };
-                read(0, part[0]);
-#pragma unroll
-                for (int m = 0; m < NS; ++m) {  // reads of the next step under the products of this one
-                    if (m + 1 < NS) read(m + 1, part[m % 2 ^ 1]);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-#pragma unroll
-                        for (int d = 0; d < DB; ++d) y[d] = Mfma4(part[m % 2][d][e], q[m][e], y[d]);
-                    }
-                    __builtin_amdgcn_sched_barrier(0);
-                }
-                const float from_start = __builtin_amdgcn_exp2f(high + low);
-#pragma unroll
-                for (int d = 0; d < DB; ++d) y[d] *= from_start;
-            }
+        if (live) {
             attend4_t a[4]{};
             {
                 const float* const at = ks + lane % 16 * KP + 4 * quarter;
@@ -260,7 +274,7 @@ __global__ __launch_bounds__(256, KD == 64 ? 3 : 1) void AttendKernel(AttendArgs
                 }
             }
             float* const to = yp + static_cast<int64_t>(own_row()) * y_row;
-            const bool live = r0 + own_row() < rows;
+            const bool there = r0 + own_row() < rows;
             float dot = 0;
 #pragma unroll
             for (int d = 0; d < DB; ++d) {
@@ -268,7 +282,7 @@ __global__ __launch_bounds__(256, KD == 64 ? 3 : 1) void AttendKernel(AttendArgs
                 AttendPiece<float, 4> out;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) out.v[e] = y[d][e] * run.out_scale;
-                if (!live) continue;
+                if (!there) continue;
                 if (with_dots) {
                     const float* const row = dp + static_cast<int64_t>(own_row()) * d_row;
                     const AttendPiece<float, 4> with = AttendPlace<WIDTHS>(AttendFetch<WIDTHS, 4>(row, j, cols), j, cols);
@@ -287,7 +301,7 @@ __global__ __launch_bounds__(256, KD == 64 ? 3 : 1) void AttendKernel(AttendArgs
             if (with_dots) {
                 dot += __shfl_xor(dot, 16);
                 dot += __shfl_xor(dot, 32);
-                if (quarter == 0 && live) dots[row0 + way * (r0 + own_row())] = dot;
+                if (quarter == 0 && there) dots[row0 + way * (r0 + own_row())] = dot;
                 dp += static_cast<int64_t>(d_row) * C;
             }
             yp += static_cast<int64_t>(y_row) * C;
@@ -325,12 +339,16 @@ __global__ __launch_bounds__(256, KD == 64 ? 3 : 1) void AttendKernel(AttendArgs
                 }
             }
         }
-        __syncthreads();  // the copy of the state, and the rows of k and v, have been read
+        __syncthreads();  // the rows of k and v have been read
         if (OUT) keep_state();
+        if (kTurns) __syncthreads();
     }
 
     if (OUT && r0 < rows) {
         // row by row, on the copy
+        __syncthreads();
+        keep_state();
+        __syncthreads();
         const int j = lane;
         for (; r0 < rows; ++r0) {
             const int64_t row = row0 + way * r0;
@@ -602,7 +620,7 @@ bool AttendSizesOf(const hipcx_array* q, const hipcx_array* v, AttendCall* c) {
     if (q->shape[0] < 0 || q->shape[1] < 0 || q->shape[1] >= (int64_t{1} << 30) || kh < 1 || h < 1 || h >= (1 << 20) || h % kh != 0) return false;
     if (q->shape[3] < 1 || q->shape[3] > kMaxAttend || v->shape[3] < 1 || v->shape[3] > kMaxAttend || q->shape[0] > kBlocksPerLaunch / h) return false;
     c->p.batch = q->shape[0], c->p.length = q->shape[1], c->p.heads = static_cast<int>(h);
-    c->keys = static_cast<int>(q->shape[3]), c->values = static_cast<int>(v->shape[3]), c->key_heads = static_cast<int>(kh), c->dtype = q->dtype;
+    c->keys = static_cast<int>(q->shape[3]), c->values = static_cast<int>(v->shape[3]), c->key_heads = static_cast<int>(kh);
     return true;
 }
 
@@ -654,7 +672,7 @@ constexpr int kAttendTokens = 8;
 
 void CutForward(AttendCall* c, bool padded) {
     if (c->p.length <= kAttendTokens) c->p.segments = 1, c->p.segment_rows = kAttendTile;
-    else CutAttend(&c->p, padded, AttendBlocks(c->values), AttendBlocks(c->values), AttendResident(c->dtype, c->keys), static_cast<int64_t>(c->keys) * c->values);
+    else CutAttend(&c->p, padded, AttendBlocks(c->values), AttendBlocks(c->values), AttendResident(c->keys), static_cast<int64_t>(c->keys) * c->values);
 }
 
 size_t ForwardWorkspace(const AttendCall& c) {
