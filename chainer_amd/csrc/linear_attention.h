@@ -64,28 +64,12 @@ constexpr int kAttendTile = 64;      // rows that are taken at once
 constexpr int kAttendColumns = 64;   // columns of v to a workgroup
 constexpr int kMaxAttend = 256;      // keys, values
 
-typedef float attend16_t __attribute__((ext_vector_type(16)));
 typedef float attend4_t __attribute__((ext_vector_type(4)));
 
 template <typename T, int N>
 struct __attribute__((packed, aligned(alignof(T)))) AttendPiece {
     T v[N];
 };
-
-// N elements of a row from `at` on, zeros from `end` on.
-template <typename T, int N>
-__device__ __forceinline__ AttendPiece<T, N> AttendLoad(const T* row, int at, int end) {
-    AttendPiece<T, N> r{};
-    if (at + N <= end) {
-        r = *reinterpret_cast<const AttendPiece<T, N>*>(row + at);
-    } else {
-#pragma unroll
-        for (int e = 0; e < N; ++e) {
-            if (at + e < end) r.v[e] = row[at + e];
-        }
-    }
-    return r;
-}
 
 // How the rows of a pass fall into pieces of 16 bytes: all whole; the last one not; rows of less than a piece.
 enum AttendWidths { kAttendWhole, kAttendPart, kAttendNarrow };

@@ -13,7 +13,9 @@ struct AttendTag {};
 //   P[t][s] = exp(G[t] - G[s]) q[t] k[s] for s <= t,  y = P v + exp(G) q S,  S <- exp(G[63]) S + (exp(G[63] - G) k)^T v.
 // A workgroup of four waves has 64 columns of v: a wave has sixteen rows of y, and sixteen columns of S in its accumulators (a copy is in LDS, turned, for the products with q).
 // P stays in registers: as k q^T its column t is a lane, whose rows s are the reduction of the product v^T P.
-// Products run on the float pipe (v_mfma_f32_16x16x4_f32), with the reduction's elements in an order that gives a lane four neighbours.
+// Products run on the float pipe (v_mfma_f32_16x16x4_f32), with the reduction's elements in an order that gives a lane four neighbours.  Bound by a tile's chain: at 64 keys and values the wave of the
+// last rows multiplies for 8.2 thousand cycles of a tile's 16, and three workgroups share a compute unit.  20 padded prompts of up to 777 rows, 13 heads of 50 x 50: 61 us, the states of their three
+// segments before it 30; rows of 32 to a wave, and loads that waited for one another, took 222 in one segment.  At 128 keys and values 24 x 478 rows of 11 heads with gradients run at 72 TFLOP/s.
 // GRAD: what the passes of the gradients have beyond the forward one.
 template <int KD, bool OUT>
 struct AttendLds {
@@ -458,7 +460,8 @@ __global__ __launch_bounds__(256) void AttendStartsKernel(AttendStates at, Atten
     }
 }
 
-// Few rows, one after another: a workgroup has 64 columns of the state in its registers, four of them and every sixteenth row to a thread.  Bound by the state, read and written once.
+// Few rows, one after another: a workgroup has 64 columns of the state in its registers, four of them and every sixteenth row to a thread.  Bound by the state, read and written once: one row of 128
+// sequences, 16 heads of 128 x 128 in float16, takes 44.6 us, 6.0 TB/s (with loads behind branches 58).  Up to eight rows it is quicker than a tile, which multiplies for sixteen at least.
 // Rows of the state that are not there are read as the last one; their q and k are zeros.
 template <typename T, int KD, int WIDTHS>
 __global__ __launch_bounds__(256) void AttendTokensKernel(AttendArgs p) {

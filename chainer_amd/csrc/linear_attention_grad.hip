@@ -1,5 +1,5 @@
 // The gradients of linear attention: its three passes (linear_attention.h), and what they have of the log decays.
-#include <cstdlib>
+#include <utility>
 
 #include "linear_attention.h"
 
