@@ -207,7 +207,8 @@ __global__ __launch_bounds__(256, KD == 64 ? 3 : KD == 128 ? 2 : 1) void AttendK
             };
             read(0, part[0]);
 #pragma unroll
-            for (int m = 0; m < NS; ++m) {  // reads of the next step under the products of this one
+            for (int m = 0; m < NS; ++m) {  // reads of the next step under the products of this one; nothing for sixteen keys that are not there
+                if (16 * m >= keys) break;
                 if (m + 1 < NS) read(m + 1, part[m % 2 ^ 1]);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
@@ -242,6 +243,7 @@ __global__ __launch_bounds__(256, KD == 64 ? 3 : KD == 128 ? 2 : 1) void AttendK
                 read(0, part[0]);
 #pragma unroll
                 for (int m = 0; m < NS; ++m) {
+                    if (16 * m >= keys) break;
                     if (m + 1 < NS) read(m + 1, part[m % 2 ^ 1]);
 #pragma unroll
                     for (int sb = 0; sb < 4; ++sb) {
@@ -317,7 +319,7 @@ __global__ __launch_bounds__(256, KD == 64 ? 3 : KD == 128 ? 2 : 1) void AttendK
 #pragma unroll
             for (int n = 0; n < NS; ++n) s[n] *= all;
             const float *const from = vs + 4 * quarter * VP + state_col(), *const at = ks + 4 * quarter * KP + lane % 16;
-            constexpr int N = NS < 8 ? NS : 8;  // accumulators between the reads
+            constexpr int N = 4;  // accumulators between the reads
 #pragma unroll
             for (int sb = 0; sb < 4; ++sb) {
                 if (16 * sb >= here) break;
@@ -327,6 +329,7 @@ __global__ __launch_bounds__(256, KD == 64 ? 3 : KD == 128 ? 2 : 1) void AttendK
                 for (int e = 0; e < 4; ++e) v[e] = from[(16 * sb + e) * VP] * end[e];
 #pragma unroll
                 for (int n0 = 0; n0 < NS; n0 += N) {
+                    if (16 * n0 >= keys) break;
                     float k[4][N];
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
