@@ -201,7 +201,7 @@ __device__ __forceinline__ double AttendStep(const AttendArgs& p, const AttendRu
     return t + 1 < length ? AttendDecay(p, b, h, t + 1) : 0;
 }
 
-// How the time axis is cut: into segments of whole tiles, four at least, of the number that costs least.  Costs are in a tile's time with the compute units full (`resident` workgroups to each):
+// How the time axis is cut: into segments of whole tiles, two at least, of the number that costs least.  Costs are in a tile's time with the compute units full (`resident` workgroups to each):
 // a round of workgroups takes a segment's tiles and three more for what comes before and behind them, six tenths of that where there is a workgroup to a compute unit at most and between them in
 // proportion; segments need the states that they start from first, which takes 0.4 of a tile each, and a pass over the states.  Of a padded batch half of the workgroups are taken to have work.
 // `blocks`: workgroups to a head and segment; `states`: those of the states alone.
@@ -217,7 +217,7 @@ inline void CutAttend(AttendArgs* p, bool padded, int64_t blocks, int64_t states
     };
     int64_t best = 1;
     double least = 0;
-    for (int64_t n = 1; n <= std::max<int64_t>(1, std::min<int64_t>(tiles / 4, 64)); ++n) {
+    for (int64_t n = 1; n <= std::max<int64_t>(1, std::min<int64_t>(tiles / 2, 64)); ++n) {
         const int64_t each = (tiles + n - 1) / n;
         double cost = rounds(heads * blocks * n, units * resident) * static_cast<double>(each + 3);
         if (n > 1) cost += rounds(heads * states * (n - 1), units * 4) * (0.4 * static_cast<double>(each) + 2) + 0.6 + static_cast<double>(heads * n * matrix) * 3e-7;
