@@ -125,6 +125,25 @@ def test_layer_norm_means_of_float16_are_those_of_its_values(chx, cols):
     assert (np.abs(state.mean.get() - want) <= 2.0 ** -19.5 / cols ** 0.5 + 2.0 ** -23 * np.abs(want)).all()
 
 
+@pytest.mark.parametrize('rows,cols,dtype', [(20003, 64, 'float16'), (9001, 600, 'float16'), (4099, 2500, 'float16'), (300, 5, 'float32'), (3, 20001, 'float32')])
+def test_layer_norm_keeps_to_the_row(chx, rows, cols, dtype):
+    """A row with an infinity or NaN is NaN; those that are taken with it are as without it."""
+    x, gamma, beta, gy = norm_case(rows, cols, dtype, dtype)
+    args = [up(chx, a) for a in (gamma, beta)]
+    y, state = chx.layer_norm(up(chx, x), *args)
+    gx = chx.layer_norm_grad(up(chx, x), args[0], up(chx, gy), state)[0].get()
+    bad = x.copy()
+    touched = [0, rows // 2, rows - 1] if rows > 3 else [1]
+    for n, row in enumerate(touched):
+        bad[row, n * 7 % cols] = (np.inf, np.nan, -np.inf)[n]
+    y2, state2 = chx.layer_norm(up(chx, bad), *args)
+    gx2 = chx.layer_norm_grad(up(chx, bad), args[0], up(chx, gy), state2)[0].get()
+    others = np.setdiff1d(np.arange(rows), touched)
+    for got, want in ((y2.get(), y.get()), (state2.mean.get(), state.mean.get()), (state2.inv_std.get(), state.inv_std.get()), (gx2, gx)):
+        assert np.array_equal(got[others], want[others])
+    assert np.isnan(y2.get()[touched]).all() and np.isnan(gx2[touched]).all()
+
+
 def test_layer_norm_gradients_against_differences(chx):
     """In float64: central differences of sum(y * gy), whose error is h^2 / 6 of the third derivative (of order 1 here) and 2^-53 of the sum (of order 20) over h."""
     x, gamma, beta, gy = norm_case(3, 11, 'float64', 'float64')
@@ -263,6 +282,23 @@ def test_linear_attention_keeps_what_comes_before_an_infinity(chx, length, dtype
             # elsewhere as without it; a tile that has one goes row by row, in another order
             limit = 2 * far + (np.finfo(dtype).eps * ab_of(want) if got is y else 0)
             assert (np.abs(got - want) <= limit + 1e-7)[~at].all(), name
+
+
+@pytest.mark.parametrize('dtype', ['float16', 'float32'])
+@pytest.mark.parametrize('length', [5, 100, 900])
+def test_linear_attention_of_a_state_that_is_not_finite(chx, length, dtype):
+    """An infinity or NaN in a state stays in its column of values, its head and its sequence, whatever power of two the others are counted in."""
+    c = attend_case((2, length, 2, 1, 40, 70), dtype)
+    args, decay = [up(chx, c[k]) for k in ('q', 'k', 'v')], up(chx, c['log_decay'])
+    plain, plain_new = (x.get() for x in chx.linear_attention(*args, decay, state=up(chx, c['state'])))
+    for value in (np.inf, np.nan):
+        state = c['state'].copy()
+        state[1, 0, 7, 17] = value
+        y, new = (x.get() for x in chx.linear_attention(*args, decay, state=up(chx, state)))
+        touched, touched_new = np.zeros(y.shape, bool), np.zeros(new.shape, bool)
+        touched[1, :, 0, 17] = touched_new[1, 0, :, 17] = True
+        assert not np.isfinite(new[1, 0, 7, 17]) and not np.isfinite(y[1, 0, 0, 17])
+        assert np.array_equal(y[~touched], plain[~touched]) and np.array_equal(new[~touched_new], plain_new[~touched_new])
 
 
 def ab_of(x):
@@ -562,6 +598,28 @@ def test_linear_attention_of_strides_that_repeat_and_run_backwards(chx, length, 
         odd = [chx.ndarray(a._buf, a._offset, a.shape, (a.strides[0], far) + a.strides[2:], a.dtype) for a in (q, k, v)]
         for got, w in zip(chx.linear_attention(*odd), want):
             assert np.array_equal(got.get(), w.get())
+
+
+@pytest.mark.parametrize('seed', range(16))
+def test_layers_of_drawn_sizes(chx, seed):
+    """Any widths, lengths, heads and shares, padded and not, in both types; rows of any number and width."""
+    rng = np.random.default_rng(1000 + seed)
+    share = int(rng.choice([1, 1, 2, 3]))
+    sizes = (int(rng.integers(1, 4)), int(np.exp(rng.uniform(0, np.log(420)))), share * int(rng.integers(1, 3)), share, int(rng.integers(1, 257)), int(rng.integers(1, 257)))
+    dtype, ragged, decay = ('float16', 'float32')[seed % 2], bool(rng.integers(2)), (None, 'rows', 'heads')[int(rng.integers(3))]
+    c = attend_case(sizes, dtype, seed=seed, ragged=ragged, decay=decay)
+    if decay is None:
+        c['v'] = c['v'] * np.asarray(0.1, dtype)
+    check_attend(chx, c, (lambda a: apart(chx, a)) if rng.integers(2) else (lambda a: up(chx, a)), None, bool(rng.integers(2)), bool(rng.integers(2)), '%s %s' % (sizes, dtype))
+    rows, cols = int(np.exp(rng.uniform(0, np.log(3000)))), int(np.exp(rng.uniform(0, np.log(9000))))
+    x, gamma, beta, gy = norm_case(rows, cols, dtype, 'float32', seed=seed)
+    y, state = chx.layer_norm(apart(chx, x, 5), up(chx, gamma), up(chx, beta))
+    want, off = ref.layer_norm(x, gamma, beta, 2e-5)
+    for name, got in (('y', y), ('mean', state.mean), ('inv_std', state.inv_std)):
+        ref.assert_off(got.get(), want[name], off[name], '%d x %d %s' % (rows, cols, name))
+    want, off = ref.layer_norm_grad(x, gamma, gy, 2e-5)
+    for name, got in zip(('gx', 'ggamma', 'gbeta'), chx.layer_norm_grad(up(chx, x), up(chx, gamma), apart(chx, gy, 2), state)):
+        ref.assert_off(got.get(), want[name].reshape(got.shape), off[name].reshape(got.shape), '%d x %d %s' % (rows, cols, name))
 
 
 # ---------------------------------------------------------------------------------------------
