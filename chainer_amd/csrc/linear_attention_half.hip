@@ -82,7 +82,7 @@ struct AttendHalfLds {
 // and 43 for the states of its 16 segments; on the float pipe 1.1 ms.  Gradients of 4 x 2048 rows, 16 heads of 128 x 128, three passes: 220 us.
 // GRAD: what the passes of the gradients have beyond the forward one.
 template <int KD, bool OUT, int WIDTHS, bool GRAD>
-__global__ __launch_bounds__(256, KD == 256 ? 1 : 2) void AttendHalfKernel(AttendArgs p) {
+__global__ __launch_bounds__(256, KD == 256 ? 1 : KD == 128 ? 2 : 3) void AttendHalfKernel(AttendArgs p) {
     using T = half_t;
     constexpr bool EVEN = WIDTHS == kAttendWhole;
     using Lds = AttendHalfLds<KD, OUT>;
