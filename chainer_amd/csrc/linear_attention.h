@@ -202,17 +202,17 @@ __device__ __forceinline__ double AttendStep(const AttendArgs& p, const AttendRu
 }
 
 // How the time axis is cut: into segments of whole tiles, two at least, of the number that costs least.  Costs are in a tile's time with the compute units full (`resident` workgroups to each):
-// a round of workgroups takes a segment's tiles and three more for what comes before and behind them, six tenths of that where there is a workgroup to a compute unit at most and between them in
-// proportion; segments need the states that they start from first, which takes 0.4 of a tile each, and a pass over the states.  Of a padded batch half of the workgroups are taken to have work.
+// a round of workgroups takes a segment's tiles and three more for what comes before and behind them, `alone` (float16 0.85, float32 0.6) of that where there is a workgroup to a compute unit at most
+// and between them in proportion; segments need the states that they start from first, which takes 0.4 of a tile each, and a pass over the states.  Of a padded batch half of the workgroups are taken to have work.
 // `blocks`: workgroups to a head and segment; `states`: those of the states alone.
 // One sequence of 16384 rows, 16 heads of 128 x 128 in float16, in 8, 16, 24 and 48 segments: 179, 141, 154 and 170 us, and 16 are taken; 20 padded ones of up to 777, 13 heads of 50 x 50 in
-// float32, in 1, 2 and 3: 114, 110 and 95, and 3 are taken.
-inline void CutAttend(AttendArgs* p, bool padded, int64_t blocks, int64_t states, int64_t resident, int64_t matrix) {
+// float32, in 1, 2 and 3: 114, 110 and 95, and 3 are taken; 9 of 2533, 11 heads of 100 x 100 in float16, in 1, 2, 5 and 8: 186, 178, 161 and 179, and 5 are taken.
+inline void CutAttend(AttendArgs* p, double alone, bool padded, int64_t blocks, int64_t states, int64_t resident, int64_t matrix) {
     const int64_t tiles = (p->length + kAttendTile - 1) / kAttendTile, heads = p->batch * p->heads, units = NumCUs();
     const auto rounds = [&](int64_t workgroups, int64_t at_once) {
         if (padded) workgroups = (workgroups + 1) / 2;
         const int64_t rest = workgroups % at_once;
-        const double part = at_once > units ? 0.6 + 0.4 * static_cast<double>(std::max<int64_t>(0, rest - units)) / static_cast<double>(at_once - units) : 1;
+        const double part = at_once > units ? alone + (1 - alone) * static_cast<double>(std::max<int64_t>(0, rest - units)) / static_cast<double>(at_once - units) : 1;
         return static_cast<double>(workgroups / at_once) + (rest == 0 ? 0 : part);
     };
     int64_t best = 1;
@@ -231,7 +231,7 @@ inline void CutAttend(AttendArgs* p, bool padded, int64_t blocks, int64_t states
 struct AttendCall {
     AttendArgs p{};
     AttendRows q, k, v;
-    int keys, values, key_heads;
+    int keys, values, key_heads, dtype;
     const float* state;
 };
 bool AttendSizesOf(const hipcx_array* q, const hipcx_array* v, AttendCall* c);
@@ -267,6 +267,7 @@ void VisitWidths(AttendWidths widths, bool grad, F&& f) {
     else grad ? f(std::integral_constant<int, kAttendPart>{}, std::true_type{}) : f(std::integral_constant<int, kAttendPart>{}, std::false_type{});
 }
 
+inline double AttendAlone(int dtype) { return dtype == HIPCX_FLOAT16 ? 0.85 : 0.6; }
 // Workgroups that a compute unit holds, as registers and LDS let them.
 inline int64_t AttendResident(int keys) { return keys <= 64 ? 3 : keys <= 128 ? 2 : 1; }
 

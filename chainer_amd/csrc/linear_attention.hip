@@ -626,7 +626,7 @@ bool AttendSizesOf(const hipcx_array* q, const hipcx_array* v, AttendCall* c) {
     if (q->shape[0] < 0 || q->shape[1] < 0 || q->shape[1] >= (int64_t{1} << 30) || kh < 1 || h < 1 || h >= (1 << 20) || h % kh != 0) return false;
     if (q->shape[3] < 1 || q->shape[3] > kMaxAttend || v->shape[3] < 1 || v->shape[3] > kMaxAttend || q->shape[0] > kBlocksPerLaunch / h) return false;
     c->p.batch = q->shape[0], c->p.length = q->shape[1], c->p.heads = static_cast<int>(h);
-    c->keys = static_cast<int>(q->shape[3]), c->values = static_cast<int>(v->shape[3]), c->key_heads = static_cast<int>(kh);
+    c->keys = static_cast<int>(q->shape[3]), c->values = static_cast<int>(v->shape[3]), c->key_heads = static_cast<int>(kh), c->dtype = q->dtype;
     return true;
 }
 
@@ -678,7 +678,7 @@ constexpr int kAttendTokens = 8;
 
 void CutForward(AttendCall* c, bool padded) {
     if (c->p.length <= kAttendTokens) c->p.segments = 1, c->p.segment_rows = kAttendTile;
-    else CutAttend(&c->p, padded, AttendBlocks(c->values), AttendBlocks(c->values), AttendResident(c->keys), static_cast<int64_t>(c->keys) * c->values);
+    else CutAttend(&c->p, AttendAlone(c->dtype), padded, AttendBlocks(c->values), AttendBlocks(c->values), AttendResident(c->keys), static_cast<int64_t>(c->keys) * c->values);
 }
 
 size_t ForwardWorkspace(const AttendCall& c) {
