@@ -207,9 +207,9 @@ SIGNATURES = {
     'hipcx_selective_scan': (_INT, [_A] * 8 + [_INT] + [_A] * 4 + [_V, _SZ, _V]),
     'hipcx_selective_scan_grad_workspace_size': (_SZ, [_A, _A, _A]),
     'hipcx_selective_scan_grad': (_INT, [_A] * 8 + [_INT] + [_A] * 13 + [_V, _SZ, _V]),
-    'hipcx_linear_attention_workspace_size': (_SZ, [_A, _A]),
+    'hipcx_linear_attention_workspace_size': (_SZ, [_A, _A, _A]),
     'hipcx_linear_attention': (_INT, [_A] * 4 + [ctypes.c_double] + [_A] * 4 + [_V, _SZ, _V]),
-    'hipcx_linear_attention_grad_workspace_size': (_SZ, [_A, _A, _A]),
+    'hipcx_linear_attention_grad_workspace_size': (_SZ, [_A, _A, _A, _A]),
     'hipcx_linear_attention_grad': (_INT, [_A] * 4 + [ctypes.c_double] + [_A] * 9 + [_V, _SZ, _V]),
     'hipcx_layer_norm': (_INT, [_A] * 3 + [ctypes.c_double] + [_A] * 3 + [_V]),
     'hipcx_layer_norm_grad_workspace_size': (_SZ, [_A]),

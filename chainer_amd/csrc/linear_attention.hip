@@ -621,7 +621,7 @@ AttendRows AttendRowsOf(const hipcx_array* a, int heads, const std::string& what
 }  // namespace
 
 bool AttendSizesOf(const hipcx_array* q, const hipcx_array* v, AttendCall* c) {
-    if (q == nullptr || v == nullptr || q->ndim != 4 || v->ndim != 4 || q->shape[0] != v->shape[0] || q->shape[1] != v->shape[1]) return false;
+    if (q == nullptr || v == nullptr || (q->dtype != HIPCX_FLOAT16 && q->dtype != HIPCX_FLOAT32) || q->ndim != 4 || v->ndim != 4 || q->shape[0] != v->shape[0] || q->shape[1] != v->shape[1]) return false;
     const int64_t kh = q->shape[2], h = v->shape[2];
     if (q->shape[0] < 0 || q->shape[1] < 0 || q->shape[1] >= (int64_t{1} << 30) || kh < 1 || h < 1 || h >= (1 << 20) || h % kh != 0) return false;
     if (q->shape[3] < 1 || q->shape[3] > kMaxAttend || v->shape[3] < 1 || v->shape[3] > kMaxAttend || q->shape[0] > kBlocksPerLaunch / h) return false;
@@ -693,15 +693,11 @@ using namespace hipcx;
 
 extern "C" {
 
-size_t hipcx_linear_attention_workspace_size(const hipcx_array* q, const hipcx_array* v) {
+size_t hipcx_linear_attention_workspace_size(const hipcx_array* q, const hipcx_array* v, const hipcx_array* lengths) {
     AttendCall c;
     if (!AttendSizesOf(q, v, &c)) return 0;
-    size_t bytes = 0;
-    for (const bool padded : {false, true}) {
-        CutForward(&c, padded);
-        bytes = std::max(bytes, ForwardWorkspace(c));
-    }
-    return bytes;
+    CutForward(&c, lengths != nullptr);
+    return ForwardWorkspace(c);
 }
 
 int hipcx_linear_attention(const hipcx_array* q, const hipcx_array* k, const hipcx_array* v, const hipcx_array* log_decay, double scale, const hipcx_array* state,

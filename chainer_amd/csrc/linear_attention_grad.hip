@@ -129,15 +129,11 @@ using namespace hipcx;
 
 extern "C" {
 
-size_t hipcx_linear_attention_grad_workspace_size(const hipcx_array* q, const hipcx_array* v, const hipcx_array* log_decay) {
+size_t hipcx_linear_attention_grad_workspace_size(const hipcx_array* q, const hipcx_array* v, const hipcx_array* log_decay, const hipcx_array* lengths) {
     AttendCall c;
     if (!AttendSizesOf(q, v, &c)) return 0;
-    size_t bytes = 0;
-    for (const bool padded : {false, true}) {
-        CutGrad(&c, padded);
-        bytes = std::max(bytes, GradWorkspace(c, log_decay != nullptr, log_decay != nullptr && log_decay->ndim == 1).bytes);
-    }
-    return bytes;
+    CutGrad(&c, lengths != nullptr);
+    return GradWorkspace(c, log_decay != nullptr, log_decay != nullptr && log_decay->ndim == 1).bytes;
 }
 
 int hipcx_linear_attention_grad(const hipcx_array* q, const hipcx_array* k, const hipcx_array* v, const hipcx_array* log_decay, double scale, const hipcx_array* state,

@@ -192,7 +192,7 @@ HOST_FN(LinearAttention) {
     const int64_t of_state[4] = {queries->d.shape[0], values->d.shape[2], queries->d.shape[3], values->d.shape[3]};
     Ref new_state = Given(arg[7]) ? NewRef(AsArray(arg[7], "out_state")) : Empty(4, of_state, HIPCX_FLOAT32);
     Ref y = EmptyLike(values, values->d.dtype);
-    Workspace scratch(hipcx_linear_attention_workspace_size(q.d(), v.d()));
+    Workspace scratch(hipcx_linear_attention_workspace_size(q.d(), v.d(), Descriptor(lengths)));
     void* stream = Stream();
     Call([&] {
         return hipcx_linear_attention(q.d(), k.d(), v.d(), Descriptor(decay), scale, state.d(), Descriptor(lengths), y.d(), new_state.d(), scratch.ptr, scratch.bytes, stream);
@@ -213,7 +213,7 @@ HOST_FN(LinearAttentionGrad) {
     const double scale = ScaleOf(arg[5], queries);
     Ref state = ContiguousOrNone(first), gnew = ContiguousOrNone(Optional(arg[8], "gnew_state"));
     Ref gq = EmptyLikeOrNone(queries), gk = EmptyLikeOrNone(keys), gv = EmptyLikeOrNone(values), gdecay = EmptyLikeOrNone(decay), gstate = EmptyLikeOrNone(first);
-    Workspace scratch(hipcx_linear_attention_grad_workspace_size(q.d(), v.d(), Descriptor(decay)));
+    Workspace scratch(hipcx_linear_attention_grad_workspace_size(q.d(), v.d(), Descriptor(decay), Descriptor(lengths)));
     void* stream = Stream();
     Call([&] {
         return hipcx_linear_attention_grad(q.d(), k.d(), v.d(), Descriptor(decay), scale, state.d(), Descriptor(lengths), gy.d(), gnew.d(), gq.d(), gk.d(), gv.d(), gdecay.d(),

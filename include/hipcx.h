@@ -513,11 +513,11 @@ int hipcx_selective_scan_grad(const hipcx_array* u, const hipcx_array* delta, co
  * hipcx_linear_attention_grad: from gy and gnew_state (or NULL, zeros) the gradients of q, k, v, and of log_decay (in its shape, C-contiguous) and state (C-contiguous), which may be NULL.
  *   Those of log_decay are differences of q gq and k gk summed up from the last row of a segment, in 64 bits.  All sums run in an order that depends on the sizes, and on whether there are lengths, alone.  The workspace holds, for
  *   key heads that are shared, every head's gradients of q and k in float32, with log_decay some 16 bytes a row, head and 64 keys, and where time is cut two states a segment and head. */
-size_t hipcx_linear_attention_workspace_size(const hipcx_array* q, const hipcx_array* v);
+size_t hipcx_linear_attention_workspace_size(const hipcx_array* q, const hipcx_array* v, const hipcx_array* lengths);
 int hipcx_linear_attention(const hipcx_array* q, const hipcx_array* k, const hipcx_array* v, const hipcx_array* log_decay, double scale,
                            const hipcx_array* state, const hipcx_array* lengths, const hipcx_array* y, const hipcx_array* new_state, void* workspace,
                            size_t workspace_bytes, void* stream);
-size_t hipcx_linear_attention_grad_workspace_size(const hipcx_array* q, const hipcx_array* v, const hipcx_array* log_decay);
+size_t hipcx_linear_attention_grad_workspace_size(const hipcx_array* q, const hipcx_array* v, const hipcx_array* log_decay, const hipcx_array* lengths);
 int hipcx_linear_attention_grad(const hipcx_array* q, const hipcx_array* k, const hipcx_array* v, const hipcx_array* log_decay, double scale,
                                 const hipcx_array* state, const hipcx_array* lengths, const hipcx_array* gy, const hipcx_array* gnew_state,
                                 const hipcx_array* gq, const hipcx_array* gk, const hipcx_array* gv, const hipcx_array* glog_decay, const hipcx_array* gstate,

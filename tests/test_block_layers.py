@@ -154,15 +154,17 @@ def test_linear_attention_workspaces():
     from chainer_amd import _lib
     lib = _lib.load()
 
-    def sizes(q, v, decay=True):
-        q, v = described(q), described(v)
-        g = ctypes.byref(described((v.shape[0], v.shape[1], v.shape[2]))) if decay else None
-        return lib.hipcx_linear_attention_workspace_size(ctypes.byref(q), ctypes.byref(v)), lib.hipcx_linear_attention_grad_workspace_size(ctypes.byref(q), ctypes.byref(v), g)
+    def sizes(q, v, decay=True, padded=False, dtype=F32):
+        q, v = described(q, dtype), described(v, dtype)
+        g, n = ctypes.byref(described((v.shape[0], v.shape[1], v.shape[2]))) if decay else None, ctypes.byref(described((v.shape[0],), I32)) if padded else None
+        return (lib.hipcx_linear_attention_workspace_size(ctypes.byref(q), ctypes.byref(v), n), lib.hipcx_linear_attention_grad_workspace_size(ctypes.byref(q), ctypes.byref(v), g, n))
 
     assert sizes((128, 1, 16, 128), (128, 1, 16, 128))[0] == 0  # next tokens take none
     forward, grad = sizes((1, 16384, 16, 128), (1, 16384, 16, 128))
     assert forward % (16 * 4 * (128 * 128 + 1)) == 0 and forward > 0  # (segments are counted for each by itself)
     assert sizes((1, 16384, 16, 128), (1, 16384, 16, 128), False)[1] < grad < sizes((1, 16384, 4, 128), (1, 16384, 16, 128))[1]
+    assert sizes((1, 16384, 16, 128), (1, 16384, 16, 128), padded=True)[0] % (16 * 4 * (128 * 128 + 1)) == 0
+    assert sizes((1, 16384, 16, 128), (1, 16384, 16, 128), dtype=F64) == (0, 0)
     for q, v in (((2, 70, 2, 257), (2, 70, 4, 10)), ((2, 70, 2, 6), (2, 70, 3, 10)), ((2, 70, 2, 6), (2, 71, 4, 10)), ((70, 2, 6), (2, 70, 4, 10)), ((2, 1 << 30, 2, 6), (2, 1 << 30, 4, 10))):
         assert sizes(q, v) == (0, 0)
 
