@@ -144,6 +144,18 @@ def test_layer_norm_keeps_to_the_row(chx, rows, cols, dtype):
     assert np.isnan(y2.get()[touched]).all() and np.isnan(gx2[touched]).all()
 
 
+@pytest.mark.parametrize('rows,cols,dtype', [(40, 5, 'float16'), (9, 70, 'float32'), (20001, 100, 'float16'), (4099, 2500, 'float16'), (7, 4100, 'float32'), (3, 40000, 'float16')])
+def test_layer_norm_in_place(chx, rows, cols, dtype):
+    """y may be x, for which the routine has no argument: the entry itself."""
+    x, gamma, beta, _ = norm_case(rows, cols, dtype, 'float32')
+    want, state = chx.layer_norm(up(chx, x), up(chx, gamma), up(chx, beta))
+    a, g, b, mean, inv = up(chx, x), up(chx, gamma), up(chx, beta), chx.zeros((rows,)), chx.zeros((rows,))
+    chx._lib.call('hipcx_layer_norm', a.desc(), g.desc(), b.desc(), 2e-5, a.desc(), mean.desc(), inv.desc(), None)
+    chx.synchronize()
+    for got, w in ((a, want), (mean, state.mean), (inv, state.inv_std)):
+        assert np.array_equal(got.get(), w.get())
+
+
 def test_layer_norm_gradients_against_differences(chx):
     """In float64: central differences of sum(y * gy), whose error is h^2 / 6 of the third derivative (of order 1 here) and 2^-53 of the sum (of order 20) over h."""
     x, gamma, beta, gy = norm_case(3, 11, 'float64', 'float64')
