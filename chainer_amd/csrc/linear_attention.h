@@ -130,7 +130,6 @@ struct AttendDecays {
     alignas(16) float high[kAttendTile], low[kAttendTile];
     float end[kAttendTile];  // from a row to the tile's end, as a factor, times kv_scale
     float near[kAttendTile]; // from a row to the last of its sixteen, as a factor
-    float step[kAttendTile]; // a row's own, as a factor
     float all;               // the tile's
     double sum;              // the tile's, in powers of two
 };
@@ -178,7 +177,6 @@ __device__ __forceinline__ void SumDecays(AttendDecays* to, double g, int here, 
     to->high[lane] = high, to->low[lane] = static_cast<float>(sum - high);
     to->end[lane] = lane < here ? __builtin_amdgcn_exp2f(static_cast<float>(all - sum)) * kv_scale : 0.f;
     to->near[lane] = __builtin_amdgcn_exp2f(static_cast<float>(OfLaneInRow<15>(sum) - sum));
-    to->step[lane] = __builtin_amdgcn_exp2f(static_cast<float>(g));
     if (lane == 0) to->all = __builtin_amdgcn_exp2f(static_cast<float>(all)), to->sum = all;
 }
 
@@ -192,14 +190,6 @@ struct AttendSpan {
         end = end < first ? first : end;
     }
 };
-
-// The row of the sequence that a pass takes as its row r of the segment, and the row whose decay takes the state there (-1: none).
-__device__ __forceinline__ int64_t AttendRowOf(const AttendSpan& s, int back, int64_t r) { return back ? s.end - 1 - r : s.first + r; }
-__device__ __forceinline__ double AttendStep(const AttendArgs& p, const AttendRun& run, const AttendSpan& s, int64_t b, int h, int64_t length, int64_t r) {
-    const int64_t t = AttendRowOf(s, run.back, r);
-    if (!run.back) return AttendDecay(p, b, h, t);
-    return t + 1 < length ? AttendDecay(p, b, h, t + 1) : 0;
-}
 
 // How the time axis is cut: into segments of whole tiles, two at least, of the number that costs least.  Costs are in a tile's time with the compute units full (`resident` workgroups to each):
 // a round of workgroups takes a segment's tiles and three more for what comes before and behind them, `alone` (float16 0.85, float32 0.6) of that where there is a workgroup to a compute unit at most
