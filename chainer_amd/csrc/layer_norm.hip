@@ -547,14 +547,16 @@ int64_t PitchOf(const hipcx_array* x, const char* what) {
     if (TotalSize(x) == 0) return x->shape[last];
     HIPCX_REQUIRE(x->shape[last] == 1 || x->strides[last] == it, HIPCX_DIMENSION_ERROR, std::string("layer_norm: ") + what + " must have a dense last axis");
     int64_t pitch = 0, expect = 0;
+    bool seen = false;  // an inner axis (of a stride of 0, perhaps)
     for (int i = last - 1; i >= 0; --i) {
         if (x->shape[i] == 1) continue;
-        if (expect == 0) {
+        if (!seen) {
             HIPCX_REQUIRE(x->strides[i] % it == 0, HIPCX_DIMENSION_ERROR, std::string("layer_norm: strides of ") + what + " must be whole elements");
             pitch = x->strides[i] / it;
         } else {
             HIPCX_REQUIRE(x->strides[i] == expect, HIPCX_DIMENSION_ERROR, std::string("layer_norm: rows of ") + what + " must be equally far apart");
         }
+        seen = true;
         expect = x->strides[i] * x->shape[i];
     }
     return pitch;

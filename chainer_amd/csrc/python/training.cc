@@ -15,9 +15,11 @@ Ref EvenRows(Array* a) {
     if (last < 0 || Size(a) == 0) return NewRef(a);
     bool even = a->d.shape[last] == 1 || a->d.strides[last] == it;
     int64_t expect = 0;
+    bool seen = false;  // an inner axis (of a stride of 0, perhaps)
     for (int i = last - 1; i >= 0 && even; --i) {
         if (a->d.shape[i] == 1) continue;
-        even = expect == 0 ? a->d.strides[i] % it == 0 : a->d.strides[i] == expect;
+        even = seen ? a->d.strides[i] == expect : a->d.strides[i] % it == 0;
+        seen = true;
         expect = a->d.strides[i] * a->d.shape[i];
     }
     return even ? NewRef(a) : CopyOf(a, a->d.dtype);
