@@ -9,6 +9,7 @@
 // So one kernel does all of them (AttendRun).
 #pragma once
 
+#include "attend_decay_row.h"
 #include "sequence.h"
 
 namespace hipcx {

@@ -113,9 +113,8 @@ __global__ __launch_bounds__(256, KD == 64 ? 3 : KD == 128 ? 2 : 1) void AttendK
     const int y_row = OUT ? way * static_cast<int>(run.y.row) : 0;
     const float* dp = with_dots ? static_cast<const float*>(run.dot.data) + b * run.dot.batch + (h / run.dot.share) * run.dot.head + row0 * run.dot.row + col0 : nullptr;
     const int d_row = with_dots ? way * static_cast<int>(run.dot.row) : 0;
-    const float* gp = p.decay != nullptr ? p.decay + b * p.decay_batch + h * p.decay_head + (row0 + (back ? 1 : 0)) * p.decay_row : nullptr;
-    const int64_t g_row = way * p.decay_row;
-    const int64_t g_rows = back && span.end == length ? 1 : 0;  // the first row has no decay: none follows it
+    const float* gp = p.decay != nullptr ? p.decay + b * p.decay_batch + h * p.decay_head : nullptr;
+    const int64_t g_rows = AttendNoDecay(span.end, length, back);
     AttendPiece<float, 4> k_next[NK], v_next[NV], q_next[OUT ? NS : 1];
     const auto placed = [&](const AttendPiece<float, 4>& piece, int col, int end) {
         const AttendPiece<float, 4> there = AttendPlace<WIDTHS>(piece, col, end);
@@ -139,10 +138,9 @@ __global__ __launch_bounds__(256, KD == 64 ? 3 : KD == 128 ? 2 : 1) void AttendK
     };
     // Log decays, by one wave, a lane to a row: summed up a tile ahead, on their way two tiles ahead, so that nothing waits for what was asked for in the same tile.
     float g_now = 0, g_next = 0;
+    const auto decay_at = [&](int64_t r) { return gp[AttendDecayRow(span.first, span.end, length, back, r) * p.decay_row]; };
     const auto load_decays = [&](int64_t r0) {  // of a row that is there; sum_decays takes those that count
-        if (gp == nullptr) return;
-        const int64_t r = r0 + lane < rows ? r0 + lane : rows - 1;
-        g_next = gp[(r < g_rows ? g_rows : r) * g_row * (rows > g_rows ? 1 : 0)];
+        if (gp != nullptr) g_next = decay_at(r0 + lane);
     };
     const auto sum_decays = [&](int64_t r0, AttendDecays* to) {
         const int here = static_cast<int>(rows - r0 < C ? rows - r0 : C);
@@ -360,7 +358,7 @@ __global__ __launch_bounds__(256, KD == 64 ? 3 : KD == 128 ? 2 : 1) void AttendK
             const float* const k = static_cast<const float*>(run.k.data) + b * run.k.batch + (h / run.k.share) * run.k.head + row * run.k.row;
             const float* const x = static_cast<const float*>(run.q.data) + b * run.q.batch + (h / run.q.share) * run.q.head + row * run.q.row;
             const float* const of_v = static_cast<const float*>(run.v.data) + b * run.v.batch + (h / run.v.share) * run.v.head + row * run.v.row + col0;
-            const float step = gp != nullptr && r0 >= g_rows ? __builtin_amdgcn_exp2f(static_cast<float>(LogOfDecay(gp[r0 * g_row]))) : 1.f, v = j < cols ? of_v[j] * kv_scale : 0.f;
+            const float step = gp != nullptr && r0 >= g_rows ? __builtin_amdgcn_exp2f(static_cast<float>(LogOfDecay(decay_at(r0)))) : 1.f, v = j < cols ? of_v[j] * kv_scale : 0.f;
             float y = 0;
             for (int i = wave * (KD / 4); i < (wave + 1) * (KD / 4) && i < keys; ++i) {
                 const float now = ss[j * KP + i] * step + k[i] * v;

@@ -1,0 +1,35 @@
+"""Linear attention on the device where a segment, a row or a number is an extreme one, against plain forms (block_reference.py)."""
+import numpy as np
+import pytest
+
+import block_reference as ref
+from test_gpu_block_layers import attend_case, check_attend, chx, up  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize('dtype', ['float16', 'float32'])
+@pytest.mark.parametrize('length,heads', [(1, 1), (1, 3), (2, 1), (65, 2), (129, 1), (385, 1), (385, 2), (769, 1), (769, 4), (1153, 2)])
+def test_gradients_of_a_sequence_whose_last_row_is_a_segment(chx, length, heads, dtype):  # noqa: F811
+    """Time is cut into segments of whole tiles, so that one may hold a last row alone, which no decay follows: what lies behind the log decays has no part in it."""
+    c = attend_case((1, length, heads, 1, 64, 64), dtype, seed=length)
+    check_attend(chx, c, lambda a: up(chx, a), None, True, True, '%d rows %s' % (length, dtype))
+    args = [up(chx, c[k]) for k in ('q', 'k', 'v', 'gy')]
+    more = dict(state=up(chx, c['state']), gnew_state=up(chx, c['gnew']))
+    want = [g.get() for g in chx.linear_attention_grad(*args, up(chx, c['log_decay']), **more)]
+    for behind in (np.nan, np.inf, -3.0):
+        wide = np.full((1, length + 1, heads), behind, np.float32)
+        wide[:, :length] = c['log_decay']
+        for got, w in zip(chx.linear_attention_grad(*args, chx.array(wide)[:, :length], **more), want):
+            assert np.array_equal(got.get(), w)
+
+
+@pytest.mark.parametrize('dtype', ['float16', 'float32'])
+def test_gradients_of_padded_sequences_of_one_row(chx, dtype):  # noqa: F811
+    """The batch's log decays are not a number behind each sequence's only row."""
+    c = attend_case((5, 70, 2, 1, 20, 30), dtype, seed=2)
+    c['lengths'] = np.array([1, 70, 0, 65, 1], np.int32)
+    behind = np.arange(70) >= c['lengths'][:, None]
+    for k in ('q', 'k', 'v', 'gy', 'log_decay'):
+        c[k][behind] = np.nan
+    check_attend(chx, c, lambda a: up(chx, a), None, True, True, dtype)
