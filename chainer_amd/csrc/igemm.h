@@ -24,15 +24,19 @@ namespace hipcx {
 // Raises a kernel's dynamic LDS limit when a launch needs more than it has been given so far.  The limit is a property of the
 // function on one device; several host threads may launch the same kernel, so the bookkeeping is per kernel instantiation
 // (the Tag type), per device, and serialised (the reference serialises its launchers on a mutex too, CX/cuda/elementwise.cuh:38).
+// A tag that two kernels share would hide the second one's need behind the first one's: the call throws.
 template <typename Tag>
 void EnsureDynamicLds(const void* kernel, int lds_bytes) {
     constexpr int kMaxDevices = 64;
     static std::mutex mu;
+    static const void* of = nullptr;
     static int configured[kMaxDevices] = {};
     int dev = 0;
     HIPCX_CHECK_HIP(hipGetDevice(&dev));
     HIPCX_REQUIRE(dev >= 0 && dev < kMaxDevices, HIPCX_DEVICE_ERROR, "device index out of range");
     std::lock_guard<std::mutex> lock(mu);
+    if (of == nullptr) of = kernel;
+    HIPCX_REQUIRE(of == kernel, HIPCX_CHAINERX_ERROR, "a kernel's dynamic LDS is kept in the books of another one");
     if (lds_bytes > configured[dev]) {
         HIPCX_CHECK_HIP(hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, lds_bytes));
         configured[dev] = lds_bytes;

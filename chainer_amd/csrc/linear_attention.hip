@@ -7,8 +7,6 @@
 namespace hipcx {
 namespace {
 
-struct AttendTag {};
-
 // Tiles of 64 rows, one after another.  With G the decays summed up from the tile's first row and S the state before it,
 //   P[t][s] = exp(G[t] - G[s]) q[t] k[s] for s <= t,  y = P v + exp(G) q S,  S <- exp(G[63]) S + (exp(G[63] - G) k)^T v.
 // A workgroup of four waves has 64 columns of v: a wave has sixteen rows of y, and sixteen columns of S in its accumulators (a copy is in LDS, turned, for the products with q).
@@ -582,7 +580,8 @@ void LaunchAttend(const AttendArgs& args, int dtype, bool states_alone, hipStrea
         const auto kernel = [&](auto out, auto rows, auto grad) {
             constexpr int KD = decltype(kd)::value, kLds = AttendLds<KD, decltype(out)::value>::kBytes;
             void (*const k)(AttendArgs) = AttendKernel<KD, decltype(out)::value, decltype(rows)::value, decltype(grad)::value>;
-            EnsureDynamicLds<AttendTag>(reinterpret_cast<const void*>(k), kLds);
+            struct Tag {};  // a type of its own for every instantiation of this lambda
+            EnsureDynamicLds<Tag>(reinterpret_cast<const void*>(k), kLds);
             hipLaunchKernelGGL(k, dim3(static_cast<unsigned>(blocks)), dim3(256), kLds, stream, p);
             CheckLaunch("linear_attention");
         };

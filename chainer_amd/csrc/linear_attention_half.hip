@@ -5,8 +5,6 @@
 namespace hipcx {
 namespace {
 
-struct AttendHalfTag {};
-
 typedef short attend_short4_t __attribute__((ext_vector_type(4)));
 typedef _Float16 attend_half2_t __attribute__((ext_vector_type(2)));
 typedef _Float16 attend_half4_t __attribute__((ext_vector_type(4)));
@@ -617,7 +615,8 @@ void LaunchAttendHalf(const AttendArgs& p, int keys, int64_t blocks, bool states
         const auto kernel = [&](auto out, auto rows, auto grad) {
             constexpr int KD = decltype(kd)::value, kLds = AttendHalfLds<KD, decltype(out)::value>::kBytes;
             void (*const k)(AttendArgs) = AttendHalfKernel<KD, decltype(out)::value, decltype(rows)::value, decltype(grad)::value>;
-            EnsureDynamicLds<AttendHalfTag>(reinterpret_cast<const void*>(k), kLds);
+            struct Tag {};  // a type of its own for every instantiation of this lambda
+            EnsureDynamicLds<Tag>(reinterpret_cast<const void*>(k), kLds);
             hipLaunchKernelGGL(k, dim3(static_cast<unsigned>(blocks)), dim3(256), kLds, stream, p);
             CheckLaunch("linear_attention");
         };

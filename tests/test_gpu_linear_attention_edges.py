@@ -33,3 +33,12 @@ def test_gradients_of_padded_sequences_of_one_row(chx, dtype):  # noqa: F811
     for k in ('q', 'k', 'v', 'gy', 'log_decay'):
         c[k][behind] = np.nan
     check_attend(chx, c, lambda a: up(chx, a), None, True, True, dtype)
+
+
+@pytest.mark.parametrize('dtype', ['float16', 'float32'])
+def test_every_width_after_the_widest(chx, dtype):  # noqa: F811
+    """Each kernel has its own share of LDS raised, whatever another has had before: 256 keys first, then fewer, forms for whole and for odd widths, with gradients and without, states alone."""
+    for keys, values in ((256, 256), (256, 255), (128, 128), (128, 127), (127, 30), (64, 64), (63, 64), (3, 2)):
+        for length in (70, 1100):
+            c = attend_case((1, length, 1, 1, keys, values), dtype, seed=keys)
+            check_attend(chx, c, lambda a: up(chx, a), None, True, True, '%d rows, %d keys, %d values' % (length, keys, values))
