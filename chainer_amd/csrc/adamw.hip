@@ -258,15 +258,16 @@ extern "C" int hipcx_adamw_many(const hipcx_array* const* params, const hipcx_ar
         HIPCX_REQUIRE(beta1 >= 0 && beta1 < 1 && beta2 >= 0 && beta2 < 1, HIPCX_CHAINERX_ERROR, "adamw: beta1 and beta2 must be at least 0 and less than 1");
         HIPCX_REQUIRE(eps >= 0 && eps < HUGE_VAL, HIPCX_CHAINERX_ERROR, "adamw: eps must be finite and not negative");
         HIPCX_REQUIRE(std::isfinite(alpha) && std::isfinite(eta) && std::isfinite(weight_decay_rate), HIPCX_CHAINERX_ERROR, "adamw: alpha, eta and weight_decay_rate must be finite");
+        std::vector<Extent> extents;
+        extents.reserve(static_cast<size_t>(n) * 7 + 1);
         if (t_array != nullptr) {
             ValidateArray(t_array, "t");
             HIPCX_REQUIRE(t_array->dtype == HIPCX_INT64, HIPCX_DTYPE_ERROR, std::string("adamw: t is an int64 array, got ") + DtypeName(t_array->dtype));
             HIPCX_REQUIRE(TotalSize(t_array) == 1, HIPCX_DIMENSION_ERROR, "adamw: t is an array of one element, got shape " + ShapeStr(t_array));
+            extents.push_back({static_cast<const char*>(t_array->data), static_cast<const char*>(t_array->data) + sizeof(int64_t), false});
         } else {
             HIPCX_REQUIRE(t >= 1, HIPCX_CHAINERX_ERROR, "adamw: t counts steps from 1");
         }
-        std::vector<Extent> extents;
-        extents.reserve(static_cast<size_t>(n) * 7);
         for (int i = 0; i < n; ++i) {
             const hipcx_array *p = params[i], *g = grads[i], *m = ms[i], *v = vs[i], *m_scale = m_scales[i], *v_scale = v_scales[i], *master = masters[i];
             const auto require = [&](const hipcx_array* a, const char* what, std::initializer_list<int> dtypes, bool written) {
@@ -307,7 +308,7 @@ extern "C" int hipcx_adamw_many(const hipcx_array* const* params, const hipcx_ar
         Extent reach{}, written_reach{};  // of what begins before: the farthest end, and the farthest of what is written
         for (const Extent& e : extents) {
             HIPCX_REQUIRE(!(e.from < written_reach.to || (e.written && e.from < reach.to)), HIPCX_CHAINERX_ERROR,
-                          "adamw: arrays that are updated share memory with each other or with gradients");
+                          "adamw: arrays that are updated share memory with each other, with gradients or with t");
             if (e.to > reach.to) reach = e;
             if (e.written && e.to > written_reach.to) written_reach = e;
         }
