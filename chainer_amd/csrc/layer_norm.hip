@@ -135,23 +135,24 @@ struct RowPiece {
     }
 };
 
-// What a row's values are taken relative to: the mean.  float16's values have eleven bits, and their differences from a mean of 24 would all be rounded alike and shift the second sum by it; from
-// the mean in twelve bits, or from 0 where it is less than half of the mean of their absolute values (`sum[1]`), they are exact.
-template <typename T>
-constexpr int kFirstSums = std::is_same<T, half_t>::value ? 2 : 1;
-template <typename T, typename C>
+// What a row's values are taken relative to: the mean, and 0 where that is less than half of the mean of their absolute values (`sum[1]`).  Values of one power of two have their last bit in one
+// place, so that differences from a mean with bits beyond it are all rounded alike and shift the second sum by up to 2^-24 of the values, which is nothing next to a mean of their size, but more
+// than the first sum's error next to a small one; and from a mean that small, cancellation takes less than half a bit of the variance.  float16's values, of eleven bits, are taken relative to
+// the mean in twelve, from which their differences are exact.
+template <typename C>
 __device__ __forceinline__ void AddFirst(C* sum, C v) {
     sum[0] += v;
-    if constexpr (kFirstSums<T> == 2) sum[1] += fabsf(v);
+    sum[1] += __builtin_elementwise_abs(v);
 }
 template <typename T, typename C>
 __device__ __forceinline__ C NearMean(const C* sum, C n) {
+    if (__builtin_elementwise_abs(sum[0]) < static_cast<C>(0.5) * sum[1]) return static_cast<C>(0);
     const C mean = sum[0] / n;
-    if constexpr (kFirstSums<T> == 2) return fabsf(sum[0]) < 0.5f * sum[1] ? 0.f : __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, mean) & 0xfffff000u);
+    if constexpr (std::is_same<T, half_t>::value) return __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, mean) & 0xfffff000u);
     else return mean;
 }
 
-// The first sum gives a mean that is off by its rounding, and the sum of the differences from it corrects both the mean and the variance: two passes over registers.  R rows at once: their loads
+// The first sum gives a number near the mean, and the sums of the differences from it and of their squares the mean and the variance: two passes over registers.  R rows at once: their loads
 // are under way together, their sums meet together, and the parameters are read once for all of them.  Bound by memory: 16384 rows of 4096 in float16, parameters in float32, take 51 us
 // (5.2 TB/s; one row at a time, 95 us: each row's parameters are four times its bytes from L2), 4480 rows of 650 in float32 6.9 us, of which some 3 are the launch.
 template <typename T, typename P, int G, int V, int R, bool NARROW>
@@ -182,12 +183,10 @@ __global__ __launch_bounds__(G > 256 ? G : 256) void LayerNormKernel(NormArgs p)
 #pragma unroll
         for (int j = 0; j < V; ++j) load(j);
     }
-    constexpr int F = kFirstSums<T>;
-    C v[R][V][E], sum[F * R], more[2 * R];
+    C v[R][V][E], sum[2 * R], more[2 * R];
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-#pragma unroll
-        for (int i = 0; i < F; ++i) sum[F * r + i] = 0;
+        sum[2 * r] = sum[2 * r + 1] = 0;
 #pragma unroll
         for (int j = 0; j < V; ++j) {
             const Piece piece(l, j, cols);
@@ -195,15 +194,15 @@ __global__ __launch_bounds__(G > 256 ? G : 256) void LayerNormKernel(NormArgs p)
 #pragma unroll
             for (int e = 0; e < E; ++e) {
                 v[r][j][e] = static_cast<C>(raw[r][j].v[e]);
-                AddFirst<T>(sum + F * r, all || piece.Counts(e) ? v[r][j][e] : static_cast<C>(0));
+                AddFirst(sum + 2 * r, all || piece.Counts(e) ? v[r][j][e] : static_cast<C>(0));
             }
         }
     }
     RowSum<G, 2 * R>(sum, meet, turn);
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-        const C about = NearMean<T>(sum + F * r, n);
-        sum[F * r] = about;
+        const C about = NearMean<T>(sum + 2 * r, n);
+        sum[2 * r] = about;
         more[2 * r] = more[2 * r + 1] = 0;
 #pragma unroll
         for (int j = 0; j < V; ++j) {
@@ -228,7 +227,7 @@ __global__ __launch_bounds__(G > 256 ? G : 256) void LayerNormKernel(NormArgs p)
         var = var < 0 ? static_cast<C>(0) : var;
         const C inv = static_cast<C>(1) / static_cast<C>(sqrt(var + static_cast<C>(p.eps)));
         if (l == 0) {
-            static_cast<C*>(p.mean)[row] = sum[F * r] + off;
+            static_cast<C*>(p.mean)[row] = sum[2 * r] + off;
             static_cast<C*>(p.inv_std)[row] = inv;
         }
 #pragma unroll
@@ -256,8 +255,8 @@ __global__ __launch_bounds__(1024) void LayerNormLongKernel(NormArgs p) {
     for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x) {
         const T* const x = static_cast<const T*>(p.x) + row * p.x_pitch;
         T* const y = static_cast<T*>(p.out) + row * p.cols;
-        C sum[kFirstSums<T>] = {}, more[2] = {0, 0};
-        for (int64_t i = threadIdx.x; i < p.cols; i += 1024) AddFirst<T>(sum, static_cast<C>(x[i]));
+        C sum[2] = {0, 0}, more[2] = {0, 0};
+        for (int64_t i = threadIdx.x; i < p.cols; i += 1024) AddFirst(sum, static_cast<C>(x[i]));
         RowSum<1024, 2>(sum, meet, turn);
         const C about = NearMean<T>(sum, n);
         for (int64_t i = threadIdx.x; i < p.cols; i += 1024) {
