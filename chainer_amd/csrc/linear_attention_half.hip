@@ -1,4 +1,4 @@
-// Linear attention of float16: the passes of linear_attention.h on the float16 matrix pipe, with nothing that was computed in fewer than 22 bits.
+// Linear attention of float16: the passes of linear_attention.h on the float16 matrix pipe, with nothing that was computed in fewer than 23 bits.
 #include "igemm.h"
 #include "linear_attention.h"
 
@@ -42,14 +42,16 @@ struct Scale {
 __device__ __forceinline__ int ExponentOf(float v) { return (__builtin_bit_cast(int, v) >> 23) - 127; }  // of v >= 0
 __device__ __forceinline__ float Power(int e) { return __builtin_bit_cast(float, (127 + e) << 23); }       // of -126 to 127
 
-// Values of at most 2^15 as the sum of two float16: 22 bits of those from 2^-14 on.  `minus`: -1, which the compiler is not to know, so that the difference is one instruction that takes a
-// float16 as it is.
+// Values of at most 2^15 as the sum of two float16, each rounded to nearest: 23 bits and a sign of those from 2^-2 on, 2^-25 of the others.  (Cut off instead, as quickly, they kept 21 bits and
+// all errors had one sign.)  `minus`: -1, which the compiler is not to know, so that the difference is one instruction that takes a float16 as it is.
 template <int N>
 __device__ __forceinline__ void Split(const float (&v)[N], float minus, _Float16 __attribute__((ext_vector_type(N)))* high, _Float16 __attribute__((ext_vector_type(N)))* low) {
+    typedef float float2_t __attribute__((ext_vector_type(2)));
 #pragma unroll
     for (int e = 0; e < N; e += 2) {
-        const auto hi = __builtin_amdgcn_cvt_pkrtz(v[e], v[e + 1]);
-        const auto lo = __builtin_amdgcn_cvt_pkrtz(__builtin_fmaf(static_cast<float>(hi[0]), minus, v[e]), __builtin_fmaf(static_cast<float>(hi[1]), minus, v[e + 1]));
+        const attend_half2_t hi = __builtin_convertvector((float2_t{v[e], v[e + 1]}), attend_half2_t);
+        const float2_t rest{__builtin_fmaf(static_cast<float>(hi[0]), minus, v[e]), __builtin_fmaf(static_cast<float>(hi[1]), minus, v[e + 1])};
+        const attend_half2_t lo = __builtin_convertvector(rest, attend_half2_t);
         (*high)[e] = hi[0], (*high)[e + 1] = hi[1], (*low)[e] = lo[0], (*low)[e + 1] = lo[1];
     }
 }
@@ -72,7 +74,7 @@ struct AttendHalfLds {
 //   y^T = S^T Q^T, S in two parts of float16 in LDS;
 //   P^T = K Q^T (rows s, a lane to a row t) from float16 as they come; times the weights, brought to float16's range by a power of two for each t, in two parts; y^T += V^T P^T;
 //   S <- exp(G[63]) S + K^T (exp(G[63] - G) V), V's products in two parts.
-// S and what is added to it are counted in a power of two for each column (`unit`), which changes when the column's largest element leaves 2^4 to 2^15 of it, so that parts of float16 keep 22
+// S and what is added to it are counted in a power of two for each column (`unit`), which changes when the column's largest element leaves 2^4 to 2^15 of it, so that parts of float16 keep 23
 // bits of anything that counts next to it.
 // A reduction over 32 rows s takes them in the order in which accumulators have them, eight to a lane, for both operands: 4 q + j and 16 + 4 q + j for quarter q of a wave.
 // (32 rows by 32 columns of y to a wave have every block of P computed by two waves; half of the keys by 32 columns of S every product with V.)

@@ -42,3 +42,19 @@ def test_every_width_after_the_widest(chx, dtype):  # noqa: F811
         for length in (70, 1100):
             c = attend_case((1, length, 1, 1, keys, values), dtype, seed=keys)
             check_attend(chx, c, lambda a: up(chx, a), None, True, True, '%d rows, %d keys, %d values' % (length, keys, values))
+
+
+def test_products_of_float16_inputs_keep_the_bits_of_float32(chx):  # noqa: F811
+    """The state's gradient where each element is one product, scale * gy, as q's rows are unit vectors: what is multiplied on the float16 pipe in two parts has lost no more than a rounding or two.
+
+    The product is rounded by half a step of float32, 2^-24 of it.  Its first part, rounded to eleven bits, leaves at most 2^-11 of its power of two, a multiple of the last of 24 bits; the second
+    one, of eleven bits, rounds that by half of 2^-22 at most.  Both are the same multiples and their sum has 24 bits, so that no addition rounds: 2^-24 + 2^-23.  (Parts that are cut off instead of
+    rounded lose up to three times 2^-23, always towards zero.)"""
+    rng = np.random.default_rng(3)
+    zeros = np.zeros((1, 64, 1, 64), np.float16)
+    q = np.eye(64, dtype=np.float16)[rng.permutation(64)].reshape(1, 64, 1, 64)
+    gy = (rng.choice([-1, 1], (1, 64, 1, 64)) * (1 + rng.integers(0, 1024, (1, 64, 1, 64)) / 1024)).astype(np.float16)
+    for scale in (0.3, 0.7):
+        g = chx.linear_attention_grad(up(chx, q), up(chx, zeros), up(chx, zeros), up(chx, gy), scale=scale, state=chx.zeros((1, 1, 64, 64)))
+        want = q[0, :, 0].astype(np.float64).T @ gy[0, :, 0] * np.float64(np.float32(scale))
+        assert (np.abs(g.state.get()[0, 0] - want) <= 1.5 * 2.0 ** -23 * np.abs(want)).all(), scale
