@@ -130,7 +130,6 @@ __device__ __forceinline__ double AttendDecay(const AttendArgs& p, int64_t b, in
 struct AttendDecays {
     alignas(16) float high[kAttendTile], low[kAttendTile];
     float end[kAttendTile];  // from a row to the tile's end, as a factor, times kv_scale
-    float near[kAttendTile]; // from a row to the last of its sixteen, as a factor
     float all;               // the tile's
     double sum;              // the tile's, in powers of two
 };
@@ -154,16 +153,8 @@ __device__ __forceinline__ double AddMoved(double v) {
     return v + __builtin_bit_cast(double, static_cast<uint64_t>(hi) << 32 | lo);
 }
 
-// The value of lane L of a row of 16 lanes.
-template <int L>
-__device__ __forceinline__ double OfLaneInRow(double v) {
-    const uint64_t b = __builtin_bit_cast(uint64_t, v);
-    const uint32_t lo = __builtin_amdgcn_mov_dpp(static_cast<int>(b), 0x150 + L, 0xf, 0xf, true), hi = __builtin_amdgcn_mov_dpp(static_cast<int>(b >> 32), 0x150 + L, 0xf, 0xf, true);
-    return __builtin_bit_cast(double, static_cast<uint64_t>(hi) << 32 | lo);
-}
-
-// By one wave, a lane to a row, of which `here` are there; g in powers of two, 0 for the others.
-__device__ __forceinline__ void SumDecays(AttendDecays* to, double g, int here, float kv_scale) {
+// By one wave, a lane to a row, of which `here` are there; g in powers of two, 0 for the others.  Returns the sum up to the lane's row.
+__device__ __forceinline__ double SumDecays(AttendDecays* to, double g, int here, float kv_scale) {
     const int lane = threadIdx.x % 64;
     double sum = AddMoved<0x111, 0xf>(g);  // from 1, 2, 4 and 8 lanes before in the row of 16, then from the rows' last lanes
     sum = AddMoved<0x112, 0xf>(sum);
@@ -177,8 +168,8 @@ __device__ __forceinline__ void SumDecays(AttendDecays* to, double g, int here, 
     const float high = static_cast<float>(sum);
     to->high[lane] = high, to->low[lane] = static_cast<float>(sum - high);
     to->end[lane] = lane < here ? __builtin_amdgcn_exp2f(static_cast<float>(all - sum)) * kv_scale : 0.f;
-    to->near[lane] = __builtin_amdgcn_exp2f(static_cast<float>(OfLaneInRow<15>(sum) - sum));
     if (lane == 0) to->all = __builtin_amdgcn_exp2f(static_cast<float>(all)), to->sum = all;
+    return sum;
 }
 
 // Rows of a segment: [first, end) of the sequence's.

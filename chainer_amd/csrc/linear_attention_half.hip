@@ -58,6 +58,26 @@ __device__ __forceinline__ void Split(const float (&v)[N], float minus, _Float16
 
 __device__ __forceinline__ attend4_t Mfma(attend_half8_t a, attend_half8_t b, attend4_t c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
 
+// The value of lane L of a row of 16 lanes.
+template <int L>
+__device__ __forceinline__ double OfLaneInRow(double v) {
+    const uint64_t b = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = __builtin_amdgcn_mov_dpp(static_cast<int>(b), 0x150 + L, 0xf, 0xf, true), hi = __builtin_amdgcn_mov_dpp(static_cast<int>(b >> 32), 0x150 + L, 0xf, 0xf, true);
+    return __builtin_bit_cast(double, static_cast<uint64_t>(hi) << 32 | lo);
+}
+
+// Factors of P's rows s, 0 for rows whose v is zeros: they have no part in the power of two of the others.
+struct AttendHalfDecays : AttendDecays {
+    alignas(16) float near[kAttendTile];  // from a row to the last of its sixteen, as a factor
+    alignas(16) float own[kAttendTile];   // `low`, or infinity, which takes exp2(high - high[s] + low - own[s]) to 0
+};
+// 0 for a piece of zeros.
+__device__ __forceinline__ uint32_t AnyOf(AttendPiece<half_t, 8> piece) {
+    typedef uint32_t registers_t __attribute__((ext_vector_type(4)));
+    const registers_t d = __builtin_bit_cast(registers_t, piece);
+    return (d[0] | d[1] | d[2] | d[3]) & 0x7fff7fffu;
+}
+
 // LDS of a workgroup, in bytes.  Rows' pitches keep the banks apart.  Clocks of a wave's instruction (eight waves at work), at 128 keys: k and the state's copies read by rows, sixteen rows of 64
 // bytes each, 4.0 with 32 or 96 bytes more than a multiple of 256, 7.9 with 16, 6.6 with 80; v in blocks of 4 x 16, sixteen rows, 2.6 with 32 more than 128, 4.0 with 64; the state's copies
 // written, 8.0 with 32, 5.0 with 16.
@@ -66,16 +86,17 @@ struct AttendHalfLds {
     static constexpr int kKeyPitch = KD * 2 + 96, kValuePitch = kAttendColumns * 2 + 32, kStatePitch = KD * 2 + 32;
     static constexpr int kValues = kAttendTile * kKeyPitch, kStates = kValues + kAttendTile * kValuePitch,
                          kLow = kStates + (OUT ? kAttendColumns * kStatePitch : 0), kScales = kLow + (OUT ? kAttendColumns * kStatePitch : 0), kSums = kScales + kAttendColumns * 4, kDecays = kSums + 4 * kAttendColumns * 4,
-                         kOdd = kDecays + 2 * static_cast<int>(sizeof(AttendDecays)), kBytes = kOdd + 16;
-    static_assert(kValues % 16 == 0 && kStates % 16 == 0 && kDecays % 16 == 0 && sizeof(AttendDecays) % 16 == 0, "aligned parts");
+                         kOdd = kDecays + 2 * static_cast<int>(sizeof(AttendHalfDecays)), kBytes = kOdd + 16;
+    static_assert(kValues % 16 == 0 && kStates % 16 == 0 && kDecays % 16 == 0 && sizeof(AttendHalfDecays) % 16 == 0, "aligned parts");
 };
 
 // As AttendKernel (linear_attention.hip): a wave has sixteen rows of y with all 64 columns, and sixteen columns of the state with all keys in its accumulators.
 //   y^T = S^T Q^T, S in two parts of float16 in LDS;
 //   P^T = K Q^T (rows s, a lane to a row t) from float16 as they come; times the weights, brought to float16's range by a power of two for each t, in two parts; y^T += V^T P^T;
 //   S <- exp(G[63]) S + K^T (exp(G[63] - G) V), V's products in two parts.
-// S and what is added to it are counted in a power of two for each column (`unit`), which changes when the column's largest element leaves 2^4 to 2^15 of it, so that parts of float16 keep 23
-// bits of anything that counts next to it.
+// S and what is added to it are counted in a power of two for each column (`unit`), which changes when the largest element of the column or of what is added (V's products) leaves 2^4 to 2^15 of
+// it, so that parts of float16 keep 23 bits, or 2^-29 of that largest element; a row of P in one of its own, so that they keep 23 bits or 2^-39 of its largest.  Rows of k that are zeros have no part
+// in the largest of what is added, nor rows of v that are zeros in P's, whatever a mask has left on the other side (prompt of 16384 rows 135 -> 136 us, training on 2048 rows 294 -> 298).
 // A reduction over 32 rows s takes them in the order in which accumulators have them, eight to a lane, for both operands: 4 q + j and 16 + 4 q + j for quarter q of a wave.
 // (32 rows by 32 columns of y to a wave have every block of P computed by two waves; half of the keys by 32 columns of S every product with V.)
 // Bound by a tile's chain at two workgroups to a compute unit: of its cycles the vector units work in 45 %, LDS in 40, the matrix pipes in 17.  One sequence of 16384 rows, 16 heads of 128 x 128: 102 us
@@ -91,7 +112,7 @@ __global__ __launch_bounds__(256, KD == 256 ? 1 : KD == 128 ? 2 : 3) void Attend
     char *const ks = lds, *const vs = lds + Lds::kValues, *const high_copy = lds + Lds::kStates, *const low_copy = lds + Lds::kLow;
     float* const scales = reinterpret_cast<float*>(lds + Lds::kScales);  // [2][VB]
     float* const sums = reinterpret_cast<float*>(lds + Lds::kSums);      // [4][VB]
-    AttendDecays* const decays = reinterpret_cast<AttendDecays*>(lds + Lds::kDecays);
+    AttendHalfDecays* const decays = reinterpret_cast<AttendHalfDecays*>(lds + Lds::kDecays);
     int* const odd = reinterpret_cast<int*>(lds + Lds::kOdd);            // v has infinities or what is not a number
 
     int id = AttendNumber(p);
@@ -237,9 +258,13 @@ __global__ __launch_bounds__(256, KD == 256 ? 1 : KD == 128 ? 2 : 3) void Attend
     const auto load_decays = [&](int64_t r0) {  // of a row that is there; sum_decays takes those that count
         if (gp != nullptr) g_next = decay_at(r0 + lane);
     };
-    const auto sum_decays = [&](int64_t r0, AttendDecays* to) {
+    const auto sum_decays = [&](int64_t r0, AttendHalfDecays* to) {
         const int here = static_cast<int>(rows - r0 < C ? rows - r0 : C);
-        SumDecays(to, gp != nullptr && lane < here && r0 + lane >= g_rows ? LogOfDecay(g_now) : 0, here, kv_scale);
+        const double sum = SumDecays(to, gp != nullptr && lane < here && r0 + lane >= g_rows ? LogOfDecay(g_now) : 0, here, kv_scale);
+        if (OUT) {
+            to->near[lane] = __builtin_amdgcn_exp2f(static_cast<float>(OfLaneInRow<15>(sum) - sum));
+            to->own[lane] = static_cast<float>(sum - static_cast<float>(sum));
+        }
     };
     if (EVEN) {
 #pragma unroll
@@ -269,11 +294,13 @@ __global__ __launch_bounds__(256, KD == 256 ? 1 : KD == 128 ? 2 : 3) void Attend
     for (; r0 < rows; r0 += C, turn ^= 1) {
         asm volatile("" : "+v"(lane));
         asm volatile("" : "+s"(keys));
-        const AttendDecays* const dec = decays + turn;
+        AttendHalfDecays* const dec = decays + turn;
         // (the last tile's rows of k and v have been read by all)
+        uint32_t some = ~0u;  // 0 where a piece is zeros
 #pragma unroll
         for (int n = 0; n < NK; ++n) {
             if (!EVEN || key_col < keys) *reinterpret_cast<attend_half8_t*>(ks + (key_row + n * (2048 / KD)) * Lds::kKeyPitch + key_col * 2) = placed(k_next[n], key_col, keys);
+            some = min(some, AnyOf(k_next[n]));
         }
         attend_half2_t finite{};  // 0, or not a number
 #pragma unroll
@@ -282,6 +309,21 @@ __global__ __launch_bounds__(256, KD == 256 ? 1 : KD == 128 ? 2 : 3) void Attend
             if (!EVEN || value_col < cols) *reinterpret_cast<attend_half8_t*>(vs + (value_row + n * 32) * Lds::kValuePitch + value_col * 2) = v;
 #pragma unroll
             for (int e = 0; e < 8; e += 2) finite = __builtin_elementwise_fma(attend_half2_t{v[e], v[e + 1]}, attend_half2_t{}, finite);
+            if (OUT) some = min(some, AnyOf(v_next[n]));
+        }
+        if (__any(some == 0)) {
+            // Rows of zeros: what they are multiplied with, which a mask may have left as it was, is not to decide the power of two that the others are counted in.
+            const auto zeros = [&](const AttendPiece<T, 8>& piece, int lanes) {  // of `lanes` neighbours, whose pieces are a row
+                return (__ballot(AnyOf(piece) != 0) >> (lane & -lanes) & (~uint64_t{0} >> (64 - lanes))) == 0;
+            };
+#pragma unroll
+            for (int n = 0; n < NK; ++n) {
+                if (zeros(k_next[n], KD / 8)) dec->end[key_row + n * (2048 / KD)] = 0;
+            }
+#pragma unroll
+            for (int n = 0; n < NV; ++n) {
+                if (OUT && zeros(v_next[n], VB / 8)) dec->near[value_row + n * 32] = 0, dec->own[value_row + n * 32] = HUGE_VALF;
+            }
         }
         if (OUT && !(finite[0] + finite[1] == 0)) odd[turn] = 1;
         __syncthreads();
@@ -399,10 +441,10 @@ __global__ __launch_bounds__(256, KD == 256 ? 1 : KD == 128 ? 2 : 3) void Attend
                 if (sb > wave) continue;
                 const int first = 16 * sb + 4 * quarter;
                 if (sb == wave) {
-                    const attend4_t highs = *reinterpret_cast<const attend4_t*>(dec->high + first), lows = *reinterpret_cast<const attend4_t*>(dec->low + first);
+                    const attend4_t highs = *reinterpret_cast<const attend4_t*>(dec->high + first), owns = *reinterpret_cast<const attend4_t*>(dec->own + first);
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        const float weighted = a[sb][e] * __builtin_amdgcn_exp2f((high - highs[e]) + (low - lows[e]));
+                        const float weighted = a[sb][e] * __builtin_amdgcn_exp2f((high - highs[e]) + (low - owns[e]));
                         a[sb][e] = 4 * quarter + e <= lane % 16 ? weighted : 0.f;
                     }
                     since[sb] = 1;

@@ -3,7 +3,7 @@ import numpy as np
 import pytest
 
 import block_reference as ref
-from test_gpu_block_layers import attend_case, check_attend, chx, up  # noqa: F401
+from test_gpu_block_layers import attend_case, check_attend, check_attend_outputs, chx, up  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -58,3 +58,20 @@ def test_products_of_float16_inputs_keep_the_bits_of_float32(chx):  # noqa: F811
         g = chx.linear_attention_grad(up(chx, q), up(chx, zeros), up(chx, zeros), up(chx, gy), scale=scale, state=chx.zeros((1, 1, 64, 64)))
         want = q[0, :, 0].astype(np.float64).T @ gy[0, :, 0] * np.float64(np.float32(scale))
         assert (np.abs(g.state.get()[0, 0] - want) <= 1.5 * 2.0 ** -23 * np.abs(want)).all(), scale
+
+
+@pytest.mark.parametrize('length', [70, 300, 1100])
+@pytest.mark.parametrize('zero,large', [('k', 'v'), ('v', 'k'), ('q', 'gy'), ('gy', 'q')])
+@pytest.mark.parametrize('dtype', ['float16', 'float32'])
+def test_rows_of_zeros_next_to_large_numbers(chx, zero, large, length, dtype):  # noqa: F811
+    """Rows that a mask has made zeros on one side and left as they are on the other, some 2^25 times the others' size: no other row has fewer bits for them."""
+    c = attend_case((2, length, 2, 1, 40, 72), dtype, seed=7)
+    rng = np.random.default_rng(8)
+    c['v'], c['gy'], c['gnew'] = (c['v'] * 1e-3).astype(dtype), (c['gy'] * 1e-2).astype(dtype), c['gnew'] * np.float32(1e-2)
+    c['q'], c['k'] = (c['q'] * 0.1).astype(dtype), (c['k'] * 0.1).astype(dtype)
+    c['state'] = c['state'] * np.float32(1e-3)
+    masked = rng.random((2, length, 2)) < 0.2
+    masked[:, 0] = masked[:, -1] = True
+    c[zero][masked] = 0
+    c[large][masked] = (rng.choice([-1, 1], (masked.sum(), c[large].shape[3])) * rng.integers(20000, 60000, (masked.sum(), c[large].shape[3]))).astype(dtype)
+    check_attend_outputs(chx, c, None)  # (element by element: many results are subnormal numbers of float16, whose half step, 2^-25, is no part of their norm)
