@@ -75,3 +75,24 @@ def test_rows_of_zeros_next_to_large_numbers(chx, zero, large, length, dtype):  
     c[zero][masked] = 0
     c[large][masked] = (rng.choice([-1, 1], (masked.sum(), c[large].shape[3])) * rng.integers(20000, 60000, (masked.sum(), c[large].shape[3]))).astype(dtype)
     check_attend_outputs(chx, c, None)  # (element by element: many results are subnormal numbers of float16, whose half step, 2^-25, is no part of their norm)
+
+
+@pytest.mark.parametrize('dtype', ['float16', 'float32'])
+@pytest.mark.parametrize('length,row', [(70, 69), (100, 41), (900, 540), (900, 899)])
+def test_an_infinite_key_stays_in_its_place(chx, length, row, dtype):  # noqa: F811
+    """From its row on, in its head and sequence; in the state, in its key alone: nothing finite there, and elsewhere what is without it, but for other powers of two."""
+    c = attend_case((2, length, 2, 1, 40, 70), dtype)
+    args = lambda c: ([up(chx, c[k]) for k in ('q', 'k', 'v')], dict(log_decay=up(chx, c['log_decay']), state=up(chx, c['state'])))  # noqa: E731
+    a, more = args(c)
+    plain, plain_new = (x.get() for x in chx.linear_attention(*a, **more))
+    _, (off, off_new) = ref.linear_attention(c['q'], c['k'], c['v'], c['log_decay'], None, c['state'])
+    for value in (np.inf, -np.inf):
+        bad = dict(c, k=c['k'].copy())
+        bad['k'][1, row, 0, 17] = value
+        a, more = args(bad)
+        y, new = (x.get() for x in chx.linear_attention(*a, **more))
+        touched, touched_new = np.zeros(y.shape, bool), np.zeros(new.shape, bool)
+        touched[1, row:, 0] = touched_new[1, 0, 17] = True
+        assert not np.isfinite(y[touched]).any() and not np.isfinite(new[touched_new]).any()
+        for got, want, at, far, half in ((y, plain, touched, off, np.finfo(dtype).eps / 2), (new, plain_new, touched_new, off_new, 0)):
+            assert (np.abs(got.astype(np.float64) - want) <= 2 * far + 2 * half * np.abs(want.astype(np.float64)) + 2.0 ** -24)[~at].all()
