@@ -184,13 +184,16 @@ struct AttendSpan {
 };
 
 // How the time axis is cut: into segments of whole tiles, two at least, of the number that costs least.  Costs are in a tile's time with the compute units full (`resident` workgroups to each):
-// a round of workgroups takes a segment's tiles and three more for what comes before and behind them, `alone` (float16 0.85, float32 0.6) of that where there is a workgroup to a compute unit at most
+// a round of workgroups takes a segment's tiles and three more for what comes before and behind them, 0.85 of that where there is a workgroup to a compute unit at most
 // and between them in proportion; segments need the states that they start from first, which takes 0.4 of a tile each, and a pass over the states.  Of a padded batch half of the workgroups are taken to have work.
 // `blocks`: workgroups to a head and segment; `states`: those of the states alone.
 // One sequence of 16384 rows, 16 heads of 128 x 128 in float16, in 8, 16, 24 and 48 segments: 179, 141, 154 and 170 us, and 16 are taken; 20 padded ones of up to 777, 13 heads of 50 x 50 in
 // float32, in 1, 2 and 3: 114, 110 and 95, and 3 are taken; 9 of 2533, 11 heads of 100 x 100 in float16, in 1, 2, 5 and 8: 186, 178, 161 and 179, and 5 are taken.
-inline void CutAttend(AttendArgs* p, double alone, bool padded, int64_t blocks, int64_t states, int64_t resident, int64_t matrix) {
+// float32 with up to 64 keys, cut for three workgroups to a compute unit where two fit, and for two: forward pass of 4 x 2048 rows of 8 heads 61 and 53 us, gradients of one sequence of 5000 rows of 10
+// heads 127 and 115, of 2 x 3868 rows, 14 heads of 16 keys and 80 values, 331 and 298.
+inline void CutAttend(AttendArgs* p, bool padded, int64_t blocks, int64_t states, int64_t resident, int64_t matrix) {
     const int64_t tiles = (p->length + kAttendTile - 1) / kAttendTile, heads = p->batch * p->heads, units = NumCUs();
+    constexpr double alone = 0.85;
     const auto rounds = [&](int64_t workgroups, int64_t at_once) {
         if (padded) workgroups = (workgroups + 1) / 2;
         const int64_t rest = workgroups % at_once;
@@ -249,9 +252,9 @@ void VisitWidths(AttendWidths widths, bool grad, F&& f) {
     else grad ? f(std::integral_constant<int, kAttendPart>{}, std::true_type{}) : f(std::integral_constant<int, kAttendPart>{}, std::false_type{});
 }
 
-inline double AttendAlone(int dtype) { return dtype == HIPCX_FLOAT16 ? 0.85 : 0.6; }
 // Workgroups that a compute unit holds, as registers and LDS let them.
-inline int64_t AttendResident(int keys) { return keys <= 64 ? 3 : keys <= 128 ? 2 : 1; }
+constexpr int kLdsOfUnit = 160 * 1024;
+constexpr int AttendResident(bool half, int keys) { return keys <= 64 && half ? 3 : keys <= 128 ? 2 : 1; }
 
 void LaunchAttend(const AttendArgs& p, int dtype, bool states_alone, hipStream_t stream);
 void LaunchAttendHalf(const AttendArgs& p, int keys, int64_t blocks, bool states_alone, hipStream_t stream);  // float16

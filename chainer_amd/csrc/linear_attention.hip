@@ -12,7 +12,7 @@ namespace {
 // A workgroup of four waves has 64 columns of v: a wave has sixteen rows of y, and sixteen columns of S in its accumulators (a copy is in LDS, turned, for the products with q).
 // P stays in registers: as k q^T its column t is a lane, whose rows s are the reduction of the product v^T P.
 // Products run on the float pipe (v_mfma_f32_16x16x4_f32), with the reduction's elements in an order that gives a lane four neighbours.  Bound by a tile's chain: at 64 keys and values the wave of the
-// last rows multiplies for 8.2 thousand cycles of a tile's 16, and three workgroups share a compute unit.  20 padded prompts of up to 777 rows, 13 heads of 50 x 50: 61 us, the states of their three
+// last rows multiplies for 8.2 thousand cycles of a tile's 16, and two workgroups share a compute unit.  20 padded prompts of up to 777 rows, 13 heads of 50 x 50: 61 us, the states of their three
 // segments before it 30; rows of 32 to a wave, and loads that waited for one another, took 222 in one segment.  At 128 keys and values 24 x 478 rows of 11 heads with gradients run at 72 TFLOP/s.
 // GRAD: what the passes of the gradients have beyond the forward one.
 template <int KD, bool OUT>
@@ -20,18 +20,20 @@ struct AttendLds {
     static_assert(kAttendTile == kAttendColumns, "the rows of k and the columns of the state share a place");
     static constexpr int kPitch = KD + 4, kValuePitch = kAttendColumns + 4;  // floats; four rows on is sixteen banks on
     // At 128 keys the copy of the state and the rows of k, as many, take turns in one place, so that two workgroups fit into a compute unit: for two more barriers a tile, 24 x 478 rows of 11 heads
-    // with gradients 898 -> 723 us.  64 keys fit three times either way (20 padded prompts of 777 rows: 94 us, with turns 109), 256 once.
+    // with gradients 898 -> 723 us.  64 keys fit twice as they are; with turns three times, which is no quicker for the barriers
+    // (20 padded prompts of 777 rows: 94 us, with turns 109); 256 fit once.
     static constexpr bool kTurns = KD == 128;
     static constexpr int kValues = kAttendTile * kPitch, kStates = kTurns ? 0 : kValues + kAttendTile * kValuePitch;
     static constexpr int kSums = (kTurns ? kValues + kAttendTile * kValuePitch : kStates + (OUT ? kAttendColumns * kPitch : 0));
     static constexpr int kDecays = kSums + 4 * kAttendColumns;
     static constexpr int kBytes = kDecays * 4 + 2 * static_cast<int>(sizeof(AttendDecays)) + 16;
+    static_assert(AttendResident(false, KD) * kBytes <= kLdsOfUnit, "as many workgroups as the time axis is cut for");
 };
 
 __device__ __forceinline__ attend4_t Mfma4(float a, float b, attend4_t c) { return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0); }
 
 template <int KD, bool OUT, int WIDTHS, bool GRAD>
-__global__ __launch_bounds__(256, KD == 64 ? 3 : KD == 128 ? 2 : 1) void AttendKernel(AttendArgs p) {
+__global__ __launch_bounds__(256, AttendResident(false, KD)) void AttendKernel(AttendArgs p) {
     using Lds = AttendLds<KD, OUT>;
     constexpr int VB = kAttendColumns, C = kAttendTile, NS = KD / 16, KP = Lds::kPitch, VP = Lds::kValuePitch, DB = VB / 16;
     extern __shared__ __align__(16) float lds[];
@@ -675,7 +677,7 @@ constexpr int kAttendTokens = 8;
 
 void CutForward(AttendCall* c, bool padded) {
     if (c->p.length <= kAttendTokens) c->p.segments = 1, c->p.segment_rows = kAttendTile;
-    else CutAttend(&c->p, AttendAlone(c->dtype), padded, AttendBlocks(c->values), AttendBlocks(c->values), AttendResident(c->keys), static_cast<int64_t>(c->keys) * c->values);
+    else CutAttend(&c->p, padded, AttendBlocks(c->values), AttendBlocks(c->values), AttendResident(c->dtype == HIPCX_FLOAT16, c->keys), static_cast<int64_t>(c->keys) * c->values);
 }
 
 size_t ForwardWorkspace(const AttendCall& c) {

@@ -119,7 +119,7 @@ struct GradWorkspace {
 
 void CutGrad(AttendCall* c, bool padded) {
     const int64_t keys = AttendBlocks(c->keys), values = AttendBlocks(c->values);
-    CutAttend(&c->p, AttendAlone(c->dtype), padded, 2 * keys + values, keys + values, AttendResident(std::max(c->keys, c->values)), 2 * static_cast<int64_t>(c->keys) * c->values);
+    CutAttend(&c->p, padded, 2 * keys + values, keys + values, AttendResident(c->dtype == HIPCX_FLOAT16, std::max(c->keys, c->values)), 2 * static_cast<int64_t>(c->keys) * c->values);
 }
 
 }  // namespace

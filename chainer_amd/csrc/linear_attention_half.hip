@@ -87,6 +87,7 @@ struct AttendHalfLds {
     static constexpr int kValues = kAttendTile * kKeyPitch, kStates = kValues + kAttendTile * kValuePitch,
                          kLow = kStates + (OUT ? kAttendColumns * kStatePitch : 0), kScales = kLow + (OUT ? kAttendColumns * kStatePitch : 0), kSums = kScales + kAttendColumns * 4, kDecays = kSums + 4 * kAttendColumns * 4,
                          kOdd = kDecays + 2 * static_cast<int>(sizeof(AttendHalfDecays)), kBytes = kOdd + 16;
+    static_assert(AttendResident(true, KD) * kBytes <= kLdsOfUnit, "as many workgroups as the time axis is cut for");
     static_assert(kValues % 16 == 0 && kStates % 16 == 0 && kDecays % 16 == 0 && sizeof(AttendHalfDecays) % 16 == 0, "aligned parts");
 };
 
@@ -103,7 +104,7 @@ struct AttendHalfLds {
 // and 43 for the states of its 16 segments; on the float pipe 1.1 ms.  Gradients of 4 x 2048 rows, 16 heads of 128 x 128, three passes: 220 us.
 // GRAD: what the passes of the gradients have beyond the forward one.
 template <int KD, bool OUT, int WIDTHS, bool GRAD>
-__global__ __launch_bounds__(256, KD == 256 ? 1 : KD == 128 ? 2 : 3) void AttendHalfKernel(AttendArgs p) {
+__global__ __launch_bounds__(256, AttendResident(true, KD)) void AttendHalfKernel(AttendArgs p) {
     using T = half_t;
     constexpr bool EVEN = WIDTHS == kAttendWhole;
     using Lds = AttendHalfLds<KD, OUT>;
