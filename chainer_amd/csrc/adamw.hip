@@ -4,7 +4,8 @@
 //
 // States in 8 bits: blocks of 256 elements share a scale, the power of two that no value of the block exceeds.  A code counts eighths of a power of two, down to 2^-14 of the
 // scale for m (a sign, 4 bits of exponent) and 2^-30 for sqrt(v) (5 bits; a value that is not 0 is never stored as 0, as m is divided by it), and below that the lowest one's eighths.  Values are
-// rounded to one of the two neighbours at random, in proportion: a step changes v by a thousandth, and rounded to the nearest of 8 bits it would never change at all.  The numbers come from
+// rounded to one of the two neighbours at random, in proportion: a step changes v by a thousandth, and rounded to the nearest of 8 bits it would never change at all.
+// (sqrt(v) is what comes out right on average, so that v is larger by the variance of its roundings, some percent.)  The numbers come from
 // a counter: 16 bits each for m and v of an element.
 #include <algorithm>
 #include <cmath>
@@ -92,7 +93,7 @@ __device__ __forceinline__ uint32_t TopOf32(uint32_t v) {
 }
 
 // A pass over memory.  A thread takes eight neighbours, 32 threads a block of states in 8 bits.  25.5 M float16 weights of 161 arrays with master copies: 163 us, 4.7 TB/s.  States in 8 bits are bound by
-// the vector units, by a division and a root that round as IEEE 754 says and half a Philox counter to an element: 19.8 M weights 67 us, where their 198 MB would take 41.
+// the vector units, by a division and a root that round as IEEE 754 says and half a Philox counter to an element: 19.8 M weights 68 us, where their 198 MB would take 41.
 template <typename P, typename G, bool EIGHT, bool MASTER>
 __global__ __launch_bounds__(256) void AdamWKernel(AdamWArgs a) {
     constexpr int E = kPerThread;

@@ -1309,7 +1309,8 @@ def adamw_update(params, grads, states, t, alpha=0.001, beta1=0.9, beta2=0.999, 
     """A step of AdamW (chainer/optimizers/adam.py: AdamRule with weight_decay_rate) of many parameters in place: m += (1 - beta1) * (g - m), v += (1 - beta2) * (g * g - v),
     p -= eta * (alpha * sqrt(1 - beta2 ** t) / (1 - beta1 ** t) * m / (sqrt(v) + eps) + weight_decay_rate * p), in one launch for up to 48 arrays of a kind.  ``states``: one from
     ``adamw_state`` for every parameter, of 8 bits for some and of 32 for others as wanted.  ``t``: the step, from 1 on, or an int64 array of one element, so that a captured graph
-    goes on to the next.  ``seed``: of the numbers by which states in 8 bits are rounded; they depend on it, on t, and on a parameter's place in the list."""
+    goes on to the next.  ``seed``: of the numbers by which states in 8 bits are rounded; they depend on it, on t, and on a parameter's place in the list.  m and sqrt(v) are right on average, v in 8 bits a few
+    percent too large."""
     _host.adamw_update(params, grads, states, t, alpha, beta1, beta2, eps, eta, weight_decay_rate, seed)
 
 

@@ -200,7 +200,9 @@ int hipcx_update_many(const hipcx_array* const* xs, const hipcx_array* const* gs
  *   with m_scales and v_scales, float32 [size / 256 rounded up], the power of two that no value of a block of 256 exceeds (states of zeros: all zeros).  A code c of m stands for (8 + c % 8)
  *   2^(c / 8 % 16 - 18) of the scale, c % 8 2^-17 where c / 8 % 16 is 0, minus that from 128 on; one of sqrt(v) for (8 + c % 8) 2^(c / 8 - 34), or c 2^-33 below 8.  Values go to one of their two
  *   neighbours at random in proportion, but sqrt(v) > 0 never to 0: 16 bits each for m and v of element e of array i from Philox4x32-10's word e % 4 for counter {e / 4, i, low and high half of t}
- *   and key {low and high half of seed}.  A block that holds what is not finite, or more than 2^100, becomes NaN.  masters: float32 copies of float16 parameters, updated in
+ *   and key {low and high half of seed}.  sqrt(v) is what is right on average, so that v is
+ *   larger by the variance of its roundings: 4 % with random gradients and beta2 0.999, where an element's sqrt(v) spreads by some 15 %.  A block that holds what is not finite, or more than
+ *   2^100, becomes NaN.  masters: float32 copies of float16 parameters, updated in
  *   their place, of which the parameters are roundings; NULL for those that have none.  m_scales[i], v_scales[i]: NULL for states in 32 bits.  t: the step, from 1 on, or t_array, int64
  *   of one element in device memory, so that a captured graph takes another one's.  All arrays C-contiguous, of up to 2^33 elements; those that are written share no memory with any other. */
 int hipcx_adamw_many(const hipcx_array* const* params, const hipcx_array* const* grads, const hipcx_array* const* ms, const hipcx_array* const* vs,
@@ -526,7 +528,7 @@ int hipcx_linear_attention_grad(const hipcx_array* q, const hipcx_array* k, cons
 
 /* hipcx_layer_norm: F.layer_normalization (chainer/functions/normalization/layer_normalization.py; the reference composes it of some ten kernels): rows, the last axis, brought to mean 0 and
  *   variance 1, y = (x - mean) inv_std gamma + beta with inv_std = 1 / sqrt(var + eps) and var the mean square of what is off the mean.  x [..., columns] of a floating dtype, its rows dense and
- *   equally far apart; y like x, C-contiguous; gamma and beta [columns], each may be NULL (ones, zeros), of x's dtype or float32 where x is float16; mean and inv_std: the
+ *   equally far apart (all of them one row, perhaps; a row that repeats inside other axes is not); y like x, C-contiguous; gamma and beta [columns], each may be NULL (ones, zeros), of x's dtype or float32 where x is float16; mean and inv_std: the
  *   state that the gradient takes, x's shape without its last axis, float32 (float64 for float64), C-contiguous.  Rows of any length but 0; computed in float32 (float64), rounded
  *   once.  y may be x.
  * hipcx_layer_norm_grad: gx and, where asked for, ggamma and gbeta, sums over rows in float32 and then in 64 bits, in an order that the sizes and the device's compute units decide. */
