@@ -71,11 +71,21 @@ struct AttendHalfDecays : AttendDecays {
     alignas(16) float near[kAttendTile];  // from a row to the last of its sixteen, as a factor
     alignas(16) float own[kAttendTile];   // `low`, or infinity, which takes exp2(high - high[s] + low - own[s]) to 0
 };
-// 0 for a piece of zeros.
-__device__ __forceinline__ uint32_t AnyOf(AttendPiece<half_t, 8> piece) {
-    typedef uint32_t registers_t __attribute__((ext_vector_type(4)));
-    const registers_t d = __builtin_bit_cast(registers_t, piece);
-    return (d[0] | d[1] | d[2] | d[3]) & 0x7fff7fffu;
+typedef uint32_t attend_uint4_t __attribute__((ext_vector_type(4)));
+// Whether a piece is zeros.
+__device__ __forceinline__ bool IsZeros(AttendPiece<half_t, 8> piece) {
+    const attend_uint4_t d = __builtin_bit_cast(attend_uint4_t, piece);
+    return ((d[0] | d[1] | d[2] | d[3]) & 0x7fff7fffu) == 0;
+}
+// Whether one of some pieces may be: its first two elements, taken for a float, are one below 2^-126 then.  An instruction to two pieces (the compiler would make what is not a number quiet first).
+template <int N>
+__device__ __forceinline__ float LeastOf(const AttendPiece<half_t, 8> (&pieces)[N], float least) {
+#pragma unroll
+    for (int n = 0; n < N; n += 2) {
+        const uint32_t a = __builtin_bit_cast(attend_uint4_t, pieces[n])[0], b = __builtin_bit_cast(attend_uint4_t, pieces[n + 1 < N ? n + 1 : n])[0];
+        asm("v_min3_f32 %0, |%0|, |%1|, |%2|" : "+v"(least) : "v"(a), "v"(b));
+    }
+    return least;
 }
 
 // LDS of a workgroup, in bytes.  Rows' pitches keep the banks apart.  Clocks of a wave's instruction (eight waves at work), at 128 keys: k and the state's copies read by rows, sixteen rows of 64
@@ -97,7 +107,8 @@ struct AttendHalfLds {
 //   S <- exp(G[63]) S + K^T (exp(G[63] - G) V), V's products in two parts.
 // S and what is added to it are counted in a power of two for each column (`unit`), which changes when the largest element of the column or of what is added (V's products) leaves 2^4 to 2^15 of
 // it, so that parts of float16 keep 23 bits, or 2^-29 of that largest element; a row of P in one of its own, so that they keep 23 bits or 2^-39 of its largest.  Rows of k that are zeros have no part
-// in the largest of what is added, nor rows of v that are zeros in P's, whatever a mask has left on the other side (prompt of 16384 rows 135 -> 136 us, training on 2048 rows 294 -> 298).
+// in the largest of what is added, nor rows of v that are zeros in P's, whatever a mask has left on the other side (told by an
+// instruction to two pieces and the flag of infinities: 0.5 % of the prompt of 16384 rows; of gradients at 50 and 256 keys 3 and 2 %).
 // A reduction over 32 rows s takes them in the order in which accumulators have them, eight to a lane, for both operands: 4 q + j and 16 + 4 q + j for quarter q of a wave.
 // (32 rows by 32 columns of y to a wave have every block of P computed by two waves; half of the keys by 32 columns of S every product with V.)
 // Bound by a tile's chain at two workgroups to a compute unit: of its cycles the vector units work in 45 %, LDS in 40, the matrix pipes in 17.  One sequence of 16384 rows, 16 heads of 128 x 128: 100 us
@@ -114,7 +125,7 @@ __global__ __launch_bounds__(256, AttendResident(true, KD)) void AttendHalfKerne
     float* const scales = reinterpret_cast<float*>(lds + Lds::kScales);  // [2][VB]
     float* const sums = reinterpret_cast<float*>(lds + Lds::kSums);      // [4][VB]
     AttendHalfDecays* const decays = reinterpret_cast<AttendHalfDecays*>(lds + Lds::kDecays);
-    int* const odd = reinterpret_cast<int*>(lds + Lds::kOdd);            // v has infinities or what is not a number
+    int* const odd = reinterpret_cast<int*>(lds + Lds::kOdd);            // [2][2]: v has infinities or what is not a number; a row may be zeros
 
     int id = AttendNumber(p);
     if (id < 0) return;
@@ -277,7 +288,7 @@ __global__ __launch_bounds__(256, AttendResident(true, KD)) void AttendHalfKerne
             if (value_col >= cols) *reinterpret_cast<attend_half8_t*>(vs + (value_row + n * 32) * Lds::kValuePitch + value_col * 2) = attend_half8_t{};
         }
     }
-    if (tid == 0) odd[0] = odd[1] = 0;
+    if (tid == 0) odd[0] = odd[1] = odd[2] = odd[3] = 0;
     if (rows > 0) {
         if (wave == 0) {
             load_decays(0);
@@ -297,11 +308,9 @@ __global__ __launch_bounds__(256, AttendResident(true, KD)) void AttendHalfKerne
         asm volatile("" : "+s"(keys));
         AttendHalfDecays* const dec = decays + turn;
         // (the last tile's rows of k and v have been read by all)
-        uint32_t some = ~0u;  // 0 where a piece is zeros
 #pragma unroll
         for (int n = 0; n < NK; ++n) {
             if (!EVEN || key_col < keys) *reinterpret_cast<attend_half8_t*>(ks + (key_row + n * (2048 / KD)) * Lds::kKeyPitch + key_col * 2) = placed(k_next[n], key_col, keys);
-            some = min(some, AnyOf(k_next[n]));
         }
         attend_half2_t finite{};  // 0, or not a number
 #pragma unroll
@@ -310,27 +319,43 @@ __global__ __launch_bounds__(256, AttendResident(true, KD)) void AttendHalfKerne
             if (!EVEN || value_col < cols) *reinterpret_cast<attend_half8_t*>(vs + (value_row + n * 32) * Lds::kValuePitch + value_col * 2) = v;
 #pragma unroll
             for (int e = 0; e < 8; e += 2) finite = __builtin_elementwise_fma(attend_half2_t{v[e], v[e + 1]}, attend_half2_t{}, finite);
-            if (OUT) some = min(some, AnyOf(v_next[n]));
         }
-        if (__any(some == 0)) {
-            // Rows of zeros: what they are multiplied with, which a mask may have left as it was, is not to decide the power of two that the others are counted in.
+        // Rows of zeros: what they are multiplied with, which a mask may have left as it was, is not to decide the power of two that the others are counted in.
+        const auto leave_out_zeros = [&] {
+            int thread = tid;
+            asm volatile("" : "+v"(thread));
             const auto zeros = [&](const AttendPiece<T, 8>& piece, int lanes) {  // of `lanes` neighbours, whose pieces are a row
-                return (__ballot(AnyOf(piece) != 0) >> (lane & -lanes) & (~uint64_t{0} >> (64 - lanes))) == 0;
+                return (__ballot(!IsZeros(piece)) >> (thread % 64 & -lanes) & (~uint64_t{0} >> (64 - lanes))) == 0;
             };
 #pragma unroll
             for (int n = 0; n < NK; ++n) {
-                if (zeros(k_next[n], KD / 8)) dec->end[key_row + n * (2048 / KD)] = 0;
+                if (zeros(k_next[n], KD / 8)) dec->end[thread / (KD / 8) + n * (2048 / KD)] = 0;
             }
 #pragma unroll
-            for (int n = 0; n < NV; ++n) {
-                if (OUT && zeros(v_next[n], VB / 8)) dec->near[value_row + n * 32] = 0, dec->own[value_row + n * 32] = HUGE_VALF;
+            for (int n = 0; n < (OUT ? NV : 0); ++n) {
+                const int row = thread / (VB / 8) + n * 32;
+                if (zeros(v_next[n], VB / 8)) dec->near[row] = 0, dec->own[row] = HUGE_VALF;
             }
+        };
+        float least = LeastOf(k_next, 1.f);
+        if (OUT) least = LeastOf(v_next, least);
+        const bool bad = OUT && !(finite[0] + finite[1] == 0), empty = !(least >= 0x1p-126f);
+        if (OUT) {
+            if (bad || empty) odd[2 * turn + (bad ? 0 : 1)] = 1;
+        } else if (__builtin_expect(__any(empty), 0)) {
+            leave_out_zeros();
         }
-        if (OUT && !(finite[0] + finite[1] == 0)) odd[turn] = 1;
         __syncthreads();
         passed += dec->sum;
-        // An infinity of a later row, times P's zeros, would reach earlier ones: the rest goes row by row.
-        if (OUT && odd[turn] != 0) break;
+        if (OUT) {
+            const int any_bad = __builtin_amdgcn_readfirstlane(odd[2 * turn]), any_empty = __builtin_amdgcn_readfirstlane(odd[2 * turn + 1]);
+            if (__builtin_expect((any_bad | any_empty) != 0, 0)) {
+                // An infinity of a later row, times P's zeros, would reach earlier ones: the rest goes row by row.
+                if (any_bad != 0) break;
+                leave_out_zeros();
+                __syncthreads();
+            }
+        }
         const bool more = r0 + C < rows;
         g_now = g_next;
         load(r0 + C);
@@ -434,7 +459,7 @@ __global__ __launch_bounds__(256, AttendResident(true, KD)) void AttendHalfKerne
                 }
             }
             if (wave == 0 && more) sum_decays(r0 + C, decays + (turn ^ 1));
-            if (tid == 0) odd[turn ^ 1] = 0;
+            if (tid == 0) odd[2 * (turn ^ 1)] = odd[2 * (turn ^ 1) + 1] = 0;
             // weights: of the sixteen rows that this one is among, exp(G[t] - G[s]); of earlier ones, whose last is l, exp(G[l] - G[s]) here and exp(G[t] - G[l]) with the power of two
             float largest = 0, since[4];
 #pragma unroll

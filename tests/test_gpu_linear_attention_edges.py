@@ -96,3 +96,23 @@ def test_an_infinite_key_stays_in_its_place(chx, length, row, dtype):  # noqa: F
         assert not np.isfinite(y[touched]).any() and not np.isfinite(new[touched_new]).any()
         for got, want, at, far, half in ((y, plain, touched, off, np.finfo(dtype).eps / 2), (new, plain_new, touched_new, off_new, 0)):
             assert (np.abs(got.astype(np.float64) - want) <= 2 * far + 2 * half * np.abs(want.astype(np.float64)) + 2.0 ** -24)[~at].all()
+
+
+@pytest.mark.parametrize('dtype', ['float16', 'float32'])
+def test_rows_of_few_numbers(chx, dtype):  # noqa: F811
+    """Rows that are zeros but for one element, first, last or anywhere, and rows of zeros of both signs beside them: the first are not left out."""
+    for keys, values in ((40, 72), (64, 64), (256, 30), (7, 9)):
+        c = attend_case((2, 200, 2, 1, keys, values), dtype, seed=keys)
+        rng = np.random.default_rng(keys)
+        for name in ('q', 'k', 'v', 'gy'):
+            a = c[name]
+            width = a.shape[3]
+            kept = rng.choice([0, 1, width - 1, width // 2, -1], a.shape[:3])
+            some = np.where(kept == -1, rng.integers(0, width, a.shape[:3]), kept)
+            one = np.arange(width) == some[..., None]
+            a[...] = np.where(rng.random(a.shape[:3])[..., None] < 0.5, a, np.where(one, a, np.asarray(0, dtype)))
+            gone = rng.random(a.shape[:3]) < 0.2
+            a[gone] = np.where(rng.random((gone.sum(), width)) < 0.5, 0.0, -0.0).astype(dtype)
+        check_attend(chx, c, lambda a: up(chx, a), None, True, True, '%d keys, %d values %s' % (keys, values, dtype))
+        c['k'][:], c['v'][:] = 0, -0.0
+        check_attend(chx, c, lambda a: up(chx, a), None, True, True, 'nothing but zeros, %d keys, %d values %s' % (keys, values, dtype))
