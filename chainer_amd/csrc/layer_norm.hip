@@ -153,8 +153,8 @@ __device__ __forceinline__ C NearMean(const C* sum, C n) {
 }
 
 // The first sum gives a number near the mean, and the sums of the differences from it and of their squares the mean and the variance: two passes over registers.  R rows at once: their loads
-// are under way together, their sums meet together, and the parameters are read once for all of them.  Bound by memory: 16384 rows of 4096 in float16, parameters in float32, take 52 us
-// (5.2 TB/s; one row at a time, 95 us: each row's parameters are four times its bytes from L2), 4480 rows of 650 in float32 7.0 us, of which some 3 are the launch.
+// are under way together, their sums meet together, and the parameters are read once for all of them.  Bound by memory: 16384 rows of 4096 in float16, parameters in float32, take 53 us
+// (5.1 TB/s; one row at a time, 95 us: each row's parameters are four times its bytes from L2), 4480 rows of 650 in float32 7.0 us, of which some 3 are the launch.
 template <typename T, typename P, int G, int V, int R, bool NARROW>
 __global__ __launch_bounds__(G > 256 ? G : 256) void LayerNormKernel(NormArgs p) {
     using C = NormCompute<T>;
@@ -283,7 +283,7 @@ __global__ __launch_bounds__(1024) void LayerNormLongKernel(NormArgs p) {
 }
 
 // R rows' two sums, then their gradients, with the next rows on their way; a thread keeps its columns' sums over the rows that its workgroup walks through.  Bound by memory: 16384 rows of 4096 in
-// float16 take 84 us (4.8 TB/s; without the next rows' loads ahead, one row at a time, 160), 4480 rows of 650 in float32 9.8 us.
+// float16 take 86 us (4.7 TB/s; without the next rows' loads ahead, one row at a time, 160), 4480 rows of 650 in float32 9.7 us.
 template <typename T, typename P, int G, int V, int R, bool NARROW>
 __global__ __launch_bounds__(G > 256 ? G : 256) void LayerNormGradKernel(NormArgs p) {
     using C = NormCompute<T>;

@@ -112,7 +112,7 @@ struct AttendHalfLds {
 // A reduction over 32 rows s takes them in the order in which accumulators have them, eight to a lane, for both operands: 4 q + j and 16 + 4 q + j for quarter q of a wave.
 // (32 rows by 32 columns of y to a wave have every block of P computed by two waves; half of the keys by 32 columns of S every product with V.)
 // Bound by a tile's chain at two workgroups to a compute unit: of its cycles the vector units work in 45 %, LDS in 40, the matrix pipes in 17.  One sequence of 16384 rows, 16 heads of 128 x 128: 100 us
-// and 42 for the states of its 16 segments; on the float pipe 1.1 ms.  Gradients of 4 x 2048 rows, 16 heads of 128 x 128, three passes: 224 us.
+// and 42 for the states of its 16 segments; on the float pipe 1.1 ms.  Gradients of 4 x 2048 rows, 16 heads of 128 x 128, three passes: 227 us.
 // GRAD: what the passes of the gradients have beyond the forward one.
 template <int KD, bool OUT, int WIDTHS, bool GRAD>
 __global__ __launch_bounds__(256, AttendResident(true, KD)) void AttendHalfKernel(AttendArgs p) {

@@ -512,7 +512,8 @@ int hipcx_selective_scan_grad(const hipcx_array* u, const hipcx_array* delta, co
  *   products, and where sequences and heads are few the time axis is cut into segments whose states take the workspace.  Products and sums of float32 run in float32; float16 inputs are
  *   taken as they are, and what is computed from them in two parts of float16, every number to 23 bits or to 2^-29 of the largest of its column of the state or of what a tile of rows adds to that,
  *   whichever is larger (weights of rows: of its row), not counting rows of k or v that are zeros; sums are float32's.  Infinities and what is not a number reach the rows that the formulas
- *   say, where an infinity may have become NaN.  Rows of q, k, v, y and their gradients 2^24 elements apart or more are refused (HIPCX_NOT_IMPLEMENTED_ERROR).
+ *   say, where an infinity may have become NaN.  A decay of less than 2^-126 from one row to another leaves nothing.  Rows of q, k, v, y and their gradients 2^24 elements apart or more are
+ *   refused (HIPCX_NOT_IMPLEMENTED_ERROR).
  * hipcx_linear_attention_grad: from gy and gnew_state (or NULL, zeros) the gradients of q, k, v, and of log_decay (in its shape, C-contiguous) and state (C-contiguous), which may be NULL.
  *   Those of log_decay are differences of q gq and k gk summed up from the last row of a segment, in 64 bits, so that what is not finite in a row of these reaches all earlier ones.  All sums run in an order that depends on the sizes, and on whether there are lengths, alone.  The workspace holds, for
  *   key heads that are shared, every head's gradients of q and k in float32, with log_decay some 16 bytes a row, head and 64 keys, and where time is cut two states a segment and head. */
