@@ -510,8 +510,8 @@ int hipcx_selective_scan_grad(const hipcx_array* u, const hipcx_array* delta, co
  *   heads / key heads neighbours of which share a head of q and k; 1 to 256 keys and values.  log_decay: g, float32 [heads], [batch, time, heads] or NULL (0), of any strides;
  *   -infinity ends what was gathered.  state, new_state: float32 [batch, heads, keys, values], C-contiguous.  Up to eight rows go one after another; longer ones in tiles of 64 as matrix
  *   products, and where sequences and heads are few the time axis is cut into segments whose states take the workspace.  Products and sums of float32 run in float32; float16 inputs are
- *   taken as they are, and what is computed from them in two parts of float16, every number to 23 bits or to 2^-29 of the largest of its column of the state or of what a tile of rows adds to that,
- *   whichever is larger (weights of rows: of its row), not counting rows of k or v that are zeros; sums are float32's.  Infinities and what is not a number reach the rows that the formulas
+ *   taken as they are, and what is computed from them in two parts of float16, every number to 23 bits or, where that is more, to 2^-29 of the largest of its column: of the state, and of
+ *   v times its decays in a tile of rows, however small their k is (2^-39 of the largest of a row of weights, however small their v is); rows of k or v that are zeros do not count.  Sums are float32's.  Infinities and what is not a number reach the rows that the formulas
  *   say, where an infinity may have become NaN.  A decay of less than 2^-126 from one row to another leaves nothing.  Rows of q, k, v, y and their gradients 2^24 elements apart or more are
  *   refused (HIPCX_NOT_IMPLEMENTED_ERROR).
  * hipcx_linear_attention_grad: from gy and gnew_state (or NULL, zeros) the gradients of q, k, v, and of log_decay (in its shape, C-contiguous) and state (C-contiguous), which may be NULL.
